@@ -352,6 +352,64 @@ typedef struct osm_engine_args {
   float* scratch;               /* osm_engine_scratch_bytes, 16-byte aligned */
 } osm_engine_args;
 
+/* ---------------------------------------------------------------------------
+ * The gated delta rule: per batch row b and head h, a matrix state S [dk, dv]
+ *
+ *   S_t = e^{g_t} S_{t-1} + k_t u_t^T,   u_t = beta_t (v_t - e^{g_t} S_{t-1}^T k_t)
+ *   o_t = scale S_t^T q_t
+ *
+ * one step of gradient descent on |S^T k_t - v_t|^2 a token, at rate beta_t,
+ * after a decay e^{g_t}.  No counterpart in the reference.
+ *
+ * q and k have Hk heads, H a multiple of Hk: head h uses head h / (H / Hk) of
+ * them.  Arithmetic is fp32 throughout (products on the fp32 matrix
+ * instruction), results are rounded once to `dtype`.  g below -200 counts as
+ * -200.  Tokens at and past lengths[b] are not read, leave the state as it is
+ * and give zeros (outputs and gradients).  A NaN or infinity in a token may
+ * reach the outputs of its whole chunk of 64 tokens, and those after it. */
+typedef struct osm_rows {
+  void* p;                      /* element (b, t, h, j) at b*stride_b + t*stride_s + h*stride_h + j */
+  int64_t stride_b, stride_s, stride_h;   /* elements, >= 0 */
+} osm_rows;
+
+#define OSM_DELTA_MAX_DK 128
+
+typedef struct osm_delta_args {
+  int32_t abi_version;          /* = OSM_ABI_VERSION */
+  int32_t dtype;                /* osm_dtype of q, k, v, out and their gradients */
+  int64_t B, S, H, Hk, dk, dv;  /* dk <= OSM_DELTA_MAX_DK */
+  float scale;
+  osm_rows q, k, v, out;        /* [B,S,Hk,dk] (q, k), [B,S,H,dv] (v, out) */
+  osm_rows g, beta;             /* [B,S,H] fp32 */
+  const int32_t* lengths;       /* [B], or NULL: every row has S tokens */
+  const float* state_init;      /* [B,H,dk,dv] contiguous, or NULL: zeros */
+  float* state_out;             /* [B,H,dk,dv] contiguous, or NULL; may be state_init */
+  void* saved;                  /* osm_delta_saved_bytes for the backward, or NULL */
+} osm_delta_args;
+
+typedef struct osm_delta_bwd_args {
+  osm_rows grad_out;            /* [B,S,H,dv] of `dtype` */
+  const float* grad_state;      /* dL/d state_out [B,H,dk,dv] contiguous, or NULL */
+  osm_rows grad_q, grad_k;      /* [B,S,Hk,dk] of `dtype` */
+  osm_rows grad_v;              /* [B,S,H,dv] of `dtype` */
+  osm_rows grad_g, grad_beta;   /* [B,S,H] fp32 */
+  float* grad_init;             /* [B,H,dk,dv] contiguous, or NULL; may be grad_state */
+} osm_delta_bwd_args;
+
+/* One token a row (S = 1; stride_s unused), the states in a pool. */
+typedef struct osm_delta_step_args {
+  int32_t abi_version;          /* = OSM_ABI_VERSION */
+  int32_t dtype;                /* osm_dtype of q, k, v and out */
+  int64_t B, H, Hk, dk, dv;
+  float scale;
+  osm_rows q, k, v, out;        /* [B,Hk,dk], [B,H,dv] */
+  osm_rows g, beta;             /* [B,H] fp32 */
+  float* state;                 /* [n_slots,H,dk,dv], slots state_stride elements apart; updated in place */
+  int64_t state_stride, n_slots;
+  const int64_t* slots;         /* [B] distinct slots, or NULL: row b uses slot b.  Negative: an idle row, whose
+                                 * output is 0; past the pool: NaN.  Neither touches a state */
+} osm_delta_step_args;
+
 /* Which entry point a workspace is sized for. */
 typedef enum osm_op { OSM_OP_FWD = 0, OSM_OP_TTT = 1, OSM_OP_BWD = 2 } osm_op;
 
@@ -444,6 +502,23 @@ int osm_engine_prologue(const osm_engine_args* args, void* stream);
  * comment. */
 int osm_cheby_ema_bwd(const osm_cheby_args* args, const osm_cheby_bwd_args* bwd, void* workspace,
                       size_t workspace_bytes, void* stream);
+
+/* The gated delta rule over sequences.  `saved` (args->saved) and the workspace
+ * need no initialisation and 256-byte alignment; nothing is kept in the
+ * workspace between calls.  Three launches, or one where S is at most 16 and
+ * nothing is saved (the workspace is then 0 bytes and may be NULL). */
+size_t osm_delta_saved_bytes(const osm_delta_args* args);
+size_t osm_delta_workspace_bytes(const osm_delta_args* args);
+int osm_delta_fwd(const osm_delta_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Its backward, from the inputs and what osm_delta_fwd saved of them (out and
+ * state_out of `args` are not used). */
+size_t osm_delta_bwd_workspace_bytes(const osm_delta_args* args);
+int osm_delta_bwd(const osm_delta_args* args, const osm_delta_bwd_args* bwd, void* workspace, size_t workspace_bytes,
+                  void* stream);
+
+/* One token a row, in one launch. */
+int osm_delta_step(const osm_delta_step_args* args, void* stream);
 
 #ifdef __cplusplus
 }

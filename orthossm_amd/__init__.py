@@ -10,6 +10,8 @@ call sites in ``orthossm_amd.engine``.
 from .ops import cheby_ema, cheby_ema_backward, cheby_ema_forward, cheby_ema_ttt
 from .sdpc_kernel import apply_cheby_rkv_core, apply_cheby_rkv_v10
 from .engine import ChebyContextPath, ChebyState
+from .delta import gated_delta, gated_delta_backward, gated_delta_forward, gated_delta_step
 
 __all__ = ["cheby_ema", "cheby_ema_forward", "cheby_ema_backward", "cheby_ema_ttt", "apply_cheby_rkv_v10",
-           "apply_cheby_rkv_core", "ChebyContextPath", "ChebyState"]
+           "apply_cheby_rkv_core", "ChebyContextPath", "ChebyState", "gated_delta", "gated_delta_forward",
+           "gated_delta_backward", "gated_delta_step"]

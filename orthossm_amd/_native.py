@@ -37,6 +37,7 @@ OP_BWD = 2
 OP_LUT = 3   # key of the fixed-coefficient scan's workspaces (not an osm_op)
 V10_USE_LUT = 0x1
 ENGINE_MAX_D = 1024   # row length of osm_engine_prologue
+DELTA_MAX_DK = 128    # rows of the gated delta rule's state
 
 STATUS = {
     0: "OSM_OK",
@@ -70,6 +71,12 @@ EXPORTS = (
     "osm_cheby_ema_lut_fwd_ws",
     "osm_engine_scratch_bytes",
     "osm_engine_prologue",
+    "osm_delta_saved_bytes",
+    "osm_delta_workspace_bytes",
+    "osm_delta_fwd",
+    "osm_delta_bwd_workspace_bytes",
+    "osm_delta_bwd",
+    "osm_delta_step",
 )
 
 
@@ -274,6 +281,83 @@ class EngineArgs(ctypes.Structure):
     ]
 
 
+class Rows(ctypes.Structure):
+    """Mirror of ``osm_rows``."""
+
+    _fields_ = [
+        ("p", ctypes.c_void_p),
+        ("stride_b", ctypes.c_int64),
+        ("stride_s", ctypes.c_int64),
+        ("stride_h", ctypes.c_int64),
+    ]
+
+
+class DeltaArgs(ctypes.Structure):
+    """Mirror of ``osm_delta_args``."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("B", ctypes.c_int64),
+        ("S", ctypes.c_int64),
+        ("H", ctypes.c_int64),
+        ("Hk", ctypes.c_int64),
+        ("dk", ctypes.c_int64),
+        ("dv", ctypes.c_int64),
+        ("scale", ctypes.c_float),
+        ("q", Rows),
+        ("k", Rows),
+        ("v", Rows),
+        ("out", Rows),
+        ("g", Rows),
+        ("beta", Rows),
+        ("lengths", ctypes.c_void_p),
+        ("state_init", ctypes.c_void_p),
+        ("state_out", ctypes.c_void_p),
+        ("saved", ctypes.c_void_p),
+    ]
+
+
+class DeltaBwdArgs(ctypes.Structure):
+    """Mirror of ``osm_delta_bwd_args``."""
+
+    _fields_ = [
+        ("grad_out", Rows),
+        ("grad_state", ctypes.c_void_p),
+        ("grad_q", Rows),
+        ("grad_k", Rows),
+        ("grad_v", Rows),
+        ("grad_g", Rows),
+        ("grad_beta", Rows),
+        ("grad_init", ctypes.c_void_p),
+    ]
+
+
+class DeltaStepArgs(ctypes.Structure):
+    """Mirror of ``osm_delta_step_args``."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("B", ctypes.c_int64),
+        ("H", ctypes.c_int64),
+        ("Hk", ctypes.c_int64),
+        ("dk", ctypes.c_int64),
+        ("dv", ctypes.c_int64),
+        ("scale", ctypes.c_float),
+        ("q", Rows),
+        ("k", Rows),
+        ("v", Rows),
+        ("out", Rows),
+        ("g", Rows),
+        ("beta", Rows),
+        ("state", ctypes.c_void_p),
+        ("state_stride", ctypes.c_int64),
+        ("n_slots", ctypes.c_int64),
+        ("slots", ctypes.c_void_p),
+    ]
+
+
 class OsmError(RuntimeError):
     def __init__(self, code: int, msg: str):
         super().__init__(f"{STATUS.get(code, code)}: {msg}")
@@ -333,6 +417,16 @@ def load() -> ctypes.CDLL:
         lib.osm_engine_scratch_bytes.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64]
         lib.osm_engine_prologue.restype = ctypes.c_int
         lib.osm_engine_prologue.argtypes = [ctypes.POINTER(EngineArgs), ctypes.c_void_p]
+        for name in ("osm_delta_saved_bytes", "osm_delta_workspace_bytes", "osm_delta_bwd_workspace_bytes"):
+            getattr(lib, name).restype = ctypes.c_size_t
+            getattr(lib, name).argtypes = [ctypes.POINTER(DeltaArgs)]
+        lib.osm_delta_fwd.restype = ctypes.c_int
+        lib.osm_delta_fwd.argtypes = [ctypes.POINTER(DeltaArgs), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+        lib.osm_delta_bwd.restype = ctypes.c_int
+        lib.osm_delta_bwd.argtypes = [ctypes.POINTER(DeltaArgs), ctypes.POINTER(DeltaBwdArgs), ctypes.c_void_p,
+                                      ctypes.c_size_t, ctypes.c_void_p]
+        lib.osm_delta_step.restype = ctypes.c_int
+        lib.osm_delta_step.argtypes = [ctypes.POINTER(DeltaStepArgs), ctypes.c_void_p]
         got = lib.osm_abi_version()
         if got != ABI_VERSION:
             raise ImportError(f"orthossm_amd: library ABI {got} != binding ABI {ABI_VERSION}; rebuild")

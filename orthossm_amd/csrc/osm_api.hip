@@ -20,9 +20,9 @@
 constexpr size_t kStaticScratchBytes = size_t(32) << 20;
 static __device__ __align__(256) unsigned char scratch[kStaticScratchBytes];
 
-namespace {
+static thread_local std::string g_err;
 
-thread_local std::string g_err;
+namespace osm {
 
 int fail(int code, const char* fmt, ...) {
   char buf[512];
@@ -38,6 +38,13 @@ int ok() {
   g_err.clear();
   return OSM_OK;
 }
+
+}  // namespace osm
+
+namespace {
+
+using osm::fail;
+using osm::ok;
 
 // log2 of the look-back words per thread for the geometries that hold
 // kFwdWords: 4 words (a checkpoint every 32 tiles) where few lane-blocks have

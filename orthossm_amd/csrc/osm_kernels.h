@@ -443,4 +443,9 @@ hipError_t launch_fill_zero(void* ptr, size_t bytes, hipStream_t stream);
 hipError_t launch_copy_state(const float* src, float* dst, size_t n, hipStream_t stream);
 hipError_t launch_ws_status(void* ws, unsigned* dst, int reset, hipStream_t stream);
 
+// What osm_last_error reports on this thread: fail() sets the message and
+// returns `code`, ok() clears it and returns OSM_OK (osm_api.hip).
+int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+int ok();
+
 }  // namespace osm
