@@ -410,6 +410,52 @@ typedef struct osm_delta_step_args {
                                  * output is 0; past the pool: NaN.  Neither touches a state */
 } osm_delta_step_args;
 
+/* ---------------------------------------------------------------------------
+ * Layer norm over rows of D elements: y = (x - mean) rstd w + b, with
+ * rstd = 1 / sqrt(variance + eps), the variance over D.  fp32 arithmetic, y
+ * rounded once.  No counterpart in the reference. */
+typedef struct osm_norm_args {
+  int32_t abi_version;          /* = OSM_ABI_VERSION */
+  int32_t dtype;                /* osm_dtype of x, y, grad_y and grad_x */
+  int64_t rows, D;
+  float eps;
+  const void* x;                /* rows x_stride elements apart, elements contiguous */
+  int64_t x_stride;
+  const float* weight;          /* [D], or NULL: ones */
+  const float* bias;            /* [D], or NULL: zeros */
+  void* y;                      /* rows must not overlap; may be x */
+  int64_t y_stride;
+  float* mean;                  /* [rows], or both NULL: written by the forward, read by the backward */
+  float* rstd;
+} osm_norm_args;
+
+typedef struct osm_norm_bwd_args {
+  const void* grad_y;
+  int64_t grad_y_stride;
+  void* grad_x;                 /* or NULL */
+  int64_t grad_x_stride;
+  float* grad_weight;           /* [D], or NULL */
+  float* grad_bias;             /* [D], or NULL */
+} osm_norm_bwd_args;
+
+/* ---------------------------------------------------------------------------
+ * The 2-norm over all elements of `count` tensors, and, with OSM_CLIP_SCALE,
+ * their scaling in place by min(1, max_norm / (norm + eps)).  A NaN norm makes
+ * every element NaN, an infinite one 0 (and infinities NaN).  No counterpart in
+ * the reference. */
+#define OSM_CLIP_SCALE 0x1
+
+typedef struct osm_clip_args {
+  int32_t abi_version;          /* = OSM_ABI_VERSION */
+  int32_t flags;
+  int64_t count;
+  void* const* tensors;         /* [count] device pointers (this array and the next two are host memory) */
+  const int64_t* sizes;         /* [count] elements, dense */
+  const int32_t* dtypes;        /* [count] osm_dtype */
+  double max_norm, eps;         /* >= 0 */
+  float* norm;                  /* device scalar */
+} osm_clip_args;
+
 /* Which entry point a workspace is sized for. */
 typedef enum osm_op { OSM_OP_FWD = 0, OSM_OP_TTT = 1, OSM_OP_BWD = 2 } osm_op;
 
@@ -519,6 +565,18 @@ int osm_delta_bwd(const osm_delta_args* args, const osm_delta_bwd_args* bwd, voi
 
 /* One token a row, in one launch. */
 int osm_delta_step(const osm_delta_step_args* args, void* stream);
+
+/* Layer norm and its backward (from x, mean, rstd and weight; y and bias are
+ * not used), whose workspace needs no initialisation and 256-byte alignment. */
+int osm_layer_norm_fwd(const osm_norm_args* args, void* stream);
+size_t osm_layer_norm_bwd_workspace_bytes(const osm_norm_args* args);
+int osm_layer_norm_bwd(const osm_norm_args* args, const osm_norm_bwd_args* bwd, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/* The norm over many tensors, and clipping: two launches for up to 150 tensors
+ * (as many more for every further 150).  Workspace as above. */
+size_t osm_clip_workspace_bytes(const osm_clip_args* args);
+int osm_clip_grad_norm(const osm_clip_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -11,7 +11,10 @@ from .ops import cheby_ema, cheby_ema_backward, cheby_ema_forward, cheby_ema_ttt
 from .sdpc_kernel import apply_cheby_rkv_core, apply_cheby_rkv_v10
 from .engine import ChebyContextPath, ChebyState
 from .delta import gated_delta, gated_delta_backward, gated_delta_forward, gated_delta_step
+from .norm import layer_norm, layer_norm_backward, layer_norm_forward
+from .grad_clip import clip_grad_norm, grad_norm
 
 __all__ = ["cheby_ema", "cheby_ema_forward", "cheby_ema_backward", "cheby_ema_ttt", "apply_cheby_rkv_v10",
            "apply_cheby_rkv_core", "ChebyContextPath", "ChebyState", "gated_delta", "gated_delta_forward",
-           "gated_delta_backward", "gated_delta_step"]
+           "gated_delta_backward", "gated_delta_step", "layer_norm", "layer_norm_forward", "layer_norm_backward",
+           "clip_grad_norm", "grad_norm"]

@@ -38,6 +38,7 @@ OP_LUT = 3   # key of the fixed-coefficient scan's workspaces (not an osm_op)
 V10_USE_LUT = 0x1
 ENGINE_MAX_D = 1024   # row length of osm_engine_prologue
 DELTA_MAX_DK = 128    # rows of the gated delta rule's state
+CLIP_SCALE = 0x1
 
 STATUS = {
     0: "OSM_OK",
@@ -77,6 +78,11 @@ EXPORTS = (
     "osm_delta_bwd_workspace_bytes",
     "osm_delta_bwd",
     "osm_delta_step",
+    "osm_layer_norm_fwd",
+    "osm_layer_norm_bwd_workspace_bytes",
+    "osm_layer_norm_bwd",
+    "osm_clip_workspace_bytes",
+    "osm_clip_grad_norm",
 )
 
 
@@ -358,6 +364,55 @@ class DeltaStepArgs(ctypes.Structure):
     ]
 
 
+class NormArgs(ctypes.Structure):
+    """Mirror of ``osm_norm_args``."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("rows", ctypes.c_int64),
+        ("D", ctypes.c_int64),
+        ("eps", ctypes.c_float),
+        ("x", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("weight", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("y", ctypes.c_void_p),
+        ("y_stride", ctypes.c_int64),
+        ("mean", ctypes.c_void_p),
+        ("rstd", ctypes.c_void_p),
+    ]
+
+
+class NormBwdArgs(ctypes.Structure):
+    """Mirror of ``osm_norm_bwd_args``."""
+
+    _fields_ = [
+        ("grad_y", ctypes.c_void_p),
+        ("grad_y_stride", ctypes.c_int64),
+        ("grad_x", ctypes.c_void_p),
+        ("grad_x_stride", ctypes.c_int64),
+        ("grad_weight", ctypes.c_void_p),
+        ("grad_bias", ctypes.c_void_p),
+    ]
+
+
+class ClipArgs(ctypes.Structure):
+    """Mirror of ``osm_clip_args``."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("flags", ctypes.c_int32),
+        ("count", ctypes.c_int64),
+        ("tensors", ctypes.POINTER(ctypes.c_void_p)),
+        ("sizes", ctypes.POINTER(ctypes.c_int64)),
+        ("dtypes", ctypes.POINTER(ctypes.c_int32)),
+        ("max_norm", ctypes.c_double),
+        ("eps", ctypes.c_double),
+        ("norm", ctypes.c_void_p),
+    ]
+
+
 class OsmError(RuntimeError):
     def __init__(self, code: int, msg: str):
         super().__init__(f"{STATUS.get(code, code)}: {msg}")
@@ -427,6 +482,17 @@ def load() -> ctypes.CDLL:
                                       ctypes.c_size_t, ctypes.c_void_p]
         lib.osm_delta_step.restype = ctypes.c_int
         lib.osm_delta_step.argtypes = [ctypes.POINTER(DeltaStepArgs), ctypes.c_void_p]
+        lib.osm_layer_norm_fwd.restype = ctypes.c_int
+        lib.osm_layer_norm_fwd.argtypes = [ctypes.POINTER(NormArgs), ctypes.c_void_p]
+        lib.osm_layer_norm_bwd_workspace_bytes.restype = ctypes.c_size_t
+        lib.osm_layer_norm_bwd_workspace_bytes.argtypes = [ctypes.POINTER(NormArgs)]
+        lib.osm_layer_norm_bwd.restype = ctypes.c_int
+        lib.osm_layer_norm_bwd.argtypes = [ctypes.POINTER(NormArgs), ctypes.POINTER(NormBwdArgs), ctypes.c_void_p,
+                                           ctypes.c_size_t, ctypes.c_void_p]
+        lib.osm_clip_workspace_bytes.restype = ctypes.c_size_t
+        lib.osm_clip_workspace_bytes.argtypes = [ctypes.POINTER(ClipArgs)]
+        lib.osm_clip_grad_norm.restype = ctypes.c_int
+        lib.osm_clip_grad_norm.argtypes = [ctypes.POINTER(ClipArgs), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
         got = lib.osm_abi_version()
         if got != ABI_VERSION:
             raise ImportError(f"orthossm_amd: library ABI {got} != binding ABI {ABI_VERSION}; rebuild")
