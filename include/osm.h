@@ -369,10 +369,11 @@ typedef struct osm_engine_args {
  * reach the outputs of its whole chunk of 64 tokens, and those after it. */
 typedef struct osm_rows {
   void* p;                      /* element (b, t, h, j) at b*stride_b + t*stride_s + h*stride_h + j */
-  int64_t stride_b, stride_s, stride_h;   /* elements, >= 0 */
+  int64_t stride_b, stride_s, stride_h;   /* elements, >= 0; stride_s <= OSM_DELTA_MAX_STRIDE */
 } osm_rows;
 
 #define OSM_DELTA_MAX_DK 128
+#define OSM_DELTA_MAX_STRIDE (1 << 22)   /* of stride_s: a chunk's rows are addressed in 31 bits */
 
 typedef struct osm_delta_args {
   int32_t abi_version;          /* = OSM_ABI_VERSION */

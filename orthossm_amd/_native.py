@@ -38,6 +38,7 @@ OP_LUT = 3   # key of the fixed-coefficient scan's workspaces (not an osm_op)
 V10_USE_LUT = 0x1
 ENGINE_MAX_D = 1024   # row length of osm_engine_prologue
 DELTA_MAX_DK = 128    # rows of the gated delta rule's state
+DELTA_MAX_STRIDE = 1 << 22   # elements from token to token
 CLIP_SCALE = 0x1
 
 STATUS = {

@@ -5,11 +5,14 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace osm {
 
 constexpr int kDeltaChunk = 64;      // tokens a chunk
 constexpr int kDeltaMaxDk = 128;     // rows of the state
-constexpr int kDeltaSlice = 16;      // columns of the state a scan workgroup holds
+constexpr int kDeltaSlice = 16;      // columns of the state a scan workgroup, or a wave of a walk, holds
+constexpr int kGateFloats = 320;     // a chunk's hi, lo, beta, gam, end (delta::Gates)
 
 // Rows of a token tensor: element (b, t, h, j) at b*sb + t*ss + h*sh + j.
 struct DeltaRows {
@@ -24,14 +27,17 @@ struct DeltaParams {
   const float* init;                 // [B,H,dk,dv], or NULL
   float* fin;                        // [B,H,dk,dv], or NULL
   float* z;                          // [B,H,N][64][64]
-  float* a;                          // [B,H,N][dkp][dkp]
-  float* s;                          // [B,H,N][dkp][dvp]
+  float* gates;                      // [B,H,N][kGateFloats]
+  float* s;                          // [B,H,N][dkp][dvp] states before the chunks, or NULL
+  float* a;                          // maps of the segments [B,H,segs][dkp][dkp] (backward: of the chunks)
+  float* x;                          // and what they add, then the states before them [B,H,segs][dkp][dvp]
   // the backward's
   DeltaRows dout, dq, dk, dv, dg, dbeta;
   const float* grad_state;           // [B,H,dk,dv], or NULL
   float* grad_init;                  // [B,H,dk,dv], or NULL
   float* d;                          // [B,H,N][dkp][dvp]
-  int B, S, H, Hk, dk_, dv_, dkp, dvp, N;
+  int B, S, H, Hk, dk_, dv_, dkp, dvp, N;   // dkp: dk up to a multiple of 32, dvp: dv of 16, N: chunks of a row
+  int seg, segs;                     // chunks a segment, segments a row
   float scale;
   int vec;                           // rows of q, k, v, o, dout, dq, dk, dv start at multiples of 4 elements
 };
@@ -50,14 +56,16 @@ struct DeltaStepParams {
   float scale;
 };
 
+int delta_segment(int64_t heads, int64_t chunks);
 hipError_t launch_delta_step(const DeltaStepParams& p, int dtype, hipStream_t stream);
 hipError_t launch_delta_fwd(const DeltaParams& p, int dtype, hipStream_t stream);
 // part: 2 B S H dk floats where q and k heads are shared.
 hipError_t launch_delta_bwd(const DeltaParams& p, float* part, int dtype, hipStream_t stream);
-// The chunks' state maps S' = a S + x applied from init, x receiving the state
-// before each chunk, fin (or NULL) the last; reverse goes from the last chunk.
-hipError_t launch_delta_scan(const DeltaParams& p, const float* a, float* x, const float* init, float* fin,
-                             bool reverse, hipStream_t stream);
+// The state maps S' = a S + x of n spans of `span` tokens a row applied from
+// init, x receiving the state before each span, fin (or NULL) the last; reverse
+// goes from the last span.
+hipError_t launch_delta_scan(const DeltaParams& p, const float* a, float* x, const float* init, float* fin, int n,
+                             int span, bool reverse, hipStream_t stream);
 
 #ifdef __HIPCC__
 namespace delta {
@@ -222,6 +230,218 @@ __device__ __forceinline__ void load_gates(Gates* s, const DeltaRows& g, const D
 // e^(G_i - G_j)
 __device__ __forceinline__ float decay_between(const Gates& s, int i, int j) {
   return expf((s.hi[i] - s.hi[j]) + (s.lo[i] - s.lo[j]));
+}
+
+// ---- bf16 parts of fp32 numbers ----
+
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// bf16 numbers that hold one of T.
+template <typename T>
+constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
+
+// a and b as the sums of three bf16 numbers each, packed: the nearest, then the
+// nearest to what is left (which is exact), twice.
+__device__ __forceinline__ void split2(unsigned (&part)[3], float a, float b) {
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    part[k] = __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{a, b}, bf16x2));
+    if (k < 2) {
+      a -= __uint_as_float(part[k] << 16);
+      b -= __uint_as_float(part[k] & 0xffff0000u);
+    }
+  }
+}
+
+__device__ __forceinline__ void split4(u32x2 (&part)[3], f32x4 v) {
+  unsigned lo[3], hi[3];
+  split2(lo, v[0], v[1]);
+  split2(hi, v[2], v[3]);
+#pragma unroll
+  for (int k = 0; k < 3; ++k) part[k] = u32x2{lo[k], hi[k]};
+}
+
+// Two result tiles, rows 16 apart, as the second operand of a product over
+// their 32 rows.
+__device__ __forceinline__ void split_pair(u32x4 (&part)[3], f32x4 a, f32x4 b) {
+  u32x2 pa[3], pb[3];
+  split4(pa, a);
+  split4(pb, b);
+#pragma unroll
+  for (int k = 0; k < 3; ++k) part[k] = u32x4{pa[k][0], pa[k][1], pb[k][0], pb[k][1]};
+}
+
+// The terms of a product's 32 are kept in the order in which a pair of result
+// tiles holds them: place 8 g + 4 h + i is term 16 h + 4 g + i.  Place of the
+// four terms 4 q .. 4 q + 3 along a row:
+__device__ __forceinline__ int place4(int q) { return 32 * (q >> 3) + 8 * (q & 3) + 4 * ((q >> 2) & 1); }
+
+// The parts of 8 terms at `at` of matrices `stride` elements apart.
+template <int NP>
+__device__ __forceinline__ void read_parts(u32x4 (&f)[NP], const unsigned short* m, int stride, int at) {
+#pragma unroll
+  for (int k = 0; k < NP; ++k) f[k] = *reinterpret_cast<const u32x4*>(m + k * stride + at);
+}
+
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// acc += A B over 32 terms, A's parts in LDS, B's in registers, the smaller
+// products first.
+template <int NA, int NB>
+__device__ __forceinline__ void prod(f32x4& acc, const unsigned short* m, int stride, int at, const u32x4 (&b)[NB]) {
+  u32x4 a[NA];
+  read_parts<NA>(a, m, stride, at);
+#pragma unroll
+  for (int sum = 2; sum >= 0; --sum)
+#pragma unroll
+    for (int i = 0; i <= sum; ++i)
+      if (i < NA && sum - i < NB) acc = mfma(a[i], b[sum - i], acc);
+}
+
+__device__ __forceinline__ void store4(float* p, f32x4 v) {
+  *reinterpret_cast<f32x4*>(p) = v;
+  // two wait states before anything may overwrite the store's registers (a
+  // store wider than 64 bits was seen to lose its first word otherwise)
+  asm volatile("s_nop 1" ::: "memory");
+}
+
+// Memory through buffer descriptors: an offset past the extent reads zeros and
+// drops stores, so rows and columns outside a tensor need no branch, only kOut
+// as their offset (added to by less than 2^31 it stays out).
+typedef __amdgpu_buffer_rsrc_t Rsrc;
+constexpr unsigned kOut = 0x80000000u;
+__device__ __forceinline__ Rsrc make_rsrc(const void* base) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, 0x7fffffff, 0x00020000);
+}
+
+template <typename T>
+__device__ __forceinline__ T load_one(Rsrc r, unsigned at) {
+  if constexpr (sizeof(T) == 4)
+    return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0));
+  else
+    return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(r, at, 0, 0));
+}
+template <typename T>
+__device__ __forceinline__ void store_one(Rsrc r, unsigned at, float v) {
+  if constexpr (sizeof(T) == 4)
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), r, at, 0, 0);
+  else
+    __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, (__bf16)v), r, at, 0, 0);
+}
+
+// 64 rows of 32 KS columns of q or k in the registers of NT threads: 4x4 blocks,
+// the columns' blocks of a row in consecutive threads.
+template <typename T, int KS, int NT>
+struct Block {
+  static constexpr int kQuads = 8 * KS, kBlocks = (16 * kQuads + NT - 1) / NT;
+  static constexpr bool kAll = 16 * kQuads % NT == 0;
+  static constexpr int NP = kParts<T>;
+  typedef typename std::conditional<sizeof(T) == 4, f32x4, bf16x4>::type Quad;
+  Quad v[kBlocks][4];
+
+  // (stride 64 sizeof(T) is below 2^30: the entry points see to it)
+  __device__ __forceinline__ void load(const T* src, int64_t stride, int rows, int cols, bool vec) {
+    const Rsrc rs = make_rsrc(src);
+    const unsigned row_bytes = (unsigned)stride * sizeof(T);
+#pragma unroll
+    for (int n = 0; n < kBlocks; ++n) {
+      const int e = threadIdx.x + n * NT, q = e % kQuads, r = 4 * (e / kQuads);
+      const unsigned at = kAll || e < 16 * kQuads ? r * row_bytes + 4 * q * (unsigned)sizeof(T) : kOut;
+      if (vec) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const unsigned o = r + i < rows && 4 * q < cols ? at + i * row_bytes : kOut;
+          if constexpr (sizeof(T) == 4)
+            v[n][i] = __builtin_bit_cast(Quad, __builtin_amdgcn_raw_buffer_load_b128(rs, o, 0, 0));
+          else
+            v[n][i] = __builtin_bit_cast(Quad, __builtin_amdgcn_raw_buffer_load_b64(rs, o, 0, 0));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            v[n][i][k] = load_one<T>(rs, r + i < rows && 4 * q + k < cols ? at + i * row_bytes + k * (unsigned)sizeof(T) : kOut);
+      }
+    }
+  }
+  // rows LD elements apart, the parts `stride`
+  template <int LD>
+  __device__ __forceinline__ void put_rows(unsigned short* dst, int stride) const {
+#pragma unroll
+    for (int n = 0; n < kBlocks; ++n) {
+      const int e = threadIdx.x + n * NT, q = e % kQuads, r = 4 * (e / kQuads);
+      if (kAll || e < 16 * kQuads)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) put(dst + (r + i) * LD + place4(q), stride, v[n][i]);
+    }
+  }
+  // columns LD elements apart
+  template <int LD>
+  __device__ __forceinline__ void put_columns(unsigned short* dst, int stride) const {
+#pragma unroll
+    for (int n = 0; n < kBlocks; ++n) {
+      const int e = threadIdx.x + n * NT, q = e % kQuads, r = e / kQuads;
+      if (kAll || e < 16 * kQuads)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          put(dst + (4 * q + k) * LD + place4(r), stride, Quad{v[n][0][k], v[n][1][k], v[n][2][k], v[n][3][k]});
+    }
+  }
+
+ private:
+  static __device__ __forceinline__ void put(unsigned short* dst, int stride, Quad x) {
+    if constexpr (NP == 1) {
+      *reinterpret_cast<u32x2*>(dst) = __builtin_bit_cast(u32x2, x);
+    } else {
+      u32x2 part[3];
+      split4(part, x);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) *reinterpret_cast<u32x2*>(dst + k * stride) = part[k];
+    }
+  }
+};
+
+// A chunk's gates as the solve leaves them, 64 floats each.  hi + lo is G in
+// units of log 2, from a double sum, so that differences of long sums keep their
+// digits; g below -200 counts as -200, where e^g is 0 in fp32 already (and -inf
+// would make the differences NaN).
+constexpr int kHi = 0, kLo = 64, kBeta = 128, kGam = 192, kEnd = 256;   // .., beta, e^G, e^(G_last - G)
+
+// By the first wave; the caller synchronises.  Tokens past `rows`: g = beta = 0.
+__device__ __forceinline__ void make_gates(float* gt, const DeltaRows& g, const DeltaRows& beta, int64_t b, int64_t t0,
+                                           int64_t h, int rows) {
+  const int t = threadIdx.x;
+  if (t >= 64) return;
+  float gv = 0.0f, bv = 0.0f;
+  if (t < rows) {
+    gv = static_cast<const float*>(g.p)[b * g.sb + (t0 + t) * g.ss + h * g.sh];
+    bv = static_cast<const float*>(beta.p)[b * beta.sb + (t0 + t) * beta.ss + h * beta.sh];
+    if (gv < -200.0f) gv = -200.0f;
+  }
+  double G = (double)gv * 1.4426950408889634;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double up = __shfl_up(G, o);
+    if (t >= o) G += up;
+  }
+  const float hi = (float)G, lo = (float)(G - hi);
+  gt[kHi + t] = hi;
+  gt[kLo + t] = lo;
+  gt[kBeta + t] = bv;
+  gt[kGam + t] = exp2f(hi) * __builtin_fmaf(lo, 0.69314718f, 1.0f);
+  gt[kEnd + t] = exp2f((float)(__shfl(G, 63) - G));
+}
+
+// e^(G_i - G_j)
+__device__ __forceinline__ float decay(const float* gt, int i, int j) {
+  return exp2f((gt[kHi + i] - gt[kHi + j]) + (gt[kLo + i] - gt[kLo + j]));
 }
 
 // (b, h, chunk, tokens in use) of a workgroup's chunk.

@@ -9,15 +9,27 @@
 // its two inverses are (I + L diag(beta))^-1 = I - Z diag(beta) and
 // (I + diag(beta) L)^-1 = I - diag(beta) Z, without dividing by beta, so
 //   X = V - e^G K S,  Y = X - Z (beta X),  U = beta Y,  O = scale (e^G Q S + P U)
-// and the chunk's end state is affine in S, with Kt = e^{G_last - G} K:
-//   S' = A S + B,   A = e^{G_last} I - Kt^T W,   W = beta (e^G K - Z (beta e^G K))
-//                   B = Kt^T beta (V - Z (beta V))
+//   S' = e^{G_last} S + K^T (e^{G_last - G} U)
+// Every column of S (and of V, X, U, O) goes its own way.
 //
-// Three launches: `prepare` forms Z, A and B of every chunk at once, `scan`
-// walks the chunks of a row with one product each (its 16 columns of S stay in
-// the waves' accumulators), writing every chunk's start state over its B, and
-// `output` forms O of every chunk at once.  All products run on the fp32 matrix
-// instruction: the states and the gates' gradients are fp32 results.
+// Launches:
+//   solve   Z and the gates of every chunk at once.
+//   walk    a workgroup walks a segment of a row's chunks, each wave 16 columns
+//           of S in its accumulators.  The accumulator of one product is the
+//           second operand of the next as it stands (its rows are the terms of
+//           the sum), so X, U and S never leave the registers; K, Q, Z and P, the
+//           first operands, are shared by the waves through LDS.
+// Where the rows and heads alone do not fill the chip, rows are cut into
+// segments: a first walk from zero and from the columns of the identity gives
+// every segment's affine map of the state, `scan` joins them, and the second
+// walk gives the outputs from the right states.
+//
+// Products run on the bf16 matrix instruction at fp32's accuracy: an fp32 operand
+// is the sum of three bf16 numbers (8 bits each; the remainders are exact), bf16
+// inputs are one, and of the products of parts those of order 2^-24 and below are
+// left out: 3 instructions against a bf16 operand, 6 between two fp32 ones, where
+// the fp32 matrix instruction takes 16 times as long as the bf16 one.
+#include <algorithm>
 #include <type_traits>
 
 #include "osm_delta.h"
@@ -33,7 +45,7 @@ constexpr int kThreads = 256;
 // diagonal 16x16 blocks by substitution, row i from the rows before it (Z_i =
 // L_i - sum_j L_ij beta_j Z_j), then block pairs: for L = [[a, 0], [c, d]],
 // Z_c = (I - Z_d beta) (L_c - L_c beta Z_a), the 16-wide ones, then the 32-wide.
-__device__ void invert(float* zs, const Gates& gt) {
+__device__ void invert(float* zs, const float* beta) {
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
   if (wave == 0) {
     const int c = l & 15, o = 16 * (l >> 4);
@@ -42,10 +54,13 @@ __device__ void invert(float* zs, const Gates& gt) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float v = base[i * kLd + c];
+      f32x4 row[4];
 #pragma unroll
-      for (int j = 0; j < i; ++j) v = __builtin_fmaf(-base[i * kLd + j], bz[j], v);
+      for (int q = 0; q < (i + 3) / 4; ++q) row[q] = load4(base + i * kLd + 4 * q);
+#pragma unroll
+      for (int j = 0; j < i; ++j) v = __builtin_fmaf(-row[j / 4][j % 4], bz[j], v);
       z[i] = v;
-      bz[i] = gt.beta[o + i] * v;
+      bz[i] = beta[o + i] * v;
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // every lane has read its rows
 #pragma unroll
@@ -58,7 +73,7 @@ __device__ void invert(float* zs, const Gates& gt) {
     f32x4 acc[1], q[1];
     if (wave < 2) {
       clear(acc);
-      mma<1, false, false, true>(acc, zs, d, zs, a, a, d, gt.beta);   // L_c beta Z_a
+      mma<1, false, false, true>(acc, zs, d, zs, a, a, d, beta);   // L_c beta Z_a
       get(q, zs, d, a);
       q[0] -= acc[0];
     }
@@ -67,7 +82,7 @@ __device__ void invert(float* zs, const Gates& gt) {
     __syncthreads();
     if (wave < 2) {
       clear(acc);
-      mma<1, false, false, true>(acc, zs, d, zs, a, d, d + 16, gt.beta);   // Z_d beta (..)
+      mma<1, false, false, true>(acc, zs, d, zs, a, d, d + 16, beta);   // Z_d beta (..)
       q[0] -= acc[0];
     }
     __syncthreads();
@@ -79,14 +94,14 @@ __device__ void invert(float* zs, const Gates& gt) {
     const int r0 = 32 + 16 * (wave >> 1), c0 = 16 * (wave & 1);
     f32x4 acc[1], q[1];
     clear(acc);
-    mma<1, false, false, true>(acc, zs, r0, zs, c0, 0, 32, gt.beta);
+    mma<1, false, false, true>(acc, zs, r0, zs, c0, 0, 32, beta);
     get(q, zs, r0, c0);
     q[0] -= acc[0];
     __syncthreads();
     put(zs, q, r0, c0);
     __syncthreads();
     clear(acc);
-    mma<1, false, false, true>(acc, zs, r0, zs, c0, 32, 64, gt.beta);
+    mma<1, false, false, true>(acc, zs, r0, zs, c0, 32, 64, beta);
     q[0] -= acc[0];
     __syncthreads();
     put(zs, q, r0, c0);
@@ -94,132 +109,63 @@ __device__ void invert(float* zs, const Gates& gt) {
   }
 }
 
-// Z, A and B of a chunk.  LDS: three tiles (52 KB), so that three workgroups
-// share a CU; head sizes above 64 go by blocks of 64 columns.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) delta_prepare_kernel(const DeltaParams p) {
-  __shared__ __attribute__((aligned(16))) float zs[kTile], ks[kTile], ws[kTile];
-  __shared__ __attribute__((aligned(16))) Gates gt;
-  const At w = chunk_at(p, blockIdx.x);
+// Z and the gates of a chunk.  KS: blocks of 32 columns of k.
+template <typename T, int KS>
+__global__ void __launch_bounds__(kThreads) delta_solve_kernel(const DeltaParams p) {
+  constexpr int NP = kParts<T>, LDK = 32 * KS + 8;
+  __shared__ __attribute__((aligned(16))) float zs[kTile];
+  __shared__ __attribute__((aligned(16))) unsigned short kk[NP][64 * LDK];
+  __shared__ __attribute__((aligned(16))) float gt[kGateFloats];
+  const int64_t chunk = blockIdx.x;
+  const At w = chunk_at(p, chunk);
   if (w.rows == 0) return;
-  const int r0 = 16 * (threadIdx.x >> 6), hk = w.h / (p.H / p.Hk);
-  load_gates(&gt, p.g, p.beta, w.b, w.t0, w.h, w.rows);
-  const T* const k = row_ptr<T>(p.k, w.b, w.t0, hk);
-  const T* const v = row_ptr<T>(p.v, w.b, w.t0, w.h);
-  const bool vec = p.vec;
+  const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, r0 = 16 * wave;
+  Block<T, KS, kThreads> kb;
+  kb.load(row_ptr<T>(p.k, w.b, w.t0, w.h / (p.H / p.Hk)), p.k.ss, w.rows, p.dk_, p.vec);
+  make_gates(gt, p.g, p.beta, w.b, w.t0, w.h, w.rows);
+  kb.template put_rows<LDK>(&kk[0][0], 64 * LDK);
+  __syncthreads();
   f32x4 acc[4];
   clear(acc);
-  for (int kb = 0; kb < p.dkp; kb += 64) {
-    const int kw = min(64, p.dkp - kb);
-    if (kb) __syncthreads();
-    load_tile<kThreads>(ks, k + kb, p.k.ss, w.rows, p.dk_ - kb, kw, vec);
-    __syncthreads();
-    mma<4, false, true>(acc, ks, r0, ks, 0, 0, kw);
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    u32x4 b[NP];
+    read_parts<NP>(b, &kk[0][0], 64 * LDK, (r0 + (l & 15)) * LDK + 32 * s + 8 * (l >> 4));
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (c <= wave) prod<NP, NP>(acc[c], &kk[0][0], 64 * LDK, (16 * c + (l & 15)) * LDK + 32 * s + 8 * (l >> 4), b);
   }
+  // acc[c][i] is (K K^T)[16 c + 4 g + i][r0 + lane%16]; it is symmetric: four
+  // columns of row r0 + lane%16
+  const int row = r0 + (l & 15);
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
+  for (int c = 0; c < 4; ++c) {
+    const int col = 16 * c + 4 * (l >> 4);
+    f32x4 v;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = out_row(r0, i), col = out_col(0, c);
-      acc[c][i] = row > col ? acc[c][i] * decay_between(gt, row, col) : 0.0f;
-    }
-  put(zs, acc, r0, 0);
+    for (int i = 0; i < 4; ++i) v[i] = row > col + i ? acc[c][i] * decay(gt, row, col + i) : 0.0f;
+    *reinterpret_cast<f32x4*>(zs + row * kLd + col) = v;
+  }
   __syncthreads();
-  invert(zs, gt);
-  const int64_t chunk = blockIdx.x;
+  invert(zs, gt + kBeta);
   float* const zg = p.z + chunk * 4096;
   for (int e = threadIdx.x; e < 1024; e += kThreads)
-    *reinterpret_cast<f32x4*>(zg + 4 * e) = *reinterpret_cast<const f32x4*>(zs + (e >> 4) * kLd + 4 * (e & 15));
-  const int nkb = (p.dkp + 63) / 64;
-  int held = nkb - 1;   // the block of K in ks
-  auto hold = [&](int blk) {
-    if (blk == held) return;
-    __syncthreads();
-    load_tile<kThreads>(ks, k + 64 * blk, p.k.ss, w.rows, p.dk_ - 64 * blk, min(64, p.dkp - 64 * blk), vec);
-    held = blk;
-    __syncthreads();
-  };
-  // A by blocks of columns
-  float* const ag = p.a + chunk * p.dkp * p.dkp;
-  for (int cb = 0; cb < nkb; ++cb) {
-    const int cw = min(64, p.dkp - 64 * cb);
-    hold(cb);
-    clear(acc);
-    mma<4, false, false, true>(acc, zs, r0, ks, 0, 0, r0 + 16, gt.bgam);
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = out_row(r0, i), col = out_col(0, c);
-        acc[c][i] = gt.end[row] * gt.beta[row] * (gt.gam[row] * (col < cw ? ks[row * kLd + col] : 0.0f) - acc[c][i]);
-      }
-    __syncthreads();   // the previous block's product has read ws
-    put(ws, acc, r0, 0);
-    __syncthreads();
-    for (int rb = 0; rb < nkb; ++rb) {
-      const int rw = min(64, p.dkp - 64 * rb);
-      hold(rb);
-      if (r0 >= rw) continue;   // (hold's barriers are behind every wave)
-      clear(acc);
-      mma<4, true, false>(acc, ks, r0, ws, 0, 0, 64);
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = 64 * rb + out_row(r0, i), col = out_col(0, c);
-          if (col < cw) ag[(int64_t)row * p.dkp + 64 * cb + col] = (row == 64 * cb + col ? gt.last : 0.0f) - acc[c][i];
-        }
-    }
-  }
-  // B by blocks of columns
-  float* const sg = p.s + chunk * p.dkp * p.dvp;
-  for (int vb = 0; vb < p.dvp; vb += 64) {
-    const int vw = min(64, p.dvp - vb);
-    __syncthreads();
-    load_tile<kThreads>(ws, v + vb, p.v.ss, w.rows, p.dv_ - vb, 64, vec);
-    __syncthreads();
-    clear(acc);
-    mma<4, false, false, true>(acc, zs, r0, ws, 0, 0, r0 + 16, gt.beta);
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = out_row(r0, i);
-        acc[c][i] = gt.end[row] * gt.beta[row] * (ws[row * kLd + out_col(0, c)] - acc[c][i]);
-      }
-    __syncthreads();
-    put(ws, acc, r0, 0);
-    __syncthreads();
-    for (int rb = 0; rb < nkb; ++rb) {
-      const int rw = min(64, p.dkp - 64 * rb);
-      hold(rb);
-      if (r0 >= rw) continue;
-      clear(acc);
-      mma<4, true, false>(acc, ks, r0, ws, 0, 0, 64);
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int col = out_col(0, c);
-          if (col < vw) sg[(int64_t)(64 * rb + out_row(r0, i)) * p.dvp + vb + col] = acc[c][i];
-        }
-    }
-  }
+    store4(zg + 4 * e, *reinterpret_cast<const f32x4*>(zs + (e >> 4) * kLd + 4 * (e & 15)));
+  float* const gg = p.gates + chunk * kGateFloats;
+  for (int e = threadIdx.x; e < kGateFloats; e += kThreads) gg[e] = gt[e];
 }
 
-// S' = A S + B over the chunks of a row, in order or in reverse, for 16 columns
+// S' = A S + B over the spans of a row, in order or in reverse, for 16 columns
 // of S: wave w holds rows 16 w .. 16 w + 15 of S and of A, and S passes between
 // the waves through LDS, transposed ([column][row], so that both the
 // accumulators' four rows and the product's four terms are one 16-byte access),
-// in two buffers: one barrier a chunk.  x holds B and receives the state before
-// the chunk.  KT = dkp / 16.
-//
-// What bounds it: the chain of chunks, each KT dependent-in-pairs matrix
-// instructions of 4 KT .. plus the exchange.
+// in two buffers: one barrier a span.  x holds B and receives the state before
+// the span.  KT = dkp / 16.  What bounds it: the chain of spans, 4 KT matrix
+// instructions and the exchange each.
 template <int KT>
 __global__ void __launch_bounds__(64 * KT) delta_scan_kernel(const float* a, float* x, const float* init, float* fin,
-                                                             const int* lengths, int S, int N, int BH, int H, int dk,
-                                                             int dv, int dvp, bool reverse) {
+                                                             const int* lengths, int S, int N, int span, int BH, int H,
+                                                             int dk, int dv, int dvp, bool reverse) {
   constexpr int kDkp = 16 * KT, kRow = kDkp + 4;
   __shared__ __attribute__((aligned(16))) float st[2][16 * kRow];
   // The column slices of a head share A, so they take one XCD (workgroups go
@@ -229,7 +175,7 @@ __global__ void __launch_bounds__(64 * KT) delta_scan_kernel(const float* a, flo
   const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, r = l & 15, g = l >> 4;
   const int col = kDeltaSlice * (j % ns) + r, row = 16 * wave + 4 * g;
   const int tokens = lengths ? min(max(lengths[bh / H], 0), S) : S;
-  const int n = (tokens + kDeltaChunk - 1) / kDeltaChunk;
+  const int n = (int)(((int64_t)tokens + span - 1) / span);
   a += (int64_t)bh * N * kDkp * kDkp + (int64_t)(16 * wave + r) * kDkp + 4 * g;
   x += (int64_t)bh * N * kDkp * dvp + (int64_t)row * dvp + col;
   const int64_t io = (int64_t)bh * dk * dv + (int64_t)row * dv + col;
@@ -277,119 +223,317 @@ __global__ void __launch_bounds__(64 * KT) delta_scan_kernel(const float* a, flo
       if (row + i < dk && col < dv) fin[io + (int64_t)i * dv] = s[i];
 }
 
-// O of a chunk for 64 columns of v.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) delta_output_kernel(const DeltaParams p) {
-  __shared__ __attribute__((aligned(16))) float qs[kTile], ks[kTile], ss[kTile];
-  __shared__ __attribute__((aligned(16))) Gates gt;
-  const int nvb = (p.dvp + 63) / 64, vb = 64 * (int)(blockIdx.x % nvb);
-  const int64_t chunk = blockIdx.x / nvb;
-  const At w = chunk_at(p, chunk);
-  const int r0 = 16 * (threadIdx.x >> 6), hk = w.h / (p.H / p.Hk), vw = min(64, p.dvp - vb);
-  T* const o = row_ptr<T>(p.o, w.b, w.t0, w.h) + vb;
-  const int rows = (int)min((int64_t)kDeltaChunk, p.S - w.t0);   // of the output
-  if (w.rows == 0) {
-    for (int e = threadIdx.x; e < 64 * 64; e += kThreads)
-      if ((e >> 6) < rows && vb + (e & 63) < p.dv_) o[(e >> 6) * p.o.ss + (e & 63)] = (T)0.0f;
-    return;
+// Rows 0-31 of a lower triangular matrix of the walk have 32 columns, the others
+// 64 (plus 8 of padding: 16-byte reads of eight consecutive rows touch every bank
+// once).
+constexpr int kTri = 32 * 40 + 32 * 72;
+__device__ __forceinline__ int tri_at(int row) { return row < 32 ? row * 40 : 1280 + (row - 32) * 72; }
+
+// Walks segment blockIdx.x % segs of a head.  MAP: the segment's state map, from
+// zero for the columns of v and from the identity's columns after them; else the
+// outputs.  KS: blocks of 32 rows of S; WAVES: of 16 columns each.
+template <typename T, int KS, int WAVES, bool MAP>
+__global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaParams p, int groups) {
+  constexpr int NT = 64 * WAVES, NP = kParts<T>, DK = 32 * KS, LDK = DK + 8, LKT = 72, ST = 2 * KS;
+  // K by rows; Q by rows, then K by columns; Z; P.
+  constexpr int kSecond = (MAP || 64 * LDK < DK * LKT) ? DK * LKT : 64 * LDK;
+  __shared__ __attribute__((aligned(16))) unsigned short kk[NP][64 * LDK], second[NP][kSecond], zp[3][kTri],
+      pp[MAP ? 1 : 3][MAP ? 8 : kTri];
+  __shared__ __attribute__((aligned(16))) float gt[kGateFloats];
+  const int group = blockIdx.x % groups;
+  const int64_t id = blockIdx.x / groups;
+  const int seg = (int)(id % p.segs), bh = (int)(id / p.segs), b = bh / p.H, h = bh - b * p.H, hk = h / (p.H / p.Hk);
+  const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63, r = l & 15, g = l >> 4;
+  const int tokens = p.lengths ? min(max(p.lengths[b], 0), p.S) : p.S;
+  const int n = (tokens + kDeltaChunk - 1) / kDeltaChunk;          // chunks in use
+  const int c0 = seg * p.seg, c1 = min(min(c0 + p.seg, p.N), n);
+  const int slice = group * WAVES + wave, vs = p.dvp / kDeltaSlice;
+  const bool value = slice < vs, live = slice < vs + (MAP ? DK / kDeltaSlice : 0);
+  const int col = kDeltaSlice * slice + r;                         // of v, or dvp + of the identity
+  const bool in_v = value && col < p.dv_;
+  if (!MAP) {
+    // zeros for the chunks without tokens
+    for (int c = max(c0, n); c < min(c0 + p.seg, p.N); ++c) {
+      T* const o = row_ptr<T>(p.o, b, (int64_t)c * kDeltaChunk, h) + col;
+      if (in_v)
+        for (int t = g; t < min(kDeltaChunk, p.S - c * kDeltaChunk); t += 4) o[t * p.o.ss] = (T)0.0f;
+    }
   }
-  load_gates(&gt, p.g, p.beta, w.b, w.t0, w.h, w.rows);
-  const T* const q = row_ptr<T>(p.q, w.b, w.t0, hk);
-  const T* const k = row_ptr<T>(p.k, w.b, w.t0, hk);
-  const T* const v = row_ptr<T>(p.v, w.b, w.t0, w.h) + vb;
-  const bool vec = p.vec;
-  f32x4 P[4], kS[4], qS[4], x[4], acc[4];
-  clear(P);
-  clear(kS);
-  clear(qS);
-  for (int kb = 0; kb < p.dkp; kb += 64) {
-    const int kw = min(64, p.dkp - kb);
-    if (kb) __syncthreads();
-    load_tile<kThreads>(ks, k + kb, p.k.ss, w.rows, p.dk_ - kb, kw, vec);
-    load_tile<kThreads>(qs, q + kb, p.q.ss, w.rows, p.dk_ - kb, kw, vec);
-    load_ws<kThreads>(ss, p.s + chunk * p.dkp * p.dvp + (int64_t)kb * p.dvp + vb, p.dvp, kw, vw);
+  const bool fin = !MAP && p.fin && seg == (n > 0 ? (n - 1) / p.seg : 0);
+  if (c0 >= c1 && !fin) return;
+  // S: tile t, element i: row 16 t + 4 g + i, column col
+  f32x4 S[ST];
+  const float* const from = MAP ? nullptr : p.segs > 1 && n > 0 ? p.x + id * DK * p.dvp : p.init ? p.init + (int64_t)bh * p.dk_ * p.dv_ : nullptr;
+  const bool ws = !MAP && p.segs > 1 && n > 0;
+  const Rsrc from_rs = make_rsrc(from);
+  const unsigned from_ld = 4u * (ws ? p.dvp : p.dv_);
+  const bool from_col = from && (ws ? value : in_v);
+#pragma unroll
+  for (int t = 0; t < ST; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = 16 * t + 4 * g + i;
+      if (MAP)
+        S[t][i] = !value && row == col - p.dvp ? 1.0f : 0.0f;
+      else
+        S[t][i] = load_one<float>(from_rs, from_col && (ws || row < p.dk_) ? row * from_ld + 4u * col : kOut);
+    }
+  const T* const kp = row_ptr<T>(p.k, b, 0, hk);
+  const T* const qp = row_ptr<T>(p.q, b, 0, hk);
+  const T* const vp = row_ptr<T>(p.v, b, 0, h);
+  T* const op = MAP ? nullptr : row_ptr<T>(p.o, b, 0, h);
+  const unsigned es = sizeof(T), v_row = (unsigned)p.v.ss * es, o_row = (unsigned)p.o.ss * es;
+  const unsigned v_at = in_v ? col * es + 4 * g * v_row : kOut, o_at = in_v ? col * es + 4 * g * o_row : kOut;
+  Block<T, KS, NT> kb, qb;
+  f32x4 zr[1024 / NT], br;   // br: beta of the columns of zr
+  float vr[16], gr[2];
+  auto fetch = [&](int c) {
+    const int64_t t0 = (int64_t)c * kDeltaChunk, chunk = (int64_t)bh * p.N + c;
+    const int rows = min(kDeltaChunk, tokens - (int)t0);
+    kb.load(kp + t0 * p.k.ss, p.k.ss, rows, p.dk_, p.vec);
+    if (!MAP) qb.load(qp + t0 * p.q.ss, p.q.ss, rows, p.dk_, p.vec);
+#pragma unroll
+    for (int e = 0; e < 1024 / NT; ++e) zr[e] = load4(p.z + chunk * 4096 + 4 * (tid + e * NT));
+    br = load4(p.gates + chunk * kGateFloats + kBeta + 4 * (tid & 15));
+#pragma unroll
+    for (int e = 0; e < 2; ++e) gr[e] = p.gates[chunk * kGateFloats + min(tid + e * NT, kGateFloats - 1)];
+    const Rsrc vs_rs = make_rsrc(vp + t0 * p.v.ss);
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        vr[4 * t + i] = (float)load_one<T>(vs_rs, 16 * t + 4 * g + i < rows ? v_at + (16 * t + i) * v_row : kOut);
+  };
+  if (c0 < c1) fetch(c0);
+  for (int c = c0; c < c1; ++c) {
+    const int64_t t0 = (int64_t)c * kDeltaChunk;
+    __syncthreads();   // the chunk before has been read
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (tid + e * NT < kGateFloats) gt[tid + e * NT] = gr[e];
+    kb.template put_rows<LDK>(&kk[0][0], 64 * LDK);
+    if (MAP)
+      kb.template put_columns<LKT>(&second[0][0], kSecond);
+    else
+      qb.template put_rows<LDK>(&second[0][0], kSecond);
+    // Z beta
+#pragma unroll
+    for (int e = 0; e < 1024 / NT; ++e) {
+      const int row = (tid + e * NT) >> 4, q = (tid + e * NT) & 15;
+      if (row >= 32 || q < 8) {
+        u32x2 part[3];
+        split4(part, zr[e] * br);
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+          *reinterpret_cast<u32x2*>(&zp[k][tri_at(row) + 32 * (q >> 3) + 8 * (q & 3) + 4 * ((q >> 2) & 1)]) = part[k];
+      }
+    }
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = vr[i];
+    Block<T, KS, NT> kc = kb;
     __syncthreads();
-    mma<4, false, true>(P, qs, r0, ks, 0, 0, kw);
-    mma<4, false, false>(kS, ks, r0, ss, 0, 0, kw);
-    mma<4, false, false>(qS, qs, r0, ss, 0, 0, kw);
+    if (c + 1 < c1) fetch(c + 1);
+    f32x4 x[4], o[4];
+    if (live) {
+      if (!MAP && p.s && value) {
+        float* const sg = p.s + ((int64_t)bh * p.N + c) * DK * p.dvp + col;
+#pragma unroll
+        for (int t = 0; t < ST; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sg[(int64_t)(16 * t + 4 * g + i) * p.dvp] = S[t][i];
+      }
+      clear(x);
+      clear(o);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        u32x4 sp[3];
+        split_pair(sp, S[2 * s], S[2 * s + 1]);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int at = (16 * t + r) * LDK + 32 * s + 8 * g;
+          prod<NP, 3>(x[t], &kk[0][0], 64 * LDK, at, sp);
+          if (!MAP) prod<NP, 3>(o[t], &second[0][0], kSecond, at, sp);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const f32x4 gam = load4(gt + kGam + 16 * t + 4 * g);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[t][i] = v[4 * t + i] - gam[i] * x[t][i];
+      }
+    }
+    if (!MAP) {
+      // P: four of its columns of one row a lane, from K Q^T; WAVES / 4 waves a
+      // tile row
+      const int tr = wave & 3, i = 16 * tr + r;
+      for (int tc = wave >> 2; tc <= tr; tc += WAVES / 4) {
+        f32x4 acc = zero4();
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          u32x4 qf[NP];
+          read_parts<NP>(qf, &second[0][0], kSecond, i * LDK + 32 * s + 8 * g);
+          prod<NP, NP>(acc, &kk[0][0], 64 * LDK, (16 * tc + r) * LDK + 32 * s + 8 * g, qf);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = 16 * tc + 4 * g + e;
+          acc[e] = i >= j ? acc[e] * decay(gt, i, j) : 0.0f;
+        }
+        u32x2 part[3];
+        split4(part, acc);
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+          *reinterpret_cast<u32x2*>(&pp[MAP ? 0 : k][tri_at(i) + 32 * (tc >> 1) + 8 * g + 4 * (tc & 1)]) = part[k];
+      }
+      // the other half of a pair of tiles whose first is on the diagonal
+      if ((wave >> 2) == 0 && (tr & 1) == 0)
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+          *reinterpret_cast<u32x2*>(&pp[MAP ? 0 : k][tri_at(i) + 32 * (tr >> 1) + 8 * g + 4]) = u32x2{0, 0};
+      __syncthreads();   // P is there, Q has been read
+      kc.template put_columns<LKT>(&second[0][0], kSecond);
+    }
+    if (live) {
+      f32x4 y[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) y[t] = zero4();
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        u32x4 xp[3];
+        split_pair(xp, x[2 * s], x[2 * s + 1]);
+#pragma unroll
+        for (int t = 2 * s; t < 4; ++t) prod<3, 3>(y[t], &zp[0][0], kTri, tri_at(16 * t + r) + 32 * s + 8 * g, xp);
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const f32x4 beta = load4(gt + kBeta + 16 * t + 4 * g);
+        x[t] = beta * (x[t] - y[t]);   // U
+      }
+      if (!MAP) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) o[t] *= load4(gt + kGam + 16 * t + 4 * g);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          u32x4 up[3];
+          split_pair(up, x[2 * s], x[2 * s + 1]);
+#pragma unroll
+          for (int t = 2 * s; t < 4; ++t) prod<3, 3>(o[t], &pp[0][0], kTri, tri_at(16 * t + r) + 32 * s + 8 * g, up);
+        }
+        const int rows = tokens - (int)t0, all = p.S - (int)t0;
+        const Rsrc o_rs = make_rsrc(op + t0 * p.o.ss);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = 16 * t + 4 * g + i;
+            store_one<T>(o_rs, row < all ? o_at + (16 * t + i) * o_row : kOut, row < rows ? p.scale * o[t][i] : 0.0f);
+          }
+      }
+    }
+    if (!MAP) __syncthreads();   // K by columns is there
+    if (live) {
+      const float last = gt[kGam + 63];
+#pragma unroll
+      for (int t = 0; t < ST; ++t) S[t] *= last;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        u32x4 up[3];
+        split_pair(up, x[2 * s] * load4(gt + kEnd + 32 * s + 4 * g), x[2 * s + 1] * load4(gt + kEnd + 32 * s + 16 + 4 * g));
+#pragma unroll
+        for (int t = 0; t < ST; ++t) prod<NP, 3>(S[t], &second[0][0], kSecond, (16 * t + r) * LKT + 32 * s + 8 * g, up);
+      }
+    }
   }
+  if (MAP && live) {
+    float* const dst = value ? p.x + id * DK * p.dvp + col : p.a + id * DK * DK + (col - p.dvp);
+    const int ld = value ? p.dvp : DK;
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
+    for (int t = 0; t < ST; ++t)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = out_row(r0, i), col = out_col(0, c);
-      const bool in = row < w.rows && col < vw && vb + col < p.dv_;
-      // (columns past vw hold what the tile had before: they are not stored)
-      x[c][i] = in ? (float)v[row * p.v.ss + col] - gt.gam[row] * kS[c][i] : 0.0f;
-      P[c][i] = row >= col ? P[c][i] * decay_between(gt, row, col) : 0.0f;
-    }
-  __syncthreads();
-  put(qs, P, r0, 0);
-  put(ss, x, r0, 0);
-  load_ws<kThreads>(ks, p.z + chunk * 4096, 64, 64, 64);
-  __syncthreads();
-  clear(acc);
-  mma<4, false, false, true>(acc, ks, r0, ss, 0, 0, r0 + 16, gt.beta);
+      for (int i = 0; i < 4; ++i) dst[(int64_t)(16 * t + 4 * g + i) * ld] = S[t][i];
+  }
+  if (fin && in_v) {
+    float* const dst = p.fin + (int64_t)bh * p.dk_ * p.dv_ + col;
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
+    for (int t = 0; t < ST; ++t)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[c][i] = gt.beta[out_row(r0, i)] * (x[c][i] - acc[c][i]);
-  __syncthreads();
-  put(ss, x, r0, 0);
-  __syncthreads();
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[c][i] = gt.gam[out_row(r0, i)] * qS[c][i];
-  mma<4, false, false>(acc, qs, r0, ss, 0, 0, r0 + 16);
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = out_row(r0, i), col = out_col(0, c);
-      if (row < rows && col < vw && vb + col < p.dv_)
-        o[row * p.o.ss + col] = (T)(row < w.rows ? p.scale * acc[c][i] : 0.0f);
-    }
+      for (int i = 0; i < 4; ++i)
+        if (16 * t + 4 * g + i < p.dk_) dst[(int64_t)(16 * t + 4 * g + i) * p.dv_] = S[t][i];
+  }
+}
+
+template <typename T, int KS, bool MAP>
+void launch_walk(const DeltaParams& p, hipStream_t stream) {
+  const int slices = p.dvp / kDeltaSlice + (MAP ? p.dkp / kDeltaSlice : 0);
+  auto go = [&](auto waves) {
+    constexpr int W = decltype(waves)::value;
+    const int groups = (slices + W - 1) / W;
+    const unsigned grid = (unsigned)((int64_t)p.B * p.H * p.segs * groups);
+    hipLaunchKernelGGL((delta_walk_kernel<T, KS, W, MAP>), dim3(grid), dim3(64 * W), 0, stream, p, groups);
+  };
+  if (slices <= 4)
+    go(std::integral_constant<int, 4>{});
+  else
+    go(std::integral_constant<int, 8>{});
+}
+
+template <typename T, int KS>
+hipError_t forward(const DeltaParams& p, hipStream_t stream) {
+  const int64_t chunks = (int64_t)p.B * p.H * p.N;
+  hipLaunchKernelGGL((delta_solve_kernel<T, KS>), dim3((unsigned)chunks), dim3(kThreads), 0, stream, p);
+  hipError_t e = hipGetLastError();
+  if (e == hipSuccess && p.segs > 1) {
+    launch_walk<T, KS, true>(p, stream);
+    e = hipGetLastError();
+    if (e == hipSuccess)
+      e = launch_delta_scan(p, p.a, p.x, p.init, nullptr, p.segs, p.seg * kDeltaChunk, false, stream);
+  }
+  if (e != hipSuccess) return e;
+  launch_walk<T, KS, false>(p, stream);
+  return hipGetLastError();
 }
 
 template <typename T>
-hipError_t forward(const DeltaParams& p, hipStream_t stream) {
-  const int64_t chunks = (int64_t)p.B * p.H * p.N;
-  hipLaunchKernelGGL((delta_prepare_kernel<T>), dim3((unsigned)chunks), dim3(kThreads), 0, stream, p);
-  hipError_t e = hipGetLastError();
-  if (e == hipSuccess) e = launch_delta_scan(p, p.a, p.s, p.init, p.fin, false, stream);
-  if (e != hipSuccess) return e;
-  const int nvb = (p.dvp + 63) / 64;
-  hipLaunchKernelGGL((delta_output_kernel<T>), dim3((unsigned)(chunks * nvb)), dim3(kThreads), 0, stream, p);
-  return hipGetLastError();
+hipError_t forward_by_size(const DeltaParams& p, hipStream_t stream) {
+  switch (p.dkp / 32) {
+    case 1: return forward<T, 1>(p, stream);
+    case 2: return forward<T, 2>(p, stream);
+    case 3: return forward<T, 3>(p, stream);
+    default: return forward<T, 4>(p, stream);
+  }
 }
 
 }  // namespace
 
-hipError_t launch_delta_scan(const DeltaParams& p, const float* a, float* x, const float* init, float* fin,
-                             bool reverse, hipStream_t stream) {
+// Chunks a segment.  Heads and rows alone where they give every other CU a
+// workgroup; else as many segments as give every CU two, of at least two chunks.
+int delta_segment(int64_t heads, int64_t chunks) {
+  if (heads >= 128 || chunks <= 2) return (int)std::max<int64_t>(chunks, 1);
+  const int64_t want = (512 + heads - 1) / heads, segs = std::min(want, chunks / 2);
+  return (int)((chunks + segs - 1) / segs);
+}
+
+hipError_t launch_delta_scan(const DeltaParams& p, const float* a, float* x, const float* init, float* fin, int n,
+                             int span, bool reverse, hipStream_t stream) {
   const int BH = p.B * p.H, ns = p.dvp / kDeltaSlice;
   const dim3 grid((unsigned)(8 * (int64_t)ns * ((BH + 7) / 8)));
   auto go = [&](auto kt) {
     constexpr int KT = decltype(kt)::value;
-    hipLaunchKernelGGL((delta_scan_kernel<KT>), grid, dim3(64 * KT), 0, stream, a, x, init, fin, p.lengths, p.S, p.N,
+    hipLaunchKernelGGL((delta_scan_kernel<KT>), grid, dim3(64 * KT), 0, stream, a, x, init, fin, p.lengths, p.S, n, span,
                        BH, p.H, p.dk_, p.dv_, p.dvp, reverse);
   };
-  switch (p.dkp / 16) {
-    case 1: go(std::integral_constant<int, 1>{}); break;
-    case 2: go(std::integral_constant<int, 2>{}); break;
-    case 3: go(std::integral_constant<int, 3>{}); break;
-    case 4: go(std::integral_constant<int, 4>{}); break;
-    case 5: go(std::integral_constant<int, 5>{}); break;
-    case 6: go(std::integral_constant<int, 6>{}); break;
-    case 7: go(std::integral_constant<int, 7>{}); break;
+  switch (p.dkp / 32) {
+    case 1: go(std::integral_constant<int, 2>{}); break;
+    case 2: go(std::integral_constant<int, 4>{}); break;
+    case 3: go(std::integral_constant<int, 6>{}); break;
     default: go(std::integral_constant<int, 8>{}); break;
   }
   return hipGetLastError();
 }
 
 hipError_t launch_delta_fwd(const DeltaParams& p, int dtype, hipStream_t stream) {
-  return dtype == 0 ? forward<float>(p, stream) : forward<__bf16>(p, stream);
+  return dtype == 0 ? forward_by_size<float>(p, stream) : forward_by_size<__bf16>(p, stream);
 }
 
 }  // namespace osm

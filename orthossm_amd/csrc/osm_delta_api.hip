@@ -40,6 +40,8 @@ int check_rows(const osm_rows& r, int esize, const char* name) {
   if (!r.p) return fail(OSM_E_ARG, "%s is NULL", name);
   if ((uintptr_t)r.p % esize) return fail(OSM_E_LAYOUT, "%s is not aligned to its elements", name);
   if (r.stride_b < 0 || r.stride_s < 0 || r.stride_h < 0) return fail(OSM_E_LAYOUT, "%s has a negative stride", name);
+  if (r.stride_s > OSM_DELTA_MAX_STRIDE)
+    return fail(OSM_E_LAYOUT, "%s: %lld elements from token to token, at most %d", name, (long long)r.stride_s, OSM_DELTA_MAX_STRIDE);
   return OSM_OK;
 }
 
@@ -64,15 +66,21 @@ int check_shape(const osm_delta_args* a) {
 
 bool is_short(const osm_delta_args* a) { return !a->saved && a->S <= kShort; }
 
-// Floats of the regions of `saved` and the workspaces: per chunk Z, the start
-// (or, in the backward, end) states and the state maps; each a multiple of 64.
+int64_t up32(int64_t n) { return (n + 31) / 32 * 32; }
+
+// Floats of the regions of `saved` and the workspaces, each a multiple of 64:
+// per chunk Z, its gates, its start (or, in the backward, end) state and its
+// state map; per segment the map and the state; with shared heads q's and k's
+// gradients by head.
 struct Sizes {
-  size_t z, s, a, part;
+  size_t z, gates, s, a, seg_a, seg_x, part;
 };
 Sizes sizes_of(const osm_delta_args* a) {
-  const size_t n = (size_t)a->B * a->H * chunks_of(a->S), dkp = up16(a->dk), dvp = up16(a->dv);
-  const size_t part = a->H != a->Hk ? (size_t)2 * a->B * a->S * a->H * a->dk : 0;
-  return {n * 4096, n * dkp * dvp, n * dkp * dkp, part};
+  const size_t heads = (size_t)a->B * a->H, N = chunks_of(a->S), n = heads * N, dkp = up32(a->dk), dvp = up16(a->dv);
+  const size_t seg = N ? osm::delta_segment(heads, N) : 1, segs = (N + seg - 1) / seg;
+  const size_t m = segs > 1 ? heads * segs : 0;
+  return {n * 4096, n * osm::kGateFloats, n * dkp * dvp, n * dkp * dkp, m * dkp * dkp, m * dkp * dvp,
+          a->H != a->Hk ? (size_t)2 * a->B * a->S * a->H * a->dk : 0};
 }
 
 DeltaRows rows_of(const osm_rows& r) { return {r.p, r.stride_b, r.stride_s, r.stride_h}; }
@@ -120,9 +128,11 @@ DeltaParams params_of(const osm_delta_args* a) {
   p.Hk = (int)a->Hk;
   p.dk_ = (int)a->dk;
   p.dv_ = (int)a->dv;
-  p.dkp = (int)up16(a->dk);
+  p.dkp = (int)up32(a->dk);
   p.dvp = (int)up16(a->dv);
   p.N = (int)chunks_of(a->S);
+  p.seg = osm::delta_segment(a->B * a->H, p.N);
+  p.segs = (p.N + p.seg - 1) / p.seg;
   p.scale = a->scale;
   const int es = a->dtype == OSM_F32 ? 4 : 2;
   p.vec = a->dk % 4 == 0 && a->dv % 4 == 0 && quads(a->q, es) && quads(a->k, es) && quads(a->v, es);
@@ -143,13 +153,13 @@ extern "C" {
 size_t osm_delta_saved_bytes(const osm_delta_args* a) {
   if (check_shape(a) != OSM_OK) return 0;
   const Sizes n = sizes_of(a);
-  return (n.z + n.s) * sizeof(float);
+  return (n.z + n.s + n.gates) * sizeof(float);
 }
 
 size_t osm_delta_workspace_bytes(const osm_delta_args* a) {
   if (check_shape(a) != OSM_OK || is_short(a)) return 0;
   const Sizes n = sizes_of(a);
-  return (n.a + (a->saved ? 0 : n.z + n.s)) * sizeof(float);
+  return (n.seg_a + n.seg_x + (a->saved ? 0 : n.z + n.gates)) * sizeof(float);
 }
 
 int osm_delta_fwd(const osm_delta_args* a, void* workspace, size_t workspace_bytes, void* stream) {
@@ -188,8 +198,10 @@ int osm_delta_fwd(const osm_delta_args* a, void* workspace, size_t workspace_byt
     if ((rc = check_workspace(workspace, workspace_bytes, osm_delta_workspace_bytes(a))) != OSM_OK) return rc;
     const Sizes n = sizes_of(a);
     p.a = static_cast<float*>(workspace);
-    p.z = a->saved ? static_cast<float*>(a->saved) : p.a + n.a;
-    p.s = p.z + n.z;
+    p.x = p.a + n.seg_a;
+    p.z = a->saved ? static_cast<float*>(a->saved) : p.x + n.seg_x;
+    p.gates = p.z + n.z;
+    p.s = a->saved ? p.gates + n.gates : nullptr;
     e = osm::launch_delta_fwd(p, a->dtype, st);
   }
   return e == hipSuccess ? ok() : fail(OSM_E_HIP, "delta forward launch: %s", hipGetErrorString(e));
@@ -220,7 +232,8 @@ int osm_delta_bwd(const osm_delta_args* a, const osm_delta_bwd_args* b, void* wo
   DeltaParams p = params_of(a);
   const Sizes n = sizes_of(a);
   p.z = static_cast<float*>(a->saved);
-  p.s = p.z + n.z;
+  p.gates = p.z + n.z;
+  p.s = p.gates + n.gates;
   p.a = static_cast<float*>(workspace);
   p.d = p.a + n.a;
   p.vec = p.vec && quads(b->grad_out, es);

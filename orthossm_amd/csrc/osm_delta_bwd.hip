@@ -446,7 +446,7 @@ hipError_t backward(const DeltaParams& p, float* const part, hipStream_t stream)
   const unsigned chunks = (unsigned)((int64_t)p.B * p.H * p.N);
   hipLaunchKernelGGL((delta_adjoint_kernel<T>), dim3(chunks), dim3(kThreads), 0, stream, p);
   hipError_t e = hipGetLastError();
-  if (e == hipSuccess) e = launch_delta_scan(p, p.a, p.d, p.grad_state, p.grad_init, true, stream);
+  if (e == hipSuccess) e = launch_delta_scan(p, p.a, p.d, p.grad_state, p.grad_init, p.N, kDeltaChunk, true, stream);
   if (e != hipSuccess) return e;
   const int64_t plane = (int64_t)p.B * p.S * p.H * p.dk_;
   DeltaParams w = p;

@@ -45,7 +45,8 @@ def _set_rows(r: nat.Rows, t: torch.Tensor) -> None:
 
 
 def _unit_rows(t: torch.Tensor) -> torch.Tensor:
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    near = t.dim() < 4 or t.stride(1) <= nat.DELTA_MAX_STRIDE
+    return t if near and (t.stride(-1) == 1 or t.shape[-1] == 1) else t.contiguous()
 
 
 def _check_qkv(q, k, v, dims: int, form: str):
@@ -71,7 +72,8 @@ def _check_qkv(q, k, v, dims: int, form: str):
 def _gate(t, shape, dev, name: str) -> torch.Tensor:
     if not isinstance(t, torch.Tensor) or tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name} must be a tensor of shape {tuple(shape)}")
-    return t.to(device=dev, dtype=torch.float32)
+    t = t.to(device=dev, dtype=torch.float32)
+    return t if t.dim() < 3 or t.stride(1) <= nat.DELTA_MAX_STRIDE else t.contiguous()
 
 
 def _state(t, shape, dev, name: str) -> torch.Tensor | None:
