@@ -286,25 +286,36 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaPa
   const unsigned v_at = in_v ? col * es + 4 * g * v_row : kOut, o_at = in_v ? col * es + 4 * g * o_row : kOut;
   Block<T, KS, NT> kb, qb;
   f32x4 zr[1024 / NT], br;   // br: beta of the columns of zr
-  float vr[16], gr[2];
+  T vr[16];
+  float gr[2];
+  // The next chunk's inputs, each as soon as its registers are free (and left as
+  // loaded: a conversion would wait for them here).
+  auto rows_of = [&](int c) { return min(kDeltaChunk, tokens - c * kDeltaChunk); };
+  auto fetch_k = [&](int c) { kb.load(kp + (int64_t)c * kDeltaChunk * p.k.ss, p.k.ss, rows_of(c), p.dk_, p.vec); };
+  auto fetch_v = [&](int c) {
+    const Rsrc rs = make_rsrc(vp + (int64_t)c * kDeltaChunk * p.v.ss);
+    const int rows = rows_of(c);
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        vr[4 * t + i] = load_one<T>(rs, 16 * t + 4 * g + i < rows ? v_at + (16 * t + i) * v_row : kOut);
+  };
   auto fetch = [&](int c) {
     const int64_t t0 = (int64_t)c * kDeltaChunk, chunk = (int64_t)bh * p.N + c;
-    const int rows = min(kDeltaChunk, tokens - (int)t0);
-    kb.load(kp + t0 * p.k.ss, p.k.ss, rows, p.dk_, p.vec);
+    const int rows = rows_of(c);
     if (!MAP) qb.load(qp + t0 * p.q.ss, p.q.ss, rows, p.dk_, p.vec);
 #pragma unroll
     for (int e = 0; e < 1024 / NT; ++e) zr[e] = load4(p.z + chunk * 4096 + 4 * (tid + e * NT));
     br = load4(p.gates + chunk * kGateFloats + kBeta + 4 * (tid & 15));
 #pragma unroll
     for (int e = 0; e < 2; ++e) gr[e] = p.gates[chunk * kGateFloats + min(tid + e * NT, kGateFloats - 1)];
-    const Rsrc vs_rs = make_rsrc(vp + t0 * p.v.ss);
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        vr[4 * t + i] = (float)load_one<T>(vs_rs, 16 * t + 4 * g + i < rows ? v_at + (16 * t + i) * v_row : kOut);
   };
-  if (c0 < c1) fetch(c0);
+  if (c0 < c1) {
+    fetch_k(c0);
+    fetch(c0);
+    fetch_v(c0);
+  }
   for (int c = c0; c < c1; ++c) {
     const int64_t t0 = (int64_t)c * kDeltaChunk;
     __syncthreads();   // the chunk before has been read
@@ -328,12 +339,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaPa
           *reinterpret_cast<u32x2*>(&zp[k][tri_at(row) + 32 * (q >> 3) + 8 * (q & 3) + 4 * ((q >> 2) & 1)]) = part[k];
       }
     }
-    float v[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = vr[i];
-    Block<T, KS, NT> kc = kb;
     __syncthreads();
-    if (c + 1 < c1) fetch(c + 1);
+    if (c + 1 < c1) {
+      fetch(c + 1);
+      if (MAP) fetch_k(c + 1);
+    }
     f32x4 x[4], o[4];
     if (live) {
       if (!MAP && p.s && value) {
@@ -360,9 +370,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaPa
       for (int t = 0; t < 4; ++t) {
         const f32x4 gam = load4(gt + kGam + 16 * t + 4 * g);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[t][i] = v[4 * t + i] - gam[i] * x[t][i];
+        for (int i = 0; i < 4; ++i) x[t][i] = (float)vr[4 * t + i] - gam[i] * x[t][i];
       }
     }
+    if (c + 1 < c1) fetch_v(c + 1);
     if (!MAP) {
       // P: four of its columns of one row a lane, from K Q^T; WAVES / 4 waves a
       // tile row
@@ -392,7 +403,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaPa
         for (int k = 0; k < 3; ++k)
           *reinterpret_cast<u32x2*>(&pp[MAP ? 0 : k][tri_at(i) + 32 * (tr >> 1) + 8 * g + 4]) = u32x2{0, 0};
       __syncthreads();   // P is there, Q has been read
-      kc.template put_columns<LKT>(&second[0][0], kSecond);
+      kb.template put_columns<LKT>(&second[0][0], kSecond);
+      if (c + 1 < c1) fetch_k(c + 1);
     }
     if (live) {
       f32x4 y[4];
