@@ -12,7 +12,8 @@ namespace osm {
 constexpr int kDeltaChunk = 64;      // tokens a chunk
 constexpr int kDeltaMaxDk = 128;     // rows of the state
 constexpr int kDeltaSlice = 16;      // columns of the state a scan workgroup, or a wave of a walk, holds
-constexpr int kGateFloats = 320;     // a chunk's hi, lo, beta, gam, end (delta::Gates)
+constexpr int kGateFloats = 320;     // a chunk's gates (delta::make_gates)
+constexpr int kZFloats = 3072;       // a chunk's Z: rows 0-31 by 32 columns, rows 32-63 by 64
 
 // Rows of a token tensor: element (b, t, h, j) at b*sb + t*ss + h*sh + j.
 struct DeltaRows {
@@ -26,7 +27,7 @@ struct DeltaParams {
   const int* lengths;                // [B] tokens in use, or NULL
   const float* init;                 // [B,H,dk,dv], or NULL
   float* fin;                        // [B,H,dk,dv], or NULL
-  float* z;                          // [B,H,N][64][64]
+  float* z;                          // [B,H,N][kZFloats]
   float* gates;                      // [B,H,N][kGateFloats]
   float* s;                          // [B,H,N][dkp][dvp] states before the chunks, or NULL
   float* a;                          // maps of the segments [B,H,segs][dkp][dkp] (backward: of the chunks)
@@ -175,7 +176,19 @@ __device__ __forceinline__ void load_tile(float* dst, const T* src, int64_t stri
   }
 }
 
-// The same from a workspace matrix of fp32 rows, whole quads.
+// Row and first column of the four elements `quad` of a stored Z.
+__device__ __forceinline__ int z_row(int quad) { return quad < 256 ? quad >> 3 : 32 + ((quad - 256) >> 4); }
+__device__ __forceinline__ int z_quad(int quad) { return quad < 256 ? quad & 7 : (quad - 256) & 15; }
+
+// A stored Z into a tile.
+template <int NT>
+__device__ __forceinline__ void load_z(float* dst, const float* src) {
+  for (int e = threadIdx.x; e < kZFloats / 4; e += NT)
+    *reinterpret_cast<f32x4*>(dst + z_row(e) * kLd + 4 * z_quad(e)) = load4(src + 4 * e);
+  for (int e = threadIdx.x; e < 256; e += NT) *reinterpret_cast<f32x4*>(dst + (e >> 3) * kLd + 32 + 4 * (e & 7)) = zero4();
+}
+
+// A workspace matrix of fp32 rows, whole quads, into a tile.
 template <int NT>
 __device__ __forceinline__ void load_ws(float* dst, const float* src, int ld, int rows, int width) {
   const int quads = width >> 2;
@@ -244,35 +257,46 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 template <typename T>
 constexpr int kParts = sizeof(T) == 4 ? 3 : 1;
 
-// a and b as the sums of three bf16 numbers each, packed: the nearest, then the
-// nearest to what is left (which is exact), twice.
-__device__ __forceinline__ void split2(unsigned (&part)[3], float a, float b) {
+// a and b as the sums of N bf16 numbers each, packed: the nearest, then the
+// nearest to what is left, and again (three hold all 24 bits).  What is left,
+// x - part, is exact, and one instruction as a dot product of the packed pair.
+template <int N>
+__device__ __forceinline__ void split2(unsigned (&part)[N], float a, float b) {
+  // (-1, 0) and (0, -1), as values that the compiler does not fold: it writes the
+  // first as the instruction's inline -1.0, which the hardware reads as an fp32
+  // number, that is as (0, -1).
+  unsigned first, second;
+  asm("s_mov_b32 %0, 0xbf80" : "=s"(first));
+  asm("s_mov_b32 %0, 0xbf800000" : "=s"(second));
 #pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    part[k] = __builtin_bit_cast(unsigned, __builtin_convertvector(f32x2{a, b}, bf16x2));
-    if (k < 2) {
-      a -= __uint_as_float(part[k] << 16);
-      b -= __uint_as_float(part[k] & 0xffff0000u);
+  for (int k = 0; k < N; ++k) {
+    const bf16x2 h = __builtin_convertvector(f32x2{a, b}, bf16x2);
+    part[k] = __builtin_bit_cast(unsigned, h);
+    if (k < N - 1) {
+      a = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, first), a, false);
+      b = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, second), b, false);
     }
   }
 }
 
-__device__ __forceinline__ void split4(u32x2 (&part)[3], f32x4 v) {
-  unsigned lo[3], hi[3];
-  split2(lo, v[0], v[1]);
-  split2(hi, v[2], v[3]);
+template <int N>
+__device__ __forceinline__ void split4(u32x2 (&part)[N], f32x4 v) {
+  unsigned lo[N], hi[N];
+  split2<N>(lo, v[0], v[1]);
+  split2<N>(hi, v[2], v[3]);
 #pragma unroll
-  for (int k = 0; k < 3; ++k) part[k] = u32x2{lo[k], hi[k]};
+  for (int k = 0; k < N; ++k) part[k] = u32x2{lo[k], hi[k]};
 }
 
 // Two result tiles, rows 16 apart, as the second operand of a product over
 // their 32 rows.
-__device__ __forceinline__ void split_pair(u32x4 (&part)[3], f32x4 a, f32x4 b) {
-  u32x2 pa[3], pb[3];
-  split4(pa, a);
-  split4(pb, b);
+template <int N>
+__device__ __forceinline__ void split_pair(u32x4 (&part)[N], f32x4 a, f32x4 b) {
+  u32x2 pa[N], pb[N];
+  split4<N>(pa, a);
+  split4<N>(pb, b);
 #pragma unroll
-  for (int k = 0; k < 3; ++k) part[k] = u32x4{pa[k][0], pa[k][1], pb[k][0], pb[k][1]};
+  for (int k = 0; k < N; ++k) part[k] = u32x4{pa[k][0], pa[k][1], pb[k][0], pb[k][1]};
 }
 
 // The terms of a product's 32 are kept in the order in which a pair of result
@@ -292,13 +316,15 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
 }
 
 // acc += A B over 32 terms, A's parts in LDS, B's in registers, the smaller
-// products first.
-template <int NA, int NB>
-__device__ __forceinline__ void prod(f32x4& acc, const unsigned short* m, int stride, int at, const u32x4 (&b)[NB]) {
+// products first; products of parts i and j with i + j > ORDER (of order
+// 2^(-8 ORDER - 8) and below) are left out.
+template <int NA, int NB, int ORDER = 2, int N>
+__device__ __forceinline__ void prod(f32x4& acc, const unsigned short* m, int stride, int at, const u32x4 (&b)[N]) {
+  static_assert(NB <= N, "no more parts than there are");
   u32x4 a[NA];
   read_parts<NA>(a, m, stride, at);
 #pragma unroll
-  for (int sum = 2; sum >= 0; --sum)
+  for (int sum = ORDER; sum >= 0; --sum)
 #pragma unroll
     for (int i = 0; i <= sum; ++i)
       if (i < NA && sum - i < NB) acc = mfma(a[i], b[sum - i], acc);
@@ -401,7 +427,7 @@ struct Block {
       *reinterpret_cast<u32x2*>(dst) = __builtin_bit_cast(u32x2, x);
     } else {
       u32x2 part[3];
-      split4(part, x);
+      split4<3>(part, x);
 #pragma unroll
       for (int k = 0; k < 3; ++k) *reinterpret_cast<u32x2*>(dst + k * stride) = part[k];
     }
@@ -435,13 +461,13 @@ __device__ __forceinline__ void make_gates(float* gt, const DeltaRows& g, const 
   gt[kHi + t] = hi;
   gt[kLo + t] = lo;
   gt[kBeta + t] = bv;
-  gt[kGam + t] = exp2f(hi) * __builtin_fmaf(lo, 0.69314718f, 1.0f);
-  gt[kEnd + t] = exp2f((float)(__shfl(G, 63) - G));
+  gt[kGam + t] = __builtin_amdgcn_exp2f(hi) * __builtin_fmaf(lo, 0.69314718f, 1.0f);
+  gt[kEnd + t] = __builtin_amdgcn_exp2f((float)(__shfl(G, 63) - G));
 }
 
 // e^(G_i - G_j)
 __device__ __forceinline__ float decay(const float* gt, int i, int j) {
-  return exp2f((gt[kHi + i] - gt[kHi + j]) + (gt[kLo + i] - gt[kLo + j]));
+  return __builtin_amdgcn_exp2f((gt[kHi + i] - gt[kHi + j]) + (gt[kLo + i] - gt[kLo + j]));
 }
 
 // (b, h, chunk, tokens in use) of a workgroup's chunk.

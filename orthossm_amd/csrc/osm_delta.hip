@@ -39,120 +39,133 @@ namespace {
 
 using namespace delta;
 
-constexpr int kThreads = 256;
-
-// Z from L in place (tile zs, L strictly lower, zeros elsewhere): the four
-// diagonal 16x16 blocks by substitution, row i from the rows before it (Z_i =
-// L_i - sum_j L_ij beta_j Z_j), then block pairs: for L = [[a, 0], [c, d]],
+// Z from L in place (tile zs, L strictly lower, zeros elsewhere), by one wave: the
+// four diagonal 16x16 blocks by substitution, row i from the rows before it (Z_i
+// = L_i - sum_j L_ij beta_j Z_j), then block pairs: for L = [[a, 0], [c, d]],
 // Z_c = (I - Z_d beta) (L_c - L_c beta Z_a), the 16-wide ones, then the 32-wide.
-__device__ void invert(float* zs, const float* beta) {
-  const int wave = threadIdx.x >> 6, l = threadIdx.x & 63;
-  if (wave == 0) {
-    const int c = l & 15, o = 16 * (l >> 4);
-    float* const base = zs + o * kLd + o;
-    float z[16], bz[16];   // column c of the block's Z, and beta Z
+__device__ __forceinline__ void invert(float* zs, const float* beta) {
+  const int l = threadIdx.x & 63, c = l & 15, o = 16 * (l >> 4);
+  float* const base = zs + o * kLd + o;
+  float z[16], bz[16];   // column c of the lane's block of Z, and beta Z
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float v = base[i * kLd + c];
-      f32x4 row[4];
+  for (int i = 0; i < 16; ++i) {
+    float v = base[i * kLd + c];
+    f32x4 row[4];
 #pragma unroll
-      for (int q = 0; q < (i + 3) / 4; ++q) row[q] = load4(base + i * kLd + 4 * q);
+    for (int q = 0; q < (i + 3) / 4; ++q) row[q] = load4(base + i * kLd + 4 * q);
 #pragma unroll
-      for (int j = 0; j < i; ++j) v = __builtin_fmaf(-row[j / 4][j % 4], bz[j], v);
-      z[i] = v;
-      bz[i] = beta[o + i] * v;
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // every lane has read its rows
+    for (int j = 0; j < i; ++j) v = __builtin_fmaf(-row[j / 4][j % 4], bz[j], v);
+    z[i] = v;
+    bz[i] = beta[o + i] * v;
+  }
+  __syncthreads();   // (one wave: orders its lanes' accesses)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) base[i * kLd + c] = z[i];
+  for (int i = 0; i < 16; ++i) base[i * kLd + c] = z[i];
+  __syncthreads();
+  f32x4 acc[2][1], q[2][1];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int a = 32 * h, d = a + 16;
+    clear(acc[h]);
+    mma<1, false, false, true>(acc[h], zs, d, zs, a, a, d, beta);   // L_c beta Z_a
+    get(q[h], zs, d, a);
+    q[h][0] -= acc[h][0];
   }
   __syncthreads();
-  // 16-wide: waves 0 and 1 take the pairs (0, 1) and (2, 3).
-  {
-    const int a = 32 * (wave & 1), d = a + 16;
-    f32x4 acc[1], q[1];
-    if (wave < 2) {
-      clear(acc);
-      mma<1, false, false, true>(acc, zs, d, zs, a, a, d, beta);   // L_c beta Z_a
-      get(q, zs, d, a);
-      q[0] -= acc[0];
-    }
-    __syncthreads();
-    if (wave < 2) put(zs, q, d, a);
-    __syncthreads();
-    if (wave < 2) {
-      clear(acc);
-      mma<1, false, false, true>(acc, zs, d, zs, a, d, d + 16, beta);   // Z_d beta (..)
-      q[0] -= acc[0];
-    }
-    __syncthreads();
-    if (wave < 2) put(zs, q, d, a);
-    __syncthreads();
+  put(zs, q[0], 16, 0);
+  put(zs, q[1], 48, 32);
+  __syncthreads();
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int a = 32 * h, d = a + 16;
+    clear(acc[h]);
+    mma<1, false, false, true>(acc[h], zs, d, zs, a, d, d + 16, beta);   // Z_d beta (..)
+    q[h][0] -= acc[h][0];
   }
-  // 32-wide: a 16x16 tile a wave.
-  {
-    const int r0 = 32 + 16 * (wave >> 1), c0 = 16 * (wave & 1);
-    f32x4 acc[1], q[1];
-    clear(acc);
-    mma<1, false, false, true>(acc, zs, r0, zs, c0, 0, 32, beta);
-    get(q, zs, r0, c0);
-    q[0] -= acc[0];
-    __syncthreads();
-    put(zs, q, r0, c0);
-    __syncthreads();
-    clear(acc);
-    mma<1, false, false, true>(acc, zs, r0, zs, c0, 32, 64, beta);
-    q[0] -= acc[0];
-    __syncthreads();
-    put(zs, q, r0, c0);
-    __syncthreads();
+  __syncthreads();
+  put(zs, q[0], 16, 0);
+  put(zs, q[1], 48, 32);
+  __syncthreads();
+  f32x4 wide[2][2], w[2][2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    clear(wide[h]);
+    mma<2, false, false, true>(wide[h], zs, 32 + 16 * h, zs, 0, 0, 32, beta);
+    get(w[h], zs, 32 + 16 * h, 0);
+    w[h][0] -= wide[h][0];
+    w[h][1] -= wide[h][1];
   }
+  __syncthreads();
+  put(zs, w[0], 32, 0);
+  put(zs, w[1], 48, 0);
+  __syncthreads();
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    clear(wide[h]);
+    mma<2, false, false, true>(wide[h], zs, 32 + 16 * h, zs, 0, 32, 64, beta);
+    w[h][0] -= wide[h][0];
+    w[h][1] -= wide[h][1];
+  }
+  __syncthreads();
+  put(zs, w[0], 32, 0);
+  put(zs, w[1], 48, 0);
+  __syncthreads();
 }
 
-// Z and the gates of a chunk.  KS: blocks of 32 columns of k.
+// Z and the gates of a chunk, one wave: the steps of the inversion follow each
+// other closely and hold little, so eight chunks a CU side by side beat four waves
+// that wait for each other (8192 chunks of d = 64: 89 us so).  KS: blocks of 32
+// columns of k.
 template <typename T, int KS>
-__global__ void __launch_bounds__(kThreads) delta_solve_kernel(const DeltaParams p) {
-  constexpr int NP = kParts<T>, LDK = 32 * KS + 8;
-  __shared__ __attribute__((aligned(16))) float zs[kTile];
-  __shared__ __attribute__((aligned(16))) unsigned short kk[NP][64 * LDK];
+__global__ void __launch_bounds__(64) delta_solve_kernel(const DeltaParams p) {
+  constexpr int NP = kParts<T>, LDK = 32 * KS + 8, kBytes = NP * 64 * LDK * 2 > 4 * kTile ? NP * 64 * LDK * 2 : 4 * kTile;
+  __shared__ __attribute__((aligned(16))) unsigned char both[kBytes];   // K, then L and Z
   __shared__ __attribute__((aligned(16))) float gt[kGateFloats];
+  unsigned short* const kk = reinterpret_cast<unsigned short*>(both);
+  float* const zs = reinterpret_cast<float*>(both);
   const int64_t chunk = blockIdx.x;
   const At w = chunk_at(p, chunk);
   if (w.rows == 0) return;
-  const int wave = threadIdx.x >> 6, l = threadIdx.x & 63, r0 = 16 * wave;
-  Block<T, KS, kThreads> kb;
+  const int l = threadIdx.x, r = l & 15, g = l >> 4;
+  Block<T, KS, 64> kb;
   kb.load(row_ptr<T>(p.k, w.b, w.t0, w.h / (p.H / p.Hk)), p.k.ss, w.rows, p.dk_, p.vec);
   make_gates(gt, p.g, p.beta, w.b, w.t0, w.h, w.rows);
-  kb.template put_rows<LDK>(&kk[0][0], 64 * LDK);
+  kb.template put_rows<LDK>(kk, 64 * LDK);
   __syncthreads();
-  f32x4 acc[4];
-  clear(acc);
+  f32x4 acc[4][4];   // [c][t]: element i is (K K^T)[16 c + 4 g + i][16 t + r], for c <= t
 #pragma unroll
-  for (int s = 0; s < KS; ++s) {
-    u32x4 b[NP];
-    read_parts<NP>(b, &kk[0][0], 64 * LDK, (r0 + (l & 15)) * LDK + 32 * s + 8 * (l >> 4));
+  for (int t = 0; t < 4; ++t) {
+    clear(acc[t]);
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (c <= wave) prod<NP, NP>(acc[c], &kk[0][0], 64 * LDK, (16 * c + (l & 15)) * LDK + 32 * s + 8 * (l >> 4), b);
+    for (int s = 0; s < KS; ++s) {
+      u32x4 b[NP];
+      read_parts<NP>(b, kk, 64 * LDK, (16 * t + r) * LDK + 32 * s + 8 * g);
+#pragma unroll
+      for (int c = 0; c <= t; ++c) prod<NP, NP>(acc[t][c], kk, 64 * LDK, (16 * c + r) * LDK + 32 * s + 8 * g, b);
+    }
   }
-  // acc[c][i] is (K K^T)[16 c + 4 g + i][r0 + lane%16]; it is symmetric: four
-  // columns of row r0 + lane%16
-  const int row = r0 + (l & 15);
+  __syncthreads();
+  // (it is symmetric: four columns of row 16 t + r a lane)
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const int col = 16 * c + 4 * (l >> 4);
-    f32x4 v;
+  for (int t = 0; t < 4; ++t)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = row > col + i ? acc[c][i] * decay(gt, row, col + i) : 0.0f;
-    *reinterpret_cast<f32x4*>(zs + row * kLd + col) = v;
-  }
+    for (int c = 0; c < 4; ++c) {
+      const int row = 16 * t + r, col = 16 * c + 4 * g;
+      f32x4 v = zero4();
+      if (c <= t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = row > col + i ? acc[t][c][i] * decay(gt, row, col + i) : 0.0f;
+      *reinterpret_cast<f32x4*>(zs + row * kLd + col) = v;
+    }
   __syncthreads();
   invert(zs, gt + kBeta);
-  float* const zg = p.z + chunk * 4096;
-  for (int e = threadIdx.x; e < 1024; e += kThreads)
-    store4(zg + 4 * e, *reinterpret_cast<const f32x4*>(zs + (e >> 4) * kLd + 4 * (e & 15)));
+  float* const zg = p.z + chunk * kZFloats;
+#pragma unroll
+  for (int e = l; e < kZFloats / 4; e += 64)
+    store4(zg + 4 * e, *reinterpret_cast<const f32x4*>(zs + z_row(e) * kLd + 4 * z_quad(e)));
   float* const gg = p.gates + chunk * kGateFloats;
-  for (int e = threadIdx.x; e < kGateFloats; e += kThreads) gg[e] = gt[e];
+#pragma unroll
+  for (int e = l; e < kGateFloats; e += 64) gg[e] = gt[e];
 }
 
 // S' = A S + B over the spans of a row, in order or in reverse, for 16 columns
@@ -235,10 +248,17 @@ __device__ __forceinline__ int tri_at(int row) { return row < 32 ? row * 40 : 12
 template <typename T, int KS, int WAVES, bool MAP>
 __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaParams p, int groups) {
   constexpr int NT = 64 * WAVES, NP = kParts<T>, DK = 32 * KS, LDK = DK + 8, LKT = 72, ST = 2 * KS;
-  // K by rows; Q by rows, then K by columns; Z; P.
-  constexpr int kSecond = (MAP || 64 * LDK < DK * LKT) ? DK * LKT : 64 * LDK;
+  // Parts of what only the output sees: bf16 outputs need no more than two.
+  constexpr int OP = sizeof(T) == 4 ? 3 : 2;
+  // K by rows; K by columns; Q by rows, where two workgroups' LDS holds it, else in
+  // the place of K by columns, which then follows it; Z; P.
+  constexpr int kKt = DK * LKT, kQ = 64 * LDK;
+  constexpr bool kApart = !MAP && 2 * (NP * (kKt + 2 * kQ) + (3 + OP) * kTri) + 4 * kGateFloats <= 80 * 1024;
+  constexpr int kSecond = MAP ? kKt : kApart ? kKt + kQ : kKt > kQ ? kKt : kQ;
   __shared__ __attribute__((aligned(16))) unsigned short kk[NP][64 * LDK], second[NP][kSecond], zp[3][kTri],
-      pp[MAP ? 1 : 3][MAP ? 8 : kTri];
+      pp[MAP ? 1 : OP][MAP ? 8 : kTri];
+  unsigned short* const kt = &second[0][0];
+  unsigned short* const qq = &second[0][kApart ? kKt : 0];
   __shared__ __attribute__((aligned(16))) float gt[kGateFloats];
   const int group = blockIdx.x % groups;
   const int64_t id = blockIdx.x / groups;
@@ -285,7 +305,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaPa
   const unsigned es = sizeof(T), v_row = (unsigned)p.v.ss * es, o_row = (unsigned)p.o.ss * es;
   const unsigned v_at = in_v ? col * es + 4 * g * v_row : kOut, o_at = in_v ? col * es + 4 * g * o_row : kOut;
   Block<T, KS, NT> kb, qb;
-  f32x4 zr[1024 / NT], br;   // br: beta of the columns of zr
+  constexpr int NZ = (kZFloats / 4 + NT - 1) / NT;
+  f32x4 zr[NZ], br[NZ];   // br: beta of the columns of zr
   T vr[16];
   float gr[2];
   // The next chunk's inputs, each as soon as its registers are free (and left as
@@ -306,8 +327,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaPa
     const int rows = rows_of(c);
     if (!MAP) qb.load(qp + t0 * p.q.ss, p.q.ss, rows, p.dk_, p.vec);
 #pragma unroll
-    for (int e = 0; e < 1024 / NT; ++e) zr[e] = load4(p.z + chunk * 4096 + 4 * (tid + e * NT));
-    br = load4(p.gates + chunk * kGateFloats + kBeta + 4 * (tid & 15));
+    for (int e = 0; e < NZ; ++e) {
+      const int quad = min(tid + e * NT, kZFloats / 4 - 1);
+      zr[e] = load4(p.z + chunk * kZFloats + 4 * quad);
+      br[e] = load4(p.gates + chunk * kGateFloats + kBeta + 4 * z_quad(quad));
+    }
 #pragma unroll
     for (int e = 0; e < 2; ++e) gr[e] = p.gates[chunk * kGateFloats + min(tid + e * NT, kGateFloats - 1)];
   };
@@ -323,26 +347,23 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaPa
     for (int e = 0; e < 2; ++e)
       if (tid + e * NT < kGateFloats) gt[tid + e * NT] = gr[e];
     kb.template put_rows<LDK>(&kk[0][0], 64 * LDK);
-    if (MAP)
-      kb.template put_columns<LKT>(&second[0][0], kSecond);
-    else
-      qb.template put_rows<LDK>(&second[0][0], kSecond);
+    if (MAP || kApart) kb.template put_columns<LKT>(kt, kSecond);
+    if (!MAP) qb.template put_rows<LDK>(qq, kSecond);
     // Z beta
 #pragma unroll
-    for (int e = 0; e < 1024 / NT; ++e) {
-      const int row = (tid + e * NT) >> 4, q = (tid + e * NT) & 15;
-      if (row >= 32 || q < 8) {
+    for (int e = 0; e < NZ; ++e) {
+      const int quad = tid + e * NT;
+      if (quad < kZFloats / 4) {
         u32x2 part[3];
-        split4(part, zr[e] * br);
+        split4<3>(part, zr[e] * br[e]);
 #pragma unroll
-        for (int k = 0; k < 3; ++k)
-          *reinterpret_cast<u32x2*>(&zp[k][tri_at(row) + 32 * (q >> 3) + 8 * (q & 3) + 4 * ((q >> 2) & 1)]) = part[k];
+        for (int k = 0; k < 3; ++k) *reinterpret_cast<u32x2*>(&zp[k][tri_at(z_row(quad)) + place4(z_quad(quad))]) = part[k];
       }
     }
     __syncthreads();
     if (c + 1 < c1) {
       fetch(c + 1);
-      if (MAP) fetch_k(c + 1);
+      if (MAP || kApart) fetch_k(c + 1);
     }
     f32x4 x[4], o[4];
     if (live) {
@@ -358,12 +379,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaPa
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         u32x4 sp[3];
-        split_pair(sp, S[2 * s], S[2 * s + 1]);
+        split_pair<3>(sp, S[2 * s], S[2 * s + 1]);
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
           const int at = (16 * t + r) * LDK + 32 * s + 8 * g;
           prod<NP, 3>(x[t], &kk[0][0], 64 * LDK, at, sp);
-          if (!MAP) prod<NP, 3>(o[t], &second[0][0], kSecond, at, sp);
+          if (!MAP) prod<NP, OP, OP - 1>(o[t], qq, kSecond, at, sp);
         }
       }
 #pragma unroll
@@ -383,7 +404,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaPa
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
           u32x4 qf[NP];
-          read_parts<NP>(qf, &second[0][0], kSecond, i * LDK + 32 * s + 8 * g);
+          read_parts<NP>(qf, qq, kSecond, i * LDK + 32 * s + 8 * g);
           prod<NP, NP>(acc, &kk[0][0], 64 * LDK, (16 * tc + r) * LDK + 32 * s + 8 * g, qf);
         }
 #pragma unroll
@@ -391,20 +412,22 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaPa
           const int j = 16 * tc + 4 * g + e;
           acc[e] = i >= j ? acc[e] * decay(gt, i, j) : 0.0f;
         }
-        u32x2 part[3];
-        split4(part, acc);
+        u32x2 part[OP];
+        split4<OP>(part, acc);
 #pragma unroll
-        for (int k = 0; k < 3; ++k)
+        for (int k = 0; k < OP; ++k)
           *reinterpret_cast<u32x2*>(&pp[MAP ? 0 : k][tri_at(i) + 32 * (tc >> 1) + 8 * g + 4 * (tc & 1)]) = part[k];
       }
       // the other half of a pair of tiles whose first is on the diagonal
       if ((wave >> 2) == 0 && (tr & 1) == 0)
 #pragma unroll
-        for (int k = 0; k < 3; ++k)
+        for (int k = 0; k < OP; ++k)
           *reinterpret_cast<u32x2*>(&pp[MAP ? 0 : k][tri_at(i) + 32 * (tr >> 1) + 8 * g + 4]) = u32x2{0, 0};
       __syncthreads();   // P is there, Q has been read
-      kb.template put_columns<LKT>(&second[0][0], kSecond);
-      if (c + 1 < c1) fetch_k(c + 1);
+      if (!kApart) {
+        kb.template put_columns<LKT>(kt, kSecond);
+        if (c + 1 < c1) fetch_k(c + 1);
+      }
     }
     if (live) {
       f32x4 y[4];
@@ -413,7 +436,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaPa
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         u32x4 xp[3];
-        split_pair(xp, x[2 * s], x[2 * s + 1]);
+        split_pair<3>(xp, x[2 * s], x[2 * s + 1]);
 #pragma unroll
         for (int t = 2 * s; t < 4; ++t) prod<3, 3>(y[t], &zp[0][0], kTri, tri_at(16 * t + r) + 32 * s + 8 * g, xp);
       }
@@ -427,10 +450,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaPa
         for (int t = 0; t < 4; ++t) o[t] *= load4(gt + kGam + 16 * t + 4 * g);
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          u32x4 up[3];
-          split_pair(up, x[2 * s], x[2 * s + 1]);
+          u32x4 up[OP];
+          split_pair<OP>(up, x[2 * s], x[2 * s + 1]);
 #pragma unroll
-          for (int t = 2 * s; t < 4; ++t) prod<3, 3>(o[t], &pp[0][0], kTri, tri_at(16 * t + r) + 32 * s + 8 * g, up);
+          for (int t = 2 * s; t < 4; ++t) prod<OP, OP, OP - 1>(o[t], &pp[0][0], kTri, tri_at(16 * t + r) + 32 * s + 8 * g, up);
         }
         const int rows = tokens - (int)t0, all = p.S - (int)t0;
         const Rsrc o_rs = make_rsrc(op + t0 * p.o.ss);
@@ -443,7 +466,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaPa
           }
       }
     }
-    if (!MAP) __syncthreads();   // K by columns is there
+    if (!MAP && !kApart) __syncthreads();   // K by columns is there
     if (live) {
       const float last = gt[kGam + 63];
 #pragma unroll
@@ -451,9 +474,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaPa
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         u32x4 up[3];
-        split_pair(up, x[2 * s] * load4(gt + kEnd + 32 * s + 4 * g), x[2 * s + 1] * load4(gt + kEnd + 32 * s + 16 + 4 * g));
+        split_pair<3>(up, x[2 * s] * load4(gt + kEnd + 32 * s + 4 * g), x[2 * s + 1] * load4(gt + kEnd + 32 * s + 16 + 4 * g));
 #pragma unroll
-        for (int t = 0; t < ST; ++t) prod<NP, 3>(S[t], &second[0][0], kSecond, (16 * t + r) * LKT + 32 * s + 8 * g, up);
+        for (int t = 0; t < ST; ++t) prod<NP, 3>(S[t], kt, kSecond, (16 * t + r) * LKT + 32 * s + 8 * g, up);
       }
     }
   }
@@ -493,7 +516,7 @@ void launch_walk(const DeltaParams& p, hipStream_t stream) {
 template <typename T, int KS>
 hipError_t forward(const DeltaParams& p, hipStream_t stream) {
   const int64_t chunks = (int64_t)p.B * p.H * p.N;
-  hipLaunchKernelGGL((delta_solve_kernel<T, KS>), dim3((unsigned)chunks), dim3(kThreads), 0, stream, p);
+  hipLaunchKernelGGL((delta_solve_kernel<T, KS>), dim3((unsigned)chunks), dim3(64), 0, stream, p);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && p.segs > 1) {
     launch_walk<T, KS, true>(p, stream);

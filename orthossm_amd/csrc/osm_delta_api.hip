@@ -79,7 +79,7 @@ Sizes sizes_of(const osm_delta_args* a) {
   const size_t heads = (size_t)a->B * a->H, N = chunks_of(a->S), n = heads * N, dkp = up32(a->dk), dvp = up16(a->dv);
   const size_t seg = N ? osm::delta_segment(heads, N) : 1, segs = (N + seg - 1) / seg;
   const size_t m = segs > 1 ? heads * segs : 0;
-  return {n * 4096, n * osm::kGateFloats, n * dkp * dvp, n * dkp * dkp, m * dkp * dkp, m * dkp * dvp,
+  return {n * osm::kZFloats, n * osm::kGateFloats, n * dkp * dvp, n * dkp * dkp, m * dkp * dkp, m * dkp * dvp,
           a->H != a->Hk ? (size_t)2 * a->B * a->S * a->H * a->dk : 0};
 }
 

@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(kThreads) delta_adjoint_kernel(const DeltaPara
   const T* const q = row_ptr<T>(p.q, w.b, w.t0, hk);
   const T* const k = row_ptr<T>(p.k, w.b, w.t0, hk);
   const T* const go = row_ptr<T>(p.dout, w.b, w.t0, w.h);
-  load_ws<kThreads>(zs, p.z + chunk * 4096, 64, 64, 64);
+  load_z<kThreads>(zs, p.z + chunk * kZFloats);
   f32x4 P[4], acc[4], x[4];
   scores<kThreads, false>(P, acc, ws, ks, q, k, p, w.rows, r0, 0);
 #pragma unroll
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const DeltaPa
     return;
   }
   load_gates(&gt, p.g, p.beta, w.b, w.t0, w.h, w.rows);
-  load_ws<kGradThreads>(zs, p.z + chunk * 4096, 64, 64, 64);
+  load_z<kGradThreads>(zs, p.z + chunk * kZFloats);
   const T* const q = row_ptr<T>(p.q, w.b, w.t0, hk);
   const T* const k = row_ptr<T>(p.k, w.b, w.t0, hk);
   const T* const v = row_ptr<T>(p.v, w.b, w.t0, w.h);

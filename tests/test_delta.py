@@ -67,7 +67,7 @@ def _fwd(a, ws=None, nbytes=0):
 def test_sizes():
     lib = nat.load()
     chunks = 2 * 4 * 4                      # rows, heads, chunks of 64 tokens
-    solved, states, maps = (chunks * n * 4 for n in (64 * 64 + 320, 64 * 80, 64 * 64))   # 48 rows of a state held as 64
+    solved, states, maps = (chunks * n * 4 for n in (48 * 64 + 320, 64 * 80, 64 * 64))   # 48 rows of a state held as 64
     segments = 2 * 4 * 2 * (64 * 64 + 64 * 80) * 4                                      # two of two chunks a row
     assert lib.osm_delta_saved_bytes(ctypes.byref(_args())) == solved + states
     assert lib.osm_delta_workspace_bytes(ctypes.byref(_args())) == solved + segments
