@@ -380,7 +380,7 @@ typedef struct osm_delta_args {
   int32_t dtype;                /* osm_dtype of q, k, v, out and their gradients */
   int64_t B, S, H, Hk, dk, dv;  /* dk <= OSM_DELTA_MAX_DK */
   float scale;
-  osm_rows q, k, v, out;        /* [B,S,Hk,dk] (q, k), [B,S,H,dv] (v, out) */
+  osm_rows q, k, v, out;        /* [B,S,Hk,dk] (q, k), [B,S,H,dv] (v, out); stride_s at least the row's elements */
   osm_rows g, beta;             /* [B,S,H] fp32 */
   const int32_t* lengths;       /* [B], or NULL: every row has S tokens */
   const float* state_init;      /* [B,H,dk,dv] contiguous, or NULL: zeros */

@@ -40,7 +40,7 @@ struct DeltaParams {
   int B, S, H, Hk, dk_, dv_, dkp, dvp, N;   // dkp: dk up to a multiple of 32, dvp: dv of 16, N: chunks of a row
   int seg, segs;                     // chunks a segment, segments a row
   float scale;
-  int vec;                           // rows of q, k, v, o, dout, dq, dk, dv start at multiples of 4 elements
+  int vec;                           // q, k, v and dout are whole multiples of so many elements, strides and all (4, 2, 1)
 };
 
 // Row b's state is slot b, or slots[b] of a pool of n_slots (state_s elements
@@ -315,19 +315,35 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// acc += A B over 32 terms, A's parts in LDS, B's in registers, the smaller
-// products first; products of parts i and j with i + j > ORDER (of order
-// 2^(-8 ORDER - 8) and below) are left out.
-template <int NA, int NB, int ORDER = 2, int N>
-__device__ __forceinline__ void prod(f32x4& acc, const unsigned short* m, int stride, int at, const u32x4 (&b)[N]) {
+// acc += A B over 32 terms, the smaller products first; products of parts i and
+// j with i + j > ORDER (of order 2^(-8 ORDER - 8) and below) are left out.
+template <int NB, int ORDER, int NA, int N>
+__device__ __forceinline__ void mul(f32x4& acc, const u32x4 (&a)[NA], const u32x4 (&b)[N]) {
   static_assert(NB <= N, "no more parts than there are");
-  u32x4 a[NA];
-  read_parts<NA>(a, m, stride, at);
 #pragma unroll
   for (int sum = ORDER; sum >= 0; --sum)
 #pragma unroll
     for (int i = 0; i <= sum; ++i)
       if (i < NA && sum - i < NB) acc = mfma(a[i], b[sum - i], acc);
+}
+
+// COUNT products in turn: at(i) is where the parts of the i-th first operand are
+// in LDS, go(i, parts) its matrix instructions.  Operands are read DEPTH products
+// ahead: left to itself the compiler reads each right before its use, and a wave
+// then waits for LDS as long again as it computes.
+template <int NA, int DEPTH, int COUNT, typename At, typename Go>
+__device__ __forceinline__ void products(int stride, At at, Go go) {
+  constexpr int kStay = 0;
+  u32x4 a[DEPTH + 1][NA];
+#pragma unroll
+  for (int i = 0; i < DEPTH && i < COUNT; ++i) read_parts<NA>(a[i], at(i), stride, 0);
+#pragma unroll
+  for (int i = 0; i < COUNT; ++i) {
+    if (i + DEPTH < COUNT) read_parts<NA>(a[(i + DEPTH) % (DEPTH + 1)], at(i + DEPTH), stride, 0);
+    __builtin_amdgcn_sched_barrier(kStay);
+    go(i, a[i % (DEPTH + 1)]);
+    __builtin_amdgcn_sched_barrier(kStay);
+  }
 }
 
 __device__ __forceinline__ void store4(float* p, f32x4 v) {
@@ -337,28 +353,40 @@ __device__ __forceinline__ void store4(float* p, f32x4 v) {
   asm volatile("s_nop 1" ::: "memory");
 }
 
-// Memory through buffer descriptors: an offset past the extent reads zeros and
-// drops stores, so rows and columns outside a tensor need no branch, only kOut
-// as their offset (added to by less than 2^31 it stays out).
+// Memory through buffer descriptors: an access past the extent reads zeros and
+// drops stores.  A descriptor of a chunk's rows ends with its last row in use, so
+// rows past it need no test (a row's stride is at least its length: the entry
+// points see to it); a column outside the tensor has kOut as its offset.  The
+// row's offset is added by the scalar operand: one address register for all.
 typedef __amdgpu_buffer_rsrc_t Rsrc;
 constexpr unsigned kOut = 0x80000000u;
-__device__ __forceinline__ Rsrc make_rsrc(const void* base) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, 0x7fffffff, 0x00020000);
+__device__ __forceinline__ Rsrc make_rsrc(const void* base, unsigned extent = 0x7fffffffu) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, (int)extent, 0x00020000);
+}
+// `rows` rows of `cols` elements of T.
+template <typename T>
+__device__ __forceinline__ Rsrc rows_rsrc(const void* base, int64_t stride, int rows, int cols) {
+  return make_rsrc(base, rows > 0 ? ((unsigned)(rows - 1) * (unsigned)stride + cols) * (unsigned)sizeof(T) : 0);
 }
 
+// An element as it comes, in a register of its own, and its value.
 template <typename T>
-__device__ __forceinline__ T load_one(Rsrc r, unsigned at) {
+__device__ __forceinline__ unsigned load_raw(Rsrc r, unsigned at, unsigned row = 0) {
   if constexpr (sizeof(T) == 4)
-    return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0));
+    return __builtin_amdgcn_raw_buffer_load_b32(r, at, row, 0);
   else
-    return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(r, at, 0, 0));
+    return __builtin_amdgcn_raw_buffer_load_b16(r, at, row, 0);
 }
 template <typename T>
-__device__ __forceinline__ void store_one(Rsrc r, unsigned at, float v) {
+__device__ __forceinline__ float raw_value(unsigned v) {
+  return __uint_as_float(sizeof(T) == 4 ? v : v << 16);
+}
+template <typename T>
+__device__ __forceinline__ void store_one(Rsrc r, unsigned at, unsigned row, float v) {
   if constexpr (sizeof(T) == 4)
-    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), r, at, 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), r, at, row, 0);
   else
-    __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, (__bf16)v), r, at, 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, (__bf16)v), r, at, row, 0);
 }
 
 // 64 rows of 32 KS columns of q or k in the registers of NT threads: 4x4 blocks,
@@ -371,29 +399,34 @@ struct Block {
   typedef typename std::conditional<sizeof(T) == 4, f32x4, bf16x4>::type Quad;
   Quad v[kBlocks][4];
 
-  // (stride 64 sizeof(T) is below 2^30: the entry points see to it)
-  __device__ __forceinline__ void load(const T* src, int64_t stride, int rows, int cols, bool vec) {
-    const Rsrc rs = make_rsrc(src);
-    const unsigned row_bytes = (unsigned)stride * sizeof(T);
+  __device__ __forceinline__ void load(const T* src, int64_t stride, int rows, int cols, int vec) {
+    const Rsrc rs = rows_rsrc<T>(src, stride, rows, cols);
+    const unsigned es = sizeof(T), row_bytes = (unsigned)stride * es;
 #pragma unroll
     for (int n = 0; n < kBlocks; ++n) {
       const int e = threadIdx.x + n * NT, q = e % kQuads, r = 4 * (e / kQuads);
-      const unsigned at = kAll || e < 16 * kQuads ? r * row_bytes + 4 * q * (unsigned)sizeof(T) : kOut;
-      if (vec) {
+      const unsigned at = (kAll || e < 16 * kQuads) && 4 * q < cols ? r * row_bytes + 4 * q * es : kOut;
+      if (vec == 4) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const unsigned o = r + i < rows && 4 * q < cols ? at + i * row_bytes : kOut;
           if constexpr (sizeof(T) == 4)
-            v[n][i] = __builtin_bit_cast(Quad, __builtin_amdgcn_raw_buffer_load_b128(rs, o, 0, 0));
+            v[n][i] = __builtin_bit_cast(Quad, __builtin_amdgcn_raw_buffer_load_b128(rs, at, i * row_bytes, 0));
           else
-            v[n][i] = __builtin_bit_cast(Quad, __builtin_amdgcn_raw_buffer_load_b64(rs, o, 0, 0));
+            v[n][i] = __builtin_bit_cast(Quad, __builtin_amdgcn_raw_buffer_load_b64(rs, at, i * row_bytes, 0));
         }
+      } else if (sizeof(T) == 2 && vec == 2) {
+        const unsigned at2 = 4 * q + 2 < cols ? at + 2 * es : kOut;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if constexpr (sizeof(T) == 2)
+            v[n][i] = __builtin_bit_cast(Quad, u32x2{__builtin_amdgcn_raw_buffer_load_b32(rs, at, i * row_bytes, 0),
+                                                     __builtin_amdgcn_raw_buffer_load_b32(rs, at2, i * row_bytes, 0)});
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            v[n][i][k] = load_one<T>(rs, r + i < rows && 4 * q + k < cols ? at + i * row_bytes + k * (unsigned)sizeof(T) : kOut);
+            v[n][i][k] = (T)raw_value<T>(load_raw<T>(rs, 4 * q + k < cols ? at + k * es : kOut, i * row_bytes));
       }
     }
   }

@@ -141,7 +141,11 @@ __global__ void __launch_bounds__(64) delta_solve_kernel(const DeltaParams p) {
       u32x4 b[NP];
       read_parts<NP>(b, kk, 64 * LDK, (16 * t + r) * LDK + 32 * s + 8 * g);
 #pragma unroll
-      for (int c = 0; c <= t; ++c) prod<NP, NP>(acc[t][c], kk, 64 * LDK, (16 * c + r) * LDK + 32 * s + 8 * g, b);
+      for (int c = 0; c <= t; ++c) {
+        u32x4 a[NP];
+        read_parts<NP>(a, kk, 64 * LDK, (16 * c + r) * LDK + 32 * s + 8 * g);
+        mul<NP, 2>(acc[t][c], a, b);
+      }
     }
   }
   __syncthreads();
@@ -250,16 +254,14 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaPa
   constexpr int NT = 64 * WAVES, NP = kParts<T>, DK = 32 * KS, LDK = DK + 8, LKT = 72, ST = 2 * KS;
   // Parts of what only the output sees: bf16 outputs need no more than two.
   constexpr int OP = sizeof(T) == 4 ? 3 : 2;
-  // K by rows; K by columns; Q by rows, where two workgroups' LDS holds it, else in
-  // the place of K by columns, which then follows it; Z; P.
-  constexpr int kKt = DK * LKT, kQ = 64 * LDK;
-  constexpr bool kApart = !MAP && 2 * (NP * (kKt + 2 * kQ) + (3 + OP) * kTri) + 4 * kGateFloats <= 80 * 1024;
-  constexpr int kSecond = MAP ? kKt : kApart ? kKt + kQ : kKt > kQ ? kKt : kQ;
-  __shared__ __attribute__((aligned(16))) unsigned short kk[NP][64 * LDK], second[NP][kSecond], zp[3][kTri],
-      pp[MAP ? 1 : OP][MAP ? 8 : kTri];
-  unsigned short* const kt = &second[0][0];
-  unsigned short* const qq = &second[0][kApart ? kKt : 0];
-  __shared__ __attribute__((aligned(16))) float gt[kGateFloats];
+  // By parts: K by rows, K by columns, Q by rows; where two workgroups' LDS does not
+  // hold all three, Q first has the place of K by columns.  Then Z and P.
+  constexpr int kK = 64 * LDK, kKt = DK * LKT;
+  constexpr bool kApart = !MAP && 2 * (NP * (kKt + 2 * kK) + (3 + OP) * kTri) + 8 * kGateFloats <= 80 * 1024;
+  constexpr int kIn = kK + (MAP ? kKt : kApart ? kKt + kK : kKt > kK ? kKt : kK);
+  __shared__ __attribute__((aligned(16))) unsigned short in[NP][kIn], zp[3][kTri], pp[MAP ? 1 : OP][MAP ? 8 : kTri];
+  __shared__ __attribute__((aligned(16))) float gates[2][kGateFloats];
+  unsigned short *const kk = &in[0][0], *const kt = kk + kK, *const qq = kApart ? kt + kKt : kt;
   const int group = blockIdx.x % groups;
   const int64_t id = blockIdx.x / groups;
   const int seg = (int)(id % p.segs), bh = (int)(id / p.segs), b = bh / p.H, h = bh - b * p.H, hk = h / (p.H / p.Hk);
@@ -283,8 +285,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaPa
   if (c0 >= c1 && !fin) return;
   // S: tile t, element i: row 16 t + 4 g + i, column col
   f32x4 S[ST];
-  const float* const from = MAP ? nullptr : p.segs > 1 && n > 0 ? p.x + id * DK * p.dvp : p.init ? p.init + (int64_t)bh * p.dk_ * p.dv_ : nullptr;
   const bool ws = !MAP && p.segs > 1 && n > 0;
+  const float* const from = MAP ? nullptr : ws ? p.x + id * DK * p.dvp : p.init ? p.init + (int64_t)bh * p.dk_ * p.dv_ : nullptr;
   const Rsrc from_rs = make_rsrc(from);
   const unsigned from_ld = 4u * (ws ? p.dvp : p.dv_);
   const bool from_col = from && (ws ? value : in_v);
@@ -296,7 +298,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaPa
       if (MAP)
         S[t][i] = !value && row == col - p.dvp ? 1.0f : 0.0f;
       else
-        S[t][i] = load_one<float>(from_rs, from_col && (ws || row < p.dk_) ? row * from_ld + 4u * col : kOut);
+        S[t][i] = raw_value<float>(load_raw<float>(from_rs, from_col && (ws || row < p.dk_) ? row * from_ld + 4u * col : kOut));
     }
   const T* const kp = row_ptr<T>(p.k, b, 0, hk);
   const T* const qp = row_ptr<T>(p.q, b, 0, hk);
@@ -304,58 +306,61 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaPa
   T* const op = MAP ? nullptr : row_ptr<T>(p.o, b, 0, h);
   const unsigned es = sizeof(T), v_row = (unsigned)p.v.ss * es, o_row = (unsigned)p.o.ss * es;
   const unsigned v_at = in_v ? col * es + 4 * g * v_row : kOut, o_at = in_v ? col * es + 4 * g * o_row : kOut;
-  Block<T, KS, NT> kb, qb;
   constexpr int NZ = (kZFloats / 4 + NT - 1) / NT;
-  f32x4 zr[NZ], br[NZ];   // br: beta of the columns of zr
-  T vr[16];
+  Block<T, KS, NT> kb, qb;
+  f32x4 zr[NZ];
+  unsigned vr[16];
   float gr[2];
   // The next chunk's inputs, each as soon as its registers are free (and left as
   // loaded: a conversion would wait for them here).
   auto rows_of = [&](int c) { return min(kDeltaChunk, tokens - c * kDeltaChunk); };
   auto fetch_k = [&](int c) { kb.load(kp + (int64_t)c * kDeltaChunk * p.k.ss, p.k.ss, rows_of(c), p.dk_, p.vec); };
   auto fetch_v = [&](int c) {
-    const Rsrc rs = make_rsrc(vp + (int64_t)c * kDeltaChunk * p.v.ss);
-    const int rows = rows_of(c);
+    const Rsrc rs = rows_rsrc<T>(vp + (int64_t)c * kDeltaChunk * p.v.ss, p.v.ss, rows_of(c), p.dv_);
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        vr[4 * t + i] = load_one<T>(rs, 16 * t + 4 * g + i < rows ? v_at + (16 * t + i) * v_row : kOut);
+      for (int i = 0; i < 4; ++i) vr[4 * t + i] = load_raw<T>(rs, v_at, (16 * t + i) * v_row);
   };
   auto fetch = [&](int c) {
-    const int64_t t0 = (int64_t)c * kDeltaChunk, chunk = (int64_t)bh * p.N + c;
-    const int rows = rows_of(c);
-    if (!MAP) qb.load(qp + t0 * p.q.ss, p.q.ss, rows, p.dk_, p.vec);
+    const int64_t chunk = (int64_t)bh * p.N + c;
+    if (!MAP) qb.load(qp + (int64_t)c * kDeltaChunk * p.q.ss, p.q.ss, rows_of(c), p.dk_, p.vec);
 #pragma unroll
-    for (int e = 0; e < NZ; ++e) {
-      const int quad = min(tid + e * NT, kZFloats / 4 - 1);
-      zr[e] = load4(p.z + chunk * kZFloats + 4 * quad);
-      br[e] = load4(p.gates + chunk * kGateFloats + kBeta + 4 * z_quad(quad));
-    }
+    for (int e = 0; e < NZ; ++e) zr[e] = load4(p.z + chunk * kZFloats + 4 * min(tid + e * NT, kZFloats / 4 - 1));
 #pragma unroll
     for (int e = 0; e < 2; ++e) gr[e] = p.gates[chunk * kGateFloats + min(tid + e * NT, kGateFloats - 1)];
+  };
+  auto put_gates = [&](int c) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (tid + e * NT < kGateFloats) gates[c & 1][tid + e * NT] = gr[e];
   };
   if (c0 < c1) {
     fetch_k(c0);
     fetch(c0);
     fetch_v(c0);
+    put_gates(c0);
+    // P's zeros beside the diagonal tiles that begin a pair
+    if (!MAP)
+      for (int e = tid; e < 32 * OP * 4; e += NT) {
+        const int row = (e & 31) < 16 ? (e & 31) : 16 + (e & 31), k = (e >> 5) % OP, q = 4 * (row >> 5 << 1) + 4 + (e >> 5) / OP;
+        *reinterpret_cast<u32x2*>(&pp[MAP ? 0 : k][tri_at(row) + place4(q)]) = u32x2{0, 0};
+      }
   }
   for (int c = c0; c < c1; ++c) {
     const int64_t t0 = (int64_t)c * kDeltaChunk;
-    __syncthreads();   // the chunk before has been read
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-      if (tid + e * NT < kGateFloats) gt[tid + e * NT] = gr[e];
-    kb.template put_rows<LDK>(&kk[0][0], 64 * LDK);
-    if (MAP || kApart) kb.template put_columns<LKT>(kt, kSecond);
-    if (!MAP) qb.template put_rows<LDK>(qq, kSecond);
-    // Z beta
+    const float* const gt = gates[c & 1];
+    __syncthreads();   // the chunk before has been read, this one's gates are there
+    kb.template put_rows<LDK>(kk, kIn);
+    if (MAP || kApart) kb.template put_columns<LKT>(kt, kIn);
+    if (!MAP) qb.template put_rows<LDK>(qq, kIn);
+    // -Z beta
 #pragma unroll
     for (int e = 0; e < NZ; ++e) {
       const int quad = tid + e * NT;
       if (quad < kZFloats / 4) {
         u32x2 part[3];
-        split4<3>(part, zr[e] * br[e]);
+        split4<3>(part, -zr[e] * load4(gt + kBeta + 4 * z_quad(quad)));
 #pragma unroll
         for (int k = 0; k < 3; ++k) *reinterpret_cast<u32x2*>(&zp[k][tri_at(z_row(quad)) + place4(z_quad(quad))]) = part[k];
       }
@@ -364,6 +369,35 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaPa
     if (c + 1 < c1) {
       fetch(c + 1);
       if (MAP || kApart) fetch_k(c + 1);
+    }
+    if (!MAP) {
+      // P, ten 16x16 tiles: four columns of one row a lane, from K Q^T
+#pragma unroll
+      for (int e = 0; e < (9 + WAVES) / WAVES; ++e) {
+        const int tile = wave + WAVES * e;
+        if (tile < 10) {
+          const int tr = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, tc = tile - tr * (tr + 1) / 2, i = 16 * tr + r;
+          f32x4 acc = zero4();
+          u32x4 kf[KS][NP], qf[KS][NP];
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            read_parts<NP>(kf[s], kk, kIn, (16 * tc + r) * LDK + 32 * s + 8 * g);
+            read_parts<NP>(qf[s], qq, kIn, i * LDK + 32 * s + 8 * g);
+          }
+#pragma unroll
+          for (int s = 0; s < KS; ++s) mul<NP, 2>(acc, kf[s], qf[s]);
+          const f32x4 hi = load4(gt + kHi + 16 * tc + 4 * g), lo = load4(gt + kLo + 16 * tc + 4 * g);
+          const float hi_i = gt[kHi + i], lo_i = gt[kLo + i];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            acc[k] = i >= 16 * tc + 4 * g + k ? acc[k] * __builtin_amdgcn_exp2f((hi_i - hi[k]) + (lo_i - lo[k])) : 0.0f;
+          u32x2 part[OP];
+          split4<OP>(part, acc);
+#pragma unroll
+          for (int k = 0; k < OP; ++k)
+            *reinterpret_cast<u32x2*>(&pp[MAP ? 0 : k][tri_at(i) + 32 * (tc >> 1) + 8 * g + 4 * (tc & 1)]) = part[k];
+        }
+      }
     }
     f32x4 x[4], o[4];
     if (live) {
@@ -380,90 +414,62 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaPa
       for (int s = 0; s < KS; ++s) {
         u32x4 sp[3];
         split_pair<3>(sp, S[2 * s], S[2 * s + 1]);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const int at = (16 * t + r) * LDK + 32 * s + 8 * g;
-          prod<NP, 3>(x[t], &kk[0][0], 64 * LDK, at, sp);
-          if (!MAP) prod<NP, OP, OP - 1>(o[t], qq, kSecond, at, sp);
-        }
+        products<NP, (NP == 1 ? 3 : 1), (MAP ? 4 : 8)>(
+            kIn, [&](int i) { return (i < 4 ? kk : qq) + (16 * (i & 3) + r) * LDK + 32 * s + 8 * g; },
+            [&](int i, const u32x4(&a)[NP]) {
+              if (i < 4)
+                mul<3, 2>(x[i & 3], a, sp);
+              else
+                mul<OP, OP - 1>(o[i & 3], a, sp);
+            });
       }
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const f32x4 gam = load4(gt + kGam + 16 * t + 4 * g);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[t][i] = (float)vr[4 * t + i] - gam[i] * x[t][i];
+        for (int i = 0; i < 4; ++i) x[t][i] = raw_value<T>(vr[4 * t + i]) - gam[i] * x[t][i];
       }
     }
     if (c + 1 < c1) fetch_v(c + 1);
     if (!MAP) {
-      // P: four of its columns of one row a lane, from K Q^T; WAVES / 4 waves a
-      // tile row
-      const int tr = wave & 3, i = 16 * tr + r;
-      for (int tc = wave >> 2; tc <= tr; tc += WAVES / 4) {
-        f32x4 acc = zero4();
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          u32x4 qf[NP];
-          read_parts<NP>(qf, qq, kSecond, i * LDK + 32 * s + 8 * g);
-          prod<NP, NP>(acc, &kk[0][0], 64 * LDK, (16 * tc + r) * LDK + 32 * s + 8 * g, qf);
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int j = 16 * tc + 4 * g + e;
-          acc[e] = i >= j ? acc[e] * decay(gt, i, j) : 0.0f;
-        }
-        u32x2 part[OP];
-        split4<OP>(part, acc);
-#pragma unroll
-        for (int k = 0; k < OP; ++k)
-          *reinterpret_cast<u32x2*>(&pp[MAP ? 0 : k][tri_at(i) + 32 * (tc >> 1) + 8 * g + 4 * (tc & 1)]) = part[k];
-      }
-      // the other half of a pair of tiles whose first is on the diagonal
-      if ((wave >> 2) == 0 && (tr & 1) == 0)
-#pragma unroll
-        for (int k = 0; k < OP; ++k)
-          *reinterpret_cast<u32x2*>(&pp[MAP ? 0 : k][tri_at(i) + 32 * (tr >> 1) + 8 * g + 4]) = u32x2{0, 0};
       __syncthreads();   // P is there, Q has been read
       if (!kApart) {
-        kb.template put_columns<LKT>(kt, kSecond);
+        kb.template put_columns<LKT>(kt, kIn);
         if (c + 1 < c1) fetch_k(c + 1);
       }
     }
     if (live) {
-      f32x4 y[4];
+      // Y, on X's registers: the parts of X are taken first
+      u32x4 xp[2][3];
+      split_pair<3>(xp[0], x[0], x[1]);
+      split_pair<3>(xp[1], x[2], x[3]);
+      // tiles (t, s): (0, 0) .. (3, 0), (2, 1), (3, 1)
+      products<3, 1, 6>(
+          kTri, [&](int i) { return &zp[0][0] + tri_at(16 * (i < 4 ? i : i - 2) + r) + 32 * (i >> 2) + 8 * g; },
+          [&](int i, const u32x4(&a)[3]) { mul<3, 2>(x[i < 4 ? i : i - 2], a, xp[i >> 2]); });
 #pragma unroll
-      for (int t = 0; t < 4; ++t) y[t] = zero4();
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        u32x4 xp[3];
-        split_pair<3>(xp, x[2 * s], x[2 * s + 1]);
-#pragma unroll
-        for (int t = 2 * s; t < 4; ++t) prod<3, 3>(y[t], &zp[0][0], kTri, tri_at(16 * t + r) + 32 * s + 8 * g, xp);
-      }
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const f32x4 beta = load4(gt + kBeta + 16 * t + 4 * g);
-        x[t] = beta * (x[t] - y[t]);   // U
-      }
+      for (int t = 0; t < 4; ++t) x[t] *= load4(gt + kBeta + 16 * t + 4 * g);   // U
       if (!MAP) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) o[t] *= load4(gt + kGam + 16 * t + 4 * g);
+        u32x4 up[2][OP];
+        split_pair<OP>(up[0], x[0], x[1]);
+        split_pair<OP>(up[1], x[2], x[3]);
+        products<OP, 1, 6>(
+            kTri, [&](int i) { return &pp[0][0] + tri_at(16 * (i < 4 ? i : i - 2) + r) + 32 * (i >> 2) + 8 * g; },
+            [&](int i, const u32x4(&a)[OP]) { mul<OP, OP - 1>(o[i < 4 ? i : i - 2], a, up[i >> 2]); });
+        const int rows = tokens - (int)t0;
+        if (rows < kDeltaChunk)   // zeros past the tokens in use
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          u32x4 up[OP];
-          split_pair<OP>(up, x[2 * s], x[2 * s + 1]);
+          for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int t = 2 * s; t < 4; ++t) prod<OP, OP, OP - 1>(o[t], &pp[0][0], kTri, tri_at(16 * t + r) + 32 * s + 8 * g, up);
-        }
-        const int rows = tokens - (int)t0, all = p.S - (int)t0;
-        const Rsrc o_rs = make_rsrc(op + t0 * p.o.ss);
+            for (int i = 0; i < 4; ++i)
+              if (16 * t + 4 * g + i >= rows) o[t][i] = 0.0f;
+        const Rsrc o_rs = rows_rsrc<T>(op + t0 * p.o.ss, p.o.ss, min(kDeltaChunk, p.S - (int)t0), p.dv_);
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = 16 * t + 4 * g + i;
-            store_one<T>(o_rs, row < all ? o_at + (16 * t + i) * o_row : kOut, row < rows ? p.scale * o[t][i] : 0.0f);
-          }
+          for (int i = 0; i < 4; ++i) store_one<T>(o_rs, o_at, (16 * t + i) * o_row, p.scale * o[t][i]);
       }
     }
     if (!MAP && !kApart) __syncthreads();   // K by columns is there
@@ -471,14 +477,15 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaPa
       const float last = gt[kGam + 63];
 #pragma unroll
       for (int t = 0; t < ST; ++t) S[t] *= last;
+      u32x4 up[2][3];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        u32x4 up[3];
-        split_pair<3>(up, x[2 * s] * load4(gt + kEnd + 32 * s + 4 * g), x[2 * s + 1] * load4(gt + kEnd + 32 * s + 16 + 4 * g));
-#pragma unroll
-        for (int t = 0; t < ST; ++t) prod<NP, 3>(S[t], kt, kSecond, (16 * t + r) * LKT + 32 * s + 8 * g, up);
-      }
+      for (int s = 0; s < 2; ++s)
+        split_pair<3>(up[s], x[2 * s] * load4(gt + kEnd + 32 * s + 4 * g), x[2 * s + 1] * load4(gt + kEnd + 32 * s + 16 + 4 * g));
+      products<NP, (NP == 1 ? 3 : 1), 2 * ST>(
+          kIn, [&](int i) { return kt + (16 * (i % ST) + r) * LKT + 32 * (i / ST) + 8 * g; },
+          [&](int i, const u32x4(&a)[NP]) { mul<3, 2>(S[i % ST], a, up[i / ST]); });
     }
+    if (c + 1 < c1) put_gates(c + 1);
   }
   if (MAP && live) {
     float* const dst = value ? p.x + id * DK * p.dvp + col : p.a + id * DK * DK + (col - p.dvp);

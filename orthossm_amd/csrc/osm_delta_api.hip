@@ -45,6 +45,15 @@ int check_rows(const osm_rows& r, int esize, const char* name) {
   return OSM_OK;
 }
 
+// Rows of d elements over S tokens: a chunk's rows are told from those past it by
+// their offset.
+int check_tokens(const osm_rows& r, int esize, int64_t S, int64_t d, const char* name) {
+  const int rc = check_rows(r, esize, name);
+  if (rc == OSM_OK && S > 1 && r.stride_s < d)
+    return fail(OSM_E_LAYOUT, "%s: %lld elements from token to token, rows of %lld overlap", name, (long long)r.stride_s, (long long)d);
+  return rc;
+}
+
 int check_state(const void* p, const char* name) {
   return (uintptr_t)p % 4 ? fail(OSM_E_LAYOUT, "%s must be 4-byte aligned", name) : OSM_OK;
 }
@@ -85,8 +94,8 @@ Sizes sizes_of(const osm_delta_args* a) {
 
 DeltaRows rows_of(const osm_rows& r) { return {r.p, r.stride_b, r.stride_s, r.stride_h}; }
 
-bool quads(const osm_rows& r, int esize) {
-  return (uintptr_t)r.p % (4 * esize) == 0 && r.stride_b % 4 == 0 && r.stride_s % 4 == 0 && r.stride_h % 4 == 0;
+bool whole(const osm_rows& r, int esize, int n) {
+  return (uintptr_t)r.p % (n * esize) == 0 && r.stride_b % n == 0 && r.stride_s % n == 0 && r.stride_h % n == 0;
 }
 
 int check_inputs(const osm_delta_args* a) {
@@ -94,8 +103,8 @@ int check_inputs(const osm_delta_args* a) {
   if (rc != OSM_OK) return rc;
   const int es = a->dtype == OSM_F32 ? 4 : 2;
   if (a->B > 0 && a->S > 0) {
-    if ((rc = check_rows(a->q, es, "q")) != OSM_OK || (rc = check_rows(a->k, es, "k")) != OSM_OK ||
-        (rc = check_rows(a->v, es, "v")) != OSM_OK || (rc = check_rows(a->g, 4, "g")) != OSM_OK ||
+    if ((rc = check_tokens(a->q, es, a->S, a->dk, "q")) != OSM_OK || (rc = check_tokens(a->k, es, a->S, a->dk, "k")) != OSM_OK ||
+        (rc = check_tokens(a->v, es, a->S, a->dv, "v")) != OSM_OK || (rc = check_rows(a->g, 4, "g")) != OSM_OK ||
         (rc = check_rows(a->beta, 4, "beta")) != OSM_OK)
       return rc;
     if ((uintptr_t)a->lengths % 4) return fail(OSM_E_LAYOUT, "lengths must be 4-byte aligned");
@@ -135,7 +144,9 @@ DeltaParams params_of(const osm_delta_args* a) {
   p.segs = (p.N + p.seg - 1) / p.seg;
   p.scale = a->scale;
   const int es = a->dtype == OSM_F32 ? 4 : 2;
-  p.vec = a->dk % 4 == 0 && a->dv % 4 == 0 && quads(a->q, es) && quads(a->k, es) && quads(a->v, es);
+  for (p.vec = 4; p.vec > 1; p.vec /= 2)
+    if (a->dk % p.vec == 0 && a->dv % p.vec == 0 && whole(a->q, es, p.vec) && whole(a->k, es, p.vec) && whole(a->v, es, p.vec))
+      break;
   return p;
 }
 
@@ -169,7 +180,7 @@ int osm_delta_fwd(const osm_delta_args* a, void* workspace, size_t workspace_byt
     return rc;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (a->B == 0 || a->S == 0) return copy_state(a->state_init, a->state_out, (size_t)a->B * a->H * a->dk * a->dv, st);
-  if ((rc = check_rows(a->out, a->dtype == OSM_F32 ? 4 : 2, "out")) != OSM_OK) return rc;
+  if ((rc = check_tokens(a->out, a->dtype == OSM_F32 ? 4 : 2, a->S, a->dv, "out")) != OSM_OK) return rc;
   DeltaParams p = params_of(a);
   p.o = rows_of(a->out);
   hipError_t e;
@@ -224,8 +235,8 @@ int osm_delta_bwd(const osm_delta_args* a, const osm_delta_bwd_args* b, void* wo
   if (a->B == 0 || a->S == 0) return copy_state(b->grad_state, b->grad_init, (size_t)a->B * a->H * a->dk * a->dv, st);
   if (!a->saved) return fail(OSM_E_ARG, "saved is NULL");
   const int es = a->dtype == OSM_F32 ? 4 : 2;
-  if ((rc = check_rows(b->grad_out, es, "grad_out")) != OSM_OK || (rc = check_rows(b->grad_q, es, "grad_q")) != OSM_OK ||
-      (rc = check_rows(b->grad_k, es, "grad_k")) != OSM_OK || (rc = check_rows(b->grad_v, es, "grad_v")) != OSM_OK ||
+  if ((rc = check_tokens(b->grad_out, es, a->S, a->dv, "grad_out")) != OSM_OK || (rc = check_tokens(b->grad_q, es, a->S, a->dk, "grad_q")) != OSM_OK ||
+      (rc = check_tokens(b->grad_k, es, a->S, a->dk, "grad_k")) != OSM_OK || (rc = check_tokens(b->grad_v, es, a->S, a->dv, "grad_v")) != OSM_OK ||
       (rc = check_rows(b->grad_g, 4, "grad_g")) != OSM_OK || (rc = check_rows(b->grad_beta, 4, "grad_beta")) != OSM_OK)
     return rc;
   if ((rc = check_workspace(workspace, workspace_bytes, osm_delta_bwd_workspace_bytes(a))) != OSM_OK) return rc;
@@ -236,7 +247,7 @@ int osm_delta_bwd(const osm_delta_args* a, const osm_delta_bwd_args* b, void* wo
   p.s = p.gates + n.gates;
   p.a = static_cast<float*>(workspace);
   p.d = p.a + n.a;
-  p.vec = p.vec && quads(b->grad_out, es);
+  if (!whole(b->grad_out, es, p.vec)) p.vec = 1;
   p.dout = rows_of(b->grad_out);
   p.dq = rows_of(b->grad_q);
   p.dk = rows_of(b->grad_k);

@@ -38,8 +38,8 @@ __device__ __forceinline__ void scores(f32x4 (&qk)[CT], f32x4 (&kk)[CT], float* 
   for (int kb = 0; kb < p.dkp; kb += 64) {
     const int kw = min(64, p.dkp - kb);
     if (kb) __syncthreads();
-    load_tile<NT>(ks, k + kb, p.k.ss, rows, p.dk_ - kb, kw, p.vec);
-    load_tile<NT>(qs, q + kb, p.q.ss, rows, p.dk_ - kb, kw, p.vec);
+    load_tile<NT>(ks, k + kb, p.k.ss, rows, p.dk_ - kb, kw, p.vec == 4);
+    load_tile<NT>(qs, q + kb, p.q.ss, rows, p.dk_ - kb, kw, p.vec == 4);
     __syncthreads();
     mma<CT, false, true>(qk, qs, r0, ks, c0, 0, kw);
     if (KK) mma<CT, false, true>(kk, ks, r0, ks, c0, 0, kw);
@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(kThreads) delta_adjoint_kernel(const DeltaPara
   for (int cb = 0; cb < nkb; ++cb) {
     const int cw = min(64, p.dkp - 64 * cb);
     __syncthreads();
-    if (nkb > 1) load_tile<kThreads>(ks, k + 64 * cb, p.k.ss, w.rows, p.dk_ - 64 * cb, cw, p.vec);
+    if (nkb > 1) load_tile<kThreads>(ks, k + 64 * cb, p.k.ss, w.rows, p.dk_ - 64 * cb, cw, p.vec == 4);
     __syncthreads();
     // W and, scaled to the chunk's end, its product with K: columns cb of Kt^T W,
     // so rows cb of A^T.
@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(kThreads) delta_adjoint_kernel(const DeltaPara
       const int rw = min(64, p.dkp - 64 * rb);
       if (nkb > 1) {
         __syncthreads();
-        load_tile<kThreads>(ks, k + 64 * rb, p.k.ss, w.rows, p.dk_ - 64 * rb, rw, p.vec);
+        load_tile<kThreads>(ks, k + 64 * rb, p.k.ss, w.rows, p.dk_ - 64 * rb, rw, p.vec == 4);
         __syncthreads();
       }
       if (r0 < cw) {
@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(kThreads) delta_adjoint_kernel(const DeltaPara
     for (int vb = 0; vb < p.dvp; vb += 64) {
       const int vw = min(64, p.dvp - vb);
       __syncthreads();
-      load_tile<kThreads>(ks, go + vb, p.dout.ss, w.rows, p.dv_ - vb, vw, p.vec);
+      load_tile<kThreads>(ks, go + vb, p.dout.ss, w.rows, p.dv_ - vb, vw, p.vec == 4);
       __syncthreads();
       if (r0 < cw) {
         clear(acc);
@@ -224,13 +224,13 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const DeltaPa
   for (int vb = 0; vb < p.dvp; vb += 64) {
     const int vw = min(64, p.dvp - vb);
     __syncthreads();
-    load_tile<kGradThreads>(os, go + vb, p.dout.ss, w.rows, p.dv_ - vb, 64, p.vec);
+    load_tile<kGradThreads>(os, go + vb, p.dout.ss, w.rows, p.dv_ - vb, 64, p.vec == 4);
     clear(x);
     clear(y);
 #pragma unroll
     for (int b = 0; b < NKB; ++b) {
       if (b) __syncthreads();
-      if (NKB > 1) load_tile<kGradThreads>(ks, k + 64 * b, p.k.ss, w.rows, p.dk_ - 64 * b, width(b), p.vec);
+      if (NKB > 1) load_tile<kGradThreads>(ks, k + 64 * b, p.k.ss, w.rows, p.dk_ - 64 * b, width(b), p.vec == 4);
       load_ws<kGradThreads>(ss, sg + (int64_t)64 * b * p.dvp + vb, p.dvp, width(b), vw);
       load_ws<kGradThreads>(ds, dg + (int64_t)64 * b * p.dvp + vb, p.dvp, width(b), vw);
       __syncthreads();
@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const DeltaPa
     for (int b = 0; b < NKB; ++b) {
       if (NKB > 1) {
         __syncthreads();
-        load_tile<kGradThreads>(ks, k + 64 * b, p.k.ss, w.rows, p.dk_ - 64 * b, width(b), p.vec);
+        load_tile<kGradThreads>(ks, k + 64 * b, p.k.ss, w.rows, p.dk_ - 64 * b, width(b), p.vec == 4);
         load_ws<kGradThreads>(ss, sg + (int64_t)64 * b * p.dvp + vb, p.dvp, width(b), vw);
         load_ws<kGradThreads>(ds, dg + (int64_t)64 * b * p.dvp + vb, p.dvp, width(b), vw);
         __syncthreads();
@@ -347,8 +347,8 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const DeltaPa
   for (int b = 0; b < NKB; ++b) {
     if (NKB > 1) {
       if (b) __syncthreads();
-      load_tile<kGradThreads>(ks, k + 64 * b, p.k.ss, w.rows, p.dk_ - 64 * b, width(b), p.vec);
-      load_tile<kGradThreads>(qs, q + 64 * b, p.q.ss, w.rows, p.dk_ - 64 * b, width(b), p.vec);
+      load_tile<kGradThreads>(ks, k + 64 * b, p.k.ss, w.rows, p.dk_ - 64 * b, width(b), p.vec == 4);
+      load_tile<kGradThreads>(qs, q + 64 * b, p.q.ss, w.rows, p.dk_ - 64 * b, width(b), p.vec == 4);
       __syncthreads();
     }
 #pragma unroll

@@ -45,7 +45,7 @@ def _set_rows(r: nat.Rows, t: torch.Tensor) -> None:
 
 
 def _unit_rows(t: torch.Tensor) -> torch.Tensor:
-    near = t.dim() < 4 or t.stride(1) <= nat.DELTA_MAX_STRIDE
+    near = t.dim() < 4 or t.shape[1] <= 1 or t.shape[3] <= t.stride(1) <= nat.DELTA_MAX_STRIDE
     return t if near and (t.stride(-1) == 1 or t.shape[-1] == 1) else t.contiguous()
 
 

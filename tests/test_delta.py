@@ -118,10 +118,13 @@ def test_backward_errors():
     assert bwd(_args(), b) == -1                            # nothing saved
     assert bwd(_args(saved=0x10000), b) == -1               # no grad_out
     for name in ("grad_out", "grad_q", "grad_k", "grad_v", "grad_g", "grad_beta"):
-        getattr(b, name).p = 0x10000
+        getattr(b, name).p, getattr(b, name).stride_s = 0x10000, 320
     assert bwd(_args(saved=0x10000), b) == -5
     b.grad_init = 0x10002
     assert bwd(_args(saved=0x10000), b) == -4
+    b.grad_init, b.grad_q.stride_s = None, 47               # rows of 48 overlap
+    assert bwd(_args(saved=0x10000), b) == -4
+    assert _fwd(_args(v=nat.Rows(0x10000, 200 * 320, 79, 80))) == -4
 
 
 def test_step_errors():
