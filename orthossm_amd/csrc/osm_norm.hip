@@ -23,35 +23,29 @@
 namespace osm {
 namespace {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-
 template <typename T>
 constexpr int kUnit = 16 / (int)sizeof(T);   // elements of a 16-byte access
 
+// 16 bytes of a row as loaded, and their values.
 template <typename T>
-__device__ __forceinline__ void load_unit(float (&v)[kUnit<T>], const T* p) {
-  if constexpr (sizeof(T) == 4) {
-    const f32x4 q = *reinterpret_cast<const f32x4*>(p);
+struct Unit {
+  typedef T Vec __attribute__((ext_vector_type(kUnit<T>)));
+  Vec raw;
+  __device__ __forceinline__ void get(float (&v)[kUnit<T>]) const {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = q[i];
-  } else {
-    const bf16x8 q = *reinterpret_cast<const bf16x8*>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (float)q[i];
+    for (int i = 0; i < kUnit<T>; ++i) v[i] = (float)raw[i];
   }
-}
+};
 
 template <typename T>
 __device__ __forceinline__ void store_unit(T* p, const float (&v)[kUnit<T>]) {
-  if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
-  } else {
-    bf16x8 q;
+  typename Unit<T>::Vec q;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = (__bf16)v[i];
-    *reinterpret_cast<bf16x8*>(p) = q;
-  }
+  for (int i = 0; i < kUnit<T>; ++i) q[i] = (T)v[i];
+  __builtin_nontemporal_store(q, reinterpret_cast<typename Unit<T>::Vec*>(p));
+  // two wait states before anything may overwrite the store's registers (a
+  // store wider than 64 bits was seen to lose its first word otherwise)
+  asm volatile("s_nop 1" ::: "memory");
 }
 
 // A row's units u, u + TPR, .. of a thread; past the row's end: zeros, and no
@@ -59,23 +53,29 @@ __device__ __forceinline__ void store_unit(T* p, const float (&v)[kUnit<T>]) {
 template <typename T, int TPR, int NV>
 struct Row {
   static constexpr int U = kUnit<T>;
-  static __device__ __forceinline__ void load(float (&v)[NV][U], const T* p, int D, int u, bool vec) {
+  // As loaded, so that the next row can be on its way while this one is worked on.
+  struct Raw {
+    Unit<T> n[NV];
+    __device__ __forceinline__ void load(const T* p, int D, int u, bool vec) {
 #pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      const int c = (u + n * TPR) * U;
-      if (vec) {
-        if (c < D) {
-          load_unit<T>(v[n], p + c);
+      for (int k = 0; k < NV; ++k) {
+        const int c = (u + k * TPR) * U;
+        typename Unit<T>::Vec v = {};
+        if (vec) {
+          if (c < D) v = __builtin_nontemporal_load(reinterpret_cast<const typename Unit<T>::Vec*>(p + c));
         } else {
 #pragma unroll
-          for (int i = 0; i < U; ++i) v[n][i] = 0.0f;
+          for (int i = 0; i < U; ++i)
+            if (c + i < D) v[i] = p[c + i];
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < U; ++i) v[n][i] = c + i < D ? (float)p[c + i] : 0.0f;
+        n[k].raw = v;
       }
     }
-  }
+    __device__ __forceinline__ void get(float (&v)[NV][U]) const {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) n[k].get(v[k]);
+    }
+  };
   static __device__ __forceinline__ void store(T* p, const float (&v)[NV][U], int D, int u, bool vec) {
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
@@ -101,14 +101,30 @@ struct Row {
   }
 };
 
+// v plus its value in another lane of the 16: quads' pairs, halves, mirrors.
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float lane_of(float v, int l) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
+}
+// The sum over a wave, in every lane: within 16 lanes by DPP, then four scalars
+// (a shuffle through LDS a step takes five times as long).
+__device__ __forceinline__ float wave_total(float v) {
+  v = dpp_add<0xb1>(v);    // quad_perm 1 0 3 2
+  v = dpp_add<0x4e>(v);    // quad_perm 2 3 0 1
+  v = dpp_add<0x141>(v);   // row_half_mirror
+  v = dpp_add<0x140>(v);   // row_mirror
+  return (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
+}
+
 // Sums over the TPR threads of a row, in every one of them.  `red`: one slot a
 // wave and value; the caller's calls alternate its two halves.
 template <int TPR, int K>
 __device__ __forceinline__ void row_sum(float (&v)[K], float (*red)[K]) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1)
-#pragma unroll
-    for (int k = 0; k < K; ++k) v[k] += __shfl_xor(v[k], o);
+  for (int k = 0; k < K; ++k) v[k] = wave_total(v[k]);
   if constexpr (TPR > 64) {
     const int wave = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 0)
@@ -135,8 +151,13 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) layer_norm_fwd_kernel(c
   R::param(w, p.weight, 1.0f, p.D, u);
   R::param(b, p.bias, 0.0f, p.D, u);
   // (every thread of a workgroup runs the same trips: kRows is 1 where row_sum has barriers)
-  for (int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR; row < p.rows; row += (int64_t)gridDim.x * kRows) {
-    R::load(x, static_cast<const T*>(p.x) + row * p.x_stride, p.D, u, p.vec);
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
+  typename R::Raw next;
+  if (row < p.rows) next.load(static_cast<const T*>(p.x) + row * p.x_stride, p.D, u, p.vec);
+  for (; row < p.rows; row += step) {
+    next.get(x);
+    if (row + step < p.rows) next.load(static_cast<const T*>(p.x) + (row + step) * p.x_stride, p.D, u, p.vec);
     float s[1] = {0.0f};
 #pragma unroll
     for (int n = 0; n < NV; ++n)
@@ -179,10 +200,22 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) layer_norm_bwd_kernel(c
 #pragma unroll
     for (int i = 0; i < U; ++i) dw[n][i] = db[n][i] = 0.0f;
   int par = 0;
-  for (int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR; row < p.rows; row += (int64_t)gridDim.x * kRows) {
-    R::load(x, static_cast<const T*>(p.x) + row * p.x_stride, p.D, u, p.vec);
-    R::load(g, static_cast<const T*>(p.gy) + row * p.gy_stride, p.D, u, p.vec);
-    const float mean = p.mean[row], rstd = p.rstd[row];
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
+  typename R::Raw next_x, next_g;
+  float next_mean = 0.0f, next_rstd = 0.0f;
+  auto fetch = [&](int64_t at) {
+    next_x.load(static_cast<const T*>(p.x) + at * p.x_stride, p.D, u, p.vec);
+    next_g.load(static_cast<const T*>(p.gy) + at * p.gy_stride, p.D, u, p.vec);
+    next_mean = p.mean[at];
+    next_rstd = p.rstd[at];
+  };
+  if (row < p.rows) fetch(row);
+  for (; row < p.rows; row += step) {
+    next_x.get(x);
+    next_g.get(g);
+    const float mean = next_mean, rstd = next_rstd;
+    if (row + step < p.rows) fetch(row + step);
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int n = 0; n < NV; ++n)
@@ -342,19 +375,19 @@ __global__ void __launch_bounds__(kFoldCols * kFoldGroups) layer_norm_fold_kerne
   }
 }
 
-// Calls go(TPR, NV) for the fewest threads that hold a row in 16 registers
-// each, or long_rows() past 16384 elements.
-template <typename T, typename Go, typename Long>
+// Calls go(TPR, NV) for the fewest threads that hold a row, 16 elements each (LAST
+// in the case of 1024 threads: the backward holds five rows' worth, and spills
+// with 16), or long_rows() past 1024 LAST elements.
+template <typename T, int LAST, typename Go, typename Long>
 void by_length(int64_t D, Go go, Long long_rows) {
   const int64_t units = (D + kUnit<T> - 1) / kUnit<T>;
-  constexpr int most = 16 / kUnit<T>;
   auto pick = [&](auto tpr) {
-    constexpr int TPR = decltype(tpr)::value;
+    constexpr int TPR = decltype(tpr)::value, most = (TPR == 1024 ? LAST : 16) / kUnit<T>;
     if (units > most * TPR) return false;
     if (units <= TPR)
       go(tpr, std::integral_constant<int, 1>{});
-    else if (units <= 2 * TPR)
-      go(tpr, std::integral_constant<int, 2>{});
+    else if (most == 2 || units <= 2 * TPR)
+      go(tpr, std::integral_constant<int, most == 1 ? 1 : 2>{});
     else
       go(tpr, std::integral_constant<int, most>{});
     return true;
@@ -368,12 +401,12 @@ constexpr int kMaxGroups = 2048;
 
 template <typename T>
 hipError_t forward(const NormParams& p, hipStream_t stream) {
-  by_length<T>(
+  by_length<T, 16>(
       p.D,
       [&](auto tpr, auto nv) {
         constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, kThreads = TPR > 256 ? TPR : 256;
         const int64_t groups = (p.rows + kThreads / TPR - 1) / (kThreads / TPR);
-        hipLaunchKernelGGL((layer_norm_fwd_kernel<T, TPR, NV>), dim3((unsigned)std::min<int64_t>(groups, 8 * kMaxGroups)),
+        hipLaunchKernelGGL((layer_norm_fwd_kernel<T, TPR, NV>), dim3((unsigned)std::min<int64_t>(groups, kMaxGroups)),
                            dim3(kThreads), 0, stream, p);
       },
       [&] {
@@ -387,7 +420,7 @@ template <typename T>
 hipError_t backward(const NormParams& p, float* dw, float* db, hipStream_t stream) {
   const int lines = norm_lines(p.rows, p.D);
   hipError_t e = hipSuccess;
-  by_length<T>(
+  by_length<T, 8>(
       p.D,
       [&](auto tpr, auto nv) {
         constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, kThreads = TPR > 256 ? TPR : 256;
