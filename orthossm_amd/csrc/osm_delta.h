@@ -30,7 +30,7 @@ struct DeltaParams {
   float* z;                          // [B,H,N][kZFloats]
   float* gates;                      // [B,H,N][kGateFloats]
   float* s;                          // [B,H,N][dkp][dvp] states before the chunks, or NULL
-  float* a;                          // maps of the segments [B,H,segs][dkp][dkp] (backward: of the chunks)
+  float* a;                          // maps of the segments [B,H,segs][dkp][dkp]
   float* x;                          // and what they add, then the states before them [B,H,segs][dkp][dvp]
   // the backward's
   DeltaRows dout, dq, dk, dv, dg, dbeta;
@@ -502,6 +502,12 @@ __device__ __forceinline__ void make_gates(float* gt, const DeltaRows& g, const 
 __device__ __forceinline__ float decay(const float* gt, int i, int j) {
   return __builtin_amdgcn_exp2f((gt[kHi + i] - gt[kHi + j]) + (gt[kLo + i] - gt[kLo + j]));
 }
+
+// Rows 0-31 of a lower triangular matrix of the walk have 32 columns, the others
+// 64 (plus 8 of padding: 16-byte reads of eight consecutive rows touch every bank
+// once).
+constexpr int kTri = 32 * 40 + 32 * 72;
+__device__ __forceinline__ int tri_at(int row) { return row < 32 ? row * 40 : 1280 + (row - 32) * 72; }
 
 // (b, h, chunk, tokens in use) of a workgroup's chunk.
 struct At {

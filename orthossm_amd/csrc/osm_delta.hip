@@ -240,12 +240,6 @@ __global__ void __launch_bounds__(64 * KT) delta_scan_kernel(const float* a, flo
       if (row + i < dk && col < dv) fin[io + (int64_t)i * dv] = s[i];
 }
 
-// Rows 0-31 of a lower triangular matrix of the walk have 32 columns, the others
-// 64 (plus 8 of padding: 16-byte reads of eight consecutive rows touch every bank
-// once).
-constexpr int kTri = 32 * 40 + 32 * 72;
-__device__ __forceinline__ int tri_at(int row) { return row < 32 ? row * 40 : 1280 + (row - 32) * 72; }
-
 // Walks segment blockIdx.x % segs of a head.  MAP: the segment's state map, from
 // zero for the columns of v and from the identity's columns after them; else the
 // outputs.  KS: blocks of 32 rows of S; WAVES: of 16 columns each.

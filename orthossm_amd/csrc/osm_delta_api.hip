@@ -78,17 +78,17 @@ bool is_short(const osm_delta_args* a) { return !a->saved && a->S <= kShort; }
 int64_t up32(int64_t n) { return (n + 31) / 32 * 32; }
 
 // Floats of the regions of `saved` and the workspaces, each a multiple of 64:
-// per chunk Z, its gates, its start (or, in the backward, end) state and its
-// state map; per segment the map and the state; with shared heads q's and k's
+// per chunk Z, its gates and its start state (in the backward, the gradient to its
+// end state); per segment the map and the state; with shared heads q's and k's
 // gradients by head.
 struct Sizes {
-  size_t z, gates, s, a, seg_a, seg_x, part;
+  size_t z, gates, s, seg_a, seg_x, part;
 };
 Sizes sizes_of(const osm_delta_args* a) {
   const size_t heads = (size_t)a->B * a->H, N = chunks_of(a->S), n = heads * N, dkp = up32(a->dk), dvp = up16(a->dv);
   const size_t seg = N ? osm::delta_segment(heads, N) : 1, segs = (N + seg - 1) / seg;
   const size_t m = segs > 1 ? heads * segs : 0;
-  return {n * osm::kZFloats, n * osm::kGateFloats, n * dkp * dvp, n * dkp * dkp, m * dkp * dkp, m * dkp * dvp,
+  return {n * osm::kZFloats, n * osm::kGateFloats, n * dkp * dvp, m * dkp * dkp, m * dkp * dvp,
           a->H != a->Hk ? (size_t)2 * a->B * a->S * a->H * a->dk : 0};
 }
 
@@ -221,7 +221,7 @@ int osm_delta_fwd(const osm_delta_args* a, void* workspace, size_t workspace_byt
 size_t osm_delta_bwd_workspace_bytes(const osm_delta_args* a) {
   if (check_shape(a) != OSM_OK) return 0;
   const Sizes n = sizes_of(a);
-  return (n.a + n.s + n.part) * sizeof(float);
+  return (n.seg_a + n.seg_x + n.s + n.part) * sizeof(float);
 }
 
 int osm_delta_bwd(const osm_delta_args* a, const osm_delta_bwd_args* b, void* workspace, size_t workspace_bytes,
@@ -246,7 +246,8 @@ int osm_delta_bwd(const osm_delta_args* a, const osm_delta_bwd_args* b, void* wo
   p.gates = p.z + n.z;
   p.s = p.gates + n.gates;
   p.a = static_cast<float*>(workspace);
-  p.d = p.a + n.a;
+  p.x = p.a + n.seg_a;
+  p.d = p.x + n.seg_x;
   if (!whole(b->grad_out, es, p.vec)) p.vec = 1;
   p.dout = rows_of(b->grad_out);
   p.dq = rows_of(b->grad_q);

@@ -7,7 +7,7 @@
 //   dQ  = scale e^G dO S^T + (dP o M) K
 //   dKr = (dL o M) K - e^G dY S^T             k where it reads the state
 //   dKw = (dP o M)^T Q + (dL o M)^T K + e^{G_last - G} U D^T   where it is written
-//   dL/dS = A^T D + E,  E = (scale e^G Q - scale P W)^T dO
+//   dL/dS = e^{G_last} D + Q^T (scale e^G dO) - K^T (e^G dY)
 // g_t decays what tokens i >= t and the end state see of the start state and of
 // tokens j < t, so, with the first terms of dQ and dKr and the last of dKw,
 //   dg_t = sum_{i>=t} (q.dQ + k.dKr)_i + sum_{i>=t, j<t} C_ij + sum_{j<t} (k.dKw)_j + e^{G_last} <D, S>
@@ -15,10 +15,13 @@
 // (the sum from the right of dL/dG, with what cancels in it left out: pairs on
 // one side of t never enter).
 //
-// Three launches: `adjoint` forms A^T and E of every chunk at once, the scan of
-// the forward walks the chunks in reverse (every chunk's D over its E), and
-// `grads` forms the gradients of every chunk at once.  q/k heads that several
-// heads share get a gradient a head in fp32, which `fold` adds in order.
+// Launches: `rewalk` walks the segments of the forward's walk in reverse with D in
+// the waves' accumulators, giving dV and leaving every chunk's D (where a row has
+// several segments, a first walk gives their maps of D and the scan joins them),
+// and `grads` forms the other gradients of every chunk at once.  q/k heads that
+// several heads share get a gradient a head in fp32, which `fold` adds in order.
+#include <type_traits>
+
 #include "osm_delta.h"
 
 namespace osm {
@@ -46,106 +49,279 @@ __device__ __forceinline__ void scores(f32x4 (&qk)[CT], f32x4 (&kk)[CT], float* 
   }
 }
 
-// A^T and E of a chunk.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) delta_adjoint_kernel(const DeltaParams p) {
-  __shared__ __attribute__((aligned(16))) float zs[kTile], ps[kTile], ks[kTile], ws[kTile];
-  __shared__ __attribute__((aligned(16))) Gates gt;
-  const int64_t chunk = blockIdx.x;
-  const At w = chunk_at(p, chunk);
-  if (w.rows == 0) return;
-  const int r0 = 16 * (threadIdx.x >> 6), hk = w.h / (p.H / p.Hk);
-  load_gates(&gt, p.g, p.beta, w.b, w.t0, w.h, w.rows);
-  const T* const q = row_ptr<T>(p.q, w.b, w.t0, hk);
-  const T* const k = row_ptr<T>(p.k, w.b, w.t0, hk);
-  const T* const go = row_ptr<T>(p.dout, w.b, w.t0, w.h);
-  load_z<kThreads>(zs, p.z + chunk * kZFloats);
-  f32x4 P[4], acc[4], x[4];
-  scores<kThreads, false>(P, acc, ws, ks, q, k, p, w.rows, r0, 0);
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = out_row(r0, i), col = out_col(0, c);
-      P[c][i] = row >= col ? P[c][i] * decay_between(gt, row, col) : 0.0f;
-    }
-  put(ps, P, r0, 0);
-  const int nkb = (p.dkp + 63) / 64;
-  float* const ag = p.a + chunk * p.dkp * p.dkp;
-  float* const eg = p.d + chunk * p.dkp * p.dvp;
-  for (int cb = 0; cb < nkb; ++cb) {
-    const int cw = min(64, p.dkp - 64 * cb);
-    __syncthreads();
-    if (nkb > 1) load_tile<kThreads>(ks, k + 64 * cb, p.k.ss, w.rows, p.dk_ - 64 * cb, cw, p.vec == 4);
-    __syncthreads();
-    // W and, scaled to the chunk's end, its product with K: columns cb of Kt^T W,
-    // so rows cb of A^T.
-    clear(acc);
-    mma<4, false, false, true>(acc, zs, r0, ks, 0, 0, r0 + 16, gt.bgam);
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = out_row(r0, i), col = out_col(0, c);
-        x[c][i] = col < cw ? gt.beta[row] * (gt.gam[row] * ks[row * kLd + col] - acc[c][i]) : 0.0f;
-        acc[c][i] = gt.end[row] * x[c][i];
-      }
-    put(ws, acc, r0, 0);
-    __syncthreads();
-    for (int rb = 0; rb < nkb; ++rb) {
-      const int rw = min(64, p.dkp - 64 * rb);
-      if (nkb > 1) {
-        __syncthreads();
-        load_tile<kThreads>(ks, k + 64 * rb, p.k.ss, w.rows, p.dk_ - 64 * rb, rw, p.vec == 4);
-        __syncthreads();
-      }
-      if (r0 < cw) {
-        clear(acc);
-        mma<4, true, false>(acc, ws, r0, ks, 0, 0, 64);
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = 64 * cb + out_row(r0, i), col = out_col(0, c);
-            if (col < rw)
-              ag[(int64_t)row * p.dkp + 64 * rb + col] = (row == 64 * rb + col ? gt.last : 0.0f) - acc[c][i];
-          }
-      }
-    }
-    __syncthreads();
-    // e^G Q - P W, by columns cb, and rows cb of E
-    put(ws, x, r0, 0);
-    __syncthreads();
-    clear(acc);
-    mma<4, false, false>(acc, ps, r0, ws, 0, 0, r0 + 16);
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = out_row(r0, i), col = out_col(0, c);
-        const float qv = row < w.rows && 64 * cb + col < p.dk_ ? (float)q[row * p.q.ss + 64 * cb + col] : 0.0f;
-        acc[c][i] = p.scale * (gt.gam[row] * qv - acc[c][i]);
-      }
-    __syncthreads();
-    put(ws, acc, r0, 0);
-    for (int vb = 0; vb < p.dvp; vb += 64) {
-      const int vw = min(64, p.dvp - vb);
-      __syncthreads();
-      load_tile<kThreads>(ks, go + vb, p.dout.ss, w.rows, p.dv_ - vb, vw, p.vec == 4);
-      __syncthreads();
-      if (r0 < cw) {
-        clear(acc);
-        mma<4, true, false>(acc, ws, r0, ks, 0, 0, 64);
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int col = out_col(0, c);
-            if (col < vw) eg[(int64_t)(64 * cb + out_row(r0, i)) * p.dvp + vb + col] = acc[c][i];
-          }
-      }
+// As tri_at's matrices, for the transpose: rows 0-31 have 64 columns, the others
+// the last 32.
+__device__ __forceinline__ int upper_at(int row, int col) { return row < 32 ? row * 72 + col : 2304 + (row - 32) * 40 + col - 32; }
+
+// Walks segment blockIdx.x % segs of a head from its last chunk to its first, D =
+// dL/dS' in the waves' accumulators (16 columns each, as S in the forward's walk).
+// MAP: the segment's map of D; else dV, and every chunk's D into p.d.
+template <typename T, int KS, int WAVES, bool MAP>
+__global__ void __launch_bounds__(64 * WAVES, 2) delta_rewalk_kernel(const DeltaParams p, int groups) {
+  constexpr int NT = 64 * WAVES, NP = kParts<T>, DK = 32 * KS, LDK = DK + 8, LKT = 72, ST = 2 * KS;
+  // K and Q by rows, then both by columns in the same place.
+  constexpr int kK = 64 * LDK, kKt = DK * LKT, kOne = kK > kKt ? kK : kKt;
+  __shared__ __attribute__((aligned(16))) unsigned short in[NP][2 * kOne], zt[3][kTri], pt[3][kTri];
+  __shared__ __attribute__((aligned(16))) float gates[2][kGateFloats];
+  unsigned short *const kk = &in[0][0], *const qq = kk + kOne;
+  constexpr int kIn = 2 * kOne;
+  const int group = blockIdx.x % groups;
+  const int64_t id = blockIdx.x / groups;
+  const int seg = (int)(id % p.segs), bh = (int)(id / p.segs), b = bh / p.H, h = bh - b * p.H, hk = h / (p.H / p.Hk);
+  const int tid = threadIdx.x, wave = tid >> 6, l = tid & 63, r = l & 15, g = l >> 4;
+  const int tokens = p.lengths ? min(max(p.lengths[b], 0), p.S) : p.S;
+  const int n = (tokens + kDeltaChunk - 1) / kDeltaChunk;
+  const int c0 = seg * p.seg, c1 = min(min(c0 + p.seg, p.N), n);
+  const int slice = group * WAVES + wave, vs = p.dvp / kDeltaSlice;
+  const bool value = slice < vs, live = slice < vs + (MAP ? DK / kDeltaSlice : 0);
+  const int col = kDeltaSlice * slice + r;
+  const bool in_v = value && col < p.dv_;
+  const bool first = !MAP && p.grad_init && seg == 0;
+  if (!MAP) {
+    // zeros for the chunks without tokens
+    for (int c = max(c0, n); c < min(c0 + p.seg, p.N); ++c) {
+      T* const o = row_ptr<T>(p.dv, b, (int64_t)c * kDeltaChunk, h) + col;
+      if (in_v)
+        for (int t = g; t < min(kDeltaChunk, p.S - c * kDeltaChunk); t += 4) o[t * p.dv.ss] = (T)0.0f;
     }
   }
+  if (c0 >= c1 && !first) return;
+  f32x4 D[ST];
+  const bool ws = !MAP && p.segs > 1 && n > 0;
+  const float* const from =
+      MAP ? nullptr : ws ? p.x + id * DK * p.dvp : p.grad_state ? p.grad_state + (int64_t)bh * p.dk_ * p.dv_ : nullptr;
+  const Rsrc from_rs = make_rsrc(from);
+  const unsigned from_ld = 4u * (ws ? p.dvp : p.dv_);
+  const bool from_col = from && (ws ? value : in_v);
+#pragma unroll
+  for (int t = 0; t < ST; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = 16 * t + 4 * g + i;
+      if (MAP)
+        D[t][i] = !value && row == col - p.dvp ? 1.0f : 0.0f;
+      else
+        D[t][i] = raw_value<float>(load_raw<float>(from_rs, from_col && (ws || row < p.dk_) ? row * from_ld + 4u * col : kOut));
+    }
+  const T* const kp = row_ptr<T>(p.k, b, 0, hk);
+  const T* const qp = row_ptr<T>(p.q, b, 0, hk);
+  const T* const dop = row_ptr<T>(p.dout, b, 0, h);
+  T* const dvp = MAP ? nullptr : row_ptr<T>(p.dv, b, 0, h);
+  const unsigned es = sizeof(T), do_row = (unsigned)p.dout.ss * es, dv_row = (unsigned)p.dv.ss * es;
+  const unsigned do_at = in_v ? col * es + 4 * g * do_row : kOut, dv_at = in_v ? col * es + 4 * g * dv_row : kOut;
+  // Z by 4x4 blocks: 64 of rows 0-31, then 128
+  const int zi = tid < 64 ? 4 * (tid >> 3) : 32 + 4 * ((tid - 64) >> 4), zj = 4 * (tid < 64 ? tid & 7 : (tid - 64) & 15);
+  Block<T, KS, NT> kb, qb;
+  f32x4 zr[4];
+  unsigned dr[16];
+  float gr[2];
+  auto rows_of = [&](int c) { return min(kDeltaChunk, tokens - c * kDeltaChunk); };
+  auto fetch_kq = [&](int c) {
+    kb.load(kp + (int64_t)c * kDeltaChunk * p.k.ss, p.k.ss, rows_of(c), p.dk_, p.vec);
+    qb.load(qp + (int64_t)c * kDeltaChunk * p.q.ss, p.q.ss, rows_of(c), p.dk_, p.vec);
+  };
+  auto fetch_do = [&](int c) {
+    const Rsrc rs = rows_rsrc<T>(dop + (int64_t)c * kDeltaChunk * p.dout.ss, p.dout.ss, rows_of(c), p.dv_);
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) dr[4 * t + i] = load_raw<T>(rs, do_at, (16 * t + i) * do_row);
+  };
+  auto fetch = [&](int c) {
+    const int64_t chunk = (int64_t)bh * p.N + c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = min(zi, 60) + i, quad = row < 32 ? row * 8 + (zj >> 2) : 256 + (row - 32) * 16 + (zj >> 2);
+      zr[i] = load4(p.z + chunk * kZFloats + 4 * quad);
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) gr[e] = p.gates[chunk * kGateFloats + min(tid + e * NT, kGateFloats - 1)];
+  };
+  auto put_gates = [&](int c) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (tid + e * NT < kGateFloats) gates[c & 1][tid + e * NT] = gr[e];
+  };
+  if (c0 < c1) {
+    fetch_kq(c1 - 1);
+    fetch(c1 - 1);
+    fetch_do(c1 - 1);
+    put_gates(c1 - 1);
+    // P's zeros before the diagonal tiles that end a pair: rows 16-31 and 48-63
+    for (int e = tid; e < 32 * 3 * 4; e += NT) {
+      const int row = (e & 31) < 16 ? 16 + (e & 31) : 32 + (e & 31), k = (e >> 5) % 3, q = 4 * (row >> 5 << 1) + (e >> 5) / 3;
+      *reinterpret_cast<u32x2*>(&pt[k][upper_at(row, place4(q))]) = u32x2{0, 0};
+    }
+  }
+  for (int c = c1 - 1; c >= c0; --c) {
+    const int64_t t0 = (int64_t)c * kDeltaChunk;
+    const float* const gt = gates[c & 1];
+    __syncthreads();   // the chunk after has been read, this one's gates are there
+    kb.template put_rows<LDK>(kk, kIn);
+    qb.template put_rows<LDK>(qq, kIn);
+    if (tid < 192) {
+      // -(beta Z)^T
+#pragma unroll
+      for (int i = 0; i < 4; ++i) zr[i] *= -gt[kBeta + zi + i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        u32x2 part[3];
+        split4<3>(part, f32x4{zr[0][j], zr[1][j], zr[2][j], zr[3][j]});
+#pragma unroll
+        for (int k = 0; k < 3; ++k) *reinterpret_cast<u32x2*>(&zt[k][upper_at(zj + j, place4(zi >> 2))]) = part[k];
+      }
+    }
+    __syncthreads();
+    if (c > c0) fetch(c - 1);
+    // scale P^T: four of its columns (rows of Q) of one row a lane
+#pragma unroll
+    for (int e = 0; e < (9 + WAVES) / WAVES; ++e) {
+      const int tile = wave + WAVES * e;
+      if (tile < 10) {
+        const int ti = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, tj = tile - ti * (ti + 1) / 2, j = 16 * tj + r;
+        f32x4 acc = zero4();
+        u32x4 kf[KS][NP], qf[KS][NP];
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          read_parts<NP>(qf[s], qq, kIn, (16 * ti + r) * LDK + 32 * s + 8 * g);
+          read_parts<NP>(kf[s], kk, kIn, j * LDK + 32 * s + 8 * g);
+        }
+#pragma unroll
+        for (int s = 0; s < KS; ++s) mul<NP, 2>(acc, qf[s], kf[s]);
+        const f32x4 hi = load4(gt + kHi + 16 * ti + 4 * g), lo = load4(gt + kLo + 16 * ti + 4 * g);
+        const float hi_j = gt[kHi + j], lo_j = gt[kLo + j];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          acc[k] = 16 * ti + 4 * g + k >= j ? p.scale * acc[k] * __builtin_amdgcn_exp2f((hi[k] - hi_j) + (lo[k] - lo_j)) : 0.0f;
+        u32x2 part[3];
+        split4<3>(part, acc);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) *reinterpret_cast<u32x2*>(&pt[k][upper_at(j, place4(4 * ti + g))]) = part[k];
+      }
+    }
+    f32x4 x[4];
+    u32x4 dp[2][NP];   // dO
+    if (live) {
+      if (!MAP && value) {
+        float* const dg = p.d + ((int64_t)bh * p.N + c) * DK * p.dvp + col;
+#pragma unroll
+        for (int t = 0; t < ST; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) dg[(int64_t)(16 * t + 4 * g + i) * p.dvp] = D[t][i];
+      }
+      clear(x);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        u32x4 sp[3];
+        split_pair<3>(sp, D[2 * s], D[2 * s + 1]);
+        products<NP, (NP == 1 ? 3 : 1), 4>(
+            kIn, [&](int i) { return kk + (16 * i + r) * LDK + 32 * s + 8 * g; },
+            [&](int i, const u32x4(&a)[NP]) { mul<3, 2>(x[i], a, sp); });
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) x[t] *= load4(gt + kEnd + 16 * t + 4 * g);
+    }
+    __syncthreads();   // P is there, the rows have been read
+    kb.template put_columns<LKT>(kk, kIn);
+    qb.template put_columns<LKT>(qq, kIn);
+    if (c > c0) fetch_kq(c - 1);
+    if (live) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if constexpr (NP == 1)
+          dp[s][0] = u32x4{dr[8 * s] | dr[8 * s + 1] << 16, dr[8 * s + 2] | dr[8 * s + 3] << 16,
+                           dr[8 * s + 4] | dr[8 * s + 5] << 16, dr[8 * s + 6] | dr[8 * s + 7] << 16};
+        else
+          split_pair<NP>(dp[s], f32x4{raw_value<T>(dr[8 * s]), raw_value<T>(dr[8 * s + 1]), raw_value<T>(dr[8 * s + 2]), raw_value<T>(dr[8 * s + 3])},
+                         f32x4{raw_value<T>(dr[8 * s + 4]), raw_value<T>(dr[8 * s + 5]), raw_value<T>(dr[8 * s + 6]), raw_value<T>(dr[8 * s + 7])});
+      }
+      // tiles (t, s): (0, 0), (1, 0), (0, 1) .. (3, 1)
+      products<3, 1, 6>(
+          kTri, [&](int i) { return &pt[0][0] + upper_at(16 * (i < 2 ? i : i - 2) + r, 32 * (i >= 2) + 8 * g); },
+          [&](int i, const u32x4(&a)[3]) { mul<NP, 2>(x[i < 2 ? i : i - 2], a, dp[i >= 2]); });
+      // R, on R0's registers
+      u32x4 xp[2][3];
+      split_pair<3>(xp[0], x[0], x[1]);
+      split_pair<3>(xp[1], x[2], x[3]);
+      products<3, 1, 6>(
+          kTri, [&](int i) { return &zt[0][0] + upper_at(16 * (i < 2 ? i : i - 2) + r, 32 * (i >= 2) + 8 * g); },
+          [&](int i, const u32x4(&a)[3]) { mul<3, 2>(x[i < 2 ? i : i - 2], a, xp[i >= 2]); });
+#pragma unroll
+      for (int t = 0; t < 4; ++t) x[t] *= load4(gt + kBeta + 16 * t + 4 * g);   // dY
+      if (!MAP) {
+        const int rows = tokens - (int)t0;
+        if (rows < kDeltaChunk)   // zeros past the tokens in use
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (16 * t + 4 * g + i >= rows) x[t][i] = 0.0f;
+        const Rsrc o_rs = rows_rsrc<T>(dvp + t0 * p.dv.ss, p.dv.ss, min(kDeltaChunk, p.S - (int)t0), p.dv_);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) store_one<T>(o_rs, dv_at, (16 * t + i) * dv_row, x[t][i]);
+      }
+    }
+    __syncthreads();   // the columns are there
+    if (live) {
+      const float last = gt[kGam + 63];
+#pragma unroll
+      for (int t = 0; t < ST; ++t) D[t] *= last;
+      f32x4 gam[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) gam[t] = load4(gt + kGam + 16 * t + 4 * g);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        u32x4 yp[3], op[3];
+        split_pair<3>(yp, -x[2 * s] * gam[2 * s], -x[2 * s + 1] * gam[2 * s + 1]);
+        f32x4 o[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[t][i] = p.scale * gam[2 * s + t][i] * raw_value<T>(dr[8 * s + 4 * t + i]);
+        split_pair<3>(op, o[0], o[1]);
+        products<NP, (NP == 1 ? 3 : 1), 2 * ST>(
+            kIn, [&](int i) { return (i < ST ? kk : qq) + (16 * (i % ST) + r) * LKT + 32 * s + 8 * g; },
+            [&](int i, const u32x4(&a)[NP]) { mul<3, 2>(D[i % ST], a, i < ST ? yp : op); });
+      }
+    }
+    if (c > c0) {
+      fetch_do(c - 1);
+      put_gates(c - 1);
+    }
+  }
+  if (MAP && live) {
+    float* const dst = value ? p.x + id * DK * p.dvp + col : p.a + id * DK * DK + (col - p.dvp);
+    const int ld = value ? p.dvp : DK;
+#pragma unroll
+    for (int t = 0; t < ST; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) dst[(int64_t)(16 * t + 4 * g + i) * ld] = D[t][i];
+  }
+  if (first && in_v) {
+    float* const dst = p.grad_init + (int64_t)bh * p.dk_ * p.dv_ + col;
+#pragma unroll
+    for (int t = 0; t < ST; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (16 * t + 4 * g + i < p.dk_) dst[(int64_t)(16 * t + 4 * g + i) * p.dv_] = D[t][i];
+  }
+}
+
+template <typename T, int KS, bool MAP>
+void launch_rewalk(const DeltaParams& p, hipStream_t stream) {
+  const int slices = p.dvp / kDeltaSlice + (MAP ? p.dkp / kDeltaSlice : 0);
+  auto go = [&](auto waves) {
+    constexpr int W = decltype(waves)::value;
+    const int groups = (slices + W - 1) / W;
+    const unsigned grid = (unsigned)((int64_t)p.B * p.H * p.segs * groups);
+    hipLaunchKernelGGL((delta_rewalk_kernel<T, KS, W, MAP>), dim3(grid), dim3(64 * W), 0, stream, p, groups);
+  };
+  if (slices <= 4)
+    go(std::integral_constant<int, 4>{});
+  else
+    go(std::integral_constant<int, 8>{});
 }
 
 constexpr int kGradThreads = 512;
@@ -168,7 +344,6 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const DeltaPa
   const int hk = w.h / (p.H / p.Hk);
   const bool shared_heads = p.H != p.Hk;   // dq and dk are then fp32, by head
   const int rows = (int)min((int64_t)kDeltaChunk, p.S - w.t0);
-  T* const gv = row_ptr<T>(p.dv, w.b, w.t0, w.h);
   auto put_qk = [&](const DeltaRows& dst, int row, int col, float v) {
     if (shared_heads)
       row_ptr<float>(dst, w.b, w.t0 + row, w.h)[col] = v;
@@ -182,7 +357,6 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const DeltaPa
         put_qk(p.dq, row, e, 0.0f);
         put_qk(p.dk, row, e, 0.0f);
       }
-      for (int e = tid & 63; e < p.dv_; e += 64) gv[row * p.dv.ss + e] = (T)0.0f;
       if ((tid & 63) == 0) {
         put_gate(p.dg, row, 0.0f);
         put_gate(p.dbeta, row, 0.0f);
@@ -275,7 +449,6 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const DeltaPa
         bsum[i] = __builtin_fmaf(r, x[c][i], bsum[i]);
         x[c][i] *= beta;                                    // U
         y[c][i] = beta * r;                                 // dY
-        if (row < rows && col < vw && vb + col < p.dv_) gv[row * p.dv.ss + vb + col] = (T)y[c][i];
       }
     __syncthreads();
     put(us, x, r0, c0);
@@ -441,12 +614,29 @@ __global__ void __launch_bounds__(kThreads) delta_fold_kernel(const float* src, 
   row_ptr<T>(dst, bt / S, bt % S, hb % Hk)[j] = (T)s;
 }
 
+template <typename T, int KS>
+hipError_t walks(const DeltaParams& p, hipStream_t stream) {
+  if (p.segs > 1) {
+    launch_rewalk<T, KS, true>(p, stream);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess)
+      e = launch_delta_scan(p, p.a, p.x, p.grad_state, nullptr, p.segs, p.seg * kDeltaChunk, true, stream);
+    if (e != hipSuccess) return e;
+  }
+  launch_rewalk<T, KS, false>(p, stream);
+  return hipGetLastError();
+}
+
 template <typename T>
 hipError_t backward(const DeltaParams& p, float* const part, hipStream_t stream) {
   const unsigned chunks = (unsigned)((int64_t)p.B * p.H * p.N);
-  hipLaunchKernelGGL((delta_adjoint_kernel<T>), dim3(chunks), dim3(kThreads), 0, stream, p);
-  hipError_t e = hipGetLastError();
-  if (e == hipSuccess) e = launch_delta_scan(p, p.a, p.d, p.grad_state, p.grad_init, p.N, kDeltaChunk, true, stream);
+  hipError_t e;
+  switch (p.dkp / 32) {
+    case 1: e = walks<T, 1>(p, stream); break;
+    case 2: e = walks<T, 2>(p, stream); break;
+    case 3: e = walks<T, 3>(p, stream); break;
+    default: e = walks<T, 4>(p, stream); break;
+  }
   if (e != hipSuccess) return e;
   const int64_t plane = (int64_t)p.B * p.S * p.H * p.dk_;
   DeltaParams w = p;

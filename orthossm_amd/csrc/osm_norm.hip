@@ -351,9 +351,9 @@ __global__ void __launch_bounds__(256) layer_norm_columns_kernel(const NormParam
   line[p.D + c] = db;
 }
 
-constexpr int kFoldCols = 32, kFoldGroups = 8;
+constexpr int kFoldCols = 32, kFoldGroups = 32;
 
-// dw and db from the lines, 32 columns a workgroup: group g adds lines g, g + 8,
+// dw and db from the lines, 32 columns a workgroup: group g adds lines g, g + 32,
 // ..; then the groups in order.
 __global__ void __launch_bounds__(kFoldCols * kFoldGroups) layer_norm_fold_kernel(const float* part, float* dw, float* db,
                                                                                   int64_t D, int lines) {

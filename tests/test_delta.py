@@ -67,16 +67,16 @@ def _fwd(a, ws=None, nbytes=0):
 def test_sizes():
     lib = nat.load()
     chunks = 2 * 4 * 4                      # rows, heads, chunks of 64 tokens
-    solved, states, maps = (chunks * n * 4 for n in (48 * 64 + 320, 64 * 80, 64 * 64))   # 48 rows of a state held as 64
+    solved, states = (chunks * n * 4 for n in (48 * 64 + 320, 64 * 80))                 # 48 rows of a state held as 64
     segments = 2 * 4 * 2 * (64 * 64 + 64 * 80) * 4                                      # two of two chunks a row
     assert lib.osm_delta_saved_bytes(ctypes.byref(_args())) == solved + states
     assert lib.osm_delta_workspace_bytes(ctypes.byref(_args())) == solved + segments
     assert lib.osm_delta_workspace_bytes(ctypes.byref(_args(saved=0x10000))) == segments
     assert lib.osm_delta_workspace_bytes(ctypes.byref(_args(S=16))) == 0      # token by token
     assert lib.osm_delta_workspace_bytes(ctypes.byref(_args(S=0))) == 0
-    # the backward: maps, end states, and a gradient of q and k for each of v's heads
-    assert lib.osm_delta_bwd_workspace_bytes(ctypes.byref(_args())) == maps + states + 2 * 2 * 200 * 4 * 48 * 4
-    assert lib.osm_delta_bwd_workspace_bytes(ctypes.byref(_args(Hk=4))) == maps + states
+    # the backward: maps of the segments, the chunks' gradients, and a gradient of q and k for each of v's heads
+    assert lib.osm_delta_bwd_workspace_bytes(ctypes.byref(_args())) == segments + states + 2 * 2 * 200 * 4 * 48 * 4
+    assert lib.osm_delta_bwd_workspace_bytes(ctypes.byref(_args(Hk=4))) == segments + states
 
 
 @pytest.mark.parametrize("kw,code", [
