@@ -41,6 +41,7 @@ struct DeltaParams {
   int seg, segs;                     // chunks a segment, segments a row
   float scale;
   int vec;                           // q, k, v and dout are whole multiples of so many elements, strides and all (4, 2, 1)
+  int out_vec;                       // dq's and dk's rows start at multiples of 4 elements
 };
 
 // Row b's state is slot b, or slots[b] of a pool of n_slots (state_s elements

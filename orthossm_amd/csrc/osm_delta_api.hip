@@ -249,6 +249,8 @@ int osm_delta_bwd(const osm_delta_args* a, const osm_delta_bwd_args* b, void* wo
   p.x = p.a + n.seg_a;
   p.d = p.x + n.seg_x;
   if (!whole(b->grad_out, es, p.vec)) p.vec = 1;
+  // (gradients by head are in the workspace, rows of dk)
+  p.out_vec = a->dk % 4 == 0 && (a->H != a->Hk || (whole(b->grad_q, es, 4) && whole(b->grad_k, es, 4)));
   p.dout = rows_of(b->grad_out);
   p.dq = rows_of(b->grad_q);
   p.dk = rows_of(b->grad_k);

@@ -599,6 +599,493 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const DeltaPa
   }
 }
 
+// ---- bf16 inputs ----
+
+// Four elements of a row from `at` (kOut: zeros), `left` of them inside it.
+__device__ __forceinline__ bf16x4 load_quad(Rsrc rs, unsigned at, int left, int vec) {
+  if (vec == 4) return __builtin_bit_cast(bf16x4, __builtin_amdgcn_raw_buffer_load_b64(rs, left > 0 ? at : kOut, 0, 0));
+  if (vec == 2)
+    return __builtin_bit_cast(bf16x4, u32x2{__builtin_amdgcn_raw_buffer_load_b32(rs, left > 0 ? at : kOut, 0, 0),
+                                            __builtin_amdgcn_raw_buffer_load_b32(rs, left > 2 ? at + 4 : kOut, 0, 0)});
+  bf16x4 v;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    v[k] = __builtin_bit_cast(__bf16, __builtin_amdgcn_raw_buffer_load_b16(rs, left > k ? at + 2 * k : kOut, 0, 0));
+  return v;
+}
+__device__ __forceinline__ f32x4 wide(bf16x4 v) { return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]}; }
+
+// The gradients of a chunk but dV, from bf16 inputs: eight waves, one workgroup a
+// CU.  Waves 0-3 (`reader`) and 4-7 share the work by what it is about:
+//   1  16 columns of v a wave: Y from S, and R from D, as in the walks; their parts
+//      go to LDS by rows
+//   2  16 tokens a wave, all products transposed, so that a result of 16 tokens'
+//      columns is the second operand of the next as it stands.  A reader's tokens
+//      are i: S dO^T and S R^T for dQ and dKr, (Y dO^T)_ji and (Y R^T)_ji; the
+//      others' are j: D Y^T for dKw, (dO Y^T)_ij and (R Y^T)_ij
+//   3  the latter, with their factors dP o M = scale beta_j M_ij dO Y^T and
+//      dL o M = -beta_i beta_j M_ij R Y^T, times K, Q and K
+// dbeta is the diagonal of Y R^T.  Tile rows left of the diagonal for a reader are
+// right of it for its partner on the same SIMD, so the SIMDs' work is even.
+// LDS: K by rows, then columns; dO; Q by rows, then Y and R, then C and dKw; Z,
+// its transpose and P's, then S and D (one after the other for more than 64 rows)
+// and Q by columns.  ONE: dv <= 64, so that what part 2 adds up need not live
+// through part 1.
+template <int KS, bool ONE>
+__global__ void __launch_bounds__(512, 2) delta_grads_parts_kernel(const DeltaParams p) {
+  typedef __bf16 T;
+  constexpr int NT = 512, DK = 32 * KS, LDK = DK + 8, L = 72, ST = 2 * KS;
+  constexpr int kK = 64 * LDK, kKt = DK * L, kVal = 64 * L, kState = DK * L, LW = DK + 4;
+  constexpr bool kBoth = KS <= 2;
+  constexpr int kFirst = kK > kKt ? kK : kKt;
+  constexpr int kStates = (kBoth ? 6 : 3) * kState, kLast = 9 * kTri > kStates + kKt ? 9 * kTri : kStates + kKt;
+  static_assert(kK <= 6 * kVal && 2 * (kTile + 64 * LW) <= 6 * kVal, "Q, or C and dKw, fit the place of Y and R");
+  __shared__ __attribute__((aligned(16))) unsigned short first[kFirst], os[kVal], yr[6 * kVal], rest[kLast];
+  __shared__ __attribute__((aligned(16))) float gt[kGateFloats];
+  __shared__ float pairs[8][64], part[8], reads[64], writes[64], dbeta[64];
+  unsigned short *const zp = rest, *const zt = rest + 3 * kTri, *const pt = rest + 6 * kTri;
+  unsigned short *const sp = rest, *const dp = rest + (kBoth ? 3 * kState : 0), *const qt = rest + kStates;
+  float *const cs = reinterpret_cast<float*>(yr), *const ws = cs + kTile;
+  const int64_t chunk = blockIdx.x;
+  const At w = chunk_at(p, chunk);
+  const int tid = threadIdx.x, wave = tid >> 6, st = wave & 3, l = tid & 63, r = l & 15, g = l >> 4;
+  const bool reader = wave < 4;
+  const int tok = 16 * st + r;                          // the token of this lane in parts 2 and 3
+  const int hk = w.h / (p.H / p.Hk);
+  const bool shared_heads = p.H != p.Hk;                // dq and dk are then fp32, by head
+  const int rows = (int)min((int64_t)kDeltaChunk, p.S - w.t0);
+  auto put_qk = [&](const DeltaRows& dst, int row, int col, f32x4 v) {
+    const int left = p.dk_ - col;
+    if (shared_heads) {
+      float* const o = row_ptr<float>(dst, w.b, w.t0 + row, w.h) + col;
+      if (p.out_vec) {
+        if (left > 0) store4(o, v);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (k < left) o[k] = v[k];
+      }
+    } else {
+      T* const o = row_ptr<T>(dst, w.b, w.t0 + row, w.h) + col;
+      const bf16x4 n = __builtin_convertvector(v, bf16x4);
+      if (p.out_vec) {
+        if (left > 0) *reinterpret_cast<bf16x4*>(o) = n;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (k < left) o[k] = n[k];
+      }
+    }
+  };
+  auto put_gate = [&](const DeltaRows& dst, int row, float v) { *row_ptr<float>(dst, w.b, w.t0 + row, w.h) = v; };
+  if (w.rows == 0) {
+    for (int row = wave; row < rows; row += 8) {
+      for (int e = 4 * l; e < p.dk_; e += 256) {
+        put_qk(p.dq, row, e, zero4());
+        put_qk(p.dk, row, e, zero4());
+      }
+      if (l == 0) {
+        put_gate(p.dg, row, 0.0f);
+        put_gate(p.dbeta, row, 0.0f);
+      }
+    }
+    return;
+  }
+  const T* const q = row_ptr<T>(p.q, w.b, w.t0, hk);
+  const T* const k = row_ptr<T>(p.k, w.b, w.t0, hk);
+  const T* const v = row_ptr<T>(p.v, w.b, w.t0, w.h);
+  const T* const go = row_ptr<T>(p.dout, w.b, w.t0, w.h);
+  const float* const sg = p.s + chunk * DK * p.dvp;
+  const float* const dg = p.d + chunk * DK * p.dvp;
+  const Rsrc o_rs = rows_rsrc<T>(go, p.dout.ss, w.rows, p.dv_);
+  const Rsrc raw_rs = reader ? rows_rsrc<T>(v, p.v.ss, w.rows, p.dv_) : o_rs;
+  const unsigned raw_row = 2u * (unsigned)(reader ? p.v.ss : p.dout.ss);
+  const Rsrc state_rs = make_rsrc(reader ? sg : dg, (unsigned)DK * p.dvp * 4u);
+  const int zi = tid < 64 ? 4 * (tid >> 3) : 32 + 4 * ((tid - 64) >> 4), zj = 4 * (tid < 64 ? tid & 7 : (tid - 64) & 15);
+  Block<T, KS, NT> kb, qb;
+  kb.load(k, p.k.ss, w.rows, p.dk_, p.vec);
+  qb.load(q, p.q.ss, w.rows, p.dk_, p.vec);
+  for (int e = tid; e < kGateFloats; e += NT) gt[e] = p.gates[chunk * kGateFloats + e];
+  kb.template put_rows<LDK>(first, kFirst);
+  f32x4 a1[ST], a2[ST];                 // dQ^T and dKr^T, or dKw^T and nothing
+  f32x4 mp[4], ml[4], qk[4], kk[4];     // dO Y^T, R Y^T, and a reader's K Q^T, K K^T, by tiles of the other token
+  if (!ONE) {
+    clear(a1);
+    clear(a2);
+    clear(mp);
+    clear(ml);
+  }
+  float ending = 0.0f;
+  for (int vb = 0; vb < (ONE ? 1 : p.dvp); vb += 64) {
+    if (vb) {
+      __syncthreads();
+      qb.load(q, p.q.ss, w.rows, p.dk_, p.vec);
+    }
+    // the slice's inputs
+    const int col = vb + 16 * st + r;
+    f32x4 state[ST];
+    unsigned raw[16];
+#pragma unroll
+    for (int t = 0; t < ST; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        state[t][i] = raw_value<float>(load_raw<float>(state_rs, col < p.dvp ? (unsigned)((16 * t + 4 * g + i) * p.dvp + col) * 4u : kOut));
+    const unsigned raw_at = col < p.dv_ ? 2u * col + 4 * g * raw_row : kOut;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[4 * t + i] = load_raw<T>(raw_rs, raw_at, (16 * t + i) * raw_row);
+    bf16x4 oq[2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int e = tid + n * NT, c = vb + 4 * (e & 15);
+      oq[n] = load_quad(o_rs, (e >> 4) * 2u * (unsigned)p.dout.ss + 2u * c, p.dv_ - c, p.vec);
+    }
+    f32x4 zr[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = min(zi, 60) + i, quad = row < 32 ? row * 8 + (zj >> 2) : 256 + (row - 32) * 16 + (zj >> 2);
+      zr[i] = load4(p.z + chunk * kZFloats + 4 * quad);
+    }
+    qb.template put_rows<LDK>(yr, kK);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) *reinterpret_cast<bf16x4*>(os + ((tid + n * NT) >> 4) * L + 4 * ((tid + n * NT) & 15)) = oq[n];
+    __syncthreads();
+    if (tid < 192) {
+      const f32x4 beta = load4(gt + kBeta + zj);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        u32x2 parts[3];
+        split4<3>(parts, -zr[i] * beta);      // -Z beta
+#pragma unroll
+        for (int n = 0; n < 3; ++n) *reinterpret_cast<u32x2*>(zp + n * kTri + tri_at(zi + i) + place4(zj >> 2)) = parts[n];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) zr[i] *= -gt[kBeta + zi + i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        u32x2 parts[3];
+        split4<3>(parts, f32x4{zr[0][j], zr[1][j], zr[2][j], zr[3][j]});   // -(beta Z)^T
+#pragma unroll
+        for (int n = 0; n < 3; ++n) *reinterpret_cast<u32x2*>(zt + n * kTri + upper_at(zj + j, place4(zi >> 2))) = parts[n];
+      }
+    }
+    if (reader) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        qk[t] = kk[t] = zero4();
+        if (t <= st)
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            u32x4 a[1], bq[1], bk[1];
+            read_parts<1>(a, first, 0, (16 * t + r) * LDK + 32 * s + 8 * g);
+            read_parts<1>(bq, yr, 0, tok * LDK + 32 * s + 8 * g);
+            read_parts<1>(bk, first, 0, tok * LDK + 32 * s + 8 * g);
+            qk[t] = mfma(a[0], bq[0], qk[t]);
+            kk[t] = mfma(a[0], bk[0], kk[t]);
+          }
+      }
+    } else {
+      // scale P^T, row tok, and zeros before it in its pair of tiles
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        if (t >= (st & 2)) {
+          f32x4 acc = zero4();
+          if (t >= st) {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+              u32x4 a[1], bk[1];
+              read_parts<1>(a, yr, 0, (16 * t + r) * LDK + 32 * s + 8 * g);
+              read_parts<1>(bk, first, 0, tok * LDK + 32 * s + 8 * g);
+              acc = mfma(a[0], bk[0], acc);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int row = 16 * t + 4 * g + i;
+              acc[i] = row >= tok ? p.scale * acc[i] * decay(gt, row, tok) : 0.0f;
+            }
+          }
+          u32x2 parts[3];
+          split4<3>(parts, acc);
+#pragma unroll
+          for (int n = 0; n < 3; ++n) *reinterpret_cast<u32x2*>(pt + n * kTri + upper_at(tok, place4(4 * t + g))) = parts[n];
+        }
+    }
+    __syncthreads();
+    // the states of part 2 on their way
+    constexpr int NS = DK * 16 / NT;   // quads a thread
+    f32x4 sq[NS], dq[NS];
+#pragma unroll
+    for (int n = 0; n < NS; ++n) {
+      const int e = tid + n * NT, c = vb + 4 * (e & 15);
+      const int64_t at = (int64_t)(e >> 4) * p.dvp + c;
+      sq[n] = c < p.dvp ? load4(sg + at) : zero4();
+      dq[n] = c < p.dvp ? load4(dg + at) : zero4();
+    }
+    // 1
+    {
+      f32x4 x[4];
+      clear(x);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        u32x4 b[3];
+        split_pair<3>(b, state[2 * s], state[2 * s + 1]);
+        products<1, 3, 4>(
+            0, [&](int i) { return first + (16 * i + r) * LDK + 32 * s + 8 * g; },
+            [&](int i, const u32x4(&a)[1]) { mul<3, 2>(x[i], a, b); });
+      }
+      u32x4 xp[2][3];
+      if (reader) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const f32x4 gam = load4(gt + kGam + 16 * t + 4 * g);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[t][i] = raw_value<T>(raw[4 * t + i]) - gam[i] * x[t][i];
+        }
+        split_pair<3>(xp[0], x[0], x[1]);
+        split_pair<3>(xp[1], x[2], x[3]);
+        products<3, 1, 6>(
+            kTri, [&](int i) { return zp + tri_at(16 * (i < 4 ? i : i - 2) + r) + 32 * (i >> 2) + 8 * g; },
+            [&](int i, const u32x4(&a)[3]) { mul<3, 2>(x[i < 4 ? i : i - 2], a, xp[i >> 2]); });
+      } else {
+        u32x4 ob[2][1];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+          ob[s][0] = u32x4{raw[8 * s] | raw[8 * s + 1] << 16, raw[8 * s + 2] | raw[8 * s + 3] << 16,
+                           raw[8 * s + 4] | raw[8 * s + 5] << 16, raw[8 * s + 6] | raw[8 * s + 7] << 16};
+#pragma unroll
+        for (int t = 0; t < 4; ++t) x[t] *= load4(gt + kEnd + 16 * t + 4 * g);
+        products<3, 1, 6>(
+            kTri, [&](int i) { return pt + upper_at(16 * (i < 2 ? i : i - 2) + r, 32 * (i >= 2) + 8 * g); },
+            [&](int i, const u32x4(&a)[3]) { mul<1, 2>(x[i < 2 ? i : i - 2], a, ob[i >= 2]); });
+        split_pair<3>(xp[0], x[0], x[1]);
+        split_pair<3>(xp[1], x[2], x[3]);
+        products<3, 1, 6>(
+            kTri, [&](int i) { return zt + upper_at(16 * (i < 2 ? i : i - 2) + r, 32 * (i >= 2) + 8 * g); },
+            [&](int i, const u32x4(&a)[3]) { mul<3, 2>(x[i < 2 ? i : i - 2], a, xp[i >= 2]); });
+      }
+      // (columns past dv are zeros: the states' padding, v and dO are)
+      unsigned short* const dst = yr + (reader ? 0 : 3 * kVal) + 16 * st + r;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        u32x2 parts[3];
+        split4<3>(parts, x[t]);
+#pragma unroll
+        for (int n = 0; n < 3; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            dst[n * kVal + (16 * t + 4 * g + i) * L] = (unsigned short)(parts[n][i >> 1] >> (16 * (i & 1)));
+      }
+    }
+    __syncthreads();
+    auto put_state = [&](unsigned short* to, const f32x4(&from)[NS]) {
+#pragma unroll
+      for (int n = 0; n < NS; ++n) {
+        const int e = tid + n * NT;
+        u32x2 parts[3];
+        split4<3>(parts, from[n]);
+#pragma unroll
+        for (int m = 0; m < 3; ++m) *reinterpret_cast<u32x2*>(to + m * kState + (e >> 4) * L + 4 * (e & 15)) = parts[m];
+      }
+    };
+#pragma unroll
+    for (int n = 0; n < NS; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ending = __builtin_fmaf(sq[n][i], dq[n][i], ending);
+    put_state(sp, sq);
+    if (kBoth) put_state(dp, dq);
+    __syncthreads();
+    // 2
+    if (ONE) {
+      clear(a1);
+      clear(a2);
+      clear(mp);
+      clear(ml);
+      kb.load(k, p.k.ss, w.rows, p.dk_, p.vec);   // for part 3
+      qb.load(q, p.q.ss, w.rows, p.dk_, p.vec);
+    }
+    const unsigned short *const ys = yr, *const rs = yr + 3 * kVal;
+    u32x4 bo[2][1], b3[2][3];   // the tokens' dO and R, or Y
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      read_parts<1>(bo[s], os, 0, tok * L + 32 * s + 8 * g);
+      read_parts<3>(b3[s], reader ? rs : ys, kVal, tok * L + 32 * s + 8 * g);
+    }
+    auto by_states = [&] {
+      if (reader)
+        products<3, 1, 2 * ST>(
+            kState, [&](int i) { return sp + (16 * (i >> 1) + r) * L + 32 * (i & 1) + 8 * g; },
+            [&](int i, const u32x4(&a)[3]) {
+              mul<1, 2>(a1[i >> 1], a, bo[i & 1]);
+              mul<3, 2>(a2[i >> 1], a, b3[i & 1]);
+            });
+    };
+    auto by_gradients = [&] {
+      if (!reader)
+        products<3, 1, 2 * ST>(
+            kState, [&](int i) { return dp + (16 * (i >> 1) + r) * L + 32 * (i & 1) + 8 * g; },
+            [&](int i, const u32x4(&a)[3]) { mul<3, 2>(a1[i >> 1], a, b3[i & 1]); });
+    };
+    auto by_tokens = [&] {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        if (reader ? t > st : t < st) continue;
+        const int at = (16 * t + r) * L + 8 * g;
+        if (reader) {
+          products<3, 1, 2>(
+              kVal, [&](int i) { return ys + at + 32 * i; },
+              [&](int i, const u32x4(&a)[3]) {
+                mul<1, 2>(mp[t], a, bo[i]);
+                mul<3, 2>(ml[t], a, b3[i]);
+              });
+        } else {
+          products<3, 1, 2>(
+              kVal, [&](int i) { return rs + at + 32 * i; },
+              [&](int i, const u32x4(&a)[3]) {
+                u32x4 ao[1];
+                read_parts<1>(ao, os, 0, at + 32 * i);
+                mul<3, 2>(ml[t], a, b3[i]);
+                mul<3, 2>(mp[t], ao, b3[i]);
+              });
+        }
+      }
+    };
+    by_states();
+    if (kBoth) {
+      by_gradients();
+      by_tokens();
+    } else {
+      if (!reader) by_tokens();
+      __syncthreads();
+      put_state(dp, dq);
+      __syncthreads();
+      by_gradients();
+      if (reader) by_tokens();
+    }
+  }
+  if (!ONE) {
+    kb.load(k, p.k.ss, w.rows, p.dk_, p.vec);
+    qb.load(q, p.q.ss, w.rows, p.dk_, p.vec);
+  }
+  __syncthreads();
+  kb.template put_columns<L>(first, kFirst);
+  qb.template put_columns<L>(qt, kKt);
+  // the factors of this lane's token, and the gates' parts of what S and D gave
+  const float gam = gt[kGam + tok], beta = gt[kBeta + tok];
+  float dot = 0.0f;
+  {
+    const Rsrc k_rs = rows_rsrc<T>(k, p.k.ss, w.rows, p.dk_), q_rs = rows_rsrc<T>(q, p.q.ss, w.rows, p.dk_);
+    const unsigned k_at = tok * 2u * (unsigned)p.k.ss, q_at = tok * 2u * (unsigned)p.q.ss;
+    const float f1 = reader ? p.scale * gam : gt[kEnd + tok] * beta, f2 = -gam * beta;
+#pragma unroll
+    for (int t = 0; t < ST; ++t) {
+      const int c = 16 * t + 4 * g;
+      const f32x4 kv = wide(load_quad(k_rs, k_at + 2 * c, p.dk_ - c, p.vec));
+      a1[t] *= f1;
+      if (reader) {
+        const f32x4 qv = wide(load_quad(q_rs, q_at + 2 * c, p.dk_ - c, p.vec));
+        a2[t] *= f2;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dot += qv[i] * a1[t][i] + kv[i] * a2[t][i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dot = __builtin_fmaf(kv[i], a1[t][i], dot);
+      }
+    }
+    dot += __shfl_xor(dot, 16);
+    dot += __shfl_xor(dot, 32);
+    if (g == 0) (reader ? reads : writes)[tok] = dot;
+  }
+  // dP o M and dL o M, their pairs' part of dg, dbeta
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const f32x4 bo = load4(gt + kBeta + 16 * t + 4 * g);
+    f32x4 c = zero4();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int other = 16 * t + 4 * g + i, ri = reader ? tok : other, cj = reader ? other : tok;
+      if (reader && other == tok) dbeta[tok] = ml[t][i];
+      const float m = ri >= cj ? decay(gt, ri, cj) : 0.0f;
+      mp[t][i] = ri >= cj ? p.scale * (reader ? bo[i] : beta) * m * mp[t][i] : 0.0f;
+      ml[t][i] = ri > cj ? -beta * bo[i] * m * ml[t][i] : 0.0f;
+      if (reader && ri > cj) c[i] = mp[t][i] * qk[t][i] + ml[t][i] * kk[t][i];
+    }
+    if (reader) *reinterpret_cast<f32x4*>(cs + tok * kLd + 16 * t + 4 * g) = c;
+  }
+  __syncthreads();
+  // 3
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    if (reader ? 2 * s > st : 2 * s + 1 < st) continue;
+    u32x4 bp[3], bl[3];
+    split_pair<3>(bp, mp[2 * s], mp[2 * s + 1]);
+    split_pair<3>(bl, ml[2 * s], ml[2 * s + 1]);
+    if (reader)
+      products<1, 2, ST>(
+          0, [&](int i) { return first + (16 * i + r) * L + 32 * s + 8 * g; },
+          [&](int i, const u32x4(&a)[1]) {
+            mul<3, 2>(a1[i], a, bp);
+            mul<3, 2>(a2[i], a, bl);
+          });
+    else
+      products<1, 2, 2 * ST>(
+          0, [&](int i) { return (i < ST ? qt : first) + (16 * (i % ST) + r) * L + 32 * s + 8 * g; },
+          [&](int i, const u32x4(&a)[1]) { mul<3, 2>(a1[i % ST], a, i < ST ? bp : bl); });
+  }
+  if (!reader)
+#pragma unroll
+    for (int t = 0; t < ST; ++t) *reinterpret_cast<f32x4*>(ws + tok * LW + 16 * t + 4 * g) = a1[t];
+  {
+    // C over its rows i in [8 wave, 8 wave + 8) for every t, lane t: over j < t by a
+    // scan along the row, then over the rows at and past t.
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = 8 * wave + i;
+      float c = cs[row * kLd + l];
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const float up = __shfl_up(c, o);
+        if (l >= o) c += up;
+      }
+      const float before = __shfl_up(c, 1);   // sum_{j < t}
+      if (l > 0 && row >= l) sum += before;
+    }
+    pairs[wave][l] = sum;
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) ending += __shfl_xor(ending, o);
+  if (l == 0) part[wave] = ending;
+  __syncthreads();
+  if (reader && tok < rows)
+#pragma unroll
+    for (int t = 0; t < ST; ++t) {
+      const int c = 16 * t + 4 * g;
+      put_qk(p.dq, tok, c, a1[t]);
+      put_qk(p.dk, tok, c, a2[t] + *reinterpret_cast<const f32x4*>(ws + tok * LW + c));
+    }
+  if (wave == 7) {
+    float from = reads[l], upto = writes[l];
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const float down = __shfl_down(from, o), up = __shfl_up(upto, o);
+      if (l + o < 64) from += down;
+      if (l >= o) upto += up;
+    }
+    upto = __shfl_up(upto, 1);
+    float sum = from + (l > 0 ? upto : 0.0f), whole = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      sum += pairs[i][l];
+      whole += part[i];
+    }
+    if (l < rows) {
+      put_gate(p.dg, l, l < w.rows ? sum + gt[kGam + 63] * whole : 0.0f);
+      put_gate(p.dbeta, l, l < w.rows ? dbeta[l] : 0.0f);
+    }
+  }
+}
+
 // dst[b,t,hk,:] = the sum over the heads that share hk, in order, of src [B,S,H,dk].
 template <typename T>
 __global__ void __launch_bounds__(kThreads) delta_fold_kernel(const float* src, DeltaRows dst, int64_t n, int S, int Hk,
@@ -646,10 +1133,25 @@ hipError_t backward(const DeltaParams& p, float* const part, hipStream_t stream)
     w.dq.p = part;
     w.dk.p = part + plane;
   }
-  if (p.dkp <= 64)
+  if constexpr (sizeof(T) == 2) {
+    auto go = [&](auto ks) {
+      constexpr int KS = decltype(ks)::value;
+      if (p.dvp <= 64)
+        hipLaunchKernelGGL((delta_grads_parts_kernel<KS, true>), dim3(chunks), dim3(512), 0, stream, w);
+      else
+        hipLaunchKernelGGL((delta_grads_parts_kernel<KS, false>), dim3(chunks), dim3(512), 0, stream, w);
+    };
+    switch (p.dkp / 32) {
+      case 1: go(std::integral_constant<int, 1>{}); break;
+      case 2: go(std::integral_constant<int, 2>{}); break;
+      case 3: go(std::integral_constant<int, 3>{}); break;
+      default: go(std::integral_constant<int, 4>{}); break;
+    }
+  } else if (p.dkp <= 64) {
     hipLaunchKernelGGL((delta_grads_kernel<T, 1>), dim3(chunks), dim3(kGradThreads), 0, stream, w);
-  else
+  } else {
     hipLaunchKernelGGL((delta_grads_kernel<T, 2>), dim3(chunks), dim3(kGradThreads), 0, stream, w);
+  }
   e = hipGetLastError();
   if (e != hipSuccess || p.H == p.Hk) return e;
   const int64_t n = (int64_t)p.B * p.S * p.Hk * p.dk_;
