@@ -535,11 +535,14 @@ def _import_ext():
     return mod
 
 
-# The functions osm_torch takes by address, in the order of its init() (the
-# last one the HIP runtime's, which the library links against).
+# The functions osm_torch takes by address, in the order of its init()
+# (hipStreamIsCapturing is the HIP runtime's, which the library links against).
 EXT_FUNCTIONS = ("osm_workspace_bytes", "osm_cheby_ema_fwd", "osm_cheby_ema_ttt", "osm_cheby_ema_bwd",
                  "osm_v10_chunked_ttt", "osm_v10_bwd", "osm_lut_fwd_workspace_bytes", "osm_cheby_ema_lut_fwd_ws",
-                 "osm_engine_scratch_bytes", "osm_engine_prologue", "hipStreamIsCapturing")
+                 "osm_engine_scratch_bytes", "osm_engine_prologue", "hipStreamIsCapturing", "osm_delta_saved_bytes",
+                 "osm_delta_workspace_bytes", "osm_delta_fwd", "osm_delta_bwd_workspace_bytes", "osm_delta_bwd",
+                 "osm_delta_step", "osm_layer_norm_fwd", "osm_layer_norm_bwd_workspace_bytes", "osm_layer_norm_bwd",
+                 "osm_clip_workspace_bytes", "osm_clip_grad_norm")
 
 
 def check(rc: int) -> None:

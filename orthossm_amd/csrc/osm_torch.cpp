@@ -20,6 +20,10 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/version.h>
 
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
 #include "osm.h"
 
 namespace {
@@ -38,7 +42,19 @@ struct Lib {
   decltype(&osm_engine_scratch_bytes) engine_bytes;
   decltype(&osm_engine_prologue) engine;
   int (*stream_is_capturing)(void* stream, int* status);   // hipStreamIsCapturing
+  decltype(&osm_delta_saved_bytes) delta_saved;
+  decltype(&osm_delta_workspace_bytes) delta_bytes;
+  decltype(&osm_delta_fwd) delta_fwd;
+  decltype(&osm_delta_bwd_workspace_bytes) delta_bwd_bytes;
+  decltype(&osm_delta_bwd) delta_bwd;
+  decltype(&osm_delta_step) delta_step;
+  decltype(&osm_layer_norm_fwd) norm_fwd;
+  decltype(&osm_layer_norm_bwd_workspace_bytes) norm_bwd_bytes;
+  decltype(&osm_layer_norm_bwd) norm_bwd;
+  decltype(&osm_clip_workspace_bytes) clip_bytes;
+  decltype(&osm_clip_grad_norm) clip;
 } lib;
+constexpr int kFunctions = 22;
 PyObject* raw_stream = nullptr;   // device index -> raw stream handle
 PyObject* ws_cache = nullptr;     // {(device index, stream, op): uint8 tensor}
 PyObject* workspace = nullptr;    // (device, stream, bytes, op) -> uint8 tensor
@@ -612,6 +628,401 @@ PyObject* run_engine(PyObject* const* p) {
   return Py_BuildValue("(NNN)", THPVariable_Wrap(xn), THPVariable_Wrap(gate), THPVariable_Wrap(mu));
 }
 
+// ---- gated delta rule, layer norm, gradient clipping (orthossm_amd/delta.py,
+// norm.py, grad_clip.py): as above, None for what is not in the kernels' form.
+// Their scratch memory is a plain allocation: nothing in it outlives the call.
+
+PyObject* wrap_or_none(const at::Tensor& t) {
+  if (t.defined()) return THPVariable_Wrap(t);
+  Py_RETURN_NONE;
+}
+
+at::Tensor scratch(size_t bytes, const at::Tensor& like) { return empty({(int64_t)bytes}, like, at::kByte); }
+
+osm_rows rows_of(const at::Tensor& t) { return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)}; }
+
+// Tokens' rows as the kernels address them.
+bool token_rows(const at::Tensor& t, int64_t dim) {
+  const int64_t s = t.size(1) > 1 ? t.stride(1) : dim;
+  return t.stride(0) >= 0 && t.stride(2) >= 0 && s >= dim && t.stride(1) >= 0 && t.stride(1) <= OSM_DELTA_MAX_STRIDE &&
+         (dim == 1 || t.stride(3) == 1);
+}
+
+// A scale: a number, or None for 1/sqrt(dk).
+bool as_scale(PyObject* o, int64_t dk, float* v) {
+  if (o == Py_None) {
+    *v = (float)(1.0 / std::sqrt((double)dk));
+    return true;
+  }
+  return as_float(o, v);
+}
+
+struct Delta {
+  const at::Tensor* t[5];        // q, k, v, g, beta
+  osm_delta_args a{};
+};
+
+// args: q, k, v, g, beta, scale, lengths.
+bool delta_common(PyObject* const* p, Delta* d) {
+  for (int i = 0; i < 5; ++i) {
+    d->t[i] = plain(p[i]);
+    if (!d->t[i] || !d->t[i]->is_cuda() || d->t[i]->dim() != (i < 3 ? 4 : 3)) return false;
+  }
+  const at::Tensor &q = *d->t[0], &k = *d->t[1], &v = *d->t[2];
+  if (!(is_f32(q) || is_bf16(q)) || k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type()) return false;
+  osm_delta_args& a = d->a;
+  a.abi_version = OSM_ABI_VERSION;
+  a.dtype = code(q);
+  a.B = q.size(0);
+  a.S = q.size(1);
+  a.Hk = q.size(2);
+  a.dk = q.size(3);
+  a.H = v.size(2);
+  a.dv = v.size(3);
+  if (k.sizes() != q.sizes() || v.size(0) != a.B || v.size(1) != a.S || a.Hk < 1 || a.H < 1 || a.H % a.Hk || a.dk < 1 ||
+      a.dk > OSM_DELTA_MAX_DK || a.dv < 1)
+    return false;
+  for (int i = 0; i < 5; ++i) {
+    const at::Tensor& t = *d->t[i];
+    if (t.device() != q.device()) return false;
+    if (i < 3 ? !token_rows(t, t.size(3))
+              : !is_f32(t) || t.size(0) != a.B || t.size(1) != a.S || t.size(2) != a.H || t.stride(0) < 0 ||
+                    t.stride(1) < 0 || t.stride(2) < 0 || t.stride(1) > OSM_DELTA_MAX_STRIDE)
+      return false;
+  }
+  a.q = rows_of(q);
+  a.k = rows_of(k);
+  a.v = rows_of(v);
+  a.g = rows_of(*d->t[3]);
+  a.beta = rows_of(*d->t[4]);
+  if (!as_scale(p[5], a.dk, &a.scale)) return false;
+  if (p[6] != Py_None) {
+    const at::Tensor* t = plain(p[6]);
+    if (!t || t->scalar_type() != at::kInt || t->dim() != 1 || t->size(0) != a.B || !t->is_contiguous() ||
+        t->device() != q.device())
+      return false;
+    a.lengths = static_cast<const int32_t*>(t->data_ptr());
+  }
+  return true;
+}
+
+// A state [B,H,dk,dv] fp32 contiguous, or None; false for another.
+bool state_ptr(PyObject* o, const Delta& d, float** out) {
+  *out = nullptr;
+  if (o == Py_None) return true;
+  const at::Tensor* t = plain(o);
+  if (!t || t->dim() != 4 || t->size(0) != d.a.B || t->size(1) != d.a.H || t->size(2) != d.a.dk || t->size(3) != d.a.dv ||
+      !f32_flat(*t, t->numel(), *d.t[0]))
+    return false;
+  *out = fptr(*t);
+  return true;
+}
+
+// delta_forward(<common 7>, state_init, want_state, save): None, or (out, state | None, saved | None).
+PyObject* run_delta_forward(PyObject* const* p) {
+  Delta d;
+  float* init;
+  if (!delta_common(p, &d) || !state_ptr(p[7], d, &init)) Py_RETURN_NONE;
+  const bool want_state = PyObject_IsTrue(p[8]) == 1, save = PyObject_IsTrue(p[9]) == 1;
+  if (PyErr_Occurred()) return nullptr;
+  const at::Tensor& q = *d.t[0];
+  osm_delta_args& a = d.a;
+  a.state_init = init;
+  Ref s_obj;
+  void* stream;
+  const c10::DeviceGuard guard(q.device());
+  if (!stream_of(q, &s_obj, &stream)) return nullptr;
+  at::Tensor out, fin, saved, ws;
+  int rc;
+  {
+    const NoGil nogil;
+    out = empty({a.B, a.S, a.H, a.dv}, q, q.scalar_type());
+    a.out = rows_of(out);
+    if (want_state) {
+      fin = empty({a.B, a.H, a.dk, a.dv}, q, at::kFloat);
+      a.state_out = fptr(fin);
+    }
+    if (save) {
+      saved = scratch(lib.delta_saved(&a), q);
+      a.saved = saved.data_ptr();
+    }
+    ws = scratch(lib.delta_bytes(&a), q);
+    rc = lib.delta_fwd(&a, ws.data_ptr(), (size_t)ws.numel(), stream);
+  }
+  if (rc != OSM_OK) return fail_rc(rc);
+  return Py_BuildValue("(NNN)", THPVariable_Wrap(out), wrap_or_none(fin), wrap_or_none(saved));
+}
+
+// delta_backward(<common 7>, saved, grad_out, grad_state, need_init): None, or the six gradients.
+PyObject* run_delta_backward(PyObject* const* p) {
+  Delta d;
+  float* gs;
+  if (!delta_common(p, &d) || !state_ptr(p[9], d, &gs)) Py_RETURN_NONE;
+  const at::Tensor &q = *d.t[0], &v = *d.t[2];
+  const at::Tensor *saved = plain(p[7]), *go = plain(p[8]);
+  if (!saved || !go || go->dim() != 4 || go->sizes() != v.sizes() || go->scalar_type() != v.scalar_type() ||
+      go->device() != q.device() || !token_rows(*go, v.size(3)))
+    Py_RETURN_NONE;
+  const bool need_init = PyObject_IsTrue(p[10]) == 1;
+  if (PyErr_Occurred()) return nullptr;
+  osm_delta_args& a = d.a;
+  a.saved = saved->data_ptr();
+  osm_delta_bwd_args b{};
+  b.grad_out = rows_of(*go);
+  b.grad_state = gs;
+  Ref s_obj;
+  void* stream;
+  const c10::DeviceGuard guard(q.device());
+  if (!stream_of(q, &s_obj, &stream)) return nullptr;
+  at::Tensor gr[5], gi, ws;
+  int rc;
+  {
+    const NoGil nogil;
+    for (int i = 0; i < 5; ++i) gr[i] = empty(d.t[i]->sizes(), q, d.t[i]->scalar_type());
+    b.grad_q = rows_of(gr[0]);
+    b.grad_k = rows_of(gr[1]);
+    b.grad_v = rows_of(gr[2]);
+    b.grad_g = rows_of(gr[3]);
+    b.grad_beta = rows_of(gr[4]);
+    if (need_init) {
+      gi = empty({a.B, a.H, a.dk, a.dv}, q, at::kFloat);
+      b.grad_init = fptr(gi);
+    }
+    ws = scratch(lib.delta_bwd_bytes(&a), q);
+    rc = lib.delta_bwd(&a, &b, ws.data_ptr(), (size_t)ws.numel(), stream);
+  }
+  if (rc != OSM_OK) return fail_rc(rc);
+  return Py_BuildValue("(NNNNNN)", THPVariable_Wrap(gr[0]), THPVariable_Wrap(gr[1]), THPVariable_Wrap(gr[2]),
+                       THPVariable_Wrap(gr[3]), THPVariable_Wrap(gr[4]), wrap_or_none(gi));
+}
+
+// delta_step(q, k, v, g, beta, state, scale, slots): None, or out.
+PyObject* run_delta_step(PyObject* const* p) {
+  const at::Tensor* t[6];
+  for (int i = 0; i < 6; ++i) {
+    t[i] = plain(p[i]);
+    if (!t[i] || !t[i]->is_cuda() || t[i]->device() != t[0]->device()) Py_RETURN_NONE;
+  }
+  const at::Tensor &q = *t[0], &k = *t[1], &v = *t[2], &state = *t[5];
+  if (q.dim() != 3 || v.dim() != 3 || k.sizes() != q.sizes() || !(is_f32(q) || is_bf16(q)) ||
+      k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type())
+    Py_RETURN_NONE;
+  osm_delta_step_args a{};
+  a.abi_version = OSM_ABI_VERSION;
+  a.dtype = code(q);
+  a.B = q.size(0);
+  a.Hk = q.size(1);
+  a.dk = q.size(2);
+  a.H = v.size(1);
+  a.dv = v.size(2);
+  if (v.size(0) != a.B || a.Hk < 1 || a.H < 1 || a.H % a.Hk || a.dk < 1 || a.dk > OSM_DELTA_MAX_DK || a.dv < 1)
+    Py_RETURN_NONE;
+  for (int i = 0; i < 5; ++i) {
+    const at::Tensor& x = *t[i];
+    if (x.stride(0) < 0 || x.stride(1) < 0) Py_RETURN_NONE;
+    if (i < 3 ? x.stride(2) != 1 && x.size(2) != 1 : x.dim() != 2 || !is_f32(x) || x.size(0) != a.B || x.size(1) != a.H)
+      Py_RETURN_NONE;
+    osm_rows* const r = i == 0 ? &a.q : i == 1 ? &a.k : i == 2 ? &a.v : i == 3 ? &a.g : &a.beta;
+    *r = {x.data_ptr(), x.stride(0), 0, x.stride(1)};
+  }
+  if (state.dim() != 4 || !is_f32(state) || state.requires_grad() || state.size(1) != a.H || state.size(2) != a.dk ||
+      state.size(3) != a.dv || state.stride(3) != 1 || state.stride(2) != a.dv || state.stride(1) != a.dk * a.dv ||
+      state.stride(0) < a.H * a.dk * a.dv)
+    Py_RETURN_NONE;
+  a.state = fptr(state);
+  a.state_stride = state.stride(0);
+  a.n_slots = state.size(0);
+  if (!as_scale(p[6], a.dk, &a.scale)) Py_RETURN_NONE;
+  if (p[7] == Py_None) {
+    if (a.n_slots < a.B) Py_RETURN_NONE;
+  } else {
+    const at::Tensor* s = plain(p[7]);
+    if (!s || s->scalar_type() != at::kLong || s->dim() != 1 || s->size(0) != a.B || !s->is_contiguous() ||
+        s->device() != q.device())
+      Py_RETURN_NONE;
+    a.slots = static_cast<const int64_t*>(s->data_ptr());
+  }
+  Ref s_obj;
+  void* stream;
+  const c10::DeviceGuard guard(q.device());
+  if (!stream_of(q, &s_obj, &stream)) return nullptr;
+  at::Tensor out;
+  int rc;
+  {
+    const NoGil nogil;
+    out = empty({a.B, a.H, a.dv}, q, q.scalar_type());
+    a.out = {out.data_ptr(), out.stride(0), 0, out.stride(1)};
+    rc = lib.delta_step(&a, stream);
+  }
+  if (rc != OSM_OK) return fail_rc(rc);
+  return THPVariable_Wrap(out);
+}
+
+// x [.., D] whose rows are D contiguous elements, one after the other.
+bool norm_rows(const at::Tensor* x) {
+  return x && x->is_cuda() && (is_f32(*x) || is_bf16(*x)) && x->dim() >= 1 && x->is_contiguous() &&
+         x->size(x->dim() - 1) >= 1;
+}
+
+// A parameter [D] fp32, or None; false for another.
+bool norm_param(PyObject* o, int64_t D, const at::Tensor& x, const float** out) {
+  *out = nullptr;
+  if (o == Py_None) return true;
+  const at::Tensor* t = plain(o);
+  if (!f32_vec(t, D, x)) return false;
+  *out = fptr(*t);
+  return true;
+}
+
+void norm_args(const at::Tensor& x, osm_norm_args* a) {
+  a->abi_version = OSM_ABI_VERSION;
+  a->dtype = code(x);
+  a->D = x.size(x.dim() - 1);
+  a->rows = x.numel() / a->D;
+  a->x = x.data_ptr();
+  a->x_stride = a->D;
+}
+
+// norm_forward(x, weight, bias, eps, stats): None, or (y, mean | None, rstd | None).
+PyObject* run_norm_forward(PyObject* const* p) {
+  const at::Tensor* const xp = plain(p[0]);
+  if (!norm_rows(xp)) Py_RETURN_NONE;
+  const at::Tensor& x = *xp;
+  osm_norm_args a{};
+  norm_args(x, &a);
+  if (!norm_param(p[1], a.D, x, &a.weight) || !norm_param(p[2], a.D, x, &a.bias) || !as_float(p[3], &a.eps)) Py_RETURN_NONE;
+  const bool stats = PyObject_IsTrue(p[4]) == 1;
+  if (PyErr_Occurred()) return nullptr;
+  Ref s_obj;
+  void* stream;
+  const c10::DeviceGuard guard(x.device());
+  if (!stream_of(x, &s_obj, &stream)) return nullptr;
+  at::Tensor y, mean, rstd;
+  int rc;
+  {
+    const NoGil nogil;
+    y = empty(x.sizes(), x, x.scalar_type());
+    a.y = y.data_ptr();
+    a.y_stride = a.D;
+    if (stats) {
+      const at::IntArrayRef lead = x.sizes().slice(0, x.dim() - 1);
+      mean = empty(lead, x, at::kFloat);
+      rstd = empty(lead, x, at::kFloat);
+      a.mean = fptr(mean);
+      a.rstd = fptr(rstd);
+    }
+    rc = lib.norm_fwd(&a, stream);
+  }
+  if (rc != OSM_OK) return fail_rc(rc);
+  return Py_BuildValue("(NNN)", THPVariable_Wrap(y), wrap_or_none(mean), wrap_or_none(rstd));
+}
+
+// norm_backward(grad_y, x, mean, rstd, weight, need_x, need_weight, need_bias): None, or
+// (grad_x | None, grad_weight | None, grad_bias | None).
+PyObject* run_norm_backward(PyObject* const* p) {
+  const at::Tensor *const gyp = plain(p[0]), *const xp = plain(p[1]), *const mp = plain(p[2]), *const rp = plain(p[3]);
+  if (!norm_rows(xp) || !norm_rows(gyp) || !mp || !rp) Py_RETURN_NONE;
+  const at::Tensor& x = *xp;
+  osm_norm_args a{};
+  norm_args(x, &a);
+  if (gyp->sizes() != x.sizes() || gyp->scalar_type() != x.scalar_type() || gyp->device() != x.device() ||
+      !f32_flat(*mp, a.rows, x) || !f32_flat(*rp, a.rows, x) || mp->dim() != x.dim() - 1 || rp->dim() != x.dim() - 1 ||
+      !norm_param(p[4], a.D, x, &a.weight))
+    Py_RETURN_NONE;
+  a.mean = fptr(*mp);
+  a.rstd = fptr(*rp);
+  bool need[3];
+  for (int i = 0; i < 3; ++i) need[i] = PyObject_IsTrue(p[5 + i]) == 1;
+  if (PyErr_Occurred()) return nullptr;
+  Ref s_obj;
+  void* stream;
+  const c10::DeviceGuard guard(x.device());
+  if (!stream_of(x, &s_obj, &stream)) return nullptr;
+  at::Tensor gx, gw, gb, ws;
+  osm_norm_bwd_args b{};
+  b.grad_y = gyp->data_ptr();
+  b.grad_y_stride = a.D;
+  int rc;
+  {
+    const NoGil nogil;
+    if (need[0]) {
+      gx = empty(x.sizes(), x, x.scalar_type());
+      b.grad_x = gx.data_ptr();
+      b.grad_x_stride = a.D;
+    }
+    if (need[1]) {
+      gw = empty({a.D}, x, at::kFloat);
+      b.grad_weight = fptr(gw);
+    }
+    if (need[2]) {
+      gb = empty({a.D}, x, at::kFloat);
+      b.grad_bias = fptr(gb);
+    }
+    ws = scratch(lib.norm_bwd_bytes(&a), x);
+    rc = lib.norm_bwd(&a, &b, ws.data_ptr(), (size_t)ws.numel(), stream);
+  }
+  if (rc != OSM_OK) return fail_rc(rc);
+  return Py_BuildValue("(NNN)", wrap_or_none(gx), wrap_or_none(gw), wrap_or_none(gb));
+}
+
+// clip(tensors, max_norm, eps, scale): None, or the norm.  tensors: a list or tuple.
+PyObject* run_clip(PyObject* const* p) {
+  if (!PyList_Check(p[0]) && !PyTuple_Check(p[0])) Py_RETURN_NONE;
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(p[0]);
+  if (n == 0) Py_RETURN_NONE;
+  const double max_norm = PyFloat_AsDouble(p[1]), eps = PyFloat_AsDouble(p[2]);
+  const bool scale = PyObject_IsTrue(p[3]) == 1;
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+  }
+  std::vector<void*> ptr(n);
+  std::vector<int64_t> size(n);
+  std::vector<int32_t> dtype(n);
+  const at::Tensor* first = nullptr;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    const at::Tensor* const t = plain(PySequence_Fast_GET_ITEM(p[0], i));
+    if (!t || !t->is_cuda() || !(is_f32(*t) || is_bf16(*t)) || !t->is_contiguous() || (scale && t->requires_grad()))
+      Py_RETURN_NONE;
+    if (!first) first = t;
+    if (t->device() != first->device()) Py_RETURN_NONE;
+    ptr[i] = t->data_ptr();
+    size[i] = t->numel();
+    dtype[i] = code(*t);
+  }
+  if (scale) {   // a tensor given twice is refused by the Python path
+    std::vector<void*> seen;
+    for (Py_ssize_t i = 0; i < n; ++i)
+      if (size[i]) seen.push_back(ptr[i]);
+    std::sort(seen.begin(), seen.end());
+    if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) Py_RETURN_NONE;
+  }
+  osm_clip_args a{};
+  a.abi_version = OSM_ABI_VERSION;
+  a.flags = scale ? OSM_CLIP_SCALE : 0;
+  a.count = n;
+  a.tensors = ptr.data();
+  a.sizes = size.data();
+  a.dtypes = dtype.data();
+  a.max_norm = max_norm;
+  a.eps = eps;
+  Ref s_obj;
+  void* stream;
+  const c10::DeviceGuard guard(first->device());
+  if (!stream_of(*first, &s_obj, &stream)) return nullptr;
+  at::Tensor norm, ws;
+  int rc;
+  {
+    const NoGil nogil;
+    norm = empty({}, *first, at::kFloat);
+    a.norm = fptr(norm);
+    ws = scratch(lib.clip_bytes(&a), *first);
+    rc = lib.clip(&a, ws.data_ptr(), (size_t)ws.numel(), stream);
+  }
+  if (rc != OSM_OK) return fail_rc(rc);
+  return THPVariable_Wrap(norm);
+}
+
 // Runs a function under the argument count and the C++ exceptions of ATen.
 template <int N, typename F>
 PyObject* guarded(PyObject* const* args, Py_ssize_t n, F f) {
@@ -640,16 +1051,23 @@ PyObject* py_v10_backward(PyObject*, PyObject* const* a, Py_ssize_t n) { return 
 PyObject* py_lut(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded<10>(a, n, run_lut); }
 PyObject* py_engine(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded<9>(a, n, run_engine); }
 
-// init(addresses of the eleven library functions, raw_stream, ws_cache, workspace, check)
+PyObject* py_delta_forward(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded<10>(a, n, run_delta_forward); }
+PyObject* py_delta_backward(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded<11>(a, n, run_delta_backward); }
+PyObject* py_delta_step(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded<8>(a, n, run_delta_step); }
+PyObject* py_norm_forward(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded<5>(a, n, run_norm_forward); }
+PyObject* py_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded<8>(a, n, run_norm_backward); }
+PyObject* py_clip(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded<4>(a, n, run_clip); }
+
+// init(addresses of the library's functions in the order of Lib, raw_stream, ws_cache, workspace, check)
 PyObject* py_init(PyObject*, PyObject* args) {
   PyObject *addr, *rs, *wc, *wf, *ck;
   if (!PyArg_ParseTuple(args, "O!OO!OO", &PyTuple_Type, &addr, &rs, &PyDict_Type, &wc, &wf, &ck)) return nullptr;
-  void* f[11];
-  if (PyTuple_GET_SIZE(addr) != 11) {
-    PyErr_SetString(PyExc_ValueError, "eleven addresses are expected");
+  void* f[kFunctions];
+  if (PyTuple_GET_SIZE(addr) != kFunctions) {
+    PyErr_Format(PyExc_ValueError, "%d addresses are expected", kFunctions);
     return nullptr;
   }
-  for (int i = 0; i < 11; ++i) f[i] = PyLong_AsVoidPtr(PyTuple_GET_ITEM(addr, i));
+  for (int i = 0; i < kFunctions; ++i) f[i] = PyLong_AsVoidPtr(PyTuple_GET_ITEM(addr, i));
   if (PyErr_Occurred()) return nullptr;
   lib.workspace_bytes = reinterpret_cast<decltype(lib.workspace_bytes)>(f[0]);
   lib.fwd = reinterpret_cast<decltype(lib.fwd)>(f[1]);
@@ -662,6 +1080,17 @@ PyObject* py_init(PyObject*, PyObject* args) {
   lib.engine_bytes = reinterpret_cast<decltype(lib.engine_bytes)>(f[8]);
   lib.engine = reinterpret_cast<decltype(lib.engine)>(f[9]);
   lib.stream_is_capturing = reinterpret_cast<decltype(lib.stream_is_capturing)>(f[10]);
+  lib.delta_saved = reinterpret_cast<decltype(lib.delta_saved)>(f[11]);
+  lib.delta_bytes = reinterpret_cast<decltype(lib.delta_bytes)>(f[12]);
+  lib.delta_fwd = reinterpret_cast<decltype(lib.delta_fwd)>(f[13]);
+  lib.delta_bwd_bytes = reinterpret_cast<decltype(lib.delta_bwd_bytes)>(f[14]);
+  lib.delta_bwd = reinterpret_cast<decltype(lib.delta_bwd)>(f[15]);
+  lib.delta_step = reinterpret_cast<decltype(lib.delta_step)>(f[16]);
+  lib.norm_fwd = reinterpret_cast<decltype(lib.norm_fwd)>(f[17]);
+  lib.norm_bwd_bytes = reinterpret_cast<decltype(lib.norm_bwd_bytes)>(f[18]);
+  lib.norm_bwd = reinterpret_cast<decltype(lib.norm_bwd)>(f[19]);
+  lib.clip_bytes = reinterpret_cast<decltype(lib.clip_bytes)>(f[20]);
+  lib.clip = reinterpret_cast<decltype(lib.clip)>(f[21]);
   PyObject** slots[4] = {&raw_stream, &ws_cache, &workspace, &check};
   PyObject* vals[4] = {rs, wc, wf, ck};
   for (int i = 0; i < 4; ++i) {
@@ -687,6 +1116,12 @@ PyMethodDef methods[] = {
     {"v10_backward", fast(py_v10_backward), METH_FASTCALL, nullptr},
     {"lut_forward", fast(py_lut), METH_FASTCALL, nullptr},
     {"engine", fast(py_engine), METH_FASTCALL, nullptr},
+    {"delta_forward", fast(py_delta_forward), METH_FASTCALL, nullptr},
+    {"delta_backward", fast(py_delta_backward), METH_FASTCALL, nullptr},
+    {"delta_step", fast(py_delta_step), METH_FASTCALL, nullptr},
+    {"norm_forward", fast(py_norm_forward), METH_FASTCALL, nullptr},
+    {"norm_backward", fast(py_norm_backward), METH_FASTCALL, nullptr},
+    {"clip", fast(py_clip), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "osm_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

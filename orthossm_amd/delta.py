@@ -31,7 +31,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native as nat
-from .ops import _current_device, _current_stream, _dtype_code
+from .ops import _current_device, _current_stream, _dtype_code, _fast
 
 
 def on_device(dev: torch.device):
@@ -125,6 +125,11 @@ def _scratch(nbytes: int, dev) -> torch.Tensor:
 
 
 def _forward(q, k, v, g, beta, scale, state_init, lengths, out, return_state, state_out, save):
+    fast = _fast()
+    if fast is not None and out is None and state_out is None:
+        res = fast.delta_forward(q, k, v, g, beta, scale, lengths, state_init, return_state, save)
+        if res is not None:
+            return (*res, (q, k, v, g, beta, state_init, lengths))
     lib = nat.load()
     a, keep = _prepare(q, k, v, g, beta, scale, state_init, lengths)
     v = keep[2]
@@ -164,9 +169,16 @@ def gated_delta_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: to
     return (out, fin) if return_state else out
 
 
-def _backward(a, keep, saved, grad_out, grad_state, need_init: bool):
-    """The C call: ``a`` and ``keep`` from _prepare, ``saved`` from _forward."""
+def _backward(inputs, scale, lengths, saved, grad_out, grad_state, need_init: bool):
+    """The six gradients; ``inputs`` (q, k, v, g, beta), ``lengths`` and
+    ``saved`` as _forward gave them."""
+    fast = _fast()
+    if fast is not None:
+        res = fast.delta_backward(*inputs, scale, lengths, saved, grad_out, grad_state, need_init)
+        if res is not None:
+            return res
     lib = nat.load()
+    a, keep = _prepare(*inputs, scale, None, lengths)
     q, k, v, g = keep[:4]
     dev = v.device
     if not isinstance(grad_out, torch.Tensor) or grad_out.shape != v.shape:
@@ -200,8 +212,7 @@ def gated_delta_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: t
     Returns (grad_q, grad_k, grad_v in the inputs' type, grad_g, grad_beta
     fp32, grad_init fp32 or None)."""
     _, _, saved, keep = _forward(q, k, v, g, beta, scale, state_init, lengths, None, False, None, True)
-    a, keep = _prepare(*keep[:5], scale, None, keep[6])
-    return _backward(a, keep, saved, grad_out, grad_state, need_init)
+    return _backward(keep[:5], scale, keep[6], saved, grad_out, grad_state, need_init)
 
 
 class _GatedDeltaFunction(torch.autograd.Function):
@@ -220,11 +231,10 @@ class _GatedDeltaFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad_out, grad_state):
         *inputs, lengths, saved = ctx.saved_tensors
-        a, keep = _prepare(*inputs, ctx.scale, None, lengths)
         if grad_out is None:
-            grad_out = torch.zeros_like(keep[2])
+            grad_out = torch.zeros_like(inputs[2])
         need = ctx.needs_input_grad
-        grads = _backward(a, keep, saved, grad_out, grad_state, need[5])
+        grads = _backward(inputs, ctx.scale, lengths, saved, grad_out, grad_state, need[5])
         return (*(t.to(dt) if n else None for t, dt, n in zip(grads, ctx.types, need)), None, None)
 
 
@@ -251,6 +261,11 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     one marks an idle row, whose output is 0; one past the pool gives NaN;
     neither touches a state.  Returns out [B,H,dv] in v's type, in ``out``
     (contiguous) if given."""
+    fast = _fast()
+    if fast is not None and out is None:
+        res = fast.delta_step(q, k, v, g, beta, state, scale, slots)
+        if res is not None:
+            return res
     lib = nat.load()
     q, k, v = _check_qkv(q, k, v, 3, "[B,heads,size]")
     dev = q.device
@@ -259,8 +274,9 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     g, beta = _gate(g, (B, H), dev, "g"), _gate(beta, (B, H), dev, "beta")
     if not isinstance(state, torch.Tensor) or state.dim() != 4 or tuple(state.shape[1:]) != (H, dk, dv) or \
             state.dtype != torch.float32 or state.device != dev or not state[:1].is_contiguous() or \
-            state.stride(0) < H * dk * dv:
-        raise ValueError(f"state must be a float32 tensor [slots,{H},{dk},{dv}] on {dev} whose slots are contiguous")
+            state.stride(0) < H * dk * dv or state.requires_grad:
+        raise ValueError(f"state must be a float32 tensor [slots,{H},{dk},{dv}] on {dev} without gradient, its slots "
+                         "contiguous")
     if slots is None:
         if state.shape[0] < B:
             raise ValueError(f"state has {state.shape[0]} slots for {B} rows")

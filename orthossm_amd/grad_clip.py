@@ -17,7 +17,7 @@ import torch
 
 from . import _native as nat
 from .delta import _scratch, on_device
-from .ops import _current_stream, _dtype_code
+from .ops import _current_stream, _dtype_code, _fast
 
 
 def _dense(t: torch.Tensor) -> bool:
@@ -34,6 +34,11 @@ def _run(grads, max_norm: float, eps: float, scale: bool) -> torch.Tensor:
     if isinstance(grads, torch.Tensor):
         grads = [grads]
     grads = list(grads)
+    fast = _fast()
+    if fast is not None:
+        norm = fast.clip(grads, max_norm, eps, scale)
+        if norm is not None:
+            return norm
     if not grads:
         raise ValueError("no tensors given")
     for i, t in enumerate(grads):

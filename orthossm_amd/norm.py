@@ -20,7 +20,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _native as nat
 from .delta import _dest, _scratch, on_device
-from .ops import _current_stream, _dtype_code
+from .ops import _current_stream, _dtype_code, _fast
 
 
 def _matrix(t: torch.Tensor) -> torch.Tensor:
@@ -63,6 +63,11 @@ def _prepare(x, weight, bias, eps):
 
 
 def _forward(x, weight, bias, eps, out, stats: bool):
+    fast = _fast()
+    if fast is not None and out is None:
+        res = fast.norm_forward(x, weight, bias, eps, stats)
+        if res is not None:
+            return res
     lib = nat.load()
     a, x, keep = _prepare(x, weight, bias, eps)
     dev = x.device
@@ -93,6 +98,11 @@ def layer_norm_backward(grad_y: torch.Tensor, x: torch.Tensor, mean: torch.Tenso
                         need_bias: bool = True):
     """(grad_x in x's type, grad_weight, grad_bias fp32), None for what is not
     needed, from dL/dy, x and what the forward gave."""
+    fast = _fast()
+    if fast is not None:
+        res = fast.norm_backward(grad_y, x, mean, rstd, weight, need_x, need_weight, need_bias)
+        if res is not None:
+            return res
     lib = nat.load()
     a, x, keep = _prepare(x, weight, None, 0.0)
     dev, D = x.device, a.D
