@@ -63,11 +63,10 @@ hipError_t launch_delta_step(const DeltaStepParams& p, int dtype, hipStream_t st
 hipError_t launch_delta_fwd(const DeltaParams& p, int dtype, hipStream_t stream);
 // part: 2 B S H dk floats where q and k heads are shared.
 hipError_t launch_delta_bwd(const DeltaParams& p, float* part, int dtype, hipStream_t stream);
-// The state maps S' = a S + x of n spans of `span` tokens a row applied from
-// init, x receiving the state before each span, fin (or NULL) the last; reverse
-// goes from the last span.
-hipError_t launch_delta_scan(const DeltaParams& p, const float* a, float* x, const float* init, float* fin, int n,
-                             int span, bool reverse, hipStream_t stream);
+// The state maps S' = a S + x of n spans of `span` tokens a row applied from init,
+// x receiving the state before each span; reverse goes from the last span.
+hipError_t launch_delta_scan(const DeltaParams& p, const float* a, float* x, const float* init, int n, int span,
+                             bool reverse, hipStream_t stream);
 
 #ifdef __HIPCC__
 namespace delta {

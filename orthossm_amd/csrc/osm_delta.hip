@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(64) delta_solve_kernel(const DeltaParams p) {
 // the span.  KT = dkp / 16.  What bounds it: the chain of spans, 4 KT matrix
 // instructions and the exchange each.
 template <int KT>
-__global__ void __launch_bounds__(64 * KT) delta_scan_kernel(const float* a, float* x, const float* init, float* fin,
+__global__ void __launch_bounds__(64 * KT) delta_scan_kernel(const float* a, float* x, const float* init,
                                                              const int* lengths, int S, int N, int span, int BH, int H,
                                                              int dk, int dv, int dvp, bool reverse) {
   constexpr int kDkp = 16 * KT, kRow = kDkp + 4;
@@ -211,15 +211,20 @@ __global__ void __launch_bounds__(64 * KT) delta_scan_kernel(const float* a, flo
 #pragma unroll
     for (int i = 0; i < 4; ++i) bn[i] = xp[(int64_t)i * dvp];
   };
-  if (n > 0) fetch(0);
+  if (n > 1) fetch(0);
   for (int c = 0; c < n; ++c) {
+    float* const xp = x + at(c) * kDkp * dvp;
+    if (c == n - 1) {   // the last span's map is not needed
+#pragma unroll
+      for (int i = 0; i < 4; ++i) xp[(int64_t)i * dvp] = s[i];
+      break;
+    }
     float* const buf = st[c & 1];
     *reinterpret_cast<f32x4*>(buf + r * kRow + row) = s;
     f32x4 ac[KT], acc0 = bn, acc1 = zero4();
 #pragma unroll
     for (int k = 0; k < KT; ++k) ac[k] = an[k];
-    float* const xp = x + at(c) * kDkp * dvp;
-    if (c + 1 < n) fetch(c + 1);
+    if (c + 2 < n) fetch(c + 1);
 #pragma unroll
     for (int i = 0; i < 4; ++i) xp[(int64_t)i * dvp] = s[i];
     __syncthreads();
@@ -234,10 +239,6 @@ __global__ void __launch_bounds__(64 * KT) delta_scan_kernel(const float* a, flo
 #pragma unroll
     for (int i = 0; i < 4; ++i) s[i] = acc0[i] + acc1[i];
   }
-  if (fin)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (row + i < dk && col < dv) fin[io + (int64_t)i * dv] = s[i];
 }
 
 // Walks segment blockIdx.x % segs of a head.  MAP: the segment's state map, from
@@ -277,6 +278,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaPa
   }
   const bool fin = !MAP && p.fin && seg == (n > 0 ? (n - 1) / p.seg : 0);
   if (c0 >= c1 && !fin) return;
+  if (MAP && c1 == n) return;   // nothing follows the last segment
   // S: tile t, element i: row 16 t + 4 g + i, column col
   f32x4 S[ST];
   const bool ws = !MAP && p.segs > 1 && n > 0;
@@ -523,7 +525,7 @@ hipError_t forward(const DeltaParams& p, hipStream_t stream) {
     launch_walk<T, KS, true>(p, stream);
     e = hipGetLastError();
     if (e == hipSuccess)
-      e = launch_delta_scan(p, p.a, p.x, p.init, nullptr, p.segs, p.seg * kDeltaChunk, false, stream);
+      e = launch_delta_scan(p, p.a, p.x, p.init, p.segs, p.seg * kDeltaChunk, false, stream);
   }
   if (e != hipSuccess) return e;
   launch_walk<T, KS, false>(p, stream);
@@ -550,13 +552,13 @@ int delta_segment(int64_t heads, int64_t chunks) {
   return (int)((chunks + segs - 1) / segs);
 }
 
-hipError_t launch_delta_scan(const DeltaParams& p, const float* a, float* x, const float* init, float* fin, int n,
-                             int span, bool reverse, hipStream_t stream) {
+hipError_t launch_delta_scan(const DeltaParams& p, const float* a, float* x, const float* init, int n, int span,
+                             bool reverse, hipStream_t stream) {
   const int BH = p.B * p.H, ns = p.dvp / kDeltaSlice;
   const dim3 grid((unsigned)(8 * (int64_t)ns * ((BH + 7) / 8)));
   auto go = [&](auto kt) {
     constexpr int KT = decltype(kt)::value;
-    hipLaunchKernelGGL((delta_scan_kernel<KT>), grid, dim3(64 * KT), 0, stream, a, x, init, fin, p.lengths, p.S, n, span,
+    hipLaunchKernelGGL((delta_scan_kernel<KT>), grid, dim3(64 * KT), 0, stream, a, x, init, p.lengths, p.S, n, span,
                        BH, p.H, p.dk_, p.dv_, p.dvp, reverse);
   };
   switch (p.dkp / 32) {

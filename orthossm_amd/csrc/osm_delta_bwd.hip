@@ -86,6 +86,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_rewalk_kernel(const Delta
     }
   }
   if (c0 >= c1 && !first) return;
+  if (MAP && c0 == 0) return;   // nothing comes before the first segment
   f32x4 D[ST];
   const bool ws = !MAP && p.segs > 1 && n > 0;
   const float* const from =
@@ -1107,7 +1108,7 @@ hipError_t walks(const DeltaParams& p, hipStream_t stream) {
     launch_rewalk<T, KS, true>(p, stream);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess)
-      e = launch_delta_scan(p, p.a, p.x, p.grad_state, nullptr, p.segs, p.seg * kDeltaChunk, true, stream);
+      e = launch_delta_scan(p, p.a, p.x, p.grad_state, p.segs, p.seg * kDeltaChunk, true, stream);
     if (e != hipSuccess) return e;
   }
   launch_rewalk<T, KS, false>(p, stream);

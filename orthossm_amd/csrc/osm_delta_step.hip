@@ -4,8 +4,10 @@
 // one read of the state:
 //   u = beta (v - e^g a),  o = scale (e^g b + (k.q) u),  S <- e^g S + k u
 //
-// A workgroup holds 32 columns of a head's state in registers, its 8 row groups
-// of R rows each added through two waves' shuffle and LDS: one barrier a token.
+// A workgroup holds 32 columns of a head's state in registers, in row groups of R
+// rows that are added through a wave's shuffles and LDS: one barrier a token.  A
+// thread holds NC neighbouring columns: four (16-byte accesses) where rows allow it
+// and the state is large, one else.
 // One token is bound by the state's bytes (read and written once, 128-byte
 // pieces of rows), or by the launch when there are few rows.
 #include "osm_delta.h"
@@ -15,92 +17,131 @@ namespace {
 
 using namespace delta;
 
-constexpr int kCols = 32, kGroups = 8, kStepThreads = kCols * kGroups;
+constexpr int kCols = 32, kStepThreads = 256;
 
-template <typename T, int R>
+template <typename T, int R, int NC>
 __global__ void __launch_bounds__(kStepThreads) delta_step_kernel(const DeltaStepParams p) {
-  constexpr int kRows = R * kGroups;
+  constexpr int kLanes = kCols / NC, kGroups = kStepThreads / kLanes, kRows = R * kGroups;
   __shared__ __attribute__((aligned(16))) float kq[2][2][kRows];
-  __shared__ float red[2][4][3][kCols];
+  __shared__ float red[2][4][2 * NC + 1][kLanes];
   const int ncb = (p.dv_ + kCols - 1) / kCols;
-  const int tid = threadIdx.x, jl = tid % kCols, kg = tid / kCols, wave = tid >> 6;
-  const int j = kCols * (int)(blockIdx.x % ncb) + jl, bh = blockIdx.x / ncb;
+  const int tid = threadIdx.x, jl = tid % kLanes, kg = tid / kLanes, wave = tid >> 6;
+  const int j = kCols * (int)(blockIdx.x % ncb) + NC * jl, bh = blockIdx.x / ncb;
   const int b = bh / p.H, h = bh - b * p.H, hk = h / (p.H / p.Hk);
   const bool live = j < p.dv_;
   const int64_t slot = p.slots ? p.slots[b] : b;
   T* const o = row_ptr<T>(p.o, b, 0, h) + j;
   if (slot < 0 || slot >= p.n_slots) {   // an idle row, or (past the pool) a wrong one: its outputs are NaN
     if (live && kg == 0)
-      for (int t = 0; t < p.S; ++t) o[t * p.o.ss] = (T)(slot < 0 ? 0.0f : __builtin_nanf(""));
+      for (int t = 0; t < p.S; ++t)
+        for (int c = 0; c < NC; ++c) o[t * p.o.ss + c] = (T)(slot < 0 ? 0.0f : __builtin_nanf(""));
     return;
   }
   const int n = p.lengths ? min(max(p.lengths[b], 0), p.S) : p.S;
   const int64_t at = slot * p.state_s + (int64_t)h * p.dk_ * p.dv_ + j;
-  float s[R];
+  typedef float Cols __attribute__((ext_vector_type(NC)));
+  Cols s[R];   // row kg + kGroups i
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    const int row = kg * R + i;
-    s[i] = p.init && live && row < p.dk_ ? p.init[at + (int64_t)row * p.dv_] : 0.0f;
+    const int row = kg + kGroups * i;
+    s[i] = p.init && live && row < p.dk_ ? *reinterpret_cast<const Cols*>(p.init + at + (int64_t)row * p.dv_) : (Cols)0.0f;
   }
-  // k and q of a token: threads 0 .. kRows-1, and the next kRows
-  const bool is_q = tid >= kRows;
-  const int e = is_q ? tid - kRows : tid;
-  auto fetch = [&](int t) {
-    if (tid >= 2 * kRows || e >= p.dk_) return 0.0f;
-    return (float)(is_q ? row_ptr<T>(p.q, b, t, hk) : row_ptr<T>(p.k, b, t, hk))[e];
+  // k and q of a token
+  auto fetch = [&](int t, int e) {
+    const bool is_q = e >= kRows;
+    e -= is_q ? kRows : 0;
+    return e < p.dk_ ? (float)(is_q ? row_ptr<T>(p.q, b, t, hk) : row_ptr<T>(p.k, b, t, hk))[e] : 0.0f;
   };
-  if (n > 0 && tid < 2 * kRows) kq[0][is_q][e] = fetch(0);
+  static_assert(2 * kRows <= 2 * kStepThreads, "two values of k and q a thread at most");
+  if (n > 0)
+    for (int e = tid; e < 2 * kRows; e += kStepThreads) (&kq[0][0][0])[e] = fetch(0, e);
   __syncthreads();
   for (int t = 0; t < n; ++t) {
     const int par = t & 1;
-    const float next = t + 1 < n ? fetch(t + 1) : 0.0f;
+    float next[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (tid + e * kStepThreads < 2 * kRows) next[e] = t + 1 < n ? fetch(t + 1, tid + e * kStepThreads) : 0.0f;
     const float decay = expf(*row_ptr<float>(p.g, b, t, h)), beta = *row_ptr<float>(p.beta, b, t, h);
-    const float v = live ? (float)row_ptr<T>(p.v, b, t, h)[j] : 0.0f;
-    float kk[R], sum[3] = {0.0f, 0.0f, 0.0f};
+    Cols v = (Cols)0.0f;
+    if (live)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) v[c] = (float)row_ptr<T>(p.v, b, t, h)[j + c];
+    float kk[R], kv = 0.0f;
+    Cols sk = (Cols)0.0f, sq = (Cols)0.0f;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      const float q = kq[par][1][kg * R + i];
-      kk[i] = kq[par][0][kg * R + i];
-      sum[0] = __builtin_fmaf(s[i], kk[i], sum[0]);
-      sum[1] = __builtin_fmaf(s[i], q, sum[1]);
-      sum[2] = __builtin_fmaf(q, kk[i], sum[2]);
+      const float q = kq[par][1][kg + kGroups * i];
+      kk[i] = kq[par][0][kg + kGroups * i];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        sk[c] = __builtin_fmaf(s[i][c], kk[i], sk[c]);
+        sq[c] = __builtin_fmaf(s[i][c], q, sq[c]);
+      }
+      kv = __builtin_fmaf(q, kk[i], kv);
+    }
+    float sum[2 * NC + 1];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      sum[c] = sk[c];
+      sum[NC + c] = sq[c];
+    }
+    sum[2 * NC] = kv;
+#pragma unroll
+    for (int c = 0; c < 2 * NC + 1; ++c) {
+#pragma unroll
+      for (int m = kLanes; m < 64; m <<= 1) sum[c] += __shfl_xor(sum[c], m);
+      if ((tid & 63) < kLanes) red[par][wave][c][jl] = sum[c];
     }
 #pragma unroll
-    for (int c = 0; c < 3; ++c) {
-      sum[c] += __shfl_xor(sum[c], 32);
-      if ((tid & 32) == 0) red[par][wave][c][jl] = sum[c];
-    }
-    if (tid < 2 * kRows) kq[par ^ 1][is_q][e] = next;
+    for (int e = 0; e < 2; ++e)
+      if (tid + e * kStepThreads < 2 * kRows) (&kq[par ^ 1][0][0])[tid + e * kStepThreads] = next[e];
     __syncthreads();
 #pragma unroll
-    for (int c = 0; c < 3; ++c)
+    for (int c = 0; c < 2 * NC + 1; ++c)
       sum[c] = (red[par][0][c][jl] + red[par][1][c][jl]) + (red[par][2][c][jl] + red[par][3][c][jl]);
-    const float u = beta * (v - decay * sum[0]);
+    Cols u;
 #pragma unroll
-    for (int i = 0; i < R; ++i) s[i] = __builtin_fmaf(kk[i], u, decay * s[i]);
-    if (live && kg == 0) o[t * p.o.ss] = (T)(p.scale * __builtin_fmaf(sum[2], u, decay * sum[1]));
+    for (int c = 0; c < NC; ++c) u[c] = beta * (v[c] - decay * sum[c]);
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) s[i][c] = __builtin_fmaf(kk[i], u[c], decay * s[i][c]);
+    if (live && kg == 0)
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        o[t * p.o.ss + c] = (T)(p.scale * __builtin_fmaf(sum[2 * NC], u[c], decay * sum[NC + c]));
   }
   if (live && kg == 0)
-    for (int t = n; t < p.S; ++t) o[t * p.o.ss] = (T)0.0f;
+    for (int t = n; t < p.S; ++t)
+      for (int c = 0; c < NC; ++c) o[t * p.o.ss + c] = (T)0.0f;
   if (p.fin && live)
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      const int row = kg * R + i;
-      if (row < p.dk_) p.fin[at + (int64_t)row * p.dv_] = s[i];
+      const int row = kg + kGroups * i;
+      if (row < p.dk_) {
+        *reinterpret_cast<Cols*>(p.fin + at + (int64_t)row * p.dv_) = s[i];
+        if (NC == 4) asm volatile("s_nop 1" ::: "memory");   // (see store4 in osm_delta.h)
+      }
     }
 }
 
 template <typename T>
 hipError_t step(const DeltaStepParams& p, hipStream_t stream) {
   const dim3 grid((unsigned)((int64_t)p.B * p.H * ((p.dv_ + kCols - 1) / kCols))), block(kStepThreads);
-  if (p.dk_ <= 16)
-    hipLaunchKernelGGL((delta_step_kernel<T, 2>), grid, block, 0, stream, p);
+  const bool quads = p.dv_ % 4 == 0 && p.state_s % 4 == 0 && ((uintptr_t)p.init | (uintptr_t)p.fin) % 16 == 0;
+  if (quads && p.dk_ > 64)
+    hipLaunchKernelGGL((delta_step_kernel<T, 4, 4>), grid, block, 0, stream, p);
+  else if (quads && p.dk_ > 32)
+    hipLaunchKernelGGL((delta_step_kernel<T, 2, 4>), grid, block, 0, stream, p);
+  else if (p.dk_ <= 16)
+    hipLaunchKernelGGL((delta_step_kernel<T, 2, 1>), grid, block, 0, stream, p);
   else if (p.dk_ <= 32)
-    hipLaunchKernelGGL((delta_step_kernel<T, 4>), grid, block, 0, stream, p);
+    hipLaunchKernelGGL((delta_step_kernel<T, 4, 1>), grid, block, 0, stream, p);
   else if (p.dk_ <= 64)
-    hipLaunchKernelGGL((delta_step_kernel<T, 8>), grid, block, 0, stream, p);
+    hipLaunchKernelGGL((delta_step_kernel<T, 8, 1>), grid, block, 0, stream, p);
   else
-    hipLaunchKernelGGL((delta_step_kernel<T, 16>), grid, block, 0, stream, p);
+    hipLaunchKernelGGL((delta_step_kernel<T, 16, 1>), grid, block, 0, stream, p);
   return hipGetLastError();
 }
 
