@@ -17,6 +17,7 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/version.h>
 
@@ -657,17 +658,75 @@ bool as_scale(PyObject* o, int64_t dk, float* v) {
   return as_float(o, v);
 }
 
+std::optional<at::Tensor> optional_tensor(PyObject* o) {
+  return o == Py_None ? std::nullopt : std::optional<at::Tensor>(*plain(o));
+}
+
+// ---- in the autograd engine's threads, which run without the interpreter's lock ----
+
+// The interpreter's lock, for a scope.
+struct Gil {
+  PyGILState_STATE s = PyGILState_Ensure();
+  ~Gil() { PyGILState_Release(s); }
+};
+
+[[noreturn]] void throw_python() {
+  python_error e;
+  e.persist();
+  throw e;
+}
+
+// The stream that the engine has made current: the forward's.
+void* engine_stream(const at::Tensor& x) {
+  const Gil gil;
+  Ref obj;
+  void* stream;
+  if (!stream_of(x, &obj, &stream)) throw_python();
+  return stream;
+}
+
+// The Python error of a status code, thrown.
+void throw_rc(int rc) {
+  if (rc == OSM_OK) return;
+  const Gil gil;
+  fail_rc(rc);
+  throw_python();
+}
+
+// Gradients that are themselves part of a graph (create_graph): the identity,
+// with a backward that refuses.
+struct Once : torch::autograd::Function<Once> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext*, at::TensorList grads, at::TensorList) {
+    torch::autograd::variable_list res;
+    for (const at::Tensor& t : grads) res.push_back(t.view_as(t));
+    return res;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, torch::autograd::variable_list) {
+    TORCH_CHECK(false, "trying to differentiate twice a function that can be differentiated once only");
+  }
+};
+torch::autograd::variable_list once(torch::autograd::variable_list res, const torch::autograd::variable_list& of) {
+  if (!at::GradMode::is_enabled()) return res;
+  torch::autograd::variable_list grads, from;
+  for (const at::Tensor& t : res)
+    if (t.defined()) grads.push_back(t);
+  for (const at::Tensor& t : of)
+    if (t.defined()) from.push_back(t);
+  const torch::autograd::variable_list refusing = Once::apply(at::TensorList(grads), at::TensorList(from));
+  size_t i = 0;
+  for (at::Tensor& t : res)
+    if (t.defined()) t = refusing[i++];
+  return res;
+}
+
 struct Delta {
   const at::Tensor* t[5];        // q, k, v, g, beta
   osm_delta_args a{};
 };
 
-// args: q, k, v, g, beta, scale, lengths.
-bool delta_common(PyObject* const* p, Delta* d) {
-  for (int i = 0; i < 5; ++i) {
-    d->t[i] = plain(p[i]);
-    if (!d->t[i] || !d->t[i]->is_cuda() || d->t[i]->dim() != (i < 3 ? 4 : 3)) return false;
-  }
+bool delta_tensors(Delta* d) {
+  for (int i = 0; i < 5; ++i)
+    if (!d->t[i]->is_cuda() || d->t[i]->dim() != (i < 3 ? 4 : 3)) return false;
   const at::Tensor &q = *d->t[0], &k = *d->t[1], &v = *d->t[2];
   if (!(is_f32(q) || is_bf16(q)) || k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type()) return false;
   osm_delta_args& a = d->a;
@@ -695,6 +754,16 @@ bool delta_common(PyObject* const* p, Delta* d) {
   a.v = rows_of(v);
   a.g = rows_of(*d->t[3]);
   a.beta = rows_of(*d->t[4]);
+  return true;
+}
+
+// args: q, k, v, g, beta, scale, lengths.
+bool delta_common(PyObject* const* p, Delta* d) {
+  for (int i = 0; i < 5; ++i)
+    if (!(d->t[i] = plain(p[i]))) return false;
+  if (!delta_tensors(d)) return false;
+  const at::Tensor& q = *d->t[0];
+  osm_delta_args& a = d->a;
   if (!as_scale(p[5], a.dk, &a.scale)) return false;
   if (p[6] != Py_None) {
     const at::Tensor* t = plain(p[6]);
@@ -718,6 +787,51 @@ bool state_ptr(PyObject* o, const Delta& d, float** out) {
   return true;
 }
 
+// A gradient of the output as the kernels read it.
+bool delta_grad_form(const at::Tensor& go, const at::Tensor& v) {
+  return go.dim() == 4 && go.sizes() == v.sizes() && go.scalar_type() == v.scalar_type() && go.device() == v.device() &&
+         token_rows(go, v.size(3));
+}
+
+// The forward into new tensors, those of `fin` and `saved` where wanted.
+int delta_forward(Delta& d, bool want_state, bool save, void* stream, at::Tensor* out, at::Tensor* fin, at::Tensor* saved) {
+  const at::Tensor& q = *d.t[0];
+  osm_delta_args& a = d.a;
+  *out = empty({a.B, a.S, a.H, a.dv}, q, q.scalar_type());
+  a.out = rows_of(*out);
+  if (want_state) {
+    *fin = empty({a.B, a.H, a.dk, a.dv}, q, at::kFloat);
+    a.state_out = fptr(*fin);
+  }
+  if (save) {
+    *saved = scratch(lib.delta_saved(&a), q);
+    a.saved = saved->data_ptr();
+  }
+  const at::Tensor ws = scratch(lib.delta_bytes(&a), q);
+  return lib.delta_fwd(&a, ws.data_ptr(), (size_t)ws.numel(), stream);
+}
+
+// The six gradients into new tensors, that of the first state where needed.
+int delta_backward(Delta& d, const at::Tensor& go, float* grad_state, bool need_init, void* stream, at::Tensor* gr) {
+  const at::Tensor& q = *d.t[0];
+  osm_delta_args& a = d.a;
+  osm_delta_bwd_args b{};
+  b.grad_out = rows_of(go);
+  b.grad_state = grad_state;
+  for (int i = 0; i < 5; ++i) gr[i] = empty(d.t[i]->sizes(), q, d.t[i]->scalar_type());
+  b.grad_q = rows_of(gr[0]);
+  b.grad_k = rows_of(gr[1]);
+  b.grad_v = rows_of(gr[2]);
+  b.grad_g = rows_of(gr[3]);
+  b.grad_beta = rows_of(gr[4]);
+  if (need_init) {
+    gr[5] = empty({a.B, a.H, a.dk, a.dv}, q, at::kFloat);
+    b.grad_init = fptr(gr[5]);
+  }
+  const at::Tensor ws = scratch(lib.delta_bwd_bytes(&a), q);
+  return lib.delta_bwd(&a, &b, ws.data_ptr(), (size_t)ws.numel(), stream);
+}
+
 // delta_forward(<common 7>, state_init, want_state, save): None, or (out, state | None, saved | None).
 PyObject* run_delta_forward(PyObject* const* p) {
   Delta d;
@@ -725,29 +839,16 @@ PyObject* run_delta_forward(PyObject* const* p) {
   if (!delta_common(p, &d) || !state_ptr(p[7], d, &init)) Py_RETURN_NONE;
   const bool want_state = PyObject_IsTrue(p[8]) == 1, save = PyObject_IsTrue(p[9]) == 1;
   if (PyErr_Occurred()) return nullptr;
-  const at::Tensor& q = *d.t[0];
-  osm_delta_args& a = d.a;
-  a.state_init = init;
+  d.a.state_init = init;
   Ref s_obj;
   void* stream;
-  const c10::DeviceGuard guard(q.device());
-  if (!stream_of(q, &s_obj, &stream)) return nullptr;
-  at::Tensor out, fin, saved, ws;
+  const c10::DeviceGuard guard(d.t[0]->device());
+  if (!stream_of(*d.t[0], &s_obj, &stream)) return nullptr;
+  at::Tensor out, fin, saved;
   int rc;
   {
     const NoGil nogil;
-    out = empty({a.B, a.S, a.H, a.dv}, q, q.scalar_type());
-    a.out = rows_of(out);
-    if (want_state) {
-      fin = empty({a.B, a.H, a.dk, a.dv}, q, at::kFloat);
-      a.state_out = fptr(fin);
-    }
-    if (save) {
-      saved = scratch(lib.delta_saved(&a), q);
-      a.saved = saved.data_ptr();
-    }
-    ws = scratch(lib.delta_bytes(&a), q);
-    rc = lib.delta_fwd(&a, ws.data_ptr(), (size_t)ws.numel(), stream);
+    rc = delta_forward(d, want_state, save, stream, &out, &fin, &saved);
   }
   if (rc != OSM_OK) return fail_rc(rc);
   return Py_BuildValue("(NNN)", THPVariable_Wrap(out), wrap_or_none(fin), wrap_or_none(saved));
@@ -760,40 +861,105 @@ PyObject* run_delta_backward(PyObject* const* p) {
   if (!delta_common(p, &d) || !state_ptr(p[9], d, &gs)) Py_RETURN_NONE;
   const at::Tensor &q = *d.t[0], &v = *d.t[2];
   const at::Tensor *saved = plain(p[7]), *go = plain(p[8]);
-  if (!saved || !go || go->dim() != 4 || go->sizes() != v.sizes() || go->scalar_type() != v.scalar_type() ||
-      go->device() != q.device() || !token_rows(*go, v.size(3)))
-    Py_RETURN_NONE;
+  if (!saved || !go || !delta_grad_form(*go, v)) Py_RETURN_NONE;
   const bool need_init = PyObject_IsTrue(p[10]) == 1;
   if (PyErr_Occurred()) return nullptr;
-  osm_delta_args& a = d.a;
-  a.saved = saved->data_ptr();
-  osm_delta_bwd_args b{};
-  b.grad_out = rows_of(*go);
-  b.grad_state = gs;
+  d.a.saved = saved->data_ptr();
   Ref s_obj;
   void* stream;
   const c10::DeviceGuard guard(q.device());
   if (!stream_of(q, &s_obj, &stream)) return nullptr;
-  at::Tensor gr[5], gi, ws;
+  at::Tensor gr[6];
   int rc;
   {
     const NoGil nogil;
-    for (int i = 0; i < 5; ++i) gr[i] = empty(d.t[i]->sizes(), q, d.t[i]->scalar_type());
-    b.grad_q = rows_of(gr[0]);
-    b.grad_k = rows_of(gr[1]);
-    b.grad_v = rows_of(gr[2]);
-    b.grad_g = rows_of(gr[3]);
-    b.grad_beta = rows_of(gr[4]);
-    if (need_init) {
-      gi = empty({a.B, a.H, a.dk, a.dv}, q, at::kFloat);
-      b.grad_init = fptr(gi);
-    }
-    ws = scratch(lib.delta_bwd_bytes(&a), q);
-    rc = lib.delta_bwd(&a, &b, ws.data_ptr(), (size_t)ws.numel(), stream);
+    rc = delta_backward(d, *go, gs, need_init, stream, gr);
   }
   if (rc != OSM_OK) return fail_rc(rc);
   return Py_BuildValue("(NNNNNN)", THPVariable_Wrap(gr[0]), THPVariable_Wrap(gr[1]), THPVariable_Wrap(gr[2]),
-                       THPVariable_Wrap(gr[3]), THPVariable_Wrap(gr[4]), wrap_or_none(gi));
+                       THPVariable_Wrap(gr[3]), THPVariable_Wrap(gr[4]), wrap_or_none(gr[5]));
+}
+
+// The differentiable form: what the Python module's autograd function keeps and
+// gives, without the interpreter between the engine and the launches.
+struct DeltaCall {
+  Delta* d;
+  void* stream;
+  int rc;
+};
+struct DeltaGrad : torch::autograd::Function<DeltaGrad> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q,
+                                                const at::Tensor& k, const at::Tensor& v, const at::Tensor& g,
+                                                const at::Tensor& beta, const std::optional<at::Tensor>& init,
+                                                const std::optional<at::Tensor>& lengths, DeltaCall* c) {
+    ctx->set_materialize_grads(false);   // an unused output's gradient stays undefined
+    at::Tensor out, fin, saved;
+    c->rc = delta_forward(*c->d, true, true, c->stream, &out, &fin, &saved);
+    ctx->save_for_backward({q, k, v, g, beta, lengths ? *lengths : at::Tensor(), saved});
+    int64_t need = 0;
+    const at::Tensor* const t[6] = {&q, &k, &v, &g, &beta, init ? &*init : nullptr};
+    for (int i = 0; i < 6; ++i) need |= (int64_t)(t[i] && t[i]->requires_grad()) << i;
+    ctx->saved_data["need"] = need;
+    ctx->saved_data["scale"] = (double)c->d->a.scale;
+    return {out, fin};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto t = ctx->get_saved_variables();
+    const int64_t need = ctx->saved_data["need"].toInt();
+    at::Tensor gr[6];
+    {
+      const at::NoGradGuard no_grad;
+      Delta d;
+      for (int i = 0; i < 5; ++i) d.t[i] = &t[i];
+      TORCH_CHECK(delta_tensors(&d), "gated_delta: a saved tensor came back in another form");
+      d.a.scale = (float)ctx->saved_data["scale"].toDouble();
+      if (t[5].defined()) d.a.lengths = static_cast<const int32_t*>(t[5].data_ptr());
+      d.a.saved = t[6].data_ptr();
+      const c10::DeviceGuard guard(t[0].device());
+      at::Tensor go = grads[0].defined() ? grads[0] : at::zeros_like(t[2]);
+      if (!delta_grad_form(go, t[2])) go = go.to(t[2].options()).contiguous();
+      const at::Tensor gs = grads[1].defined() ? grads[1].to(at::kFloat).contiguous() : at::Tensor();
+      throw_rc(delta_backward(d, go, gs.defined() ? fptr(gs) : nullptr, need >> 5 & 1, engine_stream(t[0]), gr));
+    }
+    torch::autograd::variable_list res(8);
+    for (int i = 0; i < 6; ++i)
+      if (need >> i & 1) res[i] = gr[i];
+    return once(std::move(res), {grads[0], grads[1], t[0], t[1], t[2], t[3], t[4]});
+  }
+};
+
+// gated_delta(<common 7>, state_init, return_state): None, or (out, state | None) with their gradient's function.
+PyObject* run_gated_delta(PyObject* const* p) {
+  Delta d;
+  float* init;
+  if (!delta_common(p, &d) || !state_ptr(p[7], d, &init)) Py_RETURN_NONE;
+  const bool want_state = PyObject_IsTrue(p[8]) == 1;
+  if (PyErr_Occurred()) return nullptr;
+  d.a.state_init = init;
+  Ref s_obj;
+  void* stream;
+  const c10::DeviceGuard guard(d.t[0]->device());
+  if (!stream_of(*d.t[0], &s_obj, &stream)) return nullptr;
+  const std::optional<at::Tensor> first = optional_tensor(p[7]), lengths = optional_tensor(p[6]);
+  bool grad = first && first->requires_grad();
+  for (int i = 0; i < 5; ++i) grad = grad || d.t[i]->requires_grad();
+  at::Tensor out, fin, saved;
+  int rc;
+  {
+    const NoGil nogil;
+    if (grad && at::GradMode::is_enabled()) {
+      DeltaCall c{&d, stream, OSM_OK};
+      const auto res = DeltaGrad::apply(*d.t[0], *d.t[1], *d.t[2], *d.t[3], *d.t[4], first, lengths, &c);
+      rc = c.rc;
+      out = res[0];
+      if (want_state) fin = res[1];
+    } else {
+      rc = delta_forward(d, want_state, false, stream, &out, &fin, &saved);
+    }
+  }
+  if (rc != OSM_OK) return fail_rc(rc);
+  return Py_BuildValue("(NN)", THPVariable_Wrap(out), wrap_or_none(fin));
 }
 
 // delta_step(q, k, v, g, beta, state, scale, slots): None, or out.
@@ -883,6 +1049,50 @@ void norm_args(const at::Tensor& x, osm_norm_args* a) {
   a->x_stride = a->D;
 }
 
+// A gradient of the output as the kernels read it.
+bool norm_grad_form(const at::Tensor& gy, const at::Tensor& x) {
+  return norm_rows(&gy) && gy.sizes() == x.sizes() && gy.scalar_type() == x.scalar_type() && gy.device() == x.device();
+}
+
+// The forward into new tensors, those of the statistics where wanted.
+int norm_forward(osm_norm_args& a, const at::Tensor& x, bool stats, void* stream, at::Tensor* y, at::Tensor* mean,
+                 at::Tensor* rstd) {
+  *y = empty(x.sizes(), x, x.scalar_type());
+  a.y = y->data_ptr();
+  a.y_stride = a.D;
+  if (stats) {
+    const at::IntArrayRef lead = x.sizes().slice(0, x.dim() - 1);
+    *mean = empty(lead, x, at::kFloat);
+    *rstd = empty(lead, x, at::kFloat);
+    a.mean = fptr(*mean);
+    a.rstd = fptr(*rstd);
+  }
+  return lib.norm_fwd(&a, stream);
+}
+
+// The gradients that are needed, to x, weight and bias, into new tensors.
+int norm_backward(const osm_norm_args& a, const at::Tensor& x, const at::Tensor& gy, const bool* need, void* stream,
+                  at::Tensor* gr) {
+  osm_norm_bwd_args b{};
+  b.grad_y = gy.data_ptr();
+  b.grad_y_stride = a.D;
+  if (need[0]) {
+    gr[0] = empty(x.sizes(), x, x.scalar_type());
+    b.grad_x = gr[0].data_ptr();
+    b.grad_x_stride = a.D;
+  }
+  if (need[1]) {
+    gr[1] = empty({a.D}, x, at::kFloat);
+    b.grad_weight = fptr(gr[1]);
+  }
+  if (need[2]) {
+    gr[2] = empty({a.D}, x, at::kFloat);
+    b.grad_bias = fptr(gr[2]);
+  }
+  const at::Tensor ws = scratch(lib.norm_bwd_bytes(&a), x);
+  return lib.norm_bwd(&a, &b, ws.data_ptr(), (size_t)ws.numel(), stream);
+}
+
 // norm_forward(x, weight, bias, eps, stats): None, or (y, mean | None, rstd | None).
 PyObject* run_norm_forward(PyObject* const* p) {
   const at::Tensor* const xp = plain(p[0]);
@@ -901,17 +1111,7 @@ PyObject* run_norm_forward(PyObject* const* p) {
   int rc;
   {
     const NoGil nogil;
-    y = empty(x.sizes(), x, x.scalar_type());
-    a.y = y.data_ptr();
-    a.y_stride = a.D;
-    if (stats) {
-      const at::IntArrayRef lead = x.sizes().slice(0, x.dim() - 1);
-      mean = empty(lead, x, at::kFloat);
-      rstd = empty(lead, x, at::kFloat);
-      a.mean = fptr(mean);
-      a.rstd = fptr(rstd);
-    }
-    rc = lib.norm_fwd(&a, stream);
+    rc = norm_forward(a, x, stats, stream, &y, &mean, &rstd);
   }
   if (rc != OSM_OK) return fail_rc(rc);
   return Py_BuildValue("(NNN)", THPVariable_Wrap(y), wrap_or_none(mean), wrap_or_none(rstd));
@@ -921,12 +1121,11 @@ PyObject* run_norm_forward(PyObject* const* p) {
 // (grad_x | None, grad_weight | None, grad_bias | None).
 PyObject* run_norm_backward(PyObject* const* p) {
   const at::Tensor *const gyp = plain(p[0]), *const xp = plain(p[1]), *const mp = plain(p[2]), *const rp = plain(p[3]);
-  if (!norm_rows(xp) || !norm_rows(gyp) || !mp || !rp) Py_RETURN_NONE;
+  if (!norm_rows(xp) || !gyp || !norm_grad_form(*gyp, *xp) || !mp || !rp) Py_RETURN_NONE;
   const at::Tensor& x = *xp;
   osm_norm_args a{};
   norm_args(x, &a);
-  if (gyp->sizes() != x.sizes() || gyp->scalar_type() != x.scalar_type() || gyp->device() != x.device() ||
-      !f32_flat(*mp, a.rows, x) || !f32_flat(*rp, a.rows, x) || mp->dim() != x.dim() - 1 || rp->dim() != x.dim() - 1 ||
+  if (!f32_flat(*mp, a.rows, x) || !f32_flat(*rp, a.rows, x) || mp->dim() != x.dim() - 1 || rp->dim() != x.dim() - 1 ||
       !norm_param(p[4], a.D, x, &a.weight))
     Py_RETURN_NONE;
   a.mean = fptr(*mp);
@@ -938,31 +1137,83 @@ PyObject* run_norm_backward(PyObject* const* p) {
   void* stream;
   const c10::DeviceGuard guard(x.device());
   if (!stream_of(x, &s_obj, &stream)) return nullptr;
-  at::Tensor gx, gw, gb, ws;
-  osm_norm_bwd_args b{};
-  b.grad_y = gyp->data_ptr();
-  b.grad_y_stride = a.D;
+  at::Tensor gr[3];
   int rc;
   {
     const NoGil nogil;
-    if (need[0]) {
-      gx = empty(x.sizes(), x, x.scalar_type());
-      b.grad_x = gx.data_ptr();
-      b.grad_x_stride = a.D;
-    }
-    if (need[1]) {
-      gw = empty({a.D}, x, at::kFloat);
-      b.grad_weight = fptr(gw);
-    }
-    if (need[2]) {
-      gb = empty({a.D}, x, at::kFloat);
-      b.grad_bias = fptr(gb);
-    }
-    ws = scratch(lib.norm_bwd_bytes(&a), x);
-    rc = lib.norm_bwd(&a, &b, ws.data_ptr(), (size_t)ws.numel(), stream);
+    rc = norm_backward(a, x, *gyp, need, stream, gr);
   }
   if (rc != OSM_OK) return fail_rc(rc);
-  return Py_BuildValue("(NNN)", wrap_or_none(gx), wrap_or_none(gw), wrap_or_none(gb));
+  return Py_BuildValue("(NNN)", wrap_or_none(gr[0]), wrap_or_none(gr[1]), wrap_or_none(gr[2]));
+}
+
+// The differentiable form (see DeltaGrad).
+struct NormCall {
+  osm_norm_args* a;
+  void* stream;
+  int rc;
+};
+struct NormGrad : torch::autograd::Function<NormGrad> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x,
+                            const std::optional<at::Tensor>& weight, const std::optional<at::Tensor>& bias, NormCall* c) {
+    at::Tensor y, mean, rstd;
+    c->rc = norm_forward(*c->a, x, true, c->stream, &y, &mean, &rstd);
+    ctx->save_for_backward({x, mean, rstd, weight ? *weight : at::Tensor()});
+    ctx->saved_data["need"] = (int64_t)(x.requires_grad() | (weight && weight->requires_grad()) << 1 |
+                                        (bias && bias->requires_grad()) << 2);
+    return y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto t = ctx->get_saved_variables();
+    const int64_t bits = ctx->saved_data["need"].toInt();
+    const bool need[3] = {(bits & 1) != 0, (bits & 2) != 0, (bits & 4) != 0};
+    torch::autograd::variable_list res(4);
+    {
+      const at::NoGradGuard no_grad;
+      const at::Tensor& x = t[0];
+      TORCH_CHECK(norm_rows(&x), "layer_norm: a saved tensor came back in another form");
+      osm_norm_args a{};
+      norm_args(x, &a);
+      a.mean = fptr(t[1]);
+      a.rstd = fptr(t[2]);
+      if (t[3].defined()) a.weight = fptr(t[3]);
+      const c10::DeviceGuard guard(x.device());
+      const at::Tensor gy = norm_grad_form(grads[0], x) ? grads[0] : grads[0].to(x.options()).contiguous();
+      throw_rc(norm_backward(a, x, gy, need, engine_stream(x), res.data()));
+    }
+    return once(std::move(res), {grads[0], t[0], t[3]});
+  }
+};
+
+// layer_norm(x, weight, bias, eps): None, or y with its gradient's function.
+PyObject* run_layer_norm(PyObject* const* p) {
+  const at::Tensor* const xp = plain(p[0]);
+  if (!norm_rows(xp)) Py_RETURN_NONE;
+  const at::Tensor& x = *xp;
+  osm_norm_args a{};
+  norm_args(x, &a);
+  if (!norm_param(p[1], a.D, x, &a.weight) || !norm_param(p[2], a.D, x, &a.bias) || !as_float(p[3], &a.eps)) Py_RETURN_NONE;
+  Ref s_obj;
+  void* stream;
+  const c10::DeviceGuard guard(x.device());
+  if (!stream_of(x, &s_obj, &stream)) return nullptr;
+  const std::optional<at::Tensor> weight = optional_tensor(p[1]), bias = optional_tensor(p[2]);
+  const bool grad = x.requires_grad() || (weight && weight->requires_grad()) || (bias && bias->requires_grad());
+  at::Tensor y, mean, rstd;
+  int rc;
+  {
+    const NoGil nogil;
+    if (grad && at::GradMode::is_enabled()) {
+      NormCall c{&a, stream, OSM_OK};
+      y = NormGrad::apply(x, weight, bias, &c);
+      rc = c.rc;
+    } else {
+      rc = norm_forward(a, x, false, stream, &y, &mean, &rstd);
+    }
+  }
+  if (rc != OSM_OK) return fail_rc(rc);
+  return THPVariable_Wrap(y);
 }
 
 // clip(tensors, max_norm, eps, scale): None, or the norm.  tensors: a list or tuple.
@@ -1053,9 +1304,11 @@ PyObject* py_engine(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarde
 
 PyObject* py_delta_forward(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded<10>(a, n, run_delta_forward); }
 PyObject* py_delta_backward(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded<11>(a, n, run_delta_backward); }
+PyObject* py_gated_delta(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded<9>(a, n, run_gated_delta); }
 PyObject* py_delta_step(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded<8>(a, n, run_delta_step); }
 PyObject* py_norm_forward(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded<5>(a, n, run_norm_forward); }
 PyObject* py_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded<8>(a, n, run_norm_backward); }
+PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded<4>(a, n, run_layer_norm); }
 PyObject* py_clip(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded<4>(a, n, run_clip); }
 
 // init(addresses of the library's functions in the order of Lib, raw_stream, ws_cache, workspace, check)
@@ -1118,9 +1371,11 @@ PyMethodDef methods[] = {
     {"engine", fast(py_engine), METH_FASTCALL, nullptr},
     {"delta_forward", fast(py_delta_forward), METH_FASTCALL, nullptr},
     {"delta_backward", fast(py_delta_backward), METH_FASTCALL, nullptr},
+    {"gated_delta", fast(py_gated_delta), METH_FASTCALL, nullptr},
     {"delta_step", fast(py_delta_step), METH_FASTCALL, nullptr},
     {"norm_forward", fast(py_norm_forward), METH_FASTCALL, nullptr},
     {"norm_backward", fast(py_norm_backward), METH_FASTCALL, nullptr},
+    {"layer_norm", fast(py_layer_norm), METH_FASTCALL, nullptr},
     {"clip", fast(py_clip), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -244,6 +244,11 @@ def gated_delta(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tens
     """``gated_delta_forward`` as a differentiable op: gradients flow to q, k,
     v, g, beta and state_init, from the output and the final state.  Returns
     out, or (out, final state) when ``return_state``."""
+    fast = _fast()
+    if fast is not None:
+        res = fast.gated_delta(q, k, v, g, beta, scale, lengths, state_init, return_state)
+        if res is not None:
+            return res if return_state else res[0]
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad
                                        for t in (q, k, v, g, beta, state_init)):
         out, fin = _GatedDeltaFunction.apply(q, k, v, g, beta, state_init, lengths, scale)

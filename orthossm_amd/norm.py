@@ -155,6 +155,11 @@ class _LayerNormFunction(torch.autograd.Function):
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, *,
                eps: float = 1e-5) -> torch.Tensor:
     """Layer norm over the last axis, differentiable in x, weight and bias."""
+    fast = _fast()
+    if fast is not None:
+        y = fast.layer_norm(x, weight, bias, eps)
+        if y is not None:
+            return y
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, weight, bias)):
         return _LayerNormFunction.apply(x, weight, bias, eps)
     return _forward(x, weight, bias, eps, None, False)[0]
