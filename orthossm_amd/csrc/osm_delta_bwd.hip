@@ -641,9 +641,10 @@ __global__ void __launch_bounds__(512, 2) delta_grads_parts_kernel(const DeltaPa
   constexpr int kFirst = kK > kKt ? kK : kKt;
   constexpr int kStates = (kBoth ? 6 : 3) * kState, kLast = 9 * kTri > kStates + kKt ? 9 * kTri : kStates + kKt;
   static_assert(kK <= 6 * kVal && 2 * (kTile + 64 * LW) <= 6 * kVal, "Q, or C and dKw, fit the place of Y and R");
-  __shared__ __attribute__((aligned(16))) unsigned short first[kFirst], os[kVal], yr[6 * kVal], rest[kLast];
+  __shared__ __attribute__((aligned(16))) unsigned short first[kFirst], yr[7 * kVal], rest[kLast];
   __shared__ __attribute__((aligned(16))) float gt[kGateFloats];
   __shared__ float pairs[8][64], part[8], reads[64], writes[64], dbeta[64];
+  unsigned short* const os = yr + 6 * kVal;
   unsigned short *const zp = rest, *const zt = rest + 3 * kTri, *const pt = rest + 6 * kTri;
   unsigned short *const sp = rest, *const dp = rest + (kBoth ? 3 * kState : 0), *const qt = rest + kStates;
   float *const cs = reinterpret_cast<float*>(yr), *const ws = cs + kTile;
@@ -707,7 +708,6 @@ __global__ void __launch_bounds__(512, 2) delta_grads_parts_kernel(const DeltaPa
   kb.load(k, p.k.ss, w.rows, p.dk_, p.vec);
   qb.load(q, p.q.ss, w.rows, p.dk_, p.vec);
   for (int e = tid; e < kGateFloats; e += NT) gt[e] = p.gates[chunk * kGateFloats + e];
-  kb.template put_rows<LDK>(first, kFirst);
   f32x4 a1[ST], a2[ST];                 // dQ^T and dKr^T, or dKw^T and nothing
   f32x4 mp[4], ml[4], qk[4], kk[4];     // dO Y^T, R Y^T, and a reader's K Q^T, K K^T, by tiles of the other token
   if (!ONE) {
@@ -716,6 +716,19 @@ __global__ void __launch_bounds__(512, 2) delta_grads_parts_kernel(const DeltaPa
     clear(mp);
     clear(ml);
   }
+  // K and Q for part 3, and the rows of this lane's token as its results lie
+  const Rsrc k_rs = rows_rsrc<T>(k, p.k.ss, w.rows, p.dk_), q_rs = rows_rsrc<T>(q, p.q.ss, w.rows, p.dk_);
+  bf16x4 k_tok[ST], q_tok[ST];
+  auto load_tokens = [&] {
+    kb.load(k, p.k.ss, w.rows, p.dk_, p.vec);
+    qb.load(q, p.q.ss, w.rows, p.dk_, p.vec);
+#pragma unroll
+    for (int t = 0; t < ST; ++t) {
+      const int c = 16 * t + 4 * g;
+      k_tok[t] = load_quad(k_rs, tok * 2u * (unsigned)p.k.ss + 2 * c, p.dk_ - c, p.vec);
+      if (reader) q_tok[t] = load_quad(q_rs, tok * 2u * (unsigned)p.q.ss + 2 * c, p.dk_ - c, p.vec);
+    }
+  };
   float ending = 0.0f;
   for (int vb = 0; vb < (ONE ? 1 : p.dvp); vb += 64) {
     if (vb) {
@@ -748,6 +761,7 @@ __global__ void __launch_bounds__(512, 2) delta_grads_parts_kernel(const DeltaPa
       const int row = min(zi, 60) + i, quad = row < 32 ? row * 8 + (zj >> 2) : 256 + (row - 32) * 16 + (zj >> 2);
       zr[i] = load4(p.z + chunk * kZFloats + 4 * quad);
     }
+    if (vb == 0) kb.template put_rows<LDK>(first, kFirst);   // (when all loads are on their way)
     qb.template put_rows<LDK>(yr, kK);
 #pragma unroll
     for (int n = 0; n < 2; ++n) *reinterpret_cast<bf16x4*>(os + ((tid + n * NT) >> 4) * L + 4 * ((tid + n * NT) & 15)) = oq[n];
@@ -787,30 +801,31 @@ __global__ void __launch_bounds__(512, 2) delta_grads_parts_kernel(const DeltaPa
           }
       }
     } else {
-      // scale P^T, row tok, and zeros before it in its pair of tiles
+      // scale P^T: ten tiles and the two of zeros that complete their pairs, three a wave
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-        if (t >= (st & 2)) {
-          f32x4 acc = zero4();
-          if (t >= st) {
+      for (int e = 0; e < 3; ++e) {
+        const int tr = e < 2 ? e : 2 + (st >> 1), t = e < 2 ? st : 2 + (st & 1), row = 16 * tr + r;
+        f32x4 acc = zero4();
+        if (t >= tr) {
+          u32x4 a[KS][1], bk[KS][1];
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-              u32x4 a[1], bk[1];
-              read_parts<1>(a, yr, 0, (16 * t + r) * LDK + 32 * s + 8 * g);
-              read_parts<1>(bk, first, 0, tok * LDK + 32 * s + 8 * g);
-              acc = mfma(a[0], bk[0], acc);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int row = 16 * t + 4 * g + i;
-              acc[i] = row >= tok ? p.scale * acc[i] * decay(gt, row, tok) : 0.0f;
-            }
+          for (int s = 0; s < KS; ++s) {
+            read_parts<1>(a[s], yr, 0, (16 * t + r) * LDK + 32 * s + 8 * g);
+            read_parts<1>(bk[s], first, 0, row * LDK + 32 * s + 8 * g);
           }
-          u32x2 parts[3];
-          split4<3>(parts, acc);
 #pragma unroll
-          for (int n = 0; n < 3; ++n) *reinterpret_cast<u32x2*>(pt + n * kTri + upper_at(tok, place4(4 * t + g))) = parts[n];
+          for (int s = 0; s < KS; ++s) acc = mfma(a[s][0], bk[s][0], acc);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int q_row = 16 * t + 4 * g + i;
+            acc[i] = q_row >= row ? p.scale * acc[i] * decay(gt, q_row, row) : 0.0f;
+          }
         }
+        u32x2 parts[3];
+        split4<3>(parts, acc);
+#pragma unroll
+        for (int n = 0; n < 3; ++n) *reinterpret_cast<u32x2*>(pt + n * kTri + upper_at(row, place4(4 * t + g))) = parts[n];
+      }
     }
     __syncthreads();
     // the states of part 2 on their way
@@ -902,8 +917,7 @@ __global__ void __launch_bounds__(512, 2) delta_grads_parts_kernel(const DeltaPa
       clear(a2);
       clear(mp);
       clear(ml);
-      kb.load(k, p.k.ss, w.rows, p.dk_, p.vec);   // for part 3
-      qb.load(q, p.q.ss, w.rows, p.dk_, p.vec);
+      if (kBoth) load_tokens();   // for part 3, where registers allow it
     }
     const unsigned short *const ys = yr, *const rs = yr + 3 * kVal;
     u32x4 bo[2][1], b3[2][3];   // the tokens' dO and R, or Y
@@ -940,12 +954,11 @@ __global__ void __launch_bounds__(512, 2) delta_grads_parts_kernel(const DeltaPa
                 mul<3, 2>(ml[t], a, b3[i]);
               });
         } else {
-          products<3, 1, 2>(
+          products<4, 1, 2>(   // R's parts and dO after them
               kVal, [&](int i) { return rs + at + 32 * i; },
-              [&](int i, const u32x4(&a)[3]) {
-                u32x4 ao[1];
-                read_parts<1>(ao, os, 0, at + 32 * i);
-                mul<3, 2>(ml[t], a, b3[i]);
+              [&](int i, const u32x4(&a)[4]) {
+                const u32x4 ar[3] = {a[0], a[1], a[2]}, ao[1] = {a[3]};
+                mul<3, 2>(ml[t], ar, b3[i]);
                 mul<3, 2>(mp[t], ao, b3[i]);
               });
         }
@@ -964,10 +977,7 @@ __global__ void __launch_bounds__(512, 2) delta_grads_parts_kernel(const DeltaPa
       if (reader) by_tokens();
     }
   }
-  if (!ONE) {
-    kb.load(k, p.k.ss, w.rows, p.dk_, p.vec);
-    qb.load(q, p.q.ss, w.rows, p.dk_, p.vec);
-  }
+  if (!ONE || !kBoth) load_tokens();
   __syncthreads();
   kb.template put_columns<L>(first, kFirst);
   qb.template put_columns<L>(qt, kKt);
@@ -975,16 +985,13 @@ __global__ void __launch_bounds__(512, 2) delta_grads_parts_kernel(const DeltaPa
   const float gam = gt[kGam + tok], beta = gt[kBeta + tok];
   float dot = 0.0f;
   {
-    const Rsrc k_rs = rows_rsrc<T>(k, p.k.ss, w.rows, p.dk_), q_rs = rows_rsrc<T>(q, p.q.ss, w.rows, p.dk_);
-    const unsigned k_at = tok * 2u * (unsigned)p.k.ss, q_at = tok * 2u * (unsigned)p.q.ss;
     const float f1 = reader ? p.scale * gam : gt[kEnd + tok] * beta, f2 = -gam * beta;
 #pragma unroll
     for (int t = 0; t < ST; ++t) {
-      const int c = 16 * t + 4 * g;
-      const f32x4 kv = wide(load_quad(k_rs, k_at + 2 * c, p.dk_ - c, p.vec));
+      const f32x4 kv = wide(k_tok[t]);
       a1[t] *= f1;
       if (reader) {
-        const f32x4 qv = wide(load_quad(q_rs, q_at + 2 * c, p.dk_ - c, p.vec));
+        const f32x4 qv = wide(q_tok[t]);
         a2[t] *= f2;
 #pragma unroll
         for (int i = 0; i < 4; ++i) dot += qv[i] * a1[t][i] + kv[i] * a2[t][i];
