@@ -19,8 +19,8 @@
 namespace osm {
 namespace {
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kThreads = 256;
 
@@ -45,40 +45,71 @@ __device__ __forceinline__ double block_sum(double v, double* red) {
   return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-__global__ void __launch_bounds__(kThreads) clip_sums_kernel(const ClipTable t, double* part) {
-  __shared__ double red[kThreads / 64];
-  const int chunks = t.first[t.count];
-  double sum = 0.0;
-  for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+// A chunk's place, and its elements where it is whole and aligned: 4 (bf16) or 8
+// (fp32) loads of 16 bytes a thread, all of them on their way at once.
+struct Chunk {
+  char* x;
+  int n;
+  bool bf16, whole;
+  u32x4 v[8];
+
+  __device__ __forceinline__ void load(const ClipTable& t, int c) {
     const int i = tensor_of(t, c);
     const int64_t e0 = (int64_t)(c - t.first[i]) * kClipChunk;
-    const int n = (int)min((int64_t)kClipChunk, t.n[i] - e0);
-    if (t.bf16[i]) {
-      const __bf16* const x = static_cast<const __bf16*>(t.p[i]) + e0;
-      int e = 8 * threadIdx.x;
-      if (t.vec[i])
-        for (; e + 8 <= n; e += 8 * kThreads) {
-          const bf16x8 v = *reinterpret_cast<const bf16x8*>(x + e);
+    bf16 = t.bf16[i];
+    x = static_cast<char*>(t.p[i]) + e0 * (bf16 ? 2 : 4);
+    n = (int)min((int64_t)kClipChunk, t.n[i] - e0);
+    whole = n == kClipChunk && t.vec[i];
+    if (!whole) return;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) sum = __builtin_fma((double)(float)v[k], (double)(float)v[k], sum);
-        }
-      for (; e < n; e += 8 * kThreads)
-        for (int k = e; k < min(e + 8, n); ++k) sum = __builtin_fma((double)(float)x[k], (double)(float)x[k], sum);
-    } else {
-      const float* const x = static_cast<const float*>(t.p[i]) + e0;
-      int e = 4 * threadIdx.x;
-      if (t.vec[i])
-        for (; e + 4 <= n; e += 4 * kThreads) {
-          const f32x4 v = *reinterpret_cast<const f32x4*>(x + e);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) sum = __builtin_fma((double)v[k], (double)v[k], sum);
-        }
-      for (; e < n; e += 4 * kThreads)
-        for (int k = e; k < min(e + 4, n); ++k) sum = __builtin_fma((double)x[k], (double)x[k], sum);
-    }
+    for (int k = 0; k < 8; ++k)
+      if (k < 4 || !bf16) v[k] = *reinterpret_cast<const u32x4*>(x + at(k));
   }
-  sum = block_sum(sum, red);
-  if (threadIdx.x == 0) part[t.part0 + blockIdx.x] = sum;
+  __device__ __forceinline__ static unsigned at(int k) { return 16u * (k * kThreads + threadIdx.x); }
+};
+
+__device__ __forceinline__ void add_square(double& sum, float x) { sum = __builtin_fma((double)x, (double)x, sum); }
+__device__ __forceinline__ float low(unsigned v) { return __uint_as_float(v << 16); }
+__device__ __forceinline__ float high(unsigned v) { return __uint_as_float(v & 0xffff0000u); }
+
+__device__ __forceinline__ void add_squares(double (&sum)[2], const Chunk& c) {
+  if (!c.whole) {
+    for (int e = threadIdx.x; e < c.n; e += kThreads)
+      add_square(sum[0], c.bf16 ? (float)reinterpret_cast<const __bf16*>(c.x)[e] : reinterpret_cast<const float*>(c.x)[e]);
+  } else if (c.bf16) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        add_square(sum[0], low(c.v[k][i]));
+        add_square(sum[1], high(c.v[k][i]));
+      }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) add_square(sum[i & 1], __uint_as_float(c.v[k][i]));
+  }
+}
+
+// A workgroup loads its next chunk before it adds up the one it has.
+__global__ void __launch_bounds__(kThreads) clip_sums_kernel(const ClipTable t, double* part) {
+  __shared__ double red[kThreads / 64];
+  const int chunks = t.first[t.count], turn = gridDim.x;
+  double sum[2] = {0.0, 0.0};
+  Chunk a, b;
+  int c = blockIdx.x;
+  if (c < chunks) a.load(t, c);
+  while (c < chunks) {
+    if (c + turn < chunks) b.load(t, c + turn);
+    add_squares(sum, a);
+    if (c + turn >= chunks) break;
+    if (c + 2 * turn < chunks) a.load(t, c + 2 * turn);
+    add_squares(sum, b);
+    c += 2 * turn;
+  }
+  const double all = block_sum(sum[0] + sum[1], red);
+  if (threadIdx.x == 0) part[t.part0 + blockIdx.x] = all;
 }
 
 template <bool SCALE>
@@ -93,34 +124,30 @@ __global__ void __launch_bounds__(kThreads) clip_scale_kernel(const ClipTable t,
   const float f = (float)(max_norm / (all + eps));
   if (f >= 1.0f) return;   // (a NaN norm goes on, and makes every element NaN)
   const int chunks = t.first[t.count];
-  for (int c = chunks - 1 - blockIdx.x; c >= 0; c -= gridDim.x) {
-    const int i = tensor_of(t, c);
-    const int64_t e0 = (int64_t)(c - t.first[i]) * kClipChunk;
-    const int n = (int)min((int64_t)kClipChunk, t.n[i] - e0);
-    if (t.bf16[i]) {
-      __bf16* const x = static_cast<__bf16*>(t.p[i]) + e0;
-      int e = 8 * threadIdx.x;
-      if (t.vec[i])
-        for (; e + 8 <= n; e += 8 * kThreads) {
-          bf16x8 v = *reinterpret_cast<const bf16x8*>(x + e);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] = (__bf16)((float)v[k] * f);
-          *reinterpret_cast<bf16x8*>(x + e) = v;
+  for (int i = chunks - 1 - blockIdx.x; i >= 0; i -= gridDim.x) {
+    Chunk c;
+    c.load(t, i);
+    if (!c.whole) {
+      for (int e = threadIdx.x; e < c.n; e += kThreads) {
+        if (c.bf16) {
+          __bf16* const x = reinterpret_cast<__bf16*>(c.x) + e;
+          *x = (__bf16)((float)*x * f);
+        } else {
+          reinterpret_cast<float*>(c.x)[e] *= f;
         }
-      for (; e < n; e += 8 * kThreads)
-        for (int k = e; k < min(e + 8, n); ++k) x[k] = (__bf16)((float)x[k] * f);
-    } else {
-      float* const x = static_cast<float*>(t.p[i]) + e0;
-      int e = 4 * threadIdx.x;
-      if (t.vec[i])
-        for (; e + 4 <= n; e += 4 * kThreads) {
-          f32x4 v = *reinterpret_cast<const f32x4*>(x + e);
+      }
+      continue;
+    }
 #pragma unroll
-          for (int k = 0; k < 4; ++k) v[k] *= f;
-          *reinterpret_cast<f32x4*>(x + e) = v;
-        }
-      for (; e < n; e += 4 * kThreads)
-        for (int k = e; k < min(e + 4, n); ++k) x[k] *= f;
+    for (int k = 0; k < 8; ++k) {
+      if (k >= 4 && c.bf16) break;
+      u32x4 v = c.v[k];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        v[i] = c.bf16 ? __builtin_bit_cast(unsigned, bf16x2{(__bf16)(low(v[i]) * f), (__bf16)(high(v[i]) * f)})
+                      : __float_as_uint(__uint_as_float(v[i]) * f);
+      *reinterpret_cast<u32x4*>(c.x + Chunk::at(k)) = v;
+      asm volatile("s_nop 1" ::: "memory");   // (a store wider than 64 bits: see store4 in osm_delta.h)
     }
   }
 }
