@@ -30,6 +30,7 @@
 // left out: 3 instructions against a bf16 operand, 6 between two fp32 ones, where
 // the fp32 matrix instruction takes 16 times as long as the bf16 one.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "osm_delta.h"
@@ -114,8 +115,9 @@ __device__ __forceinline__ void invert(float* zs, const float* beta) {
 
 // Z and the gates of a chunk, one wave: the steps of the inversion follow each
 // other closely and hold little, so eight chunks a CU side by side beat four waves
-// that wait for each other (8192 chunks of d = 64: 89 us so).  KS: blocks of 32
-// columns of k.
+// that wait for each other (8192 chunks of d = 64: 89 us with four waves, 59 so).
+// What bounds it: the chain of the substitution and of the block products, a third
+// of its time waiting for LDS.  KS: blocks of 32 columns of k.
 template <typename T, int KS>
 __global__ void __launch_bounds__(64) delta_solve_kernel(const DeltaParams p) {
   constexpr int NP = kParts<T>, LDK = 32 * KS + 8, kBytes = NP * 64 * LDK * 2 > 4 * kTile ? NP * 64 * LDK * 2 : 4 * kTile;
@@ -178,7 +180,8 @@ __global__ void __launch_bounds__(64) delta_solve_kernel(const DeltaParams p) {
 // accumulators' four rows and the product's four terms are one 16-byte access),
 // in two buffers: one barrier a span.  x holds B and receives the state before
 // the span.  KT = dkp / 16.  What bounds it: the chain of spans, 4 KT matrix
-// instructions and the exchange each.
+// instructions and the exchange each (32 spans of 16 heads, dk = dv = 64: 15 us;
+// maps read three spans ahead instead of one: 18).
 template <int KT>
 __global__ void __launch_bounds__(64 * KT) delta_scan_kernel(const float* a, float* x, const float* init,
                                                              const int* lengths, int S, int N, int span, int BH, int H,
@@ -244,6 +247,12 @@ __global__ void __launch_bounds__(64 * KT) delta_scan_kernel(const float* a, flo
 // Walks segment blockIdx.x % segs of a head.  MAP: the segment's state map, from
 // zero for the columns of v and from the identity's columns after them; else the
 // outputs.  KS: blocks of 32 rows of S; WAVES: of 16 columns each.
+// What bounds it: 512 chunks of 16 heads, bf16, d = 64, take 130 us for the maps and
+// 121 for the outputs, in which the vector instructions (the parts of X, U, S, Z, P)
+// fill a third to two fifths of the time, the matrix instructions a quarter, LDS two
+// fifths, and the two or three waves a SIMD has room for wait for each other in
+// between.  Tried without gain: products of two tiles in turn, a higher priority for
+// waves in their products, 128 registers for twice the waves.
 template <typename T, int KS, int WAVES, bool MAP>
 __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaParams p, int groups) {
   constexpr int NT = 64 * WAVES, NP = kParts<T>, DK = 32 * KS, LDK = DK + 8, LKT = 72, ST = 2 * KS;
@@ -510,7 +519,16 @@ void launch_walk(const DeltaParams& p, hipStream_t stream) {
     const unsigned grid = (unsigned)((int64_t)p.B * p.H * p.segs * groups);
     hipLaunchKernelGGL((delta_walk_kernel<T, KS, W, MAP>), dim3(grid), dim3(64 * W), 0, stream, p, groups);
   };
-  if (slices <= 4)
+  // Eight waves share the first operands between more columns; four, where a CU
+  // holds two such workgroups or more, wait less for each other.  Measured with four
+  // and eight, B=1 S=8192 H=16: maps of bf16 dk=64 dv=128 148 and 165 us (the whole
+  // forward), dk=dv=128 290 and 286, of fp32 dk=64 223 and 234, but dk=dv=128, one
+  // workgroup a CU, 567 and 478; outputs of bf16 dk=64 dv=128 171 and 165, dk=dv=128
+  // 393 and 285, of fp32 dk=64 285 and 234.
+  constexpr bool kFour = MAP && (sizeof(T) == 2 || KS <= 2);
+  if constexpr (kFour)
+    go(std::integral_constant<int, 4>{});
+  else if (slices <= 4)
     go(std::integral_constant<int, 4>{});
   else
     go(std::integral_constant<int, 8>{});
@@ -544,12 +562,20 @@ hipError_t forward_by_size(const DeltaParams& p, hipStream_t stream) {
 
 }  // namespace
 
-// Chunks a segment.  Heads and rows alone where they give every other CU a
-// workgroup; else as many segments as give every CU two, of at least two chunks.
+// Chunks a segment.  A segmented row is walked twice, on top of a scan, but by many
+// workgroups: worth it for up to 128 heads (bf16, d = 64, whole rows against
+// segments: 128 heads x 64 chunks 349 and 299 us, 160 x 51 289 and 298, 192 x 42 249
+// and 312; 16 x 512 2318 and 297) and from 4 chunks (8 heads x 4 32.1 and 30.5 us,
+// x 8 49.8 and 33.7).  At most as many segments as give every CU two workgroups: one
+// more and a third round of them begins (96 heads x 85 chunks: 5 segments 305 us, 6
+// 380).  Below that a walk costs its segment's length and the scan their number, so
+// the best length goes with the root of the row's: with 1, 2, 3, 4 chunks a segment
+// 8 heads x 16 chunks take 41.8, 41.3, 45.9, 52.1 us, x 47 73.6, 59.4, 57.2, 60.9,
+// x 128 163, 109, 96, 87 (8: 95); fp32 and d = 128 have theirs at the same lengths.
 int delta_segment(int64_t heads, int64_t chunks) {
-  if (heads >= 128 || chunks <= 2) return (int)std::max<int64_t>(chunks, 1);
-  const int64_t want = (512 + heads - 1) / heads, segs = std::min(want, chunks / 2);
-  return (int)((chunks + segs - 1) / segs);
+  if (heads > 128 || chunks < 4) return (int)std::max<int64_t>(chunks, 1);
+  const int64_t most = 512 / std::max<int64_t>(heads, 1);
+  return (int)std::max<int64_t>((chunks + most - 1) / most, (int64_t)(std::sqrt(chunks / 6.0) + 0.5));
 }
 
 hipError_t launch_delta_scan(const DeltaParams& p, const float* a, float* x, const float* init, int n, int span,
