@@ -362,8 +362,9 @@ typedef struct osm_engine_args {
  * after a decay e^{g_t}.  No counterpart in the reference.
  *
  * q and k have Hk heads, H a multiple of Hk: head h uses head h / (H / Hk) of
- * them.  Arithmetic is fp32 throughout (products on the fp32 matrix
- * instruction), results are rounded once to `dtype`.  g below -200 counts as
+ * them.  Arithmetic is at fp32's accuracy throughout (products on the bf16
+ * matrix instruction run on the three bf16 parts of an fp32 number, and leave
+ * out what is below 2^-24), results are rounded once to `dtype`.  g below -200 counts as
  * -200.  Tokens at and past lengths[b] are not read, leave the state as it is
  * and give zeros (outputs and gradients).  A NaN or infinity in a token may
  * reach the outputs of its whole chunk of 64 tokens, and those after it. */
@@ -552,14 +553,16 @@ int osm_cheby_ema_bwd(const osm_cheby_args* args, const osm_cheby_bwd_args* bwd,
 
 /* The gated delta rule over sequences.  `saved` (args->saved) and the workspace
  * need no initialisation and 256-byte alignment; nothing is kept in the
- * workspace between calls.  Three launches, or one where S is at most 16 and
- * nothing is saved (the workspace is then 0 bytes and may be NULL). */
+ * workspace between calls.  Two launches, four where rows are cut into segments,
+ * or one where S is at most 8 and nothing is saved (the workspace is then 0
+ * bytes and may be NULL). */
 size_t osm_delta_saved_bytes(const osm_delta_args* args);
 size_t osm_delta_workspace_bytes(const osm_delta_args* args);
 int osm_delta_fwd(const osm_delta_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Its backward, from the inputs and what osm_delta_fwd saved of them (out and
- * state_out of `args` are not used). */
+ * state_out of `args` are not used): two launches, four with segments, two more
+ * where q and k heads are shared. */
 size_t osm_delta_bwd_workspace_bytes(const osm_delta_args* args);
 int osm_delta_bwd(const osm_delta_args* args, const osm_delta_bwd_args* bwd, void* workspace, size_t workspace_bytes,
                   void* stream);

@@ -55,7 +55,10 @@ __device__ __forceinline__ int upper_at(int row, int col) { return row < 32 ? ro
 
 // Walks segment blockIdx.x % segs of a head from its last chunk to its first, D =
 // dL/dS' in the waves' accumulators (16 columns each, as S in the forward's walk).
-// MAP: the segment's map of D; else dV, and every chunk's D into p.d.
+// MAP: the segment's map of D; else dV, and every chunk's D into p.d.  What bounds
+// it is what bounds the forward's walk (64 chunks of 32 heads, bf16, d = 64: 59 us
+// for the maps, 43 for dV).  Four waves instead of eight for the maps lost 10 to 60
+// us of a backward there, and won 13 only where dk = 32, dv = 128.
 template <typename T, int KS, int WAVES, bool MAP>
 __global__ void __launch_bounds__(64 * WAVES, 2) delta_rewalk_kernel(const DeltaParams p, int groups) {
   constexpr int NT = 64 * WAVES, NP = kParts<T>, DK = 32 * KS, LDK = DK + 8, LKT = 72, ST = 2 * KS;
@@ -327,11 +330,14 @@ void launch_rewalk(const DeltaParams& p, hipStream_t stream) {
 
 constexpr int kGradThreads = 512;
 
-// The gradients of a chunk: eight waves, 16 rows by 32 columns of every product
-// each; nine tiles of LDS (157 KB), one workgroup a CU.  NKB: blocks of 64
-// columns of q and k.
-template <typename T, int NKB>
+// The gradients of a chunk but dV, from fp32 inputs, on the fp32 matrix
+// instruction: eight waves, 16 rows by 32 columns of every product each; nine tiles
+// of LDS (157 KB), one workgroup a CU.  NKB: blocks of 64 columns of q and k.  What
+// bounds it: the matrix instructions and the barriers between the products (376
+// chunks of dk = 48, dv = 80: 85 us).
+template <int NKB>
 __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const DeltaParams p) {
+  typedef float T;
   constexpr int CT = 2;
   __shared__ __attribute__((aligned(16))) float zs[kTile], ps[kTile], ks[kTile], qs[kTile], ss[kTile], ds[kTile],
       us[kTile], os[kTile], ys[kTile];
@@ -343,13 +349,9 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const DeltaPa
   const At w = chunk_at(p, chunk);
   const int tid = threadIdx.x, wave = tid >> 6, r0 = 16 * (wave & 3), c0 = 32 * (wave >> 2);
   const int hk = w.h / (p.H / p.Hk);
-  const bool shared_heads = p.H != p.Hk;   // dq and dk are then fp32, by head
   const int rows = (int)min((int64_t)kDeltaChunk, p.S - w.t0);
   auto put_qk = [&](const DeltaRows& dst, int row, int col, float v) {
-    if (shared_heads)
-      row_ptr<float>(dst, w.b, w.t0 + row, w.h)[col] = v;
-    else
-      row_ptr<T>(dst, w.b, w.t0 + row, w.h)[col] = (T)v;
+    row_ptr<T>(dst, w.b, w.t0 + row, w.h)[col] = v;   // (also where heads are shared: fp32, by head)
   };
   auto put_gate = [&](const DeltaRows& dst, int row, float v) { *row_ptr<float>(dst, w.b, w.t0 + row, w.h) = v; };
   if (w.rows == 0) {
@@ -429,7 +431,7 @@ __global__ void __launch_bounds__(kGradThreads) delta_grads_kernel(const DeltaPa
       for (int i = 0; i < 4; ++i) {
         const int row = out_row(r0, i), col = out_col(c0, c);
         const bool in = row < w.rows && vb + col < p.dv_ && col < vw;
-        x[c][i] = in ? (float)v[row * p.v.ss + vb + col] - gt.gam[row] * x[c][i] : 0.0f;
+        x[c][i] = in ? v[row * p.v.ss + vb + col] - gt.gam[row] * x[c][i] : 0.0f;
         y[c][i] = in ? p.scale * acc[c][i] + gt.end[row] * y[c][i] : 0.0f;
       }
     put(us, x, r0, c0);
@@ -631,7 +633,12 @@ __device__ __forceinline__ f32x4 wide(bf16x4 v) { return f32x4{(float)v[0], (flo
 // LDS: K by rows, then columns; dO; Q by rows, then Y and R, then C and dKw; Z,
 // its transpose and P's, then S and D (one after the other for more than 64 rows)
 // and Q by columns.  ONE: dv <= 64, so that what part 2 adds up need not live
-// through part 1.
+// through part 1 (where it does, registers spill).
+// What bounds it: 2048 chunks of d = 64 take 166 us, where their bytes take 37.  With
+// one workgroup a CU nothing covers a chunk's first loads (a fifth of its 41000
+// cycles) and the waits at the nine barriers; the two waves of a SIMD issue vector
+// instructions two fifths of the time.  Tried without gain: workgroups that go
+// through several chunks and load the next one ahead (the registers for it spill).
 template <int KS, bool ONE>
 __global__ void __launch_bounds__(512, 2) delta_grads_parts_kernel(const DeltaParams p) {
   typedef __bf16 T;
@@ -1156,9 +1163,9 @@ hipError_t backward(const DeltaParams& p, float* const part, hipStream_t stream)
       default: go(std::integral_constant<int, 4>{}); break;
     }
   } else if (p.dkp <= 64) {
-    hipLaunchKernelGGL((delta_grads_kernel<T, 1>), dim3(chunks), dim3(kGradThreads), 0, stream, w);
+    hipLaunchKernelGGL((delta_grads_kernel<1>), dim3(chunks), dim3(kGradThreads), 0, stream, w);
   } else {
-    hipLaunchKernelGGL((delta_grads_kernel<T, 2>), dim3(chunks), dim3(kGradThreads), 0, stream, w);
+    hipLaunchKernelGGL((delta_grads_kernel<2>), dim3(chunks), dim3(kGradThreads), 0, stream, w);
   }
   e = hipGetLastError();
   if (e != hipSuccess || p.H == p.Hk) return e;

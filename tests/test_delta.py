@@ -68,11 +68,12 @@ def test_sizes():
     lib = nat.load()
     chunks = 2 * 4 * 4                      # rows, heads, chunks of 64 tokens
     solved, states = (chunks * n * 4 for n in (48 * 64 + 320, 64 * 80))                 # 48 rows of a state held as 64
-    segments = 2 * 4 * 2 * (64 * 64 + 64 * 80) * 4                                      # two of two chunks a row
+    segments = 2 * 4 * 4 * (64 * 64 + 64 * 80) * 4                                      # four of one chunk a row
     assert lib.osm_delta_saved_bytes(ctypes.byref(_args())) == solved + states
     assert lib.osm_delta_workspace_bytes(ctypes.byref(_args())) == solved + segments
     assert lib.osm_delta_workspace_bytes(ctypes.byref(_args(saved=0x10000))) == segments
-    assert lib.osm_delta_workspace_bytes(ctypes.byref(_args(S=16))) == 0      # token by token
+    assert lib.osm_delta_workspace_bytes(ctypes.byref(_args(S=8))) == 0       # token by token
+    assert lib.osm_delta_workspace_bytes(ctypes.byref(_args(S=9))) > 0
     assert lib.osm_delta_workspace_bytes(ctypes.byref(_args(S=0))) == 0
     # the backward: maps of the segments, the chunks' gradients, and a gradient of q and k for each of v's heads
     assert lib.osm_delta_bwd_workspace_bytes(ctypes.byref(_args())) == segments + states + 2 * 2 * 200 * 4 * 48 * 4
