@@ -252,7 +252,8 @@ __global__ void __launch_bounds__(64 * KT) delta_scan_kernel(const float* a, flo
 // fill a third to two fifths of the time, the matrix instructions a quarter, LDS two
 // fifths, and the two or three waves a SIMD has room for wait for each other in
 // between.  Tried without gain: products of two tiles in turn, a higher priority for
-// waves in their products, 128 registers for twice the waves.
+// waves in their products, 128 registers for twice the waves, and LDS rows 160 bytes
+// apart, whose 16-byte reads meet no bank twice (their writes meet more: 144 us).
 template <typename T, int KS, int WAVES, bool MAP>
 __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaParams p, int groups) {
   constexpr int NT = 64 * WAVES, NP = kParts<T>, DK = 32 * KS, LDK = DK + 8, LKT = 72, ST = 2 * KS;
