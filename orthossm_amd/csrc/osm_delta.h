@@ -13,7 +13,7 @@ constexpr int kDeltaChunk = 64;      // tokens a chunk
 constexpr int kDeltaMaxDk = 128;     // rows of the state
 constexpr int kDeltaSlice = 16;      // columns of the state a scan workgroup, or a wave of a walk, holds
 constexpr int kGateFloats = 320;     // a chunk's gates (delta::make_gates)
-constexpr int kZFloats = 3072;       // a chunk's Z: rows 0-31 by 32 columns, rows 32-63 by 64
+constexpr int kZFloats = 32 * 32 + 32 * 64;   // a chunk's Z: rows 0-31 by 32 columns, rows 32-63 by 64
 
 // Rows of a token tensor: element (b, t, h, j) at b*sb + t*ss + h*sh + j.
 struct DeltaRows {
