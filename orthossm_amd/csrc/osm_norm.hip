@@ -4,8 +4,8 @@
 //   y = xh w + b,  xh = (x - mean) rstd
 //   dx = rstd (w dy - mean(w dy) - xh mean(w dy xh)),  dw = sum_rows dy xh,  db = sum_rows dy
 //
-// A row is held in the registers of one wave, or of four or sixteen where it is
-// longer, so x is read once in each direction and the variance is a second sum
+// A row is held in the registers of one wave, of a quarter of one where it is
+// short, or of four or sixteen where it is longer, so x is read once in each direction and the variance is a second sum
 // over registers, free of cancellation.  What bounds both: the bytes of x, y
 // (x, dy, dx); 262144 bf16 rows of 1024 take 206 us forward and 273 backward (5.2
 // and 5.9 TB/s).  The backward's workgroups walk rows a grid apart and keep their
@@ -110,13 +110,16 @@ __device__ __forceinline__ float dpp_add(float v) {
 __device__ __forceinline__ float lane_of(float v, int l) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
 }
-// The sum over a wave, in every lane: within 16 lanes by DPP, then four scalars
-// (a shuffle through LDS a step takes five times as long).
+// The sum over 16 lanes, and over a wave, in every one of them: by DPP, then four
+// scalars (a shuffle through LDS a step takes five times as long).
+__device__ __forceinline__ float lanes_total(float v) {
+  v = dpp_add<0xb1>(v);      // quad_perm 1 0 3 2
+  v = dpp_add<0x4e>(v);      // quad_perm 2 3 0 1
+  v = dpp_add<0x141>(v);     // row_half_mirror
+  return dpp_add<0x140>(v);  // row_mirror
+}
 __device__ __forceinline__ float wave_total(float v) {
-  v = dpp_add<0xb1>(v);    // quad_perm 1 0 3 2
-  v = dpp_add<0x4e>(v);    // quad_perm 2 3 0 1
-  v = dpp_add<0x141>(v);   // row_half_mirror
-  v = dpp_add<0x140>(v);   // row_mirror
+  v = lanes_total(v);
   return (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
 }
 
@@ -125,7 +128,7 @@ __device__ __forceinline__ float wave_total(float v) {
 template <int TPR, int K>
 __device__ __forceinline__ void row_sum(float (&v)[K], float (*red)[K]) {
 #pragma unroll
-  for (int k = 0; k < K; ++k) v[k] = wave_total(v[k]);
+  for (int k = 0; k < K; ++k) v[k] = TPR == 16 ? lanes_total(v[k]) : wave_total(v[k]);
   if constexpr (TPR > 64) {
     const int wave = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 0)
@@ -255,7 +258,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) layer_norm_bwd_kernel(c
         }
       __syncthreads();
       if (group == 0)
-#pragma unroll
+#pragma unroll 3
         for (int q = 0; q < kRows - 1; ++q)
 #pragma unroll
           for (int i = 0; i < U; ++i) {
@@ -380,12 +383,14 @@ __global__ void __launch_bounds__(kFoldCols * kFoldGroups) layer_norm_fold_kerne
 // in the case of 1024 threads: the backward holds five rows' worth, and spills
 // with 16), or long_rows() past 1024 LAST elements.  Measured with 64 and 256
 // threads a row, forward and backward: bf16, 262144 rows of 1024 206 and 288 us, 298
-// and 362; fp32, 15003 rows of 400 13 and 17 us, 18 and 24.
+// and 362; fp32, 15003 rows of 400 13 and 17 us, 18 and 24.  With 16 and 64, bf16,
+// 2^26 elements in rows of 16 246 and 1038 us, 306 and 1206, of 64 65 and 257, 84 and
+// 311; fp32, of 64 101 and 212, 143 and 256.
 template <typename T, int LAST, typename Go, typename Long>
 void by_length(int64_t D, Go go, Long long_rows) {
   const int64_t units = (D + kUnit<T> - 1) / kUnit<T>;
   auto pick = [&](auto tpr) {
-    constexpr int TPR = decltype(tpr)::value, most = (TPR == 1024 ? LAST : 16) / kUnit<T>;
+    constexpr int TPR = decltype(tpr)::value, most = TPR == 16 ? 1 : (TPR == 1024 ? LAST : 16) / kUnit<T>;
     if (units > most * TPR) return false;
     if (units <= TPR)
       go(tpr, std::integral_constant<int, 1>{});
@@ -395,8 +400,8 @@ void by_length(int64_t D, Go go, Long long_rows) {
       go(tpr, std::integral_constant<int, most>{});
     return true;
   };
-  if (!pick(std::integral_constant<int, 64>{}) && !pick(std::integral_constant<int, 256>{}) &&
-      !pick(std::integral_constant<int, 1024>{}))
+  if (!pick(std::integral_constant<int, 16>{}) && !pick(std::integral_constant<int, 64>{}) &&
+      !pick(std::integral_constant<int, 256>{}) && !pick(std::integral_constant<int, 1024>{}))
     long_rows();
 }
 
