@@ -257,14 +257,12 @@ __global__ void __launch_bounds__(64 * KT) delta_scan_kernel(const float* a, flo
 template <typename T, int KS, int WAVES, bool MAP>
 __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaParams p, int groups) {
   constexpr int NT = 64 * WAVES, NP = kParts<T>, DK = 32 * KS, LDK = DK + 8, LKT = 72, ST = 2 * KS;
-  // Parts of what only the output sees: bf16 outputs need no more than two.
-  constexpr int OP = sizeof(T) == 4 ? 3 : 2;
   // By parts: K by rows, K by columns, Q by rows; where two workgroups' LDS does not
   // hold all three, Q first has the place of K by columns.  Then Z and P.
   constexpr int kK = 64 * LDK, kKt = DK * LKT;
-  constexpr bool kApart = !MAP && 2 * (NP * (kKt + 2 * kK) + (3 + OP) * kTri) + 8 * kGateFloats <= 80 * 1024;
+  constexpr bool kApart = !MAP && 2 * (NP * (kKt + 2 * kK) + 6 * kTri) + 8 * kGateFloats <= 80 * 1024;
   constexpr int kIn = kK + (MAP ? kKt : kApart ? kKt + kK : kKt > kK ? kKt : kK);
-  __shared__ __attribute__((aligned(16))) unsigned short in[NP][kIn], zp[3][kTri], pp[MAP ? 1 : OP][MAP ? 8 : kTri];
+  __shared__ __attribute__((aligned(16))) unsigned short in[NP][kIn], zp[3][kTri], pp[MAP ? 1 : 3][MAP ? 8 : kTri];
   __shared__ __attribute__((aligned(16))) float gates[2][kGateFloats];
   unsigned short *const kk = &in[0][0], *const kt = kk + kK, *const qq = kApart ? kt + kKt : kt;
   const int group = blockIdx.x % groups;
@@ -348,8 +346,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaPa
     put_gates(c0);
     // P's zeros beside the diagonal tiles that begin a pair
     if (!MAP)
-      for (int e = tid; e < 32 * OP * 4; e += NT) {
-        const int row = (e & 31) < 16 ? (e & 31) : 16 + (e & 31), k = (e >> 5) % OP, q = 4 * (row >> 5 << 1) + 4 + (e >> 5) / OP;
+      for (int e = tid; e < 32 * 3 * 4; e += NT) {
+        const int row = (e & 31) < 16 ? (e & 31) : 16 + (e & 31), k = (e >> 5) % 3, q = 4 * (row >> 5 << 1) + 4 + (e >> 5) / 3;
         *reinterpret_cast<u32x2*>(&pp[MAP ? 0 : k][tri_at(row) + place4(q)]) = u32x2{0, 0};
       }
   }
@@ -397,10 +395,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaPa
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             acc[k] = i >= 16 * tc + 4 * g + k ? acc[k] * __builtin_amdgcn_exp2f((hi_i - hi[k]) + (lo_i - lo[k])) : 0.0f;
-          u32x2 part[OP];
-          split4<OP>(part, acc);
+          u32x2 part[3];
+          split4<3>(part, acc);
 #pragma unroll
-          for (int k = 0; k < OP; ++k)
+          for (int k = 0; k < 3; ++k)
             *reinterpret_cast<u32x2*>(&pp[MAP ? 0 : k][tri_at(i) + 32 * (tc >> 1) + 8 * g + 4 * (tc & 1)]) = part[k];
         }
       }
@@ -423,10 +421,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaPa
         products<NP, (NP == 1 ? 3 : 1), (MAP ? 4 : 8)>(
             kIn, [&](int i) { return (i < 4 ? kk : qq) + (16 * (i & 3) + r) * LDK + 32 * s + 8 * g; },
             [&](int i, const u32x4(&a)[NP]) {
-              if (i < 4)
-                mul<3, 2>(x[i & 3], a, sp);
-              else
-                mul<OP, OP - 1>(o[i & 3], a, sp);
+              mul<3, 2>(i < 4 ? x[i & 3] : o[i & 3], a, sp);
             });
       }
 #pragma unroll
@@ -458,12 +453,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) delta_walk_kernel(const DeltaPa
       if (!MAP) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) o[t] *= load4(gt + kGam + 16 * t + 4 * g);
-        u32x4 up[2][OP];
-        split_pair<OP>(up[0], x[0], x[1]);
-        split_pair<OP>(up[1], x[2], x[3]);
-        products<OP, 1, 6>(
+        u32x4 up[2][3];
+        split_pair<3>(up[0], x[0], x[1]);
+        split_pair<3>(up[1], x[2], x[3]);
+        products<3, 1, 6>(
             kTri, [&](int i) { return &pp[0][0] + tri_at(16 * (i < 4 ? i : i - 2) + r) + 32 * (i >> 2) + 8 * g; },
-            [&](int i, const u32x4(&a)[OP]) { mul<OP, OP - 1>(o[i < 4 ? i : i - 2], a, up[i >> 2]); });
+            [&](int i, const u32x4(&a)[3]) { mul<3, 2>(o[i < 4 ? i : i - 2], a, up[i >> 2]); });
         const int rows = tokens - (int)t0;
         if (rows < kDeltaChunk)   // zeros past the tokens in use
 #pragma unroll
