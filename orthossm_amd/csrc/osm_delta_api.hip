@@ -96,6 +96,14 @@ Sizes sizes_of(const osm_delta_args* a) {
 
 DeltaRows rows_of(const osm_rows& r) { return {r.p, r.stride_b, r.stride_s, r.stride_h}; }
 
+// Rows of d elements over S tokens as the kernels address them: a chunk's rows past
+// its tokens are told by their offset, so a single token, whose stride can be
+// anything, gets one that holds its row (a multiple of 4, as wide accesses want it).
+osm_rows token_rows(osm_rows r, int64_t S, int64_t d) {
+  if (S == 1) r.stride_s = (d + 3) / 4 * 4;
+  return r;
+}
+
 bool whole(const osm_rows& r, int esize, int n) {
   return (uintptr_t)r.p % (n * esize) == 0 && r.stride_b % n == 0 && r.stride_s % n == 0 && r.stride_h % n == 0;
 }
@@ -125,9 +133,10 @@ int check_workspace(const void* ws, size_t have, size_t need) {
 
 DeltaParams params_of(const osm_delta_args* a) {
   DeltaParams p{};
-  p.q = rows_of(a->q);
-  p.k = rows_of(a->k);
-  p.v = rows_of(a->v);
+  const osm_rows q = token_rows(a->q, a->S, a->dk), k = token_rows(a->k, a->S, a->dk), v = token_rows(a->v, a->S, a->dv);
+  p.q = rows_of(q);
+  p.k = rows_of(k);
+  p.v = rows_of(v);
   p.g = rows_of(a->g);
   p.beta = rows_of(a->beta);
   p.lengths = a->lengths;
@@ -147,7 +156,7 @@ DeltaParams params_of(const osm_delta_args* a) {
   p.scale = a->scale;
   const int es = a->dtype == OSM_F32 ? 4 : 2;
   for (p.vec = 4; p.vec > 1; p.vec /= 2)
-    if (a->dk % p.vec == 0 && a->dv % p.vec == 0 && whole(a->q, es, p.vec) && whole(a->k, es, p.vec) && whole(a->v, es, p.vec))
+    if (a->dk % p.vec == 0 && a->dv % p.vec == 0 && whole(q, es, p.vec) && whole(k, es, p.vec) && whole(v, es, p.vec))
       break;
   return p;
 }
@@ -184,7 +193,7 @@ int osm_delta_fwd(const osm_delta_args* a, void* workspace, size_t workspace_byt
   if (a->B == 0 || a->S == 0) return copy_state(a->state_init, a->state_out, (size_t)a->B * a->H * a->dk * a->dv, st);
   if ((rc = check_tokens(a->out, a->dtype == OSM_F32 ? 4 : 2, a->S, a->dv, "out")) != OSM_OK) return rc;
   DeltaParams p = params_of(a);
-  p.o = rows_of(a->out);
+  p.o = rows_of(token_rows(a->out, a->S, a->dv));
   hipError_t e;
   if (is_short(a)) {
     osm::DeltaStepParams s{};
@@ -250,13 +259,15 @@ int osm_delta_bwd(const osm_delta_args* a, const osm_delta_bwd_args* b, void* wo
   p.a = static_cast<float*>(workspace);
   p.x = p.a + n.seg_a;
   p.d = p.x + n.seg_x;
-  if (!whole(b->grad_out, es, p.vec)) p.vec = 1;
+  const osm_rows go = token_rows(b->grad_out, a->S, a->dv), gq = token_rows(b->grad_q, a->S, a->dk),
+                 gk = token_rows(b->grad_k, a->S, a->dk);
+  if (!whole(go, es, p.vec)) p.vec = 1;
   // (gradients by head are in the workspace, rows of dk)
-  p.out_vec = a->dk % 4 == 0 && (a->H != a->Hk || (whole(b->grad_q, es, 4) && whole(b->grad_k, es, 4)));
-  p.dout = rows_of(b->grad_out);
-  p.dq = rows_of(b->grad_q);
-  p.dk = rows_of(b->grad_k);
-  p.dv = rows_of(b->grad_v);
+  p.out_vec = a->dk % 4 == 0 && (a->H != a->Hk || (whole(gq, es, 4) && whole(gk, es, 4)));
+  p.dout = rows_of(go);
+  p.dq = rows_of(gq);
+  p.dk = rows_of(gk);
+  p.dv = rows_of(token_rows(b->grad_v, a->S, a->dv));
   p.dg = rows_of(b->grad_g);
   p.dbeta = rows_of(b->grad_beta);
   p.grad_state = b->grad_state;
