@@ -370,7 +370,7 @@ typedef struct osm_engine_args {
  * reach the outputs of its whole chunk of 64 tokens, and those after it. */
 typedef struct osm_rows {
   void* p;                      /* element (b, t, h, j) at b*stride_b + t*stride_s + h*stride_h + j */
-  int64_t stride_b, stride_s, stride_h;   /* elements, >= 0; stride_s <= OSM_DELTA_MAX_STRIDE */
+  int64_t stride_b, stride_s, stride_h;   /* elements, >= 0; stride_s <= OSM_DELTA_MAX_STRIDE, and unused where S = 1 */
 } osm_rows;
 
 #define OSM_DELTA_MAX_DK 128
@@ -381,7 +381,7 @@ typedef struct osm_delta_args {
   int32_t dtype;                /* osm_dtype of q, k, v, out and their gradients */
   int64_t B, S, H, Hk, dk, dv;  /* dk <= OSM_DELTA_MAX_DK */
   float scale;
-  osm_rows q, k, v, out;        /* [B,S,Hk,dk] (q, k), [B,S,H,dv] (v, out); stride_s at least the row's elements */
+  osm_rows q, k, v, out;        /* [B,S,Hk,dk] (q, k), [B,S,H,dv] (v, out); stride_s at least the row's elements (S > 1) */
   osm_rows g, beta;             /* [B,S,H] fp32 */
   const int32_t* lengths;       /* [B], or NULL: every row has S tokens */
   const float* state_init;      /* [B,H,dk,dv] contiguous, or NULL: zeros */

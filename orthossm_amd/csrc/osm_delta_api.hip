@@ -38,11 +38,13 @@ int check_common(int32_t abi, int32_t dtype, int64_t B, int64_t H, int64_t Hk, i
   return OSM_OK;
 }
 
-int check_rows(const osm_rows& r, int esize, const char* name) {
+// (the stride of a single token is not used: it can be anything)
+int check_rows(const osm_rows& r, int esize, int64_t S, const char* name) {
   if (!r.p) return fail(OSM_E_ARG, "%s is NULL", name);
   if ((uintptr_t)r.p % esize) return fail(OSM_E_LAYOUT, "%s is not aligned to its elements", name);
-  if (r.stride_b < 0 || r.stride_s < 0 || r.stride_h < 0) return fail(OSM_E_LAYOUT, "%s has a negative stride", name);
-  if (r.stride_s > OSM_DELTA_MAX_STRIDE)
+  if (r.stride_b < 0 || (S > 1 && r.stride_s < 0) || r.stride_h < 0)
+    return fail(OSM_E_LAYOUT, "%s has a negative stride", name);
+  if (S > 1 && r.stride_s > OSM_DELTA_MAX_STRIDE)
     return fail(OSM_E_LAYOUT, "%s: %lld elements from token to token, at most %d", name, (long long)r.stride_s, OSM_DELTA_MAX_STRIDE);
   return OSM_OK;
 }
@@ -50,7 +52,7 @@ int check_rows(const osm_rows& r, int esize, const char* name) {
 // Rows of d elements over S tokens: a chunk's rows are told from those past it by
 // their offset.
 int check_tokens(const osm_rows& r, int esize, int64_t S, int64_t d, const char* name) {
-  const int rc = check_rows(r, esize, name);
+  const int rc = check_rows(r, esize, S, name);
   if (rc == OSM_OK && S > 1 && r.stride_s < d)
     return fail(OSM_E_LAYOUT, "%s: %lld elements from token to token, rows of %lld overlap", name, (long long)r.stride_s, (long long)d);
   return rc;
@@ -114,8 +116,8 @@ int check_inputs(const osm_delta_args* a) {
   const int es = a->dtype == OSM_F32 ? 4 : 2;
   if (a->B > 0 && a->S > 0) {
     if ((rc = check_tokens(a->q, es, a->S, a->dk, "q")) != OSM_OK || (rc = check_tokens(a->k, es, a->S, a->dk, "k")) != OSM_OK ||
-        (rc = check_tokens(a->v, es, a->S, a->dv, "v")) != OSM_OK || (rc = check_rows(a->g, 4, "g")) != OSM_OK ||
-        (rc = check_rows(a->beta, 4, "beta")) != OSM_OK)
+        (rc = check_tokens(a->v, es, a->S, a->dv, "v")) != OSM_OK || (rc = check_rows(a->g, 4, a->S, "g")) != OSM_OK ||
+        (rc = check_rows(a->beta, 4, a->S, "beta")) != OSM_OK)
       return rc;
     if ((uintptr_t)a->lengths % 4) return fail(OSM_E_LAYOUT, "lengths must be 4-byte aligned");
     if ((uintptr_t)a->saved % 256) return fail(OSM_E_WORKSPACE, "saved must be 256-byte aligned");
@@ -248,7 +250,7 @@ int osm_delta_bwd(const osm_delta_args* a, const osm_delta_bwd_args* b, void* wo
   const int es = a->dtype == OSM_F32 ? 4 : 2;
   if ((rc = check_tokens(b->grad_out, es, a->S, a->dv, "grad_out")) != OSM_OK || (rc = check_tokens(b->grad_q, es, a->S, a->dk, "grad_q")) != OSM_OK ||
       (rc = check_tokens(b->grad_k, es, a->S, a->dk, "grad_k")) != OSM_OK || (rc = check_tokens(b->grad_v, es, a->S, a->dv, "grad_v")) != OSM_OK ||
-      (rc = check_rows(b->grad_g, 4, "grad_g")) != OSM_OK || (rc = check_rows(b->grad_beta, 4, "grad_beta")) != OSM_OK)
+      (rc = check_rows(b->grad_g, 4, a->S, "grad_g")) != OSM_OK || (rc = check_rows(b->grad_beta, 4, a->S, "grad_beta")) != OSM_OK)
     return rc;
   if ((rc = check_workspace(workspace, workspace_bytes, osm_delta_bwd_workspace_bytes(a))) != OSM_OK) return rc;
   DeltaParams p = params_of(a);
@@ -286,9 +288,9 @@ int osm_delta_step(const osm_delta_step_args* a, void* stream) {
     return fail(OSM_E_SHAPE, "n_slots=%lld, B=%lld rows without slots", (long long)a->n_slots, (long long)a->B);
   if (a->B == 0) return ok();
   const int es = a->dtype == OSM_F32 ? 4 : 2;
-  if ((rc = check_rows(a->q, es, "q")) != OSM_OK || (rc = check_rows(a->k, es, "k")) != OSM_OK ||
-      (rc = check_rows(a->v, es, "v")) != OSM_OK || (rc = check_rows(a->out, es, "out")) != OSM_OK ||
-      (rc = check_rows(a->g, 4, "g")) != OSM_OK || (rc = check_rows(a->beta, 4, "beta")) != OSM_OK)
+  if ((rc = check_rows(a->q, es, 1, "q")) != OSM_OK || (rc = check_rows(a->k, es, 1, "k")) != OSM_OK ||
+      (rc = check_rows(a->v, es, 1, "v")) != OSM_OK || (rc = check_rows(a->out, es, 1, "out")) != OSM_OK ||
+      (rc = check_rows(a->g, 4, 1, "g")) != OSM_OK || (rc = check_rows(a->beta, 4, 1, "beta")) != OSM_OK)
     return rc;
   if (!a->state && a->n_slots > 0) return fail(OSM_E_ARG, "state is NULL");
   if ((rc = check_state(a->state, "state")) != OSM_OK) return rc;

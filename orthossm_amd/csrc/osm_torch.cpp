@@ -645,8 +645,7 @@ osm_rows rows_of(const at::Tensor& t) { return {t.data_ptr(), t.stride(0), t.str
 // Tokens' rows as the kernels address them.
 bool token_rows(const at::Tensor& t, int64_t dim) {
   const int64_t s = t.size(1) > 1 ? t.stride(1) : dim;
-  return t.stride(0) >= 0 && t.stride(2) >= 0 && s >= dim && t.stride(1) >= 0 && t.stride(1) <= OSM_DELTA_MAX_STRIDE &&
-         (dim == 1 || t.stride(3) == 1);
+  return t.stride(0) >= 0 && t.stride(2) >= 0 && s >= dim && s <= OSM_DELTA_MAX_STRIDE && (dim == 1 || t.stride(3) == 1);
 }
 
 // A scale: a number, or None for 1/sqrt(dk).
@@ -746,7 +745,7 @@ bool delta_tensors(Delta* d) {
     if (t.device() != q.device()) return false;
     if (i < 3 ? !token_rows(t, t.size(3))
               : !is_f32(t) || t.size(0) != a.B || t.size(1) != a.S || t.size(2) != a.H || t.stride(0) < 0 ||
-                    t.stride(1) < 0 || t.stride(2) < 0 || t.stride(1) > OSM_DELTA_MAX_STRIDE)
+                    t.stride(2) < 0 || (a.S > 1 && (t.stride(1) < 0 || t.stride(1) > OSM_DELTA_MAX_STRIDE)))
       return false;
   }
   a.q = rows_of(q);

@@ -73,7 +73,7 @@ def _gate(t, shape, dev, name: str) -> torch.Tensor:
     if not isinstance(t, torch.Tensor) or tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name} must be a tensor of shape {tuple(shape)}")
     t = t.to(device=dev, dtype=torch.float32)
-    return t if t.dim() < 3 or t.stride(1) <= nat.DELTA_MAX_STRIDE else t.contiguous()
+    return t if t.dim() < 3 or t.shape[1] <= 1 or t.stride(1) <= nat.DELTA_MAX_STRIDE else t.contiguous()
 
 
 def _state(t, shape, dev, name: str) -> torch.Tensor | None:

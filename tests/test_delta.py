@@ -154,3 +154,20 @@ def test_step_errors():
 def test_struct_layout_matches_ctypes(cls, cname):
     from test_abi import test_struct_layout_matches_ctypes as layout
     layout(cls, cname)
+
+
+def test_a_single_tokens_stride_is_not_checked():
+    """The errors are those of a later argument, not of the strides."""
+    lib = nat.load()
+    for stride in (1 << 40, 0, -4):
+        a = _args(S=1, saved=0x10010)
+        for name in ("q", "k", "v", "g", "beta"):
+            getattr(a, name).stride_s = stride
+        assert _fwd(a) == -5
+        s = nat.DeltaStepArgs()
+        s.abi_version = nat.ABI_VERSION
+        s.B, s.H, s.Hk, s.dk, s.dv, s.n_slots = 2, 4, 2, 48, 80, 3
+        for r in (s.q, s.k, s.v, s.out, s.g, s.beta):
+            r.p, r.stride_s = 0x10000, stride
+        assert lib.osm_delta_step(ctypes.byref(s), None) == -1
+        assert lib.osm_last_error() == b"state is NULL"

@@ -50,3 +50,17 @@ def test_broadcast_gradient_of_one_value(dev):
     out = gated_delta(*leaves[:5], state_init=leaves[5])
     for i, (got, ref) in enumerate(zip(torch.autograd.grad(out.sum(), leaves), want)):
         close(got, ref, 2 * FP32 if i in (3, 4) else FP32, i)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_token_stride_past_the_limit(dev, grad):
+    """Time-major tensors of one token: a stride that no chunk could have."""
+    t = {n: x.to(dev) for n, x in make(2, 1, 2, 16).items()}
+    far = [x.as_strided(x.shape, (x.stride(0), 1 << 23, *x.stride()[2:])) for x in args(t)]
+    near, far = ([x.detach().requires_grad_(grad) for x in ins] for ins in (args(t), far))
+    want, got = (gated_delta(*ins, state_init=t["state_init"], return_state=True) for ins in (near, far))
+    assert all(torch.equal(x, y) for x, y in zip(want, got))
+    if grad:
+        go = t["grad_out"].as_strided(t["grad_out"].shape, (32, 1 << 23, 16, 1))
+        for x, y in zip(torch.autograd.grad(want[0], near, t["grad_out"]), torch.autograd.grad(got[0], far, go)):
+            assert torch.equal(x, y)
