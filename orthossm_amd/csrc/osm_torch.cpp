@@ -657,6 +657,10 @@ bool as_scale(PyObject* o, int64_t dk, float* v) {
   return as_float(o, v);
 }
 
+// Whether t is a dual number of forward-mode differentiation, which the operators
+// have no derivative for: the Python functions' autograd functions refuse it.
+bool has_tangent(const at::Tensor& t) { return t._fw_grad(0).defined(); }
+
 std::optional<at::Tensor> optional_tensor(PyObject* o) {
   return o == Py_None ? std::nullopt : std::optional<at::Tensor>(*plain(o));
 }
@@ -933,6 +937,13 @@ PyObject* run_gated_delta(PyObject* const* p) {
   Delta d;
   float* init;
   if (!delta_common(p, &d) || !state_ptr(p[7], d, &init)) Py_RETURN_NONE;
+  const std::optional<at::Tensor> first = optional_tensor(p[7]), lengths = optional_tensor(p[6]);
+  bool grad = first && first->requires_grad(), dual = first && has_tangent(*first);
+  for (int i = 0; i < 5; ++i) {
+    grad = grad || d.t[i]->requires_grad();
+    dual = dual || has_tangent(*d.t[i]);
+  }
+  if (dual) Py_RETURN_NONE;
   const bool want_state = PyObject_IsTrue(p[8]) == 1;
   if (PyErr_Occurred()) return nullptr;
   d.a.state_init = init;
@@ -940,9 +951,6 @@ PyObject* run_gated_delta(PyObject* const* p) {
   void* stream;
   const c10::DeviceGuard guard(d.t[0]->device());
   if (!stream_of(*d.t[0], &s_obj, &stream)) return nullptr;
-  const std::optional<at::Tensor> first = optional_tensor(p[7]), lengths = optional_tensor(p[6]);
-  bool grad = first && first->requires_grad();
-  for (int i = 0; i < 5; ++i) grad = grad || d.t[i]->requires_grad();
   at::Tensor out, fin, saved;
   int rc;
   {
@@ -1193,11 +1201,12 @@ PyObject* run_layer_norm(PyObject* const* p) {
   osm_norm_args a{};
   norm_args(x, &a);
   if (!norm_param(p[1], a.D, x, &a.weight) || !norm_param(p[2], a.D, x, &a.bias) || !as_float(p[3], &a.eps)) Py_RETURN_NONE;
+  const std::optional<at::Tensor> weight = optional_tensor(p[1]), bias = optional_tensor(p[2]);
+  if (has_tangent(x) || (weight && has_tangent(*weight)) || (bias && has_tangent(*bias))) Py_RETURN_NONE;
   Ref s_obj;
   void* stream;
   const c10::DeviceGuard guard(x.device());
   if (!stream_of(x, &s_obj, &stream)) return nullptr;
-  const std::optional<at::Tensor> weight = optional_tensor(p[1]), bias = optional_tensor(p[2]);
   const bool grad = x.requires_grad() || (weight && weight->requires_grad()) || (bias && bias->requires_grad());
   at::Tensor y, mean, rstd;
   int rc;

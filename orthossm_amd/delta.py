@@ -28,6 +28,7 @@ import contextlib
 import ctypes
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.function import once_differentiable
 
 from . import _native as nat
@@ -47,6 +48,14 @@ def _set_rows(r: nat.Rows, t: torch.Tensor) -> None:
 def _unit_rows(t: torch.Tensor) -> torch.Tensor:
     near = t.dim() < 4 or t.shape[1] <= 1 or t.shape[3] <= t.stride(1) <= nat.DELTA_MAX_STRIDE
     return t if near and (t.stride(-1) == 1 or t.shape[-1] == 1) else t.contiguous()
+
+
+def differentiable(*tensors) -> bool:
+    """Whether a call on these has a derivative to record, or (a dual number of
+    forward-mode differentiation) one that its autograd function refuses."""
+    ts = [t for t in tensors if isinstance(t, torch.Tensor)]
+    return (torch.is_grad_enabled() and any(t.requires_grad for t in ts)) or \
+        any(unpack_dual(t).tangent is not None for t in ts)
 
 
 def _check_qkv(q, k, v, dims: int, form: str):
@@ -249,8 +258,7 @@ def gated_delta(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tens
         res = fast.gated_delta(q, k, v, g, beta, scale, lengths, state_init, return_state)
         if res is not None:
             return res if return_state else res[0]
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad
-                                       for t in (q, k, v, g, beta, state_init)):
+    if differentiable(q, k, v, g, beta, state_init):
         out, fin = _GatedDeltaFunction.apply(q, k, v, g, beta, state_init, lengths, scale)
         return (out, fin) if return_state else out
     return gated_delta_forward(q, k, v, g, beta, scale=scale, state_init=state_init, lengths=lengths,

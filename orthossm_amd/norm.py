@@ -19,7 +19,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native as nat
-from .delta import _dest, _scratch, on_device
+from .delta import _dest, _scratch, differentiable, on_device
 from .ops import _current_stream, _dtype_code, _fast
 
 
@@ -160,6 +160,6 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
         y = fast.layer_norm(x, weight, bias, eps)
         if y is not None:
             return y
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (x, weight, bias)):
+    if differentiable(x, weight, bias):
         return _LayerNormFunction.apply(x, weight, bias, eps)
     return _forward(x, weight, bias, eps, None, False)[0]
