@@ -661,6 +661,12 @@ bool as_scale(PyObject* o, int64_t dk, float* v) {
 // have no derivative for: the Python functions' autograd functions refuse it.
 bool has_tangent(const at::Tensor& t) { return t._fw_grad(0).defined(); }
 
+// Tells autograd that a launch wrote into t: a graph that saved it refuses its
+// backward.  (Inference tensors have no version, and no graph saves them.)
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 std::optional<at::Tensor> optional_tensor(PyObject* o) {
   return o == Py_None ? std::nullopt : std::optional<at::Tensor>(*plain(o));
 }
@@ -1028,6 +1034,7 @@ PyObject* run_delta_step(PyObject* const* p) {
     rc = lib.delta_step(&a, stream);
   }
   if (rc != OSM_OK) return fail_rc(rc);
+  written(state);
   return THPVariable_Wrap(out);
 }
 
@@ -1238,6 +1245,7 @@ PyObject* run_clip(PyObject* const* p) {
   std::vector<void*> ptr(n);
   std::vector<int64_t> size(n);
   std::vector<int32_t> dtype(n);
+  std::vector<at::Tensor> scaled;   // (the list may change while the lock is released)
   const at::Tensor* first = nullptr;
   for (Py_ssize_t i = 0; i < n; ++i) {
     const at::Tensor* const t = plain(PySequence_Fast_GET_ITEM(p[0], i));
@@ -1248,6 +1256,7 @@ PyObject* run_clip(PyObject* const* p) {
     ptr[i] = t->data_ptr();
     size[i] = t->numel();
     dtype[i] = code(*t);
+    if (scale) scaled.push_back(*t);
   }
   if (scale) {   // a tensor given twice is refused by the Python path
     std::vector<void*> seen;
@@ -1279,6 +1288,7 @@ PyObject* run_clip(PyObject* const* p) {
     rc = lib.clip(&a, ws.data_ptr(), (size_t)ws.numel(), stream);
   }
   if (rc != OSM_OK) return fail_rc(rc);
+  for (const at::Tensor& t : scaled) written(t);
   return THPVariable_Wrap(norm);
 }
 

@@ -30,6 +30,7 @@ import ctypes
 import torch
 from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _native as nat
 from .ops import _current_device, _current_stream, _dtype_code, _fast
@@ -97,6 +98,17 @@ def _dest(t, shape, dtype, dev, name: str) -> None:
     if not isinstance(t, torch.Tensor) or tuple(t.shape) != tuple(shape) or t.dtype != dtype or t.device != dev or \
             not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {dev}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, which what is written into it has not")
+
+
+def written(*tensors) -> None:
+    """Tells autograd that a launch wrote into these (None: skipped): a graph
+    that saved one refuses its backward, as after torch's own in-place
+    operations."""
+    for t in tensors:
+        if t is not None and not t.is_inference():
+            increment_version(t)
 
 
 def _lengths(t, B: int, S: int, dev) -> torch.Tensor | None:
@@ -141,7 +153,7 @@ def _forward(q, k, v, g, beta, scale, state_init, lengths, out, return_state, st
             return (*res, (q, k, v, g, beta, state_init, lengths))
     lib = nat.load()
     a, keep = _prepare(q, k, v, g, beta, scale, state_init, lengths)
-    v = keep[2]
+    v, given = keep[2], (out, state_out)
     dev, shape = v.device, (a.B, a.S, a.H, a.dv)
     if out is None:
         out = torch.empty(shape, dtype=v.dtype, device=dev)
@@ -162,6 +174,7 @@ def _forward(q, k, v, g, beta, scale, state_init, lengths, out, return_state, st
     with on_device(dev):
         nat.check(lib.osm_delta_fwd(ctypes.byref(a), ctypes.c_void_p(ws.data_ptr()), ws.numel(),
                                     ctypes.c_void_p(_current_stream(dev))))
+    written(*given)
     return out, state_out, saved, keep
 
 
@@ -296,6 +309,7 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     elif not isinstance(slots, torch.Tensor) or tuple(slots.shape) != (B,) or slots.dtype != torch.int64 or \
             slots.device != dev or not slots.is_contiguous():
         raise ValueError(f"slots must be a contiguous int64 tensor of shape ({B},) on {dev}")
+    given = out
     if out is None:
         out = torch.empty((B, H, dv), dtype=v.dtype, device=dev)
     else:
@@ -311,4 +325,5 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     a.slots = slots.data_ptr() if slots is not None else None
     with on_device(dev):
         nat.check(lib.osm_delta_step(ctypes.byref(a), ctypes.c_void_p(_current_stream(dev))))
+    written(state, given)
     return out

@@ -16,7 +16,7 @@ from typing import Iterable
 import torch
 
 from . import _native as nat
-from .delta import _scratch, on_device
+from .delta import _scratch, on_device, written
 from .ops import _current_stream, _dtype_code, _fast
 
 
@@ -72,7 +72,9 @@ def _run(grads, max_norm: float, eps: float, scale: bool) -> torch.Tensor:
                                          ctypes.c_void_p(_current_stream(dev))))
     if scale:
         for t, w in zip(grads, work):
-            if w is not t:
+            if w is t:
+                written(t)
+            else:
                 t.copy_(w)
     return norm
 

@@ -19,7 +19,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native as nat
-from .delta import _dest, _scratch, differentiable, on_device
+from .delta import _dest, _scratch, differentiable, on_device, written
 from .ops import _current_stream, _dtype_code, _fast
 
 
@@ -70,7 +70,7 @@ def _forward(x, weight, bias, eps, out, stats: bool):
             return res
     lib = nat.load()
     a, x, keep = _prepare(x, weight, bias, eps)
-    dev = x.device
+    dev, given = x.device, out
     if out is None:
         out = torch.empty(x.shape, dtype=x.dtype, device=dev)
     else:
@@ -82,6 +82,7 @@ def _forward(x, weight, bias, eps, out, stats: bool):
         a.mean, a.rstd = mean.data_ptr(), rstd.data_ptr()
     with on_device(dev):
         nat.check(lib.osm_layer_norm_fwd(ctypes.byref(a), ctypes.c_void_p(_current_stream(dev))))
+    written(given)
     del keep
     return out, mean, rstd
 

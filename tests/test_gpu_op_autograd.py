@@ -4,7 +4,8 @@ import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
-from orthossm_amd import delta, gated_delta, grad_clip, layer_norm, norm, ops
+from orthossm_amd import (clip_grad_norm, delta, gated_delta, gated_delta_forward, gated_delta_step, grad_clip, grad_norm,
+                          layer_norm, layer_norm_forward, norm, ops)
 
 pytestmark = pytest.mark.gpu
 
@@ -44,3 +45,84 @@ def test_forward_mode_is_refused(dev, path, grad):
                     call(mine)
                 with torch.no_grad(), pytest.raises(NotImplementedError, match="forward mode"):
                     call(mine)
+
+
+def token(dev):
+    return [t[:, 0].contiguous() for t in delta_inputs(dev)[:5]]
+
+
+def writers(dev):
+    """name: (the tensor a call writes into, the call)."""
+    ins, (x, w, b) = delta_inputs(dev), norm_inputs(dev)
+    state, out, first = ins[5].clone(), torch.zeros(2, 2, 12, device=dev), torch.zeros(2, 20, 2, 12, device=dev)
+    last, y = ins[5].clone(), x.clone()
+    grads = [torch.ones(9, device=dev), torch.ones(20, 6, device=dev)[:, ::2]]
+    return {
+        "step's state": (state, lambda: gated_delta_step(*token(dev), state)),
+        "step's out": (out, lambda: gated_delta_step(*token(dev), ins[5].clone(), out=out)),
+        "out": (first, lambda: gated_delta_forward(*ins[:5], out=first)),
+        "state_out": (last, lambda: gated_delta_forward(*ins[:5], state_init=last, return_state=True, state_out=last)),
+        "norm's out": (y, lambda: layer_norm_forward(y, w, b, out=y)),
+        "a gradient": (grads[0], lambda: clip_grad_norm(grads, 1.0)),
+        "a gradient with gaps": (grads[1], lambda: clip_grad_norm(grads, 1.0)),
+    }
+
+
+WRITERS = ["step's state", "step's out", "out", "state_out", "norm's out", "a gradient", "a gradient with gaps"]
+
+
+@pytest.mark.parametrize("name", WRITERS)
+def test_writes_are_seen_by_graphs_that_saved_the_tensor(dev, path, name):
+    t, call = writers(dev)[name]
+    factor = torch.ones_like(t, requires_grad=True)
+    for _ in range(2):      # the second time after a write of the first
+        product = t * factor
+        (product.sum()).backward()
+        product = t * factor
+        call()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            product.sum().backward()
+
+
+def test_reads_are_not_writes(dev, path):
+    ins, (x, w, b) = delta_inputs(dev), norm_inputs(dev)
+    ts = [*ins, x, w, b]
+    before = [t._version for t in ts]
+    gated_delta_forward(*ins[:5], state_init=ins[5], return_state=True)
+    layer_norm_forward(x, w, b)
+    grad_norm(ts)
+    assert [t._version for t in ts] == before
+
+
+@pytest.mark.parametrize("name", WRITERS)
+def test_inference_tensors_are_written(dev, path, name):
+    with torch.inference_mode():
+        t, call = writers(dev)[name]
+        before = t.clone()
+        call()
+    assert not torch.equal(t, before)
+
+
+def test_a_pool_made_in_inference_mode_serves_outside_it(dev, path):
+    with torch.inference_mode():
+        state = delta_inputs(dev)[5].clone()
+    before = state.clone()
+    gated_delta_step(*token(dev), state)
+    assert not torch.equal(state, before)
+
+
+def test_outputs_that_require_a_gradient_are_refused(dev, path):
+    ins, (x, w, b) = delta_inputs(dev), norm_inputs(dev)
+
+    def leaf(*shape):
+        return torch.zeros(*shape, device=dev, requires_grad=True)
+
+    calls = (lambda: gated_delta_forward(*ins[:5], out=leaf(2, 20, 2, 12)),
+             lambda: gated_delta_forward(*ins[:5], return_state=True, state_out=leaf(2, 2, 8, 12)),
+             lambda: gated_delta_step(*token(dev), ins[5].clone(), out=leaf(2, 2, 12)),
+             lambda: layer_norm_forward(x, w, b, out=leaf(4, 40)))
+    for call in calls:
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+        with torch.no_grad():
+            call()
