@@ -451,7 +451,8 @@ typedef struct osm_clip_args {
   int32_t abi_version;          /* = OSM_ABI_VERSION */
   int32_t flags;
   int64_t count;
-  void* const* tensors;         /* [count] device pointers (this array and the next two are host memory) */
+  void* const* tensors;         /* [count] device pointers (this array and the next two are host memory); with
+                                 * OSM_CLIP_SCALE no two share memory */
   const int64_t* sizes;         /* [count] elements, dense */
   const int32_t* dtypes;        /* [count] osm_dtype */
   double max_norm, eps;         /* >= 0 */

@@ -1,6 +1,9 @@
 // C ABI of the layer norm and of gradient clipping: argument checks and
 // dispatch.  Declared in include/osm.h.
 #include <algorithm>
+#include <new>
+#include <utility>
+#include <vector>
 
 #include "osm.h"
 #include "osm_kernels.h"
@@ -72,6 +75,24 @@ int check_clip(const osm_clip_args* a) {
   if (!(a->max_norm >= 0.0) || !(a->eps >= 0.0))
     return fail(OSM_E_ARG, "max_norm=%g and eps=%g must be >= 0", a->max_norm, a->eps);
   return OSM_OK;
+}
+
+// Tensors that are scaled in place share no memory: two workgroups would read and
+// write the same elements in no order.
+int check_apart(const osm_clip_args* a) try {
+  std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+  spans.reserve(a->count);
+  for (int64_t i = 0; i < a->count; ++i) {
+    const uintptr_t p = (uintptr_t)a->tensors[i];
+    if (a->sizes[i] > 0) spans.emplace_back(p, p + (uintptr_t)a->sizes[i] * (a->dtypes[i] == OSM_F32 ? 4 : 2));
+  }
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    if (spans[i].first < spans[i - 1].second)
+      return fail(OSM_E_LAYOUT, "two of the tensors share memory, at %p", (void*)spans[i].first);
+  return OSM_OK;
+} catch (const std::bad_alloc&) {
+  return fail(OSM_E_ARG, "no host memory for %lld tensors", (long long)a->count);
 }
 
 int64_t chunks_of(int64_t n) { return (n + osm::kClipChunk - 1) / osm::kClipChunk; }
@@ -179,6 +200,7 @@ size_t osm_clip_workspace_bytes(const osm_clip_args* a) {
 
 int osm_clip_grad_norm(const osm_clip_args* a, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_clip(a);
+  if (rc == OSM_OK && a->flags & OSM_CLIP_SCALE) rc = check_apart(a);
   if (rc != OSM_OK) return rc;
   if (!a->norm || (uintptr_t)a->norm % 4) return fail(OSM_E_ARG, "norm is NULL or not 4-byte aligned");
   const size_t need = osm_clip_workspace_bytes(a);

@@ -21,7 +21,6 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/version.h>
 
-#include <algorithm>
 #include <cmath>
 #include <vector>
 
@@ -1258,13 +1257,6 @@ PyObject* run_clip(PyObject* const* p) {
     dtype[i] = code(*t);
     if (scale) scaled.push_back(*t);
   }
-  if (scale) {   // a tensor given twice is refused by the Python path
-    std::vector<void*> seen;
-    for (Py_ssize_t i = 0; i < n; ++i)
-      if (size[i]) seen.push_back(ptr[i]);
-    std::sort(seen.begin(), seen.end());
-    if (std::adjacent_find(seen.begin(), seen.end()) != seen.end()) Py_RETURN_NONE;
-  }
   osm_clip_args a{};
   a.abi_version = OSM_ABI_VERSION;
   a.flags = scale ? OSM_CLIP_SCALE : 0;
@@ -1287,6 +1279,7 @@ PyObject* run_clip(PyObject* const* p) {
     ws = scratch(lib.clip_bytes(&a), *first);
     rc = lib.clip(&a, ws.data_ptr(), (size_t)ws.numel(), stream);
   }
+  if (rc == OSM_E_LAYOUT) Py_RETURN_NONE;   // tensors that share memory: the Python path says so
   if (rc != OSM_OK) return fail_rc(rc);
   for (const at::Tensor& t : scaled) written(t);
   return THPVariable_Wrap(norm);

@@ -3,7 +3,8 @@
 ``grad_norm``       sqrt of the sum of squares over all elements of many tensors.
 ``clip_grad_norm``  the same, and every tensor times min(1, max_norm / (norm + eps)) in place.
 
-Tensors are fp32 or bf16 in any mix, of any sizes, on one device.  Sums are
+Tensors are fp32 or bf16 in any mix, of any sizes, on one device; those that are
+clipped share no memory.  Sums are
 held in double; the norm stays on the device, so nothing synchronises the host.
 A NaN norm makes every element NaN, an infinite one makes finite elements 0 and
 infinite ones NaN.  There is no CPU path.
@@ -30,6 +31,24 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
+def _share_memory(tensors) -> bool:
+    """Whether an element of these tensors (none of them empty) is in two places:
+    for dense ones by their extents, for those with gaps by a stride of zero and
+    by their first and last elements (views may lie in each other's gaps)."""
+    spans = []
+    for t in tensors:
+        start, size = t.data_ptr(), t.element_size()
+        if t.is_contiguous() or _dense(t):
+            spans.append((start, start + t.numel() * size))
+        elif any(st == 0 and n > 1 for st, n in zip(t.stride(), t.shape)):
+            return True
+        else:
+            last = start + size * sum(st * (n - 1) for st, n in zip(t.stride(), t.shape))
+            spans += [(start, start + size), (last, last + size)]
+    spans.sort()
+    return any(b[0] < a[1] for a, b in zip(spans, spans[1:]))
+
+
 def _run(grads, max_norm: float, eps: float, scale: bool) -> torch.Tensor:
     if isinstance(grads, torch.Tensor):
         grads = [grads]
@@ -54,9 +73,8 @@ def _run(grads, max_norm: float, eps: float, scale: bool) -> torch.Tensor:
             raise ValueError(f"tensor {i} requires a gradient; give the gradients")
     # (a tensor with gaps in memory is worked on in a copy)
     work = [t if t.is_contiguous() or _dense(t) else t.contiguous() for t in grads]
-    starts = [t.data_ptr() for t in work if t.numel()]
-    if scale and len(set(starts)) < len(starts):
-        raise ValueError("a tensor is given twice")
+    if scale and _share_memory([t for t in grads if t.numel()]):
+        raise ValueError("a tensor is given twice, or two share memory")
     lib = nat.load()
     dev, n = grads[0].device, len(work)
     norm = torch.empty((), dtype=torch.float32, device=dev)

@@ -136,3 +136,17 @@ def test_refusals(dev):
         with pytest.raises(OsmError):
             clip_grad_norm([x], **kw)
     assert (x == 1).all()
+
+
+@pytest.mark.gpu
+def test_tensors_that_share_memory_are_refused(dev):
+    """Before anything is written; the norm alone takes them."""
+    flat = torch.ones(240, device=dev)
+    square = flat.view(4, 60)
+    for grads in ([flat, flat[1:]], [flat, square.t()], [square[:, ::2], square[:, ::2]], [flat[10:], flat[:3].expand(2, 3)]):
+        with pytest.raises(ValueError, match="share memory"):
+            clip_grad_norm(grads, 1.0)
+        assert (flat == 1).all()
+        assert grad_norm(grads).item() == pytest.approx(norm_of(grads))
+    clip_grad_norm([square[:, ::2], square[:, 1::2]], 1.0)
+    assert abs(norm_of([flat]) - 1.0) <= 1e-5

@@ -109,3 +109,36 @@ def test_no_cpu_path():
 def test_struct_layout_matches_ctypes(cls, cname):
     from test_abi import test_struct_layout_matches_ctypes as layout
     layout(cls, cname)
+
+
+def test_clip_refuses_tensors_that_share_memory():
+    """(workspace errors, -5, come after; nothing is launched)"""
+    lib = nat.load()
+
+    def clip(sizes, dtypes, pointers, **kw):
+        return lib.osm_clip_grad_norm(ctypes.byref(_clip(sizes, dtypes, pointers, **kw)), None, 0, None)
+
+    for sizes, dtypes, pointers in (((5, 5), (0, 0), (0x10000, 0x10000)), ((5, 5), (0, 0), (0x10000, 0x10010)),
+                                    ((5, 5), (0, 0), (0x10010, 0x10000)), ((9, 1), (1, 1), (0x10000, 0x10010)),
+                                    ((100, 1, 1), (0, 1, 0), (0x10000, 0x10004, 0x20000))):
+        assert clip(sizes, dtypes, pointers) == -4
+        assert b"share memory" in lib.osm_last_error()
+        assert clip(sizes, dtypes, pointers, flags=0) == -5          # the norm alone only reads
+    for sizes, dtypes, pointers in (((5, 5), (0, 0), (0x10000, 0x10014)), ((8, 1), (1, 0), (0x10000, 0x10010)),
+                                    ((5, 0, 0), (0, 0, 1), (0x10000, 0x10004, 0x10000))):
+        assert clip(sizes, dtypes, pointers) == -5
+
+
+def test_shared_memory_of_tensors():
+    from orthossm_amd.grad_clip import _share_memory
+
+    flat = torch.zeros(240)
+    square = flat.view(4, 60)
+    shared = ([flat, flat[1:]], [flat[5:9], flat[:6]], [flat, square.t()], [square[:, ::2], square[:, ::2]],
+              [square[:, ::2], flat[:1]], [square[:, 1::2], flat[235:]], [flat[:3].expand(2, 3)], [flat[:1].expand(5)])
+    apart = ([flat[:5], flat[5:]], [square[:, ::2], square[:, 1::2]], [square[:, :5], square[:, 5:]],
+             [flat[10:20], flat[30:40].view(2, 5).t(), flat[:10]], [flat[:1], flat[1:2]], [])
+    for tensors in shared:
+        assert _share_memory(tensors) and _share_memory(tensors[::-1])
+    for tensors in apart:
+        assert not _share_memory(tensors) and not _share_memory(tensors[::-1])
