@@ -118,7 +118,7 @@ def _lengths(t, B: int, S: int, dev) -> torch.Tensor | None:
             t.dtype == torch.bool:
         raise ValueError(f"lengths must be a whole-number tensor of shape ({B},)")
     if t.dtype is not torch.int32:
-        t = t.clamp(0, S)
+        t = t.to(torch.int64).clamp(0, S)       # (in its own type S may not fit)
     return t.to(device=dev, dtype=torch.int32).contiguous()
 
 

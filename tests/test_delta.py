@@ -171,3 +171,18 @@ def test_a_single_tokens_stride_is_not_checked():
             r.p, r.stride_s = 0x10000, stride
         assert lib.osm_delta_step(ctypes.byref(s), None) == -1
         assert lib.osm_last_error() == b"state is NULL"
+
+
+@pytest.mark.parametrize("dtype,S", [(torch.int8, 200), (torch.uint8, 5001), (torch.int16, 40000), (torch.int64, 1 << 30),
+                                     (torch.uint16, 70000), (torch.int32, 100)])
+def test_lengths_of_a_type_that_does_not_hold_the_sequence(dtype, S):
+    from orthossm_amd.delta import _lengths
+
+    got = _lengths(torch.tensor([3, 0, 100], dtype=dtype), 3, S, torch.device("cpu"))
+    assert got.dtype == torch.int32 and got.tolist() == [3, 0, 100]
+
+
+def test_lengths_past_32_bits():
+    from orthossm_amd.delta import _lengths
+
+    assert _lengths(torch.tensor([1 << 40, -1 << 40, 7]), 3, 50, torch.device("cpu")).tolist() == [50, 0, 7]

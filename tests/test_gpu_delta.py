@@ -389,3 +389,11 @@ def test_refusals(dev):
     for bad in (pool[:1], pool.double(), pool.transpose(2, 3), pool[0], pool.cpu()):
         with pytest.raises(ValueError):
             gated_delta_step(*one, bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,S", [(torch.int8, 130), (torch.uint8, 300), (torch.int16, 33000)])
+def test_lengths_of_narrow_types(dev, dtype, S):
+    t = on(make(2, S, 1, 4), dev)
+    want = gated_delta_forward(*args(t), lengths=torch.tensor([120, 3], dtype=torch.int32, device=dev))
+    assert torch.equal(gated_delta_forward(*args(t), lengths=torch.tensor([120, 3], dtype=dtype, device=dev)), want)
