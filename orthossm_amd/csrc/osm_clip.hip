@@ -17,6 +17,7 @@
 #include <algorithm>
 
 #include "osm_norm.h"
+#include "osm_wide_store.h"
 
 namespace osm {
 namespace {
@@ -149,7 +150,7 @@ __global__ void __launch_bounds__(kThreads) clip_scale_kernel(const ClipTable t,
         v[i] = c.bf16 ? __builtin_bit_cast(unsigned, bf16x2{(__bf16)(low(v[i]) * f), (__bf16)(high(v[i]) * f)})
                       : __float_as_uint(__uint_as_float(v[i]) * f);
       *reinterpret_cast<u32x4*>(c.x + Chunk::at(k)) = v;
-      asm volatile("s_nop 1" ::: "memory");   // (a store wider than 64 bits: see store4 in osm_delta.h)
+      wide_store_wait();
     }
   }
 }

@@ -7,6 +7,8 @@
 
 #include <type_traits>
 
+#include "osm_wide_store.h"
+
 namespace osm {
 
 constexpr int kDeltaChunk = 64;      // tokens a chunk
@@ -348,9 +350,7 @@ __device__ __forceinline__ void products(int stride, At at, Go go) {
 
 __device__ __forceinline__ void store4(float* p, f32x4 v) {
   *reinterpret_cast<f32x4*>(p) = v;
-  // two wait states before anything may overwrite the store's registers (a
-  // store wider than 64 bits was seen to lose its first word otherwise)
-  asm volatile("s_nop 1" ::: "memory");
+  wide_store_wait();
 }
 
 // Memory through buffer descriptors: an access past the extent reads zeros and

@@ -32,16 +32,20 @@ __global__ void __launch_bounds__(kStepThreads) delta_step_kernel(const DeltaSte
   const int b = bh / p.H, h = bh - b * p.H, hk = h / (p.H / p.Hk);
   const bool live = j < p.dv_;
   const int64_t slot = p.slots ? p.slots[b] : b;
+  typedef float Cols __attribute__((ext_vector_type(NC)));
   T* const o = row_ptr<T>(p.o, b, 0, h) + j;
+  auto put_out = [&](int t, Cols v) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) o[t * p.o.ss + c] = (T)v[c];
+    if (NC * sizeof(T) > 8) wide_store_wait();   // (the compiler makes them one store)
+  };
   if (slot < 0 || slot >= p.n_slots) {   // an idle row, or (past the pool) a wrong one: its outputs are NaN
     if (live && kg == 0)
-      for (int t = 0; t < p.S; ++t)
-        for (int c = 0; c < NC; ++c) o[t * p.o.ss + c] = (T)(slot < 0 ? 0.0f : __builtin_nanf(""));
+      for (int t = 0; t < p.S; ++t) put_out(t, (Cols)(slot < 0 ? 0.0f : __builtin_nanf("")));
     return;
   }
   const int n = p.lengths ? min(max(p.lengths[b], 0), p.S) : p.S;
   const int64_t at = slot * p.state_s + (int64_t)h * p.dk_ * p.dv_ + j;
-  typedef float Cols __attribute__((ext_vector_type(NC)));
   Cols s[R];   // row kg + kGroups i
 #pragma unroll
   for (int i = 0; i < R; ++i) {
@@ -109,21 +113,22 @@ __global__ void __launch_bounds__(kStepThreads) delta_step_kernel(const DeltaSte
     for (int i = 0; i < R; ++i)
 #pragma unroll
       for (int c = 0; c < NC; ++c) s[i][c] = __builtin_fmaf(kk[i], u[c], decay * s[i][c]);
-    if (live && kg == 0)
+    if (live && kg == 0) {
+      Cols v_out;
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
-        o[t * p.o.ss + c] = (T)(p.scale * __builtin_fmaf(sum[2 * NC], u[c], decay * sum[NC + c]));
+      for (int c = 0; c < NC; ++c) v_out[c] = p.scale * __builtin_fmaf(sum[2 * NC], u[c], decay * sum[NC + c]);
+      put_out(t, v_out);
+    }
   }
   if (live && kg == 0)
-    for (int t = n; t < p.S; ++t)
-      for (int c = 0; c < NC; ++c) o[t * p.o.ss + c] = (T)0.0f;
+    for (int t = n; t < p.S; ++t) put_out(t, (Cols)0.0f);
   if (p.fin && live)
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int row = kg + kGroups * i;
       if (row < p.dk_) {
         *reinterpret_cast<Cols*>(p.fin + at + (int64_t)row * p.dv_) = s[i];
-        if (NC == 4) asm volatile("s_nop 1" ::: "memory");   // (see store4 in osm_delta.h)
+        if (NC == 4) wide_store_wait();
       }
     }
 }

@@ -16,6 +16,7 @@
 #include <type_traits>
 
 #include "osm_norm.h"
+#include "osm_wide_store.h"
 
 // Fused multiply-adds are written where they are meant: w dy - mean as one
 // would leave the rounding of w dy in a dx that is 0 (rows of one element).
@@ -48,9 +49,7 @@ __device__ __forceinline__ void store_unit(T* p, const float (&v)[kUnit<T>]) {
 #pragma unroll
   for (int i = 0; i < kUnit<T>; ++i) q[i] = (T)v[i];
   __builtin_nontemporal_store(q, reinterpret_cast<typename Unit<T>::Vec*>(p));
-  // two wait states before anything may overwrite the store's registers (a
-  // store wider than 64 bits was seen to lose its first word otherwise)
-  asm volatile("s_nop 1" ::: "memory");
+  wide_store_wait();
 }
 
 // A row's units u, u + TPR, .. of a thread; past the row's end: zeros, and no
@@ -94,7 +93,7 @@ struct Row {
 #pragma unroll
         for (int i = 0; i < U; ++i) q[i] = (T)v[n][i];
         *reinterpret_cast<typename Unit<T>::Loose*>(p + c) = q;
-        asm volatile("s_nop 1" ::: "memory");   // (as in store_unit)
+        wide_store_wait();
       } else {
 #pragma unroll
         for (int i = 0; i < U; ++i)

@@ -87,3 +87,15 @@ def test_no_wide_store_data_overwritten_by_next_valu(kernels_asm):
 def test_no_packed_fp32(kernels_asm):
     for name, asm in kernels_asm.items():
         assert not re.search(r"\bv_pk_(add|mul|fma|mov)_f32\b", asm), name
+
+
+def test_wide_stores_of_the_operators_are_followed_by_their_wait(kernels_asm):
+    """In the gated delta rule's, the layer norm's and the clipping's kernels
+    nothing stands between a wide store and its wait states, so that no change
+    of schedule can bring the pattern about."""
+    for name, asm in kernels_asm.items():
+        if not name.startswith(("osm_delta", "osm_norm", "osm_clip")):
+            continue
+        ins = list(instructions(asm))
+        bad = [pair for pair in zip(ins, ins[1:]) if WIDE_STORE.match(pair[0]) and not re.match(r"s_nop [1-9]", pair[1])]
+        assert bad == [], (name, bad[:3])
