@@ -727,6 +727,10 @@ torch::autograd::variable_list once(torch::autograd::variable_list res, const to
   return res;
 }
 
+// A hook on saved tensors can give back anything, which the kernels would read as
+// what was saved.
+constexpr const char* kAnotherForm = "a saved tensor came back in another form: ";
+
 struct Delta {
   const at::Tensor* t[5];        // q, k, v, g, beta
   osm_delta_args a{};
@@ -765,19 +769,27 @@ bool delta_tensors(Delta* d) {
   return true;
 }
 
+bool lengths_form(const at::Tensor& t, const Delta& d) {
+  return t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == d.a.B && t.is_contiguous() &&
+         t.device() == d.t[0]->device();
+}
+
+// What the forward saved of these inputs for the backward.
+bool saved_form(const at::Tensor& t, const Delta& d) {
+  return t.scalar_type() == at::kByte && (size_t)t.numel() == lib.delta_saved(&d.a) && t.is_contiguous() &&
+         t.device() == d.t[0]->device();
+}
+
 // args: q, k, v, g, beta, scale, lengths.
 bool delta_common(PyObject* const* p, Delta* d) {
   for (int i = 0; i < 5; ++i)
     if (!(d->t[i] = plain(p[i]))) return false;
   if (!delta_tensors(d)) return false;
-  const at::Tensor& q = *d->t[0];
   osm_delta_args& a = d->a;
   if (!as_scale(p[5], a.dk, &a.scale)) return false;
   if (p[6] != Py_None) {
     const at::Tensor* t = plain(p[6]);
-    if (!t || t->scalar_type() != at::kInt || t->dim() != 1 || t->size(0) != a.B || !t->is_contiguous() ||
-        t->device() != q.device())
-      return false;
+    if (!t || !lengths_form(*t, *d)) return false;
     a.lengths = static_cast<const int32_t*>(t->data_ptr());
   }
   return true;
@@ -869,7 +881,7 @@ PyObject* run_delta_backward(PyObject* const* p) {
   if (!delta_common(p, &d) || !state_ptr(p[9], d, &gs)) Py_RETURN_NONE;
   const at::Tensor &q = *d.t[0], &v = *d.t[2];
   const at::Tensor *saved = plain(p[7]), *go = plain(p[8]);
-  if (!saved || !go || !delta_grad_form(*go, v)) Py_RETURN_NONE;
+  if (!saved || !saved_form(*saved, d) || !go || !delta_grad_form(*go, v)) Py_RETURN_NONE;
   const bool need_init = PyObject_IsTrue(p[10]) == 1;
   if (PyErr_Occurred()) return nullptr;
   d.a.saved = saved->data_ptr();
@@ -920,7 +932,8 @@ struct DeltaGrad : torch::autograd::Function<DeltaGrad> {
       const at::NoGradGuard no_grad;
       Delta d;
       for (int i = 0; i < 5; ++i) d.t[i] = &t[i];
-      TORCH_CHECK(delta_tensors(&d), "gated_delta: a saved tensor came back in another form");
+      const bool inputs = delta_tensors(&d);
+      TORCH_CHECK(inputs && (!t[5].defined() || lengths_form(t[5], d)) && saved_form(t[6], d), kAnotherForm, "gated_delta");
       d.a.scale = (float)ctx->saved_data["scale"].toDouble();
       if (t[5].defined()) d.a.lengths = static_cast<const int32_t*>(t[5].data_ptr());
       d.a.saved = t[6].data_ptr();
@@ -928,6 +941,8 @@ struct DeltaGrad : torch::autograd::Function<DeltaGrad> {
       at::Tensor go = grads[0].defined() ? grads[0] : at::zeros_like(t[2]);
       if (!delta_grad_form(go, t[2])) go = go.to(t[2].options()).contiguous();
       const at::Tensor gs = grads[1].defined() ? grads[1].to(at::kFloat).contiguous() : at::Tensor();
+      TORCH_CHECK(delta_grad_form(go, t[2]) && (!gs.defined() || f32_flat(gs, d.a.B * d.a.H * d.a.dk * d.a.dv, t[0])),
+                  kAnotherForm, "gated_delta");
       throw_rc(delta_backward(d, go, gs.defined() ? fptr(gs) : nullptr, need >> 5 & 1, engine_stream(t[0]), gr));
     }
     torch::autograd::variable_list res(8);
@@ -1185,14 +1200,17 @@ struct NormGrad : torch::autograd::Function<NormGrad> {
     {
       const at::NoGradGuard no_grad;
       const at::Tensor& x = t[0];
-      TORCH_CHECK(norm_rows(&x), "layer_norm: a saved tensor came back in another form");
+      TORCH_CHECK(norm_rows(&x), kAnotherForm, "layer_norm");
       osm_norm_args a{};
       norm_args(x, &a);
+      TORCH_CHECK(f32_flat(t[1], a.rows, x) && f32_flat(t[2], a.rows, x) && (!t[3].defined() || f32_vec(&t[3], a.D, x)),
+                  kAnotherForm, "layer_norm");
       a.mean = fptr(t[1]);
       a.rstd = fptr(t[2]);
       if (t[3].defined()) a.weight = fptr(t[3]);
       const c10::DeviceGuard guard(x.device());
       const at::Tensor gy = norm_grad_form(grads[0], x) ? grads[0] : grads[0].to(x.options()).contiguous();
+      TORCH_CHECK(norm_grad_form(gy, x), kAnotherForm, "layer_norm");
       throw_rc(norm_backward(a, x, gy, need, engine_stream(x), res.data()));
     }
     return once(std::move(res), {grads[0], t[0], t[3]});

@@ -210,6 +210,9 @@ def _backward(inputs, scale, lengths, saved, grad_out, grad_state, need_init: bo
     gq, gk, gv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
     gg, gb = (torch.empty(g.shape, dtype=torch.float32, device=dev) for _ in range(2))
     gi = torch.empty((a.B, a.H, a.dk, a.dv), dtype=torch.float32, device=dev) if need_init else None
+    if saved.dtype != torch.uint8 or saved.device != dev or not saved.is_contiguous() or \
+            saved.numel() != lib.osm_delta_saved_bytes(ctypes.byref(a)):
+        raise RuntimeError("a saved tensor came back in another form: gated_delta")
     a.saved = saved.data_ptr()
     b = nat.DeltaBwdArgs()
     for name, t in (("grad_out", go), ("grad_q", gq), ("grad_k", gk), ("grad_v", gv), ("grad_g", gg),

@@ -126,3 +126,28 @@ def test_outputs_that_require_a_gradient_are_refused(dev, path):
             call()
         with torch.no_grad():
             call()
+
+
+def half_of(is_one):
+    """Hooks that give back half of the saved tensors that ``is_one`` picks."""
+    return torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t[:t.shape[0] // 2] if is_one(t) else t)
+
+
+@pytest.mark.parametrize("which", ["what the forward kept", "lengths", "statistics", "weight", "input"])
+def test_saved_tensors_of_another_form_are_refused(dev, path, which):
+    """A hook may give back anything: what does not fit is not read."""
+    lengths = torch.tensor([20, 7], dtype=torch.int32, device=dev)
+    picks = {"what the forward kept": lambda t: t.dtype == torch.uint8, "lengths": lambda t: t.dtype == torch.int32,
+             "statistics": lambda t: t.shape == (4,), "weight": lambda t: t.shape == (40,),
+             "input": lambda t: t.shape in ((2, 20, 2, 12), (4, 40))}
+    ins = [t.requires_grad_() for t in delta_inputs(dev)]
+    x = [t.requires_grad_() for t in norm_inputs(dev)]
+    with half_of(picks[which]):
+        outs = []
+        if which not in ("statistics", "weight"):
+            outs.append(gated_delta(*ins[:5], state_init=ins[5], lengths=lengths))
+        if which not in ("what the forward kept", "lengths"):
+            outs.append(layer_norm(*x))
+    for out in outs:
+        with pytest.raises((RuntimeError, ValueError)):
+            out.sum().backward()
