@@ -48,7 +48,8 @@ class GatedDeltaLayer(nn.Module):
 
     def new_state(self, slots: int, device=None) -> torch.Tensor:
         """Zero states [slots, heads, head_dim, value_dim], also a pool for ``step``."""
-        return torch.zeros(slots, self.n_heads, self.head_dim, self.value_dim, device=device or self.a_log.device)
+        return torch.zeros(slots, self.n_heads, self.head_dim, self.value_dim, dtype=torch.float32,
+                           device=self.a_log.device if device is None else device)
 
     def _project(self, x: torch.Tensor):
         lead = x.shape[:-1]

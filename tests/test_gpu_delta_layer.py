@@ -94,3 +94,13 @@ def test_example_learns_and_serves(dev):
     assert losses[-10:].mean() < losses[:10].mean()
     share, worst = ex.serve(model, gen, rows=16)
     assert 0.0 <= share <= 1.0 and worst <= 1e-3
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float64])
+def test_states_are_fp32_whatever_the_default_type(dtype):
+    m = GatedDeltaLayer(32, 2)
+    torch.set_default_dtype(dtype)
+    try:
+        assert m.new_state(3).dtype == torch.float32
+    finally:
+        torch.set_default_dtype(torch.float32)
