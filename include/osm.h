@@ -367,7 +367,8 @@ typedef struct osm_engine_args {
  * out what is below 2^-24), results are rounded once to `dtype`.  g below -200 counts as
  * -200.  Tokens at and past lengths[b] are not read, leave the state as it is
  * and give zeros (outputs and gradients).  A NaN or infinity in a token may
- * reach the outputs of its whole chunk of 64 tokens, and those after it. */
+ * reach the outputs of its whole chunk of 64 tokens, and those after it.  Outputs
+ * lie in no argument's memory, but out may be v (the same elements). */
 typedef struct osm_rows {
   void* p;                      /* element (b, t, h, j) at b*stride_b + t*stride_s + h*stride_h + j */
   int64_t stride_b, stride_s, stride_h;   /* elements, >= 0; stride_s <= OSM_DELTA_MAX_STRIDE, and unused where S = 1 */

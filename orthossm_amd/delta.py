@@ -102,6 +102,25 @@ def _dest(t, shape, dtype, dev, name: str) -> None:
         raise ValueError(f"{name} requires a gradient, which what is written into it has not")
 
 
+def _extent(t: torch.Tensor) -> tuple[int, int]:
+    """First byte of t's elements and the one after the last."""
+    last = sum(st * (n - 1) for st, n in zip(t.stride(), t.shape))
+    return t.data_ptr(), t.data_ptr() + t.element_size() * (1 + last)
+
+
+def apart(name: str, t: torch.Tensor, others: dict, may_be: str | None = None) -> None:
+    """Refuses an output ``t`` that lies in the memory of another argument, which
+    some of a launch's workgroups would read after others wrote it.  It may be
+    the one named ``may_be``, as a whole."""
+    for other, o in others.items():
+        if o is None or o is t and other == may_be or not o.numel() or not t.numel():
+            continue
+        (a, b), (c, d) = _extent(t), _extent(o)
+        whole = other == may_be and a == c and o.dtype == t.dtype and o.shape == t.shape and o.is_contiguous()
+        if not whole and a < d and c < b:
+            raise ValueError(f"{name} shares memory with {other}")
+
+
 def written(*tensors) -> None:
     """Tells autograd that a launch wrote into these (None: skipped): a graph
     that saved one refuses its backward, as after torch's own in-place
@@ -165,6 +184,11 @@ def _forward(q, k, v, g, beta, scale, state_init, lengths, out, return_state, st
         _dest(state_out, state, torch.float32, dev, "state_out")
     elif return_state:
         state_out = torch.empty(state, dtype=torch.float32, device=dev)
+    ins = dict(zip(("q", "k", "v", "g", "beta", "state_init", "lengths"), keep))
+    if given[0] is not None:
+        apart("out", out, {**ins, "state_out": state_out}, "v")
+    if given[1] is not None:
+        apart("state_out", state_out, ins, "state_init")
     a.state_out = state_out.data_ptr() if state_out is not None else None
     saved = None
     if save:
@@ -185,8 +209,9 @@ def gated_delta_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: to
     """The gated delta rule over sequences.  ``scale`` is 1/sqrt(dk) by
     default, ``state_init`` zeros.  Returns out [B,S,H,dv] in v's type, and
     the state after the last token [B,H,dk,dv] fp32 when ``return_state``.
-    ``out`` and ``state_out`` (contiguous; state_out may be state_init) receive
-    the results instead of new tensors."""
+    ``out`` and ``state_out`` (contiguous; out may be v and state_out state_init,
+    else they lie in no argument's memory) receive the results instead of new
+    tensors."""
     out, fin, _, _ = _forward(q, k, v, g, beta, scale, state_init, lengths, out, return_state, state_out, False)
     return (out, fin) if return_state else out
 
@@ -289,7 +314,7 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     slot b, or ``slots[b]`` (int64, on the device, no slot twice): a negative
     one marks an idle row, whose output is 0; one past the pool gives NaN;
     neither touches a state.  Returns out [B,H,dv] in v's type, in ``out``
-    (contiguous) if given."""
+    (contiguous; may be v, else in no argument's memory) if given."""
     fast = _fast()
     if fast is not None and out is None:
         res = fast.delta_step(q, k, v, g, beta, state, scale, slots)
@@ -317,6 +342,8 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
         out = torch.empty((B, H, dv), dtype=v.dtype, device=dev)
     else:
         _dest(out, (B, H, dv), v.dtype, dev, "out")
+    if given is not None:
+        apart("out", out, dict(q=q, k=k, v=v, g=g, beta=beta, state=state, slots=slots), "v")
     a = nat.DeltaStepArgs()
     a.abi_version, a.dtype = nat.ABI_VERSION, _dtype_code(q.dtype)
     a.B, a.H, a.Hk, a.dk, a.dv = B, H, Hk, dk, dv

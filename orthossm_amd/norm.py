@@ -19,7 +19,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native as nat
-from .delta import _dest, _scratch, differentiable, on_device, written
+from .delta import _dest, _scratch, apart, differentiable, on_device, written
 from .ops import _current_stream, _dtype_code, _fast
 
 
@@ -75,6 +75,8 @@ def _forward(x, weight, bias, eps, out, stats: bool):
         out = torch.empty(x.shape, dtype=x.dtype, device=dev)
     else:
         _dest(out, x.shape, x.dtype, dev, "out")
+        rows, weight, bias = keep
+        apart("out", out.view(rows.shape), dict(x=rows, weight=weight, bias=bias), "x")
     a.y, a.y_stride = out.data_ptr(), a.D
     mean = rstd = None
     if stats:
@@ -90,7 +92,8 @@ def _forward(x, weight, bias, eps, out, stats: bool):
 def layer_norm_forward(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, *,
                        eps: float = 1e-5, out: torch.Tensor | None = None):
     """(y in x's type, mean and rstd fp32 of x's shape without the last axis).
-    ``out`` (contiguous; may be x) receives y instead of a new tensor."""
+    ``out`` (contiguous; may be x, else in no argument's memory) receives y
+    instead of a new tensor."""
     return _forward(x, weight, bias, eps, out, True)
 
 

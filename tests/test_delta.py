@@ -186,3 +186,17 @@ def test_lengths_past_32_bits():
     from orthossm_amd.delta import _lengths
 
     assert _lengths(torch.tensor([1 << 40, -1 << 40, 7]), 3, 50, torch.device("cpu")).tolist() == [50, 0, 7]
+
+
+def test_outputs_lie_in_no_arguments_memory():
+    from orthossm_amd.delta import apart
+
+    flat = torch.zeros(240)
+    x, out = flat[:120].view(10, 12), flat[120:].view(10, 12)
+    apart("out", out, dict(x=x, w=None, none=flat[:0]), "x")
+    apart("out", x, dict(x=x, y=out), "x")
+    apart("out", x, dict(x=flat[:120].view(10, 12)), "x")
+    for others in (dict(y=x), dict(x=flat[1:121].view(10, 12)), dict(x=flat[:100].view(10, 10)), dict(y=out, z=flat[119:130]),
+                   dict(x=flat[:144].view(12, 12)[:10, :].t()), dict(x=x.view(12, 10).t()), dict(y=flat[::3])):
+        with pytest.raises(ValueError, match="out shares memory with"):
+            apart("out", x, others, "x")

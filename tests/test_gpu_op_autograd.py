@@ -151,3 +151,28 @@ def test_saved_tensors_of_another_form_are_refused(dev, path, which):
     for out in outs:
         with pytest.raises((RuntimeError, ValueError)):
             out.sum().backward()
+
+
+def test_outputs_in_an_arguments_memory(dev, path):
+    """out may be v, the norm's x, state_out the first state; nothing else."""
+    gen = torch.Generator().manual_seed(4)
+    q, k, v = (torch.randn(2, 70, 2, 16, generator=gen).to(dev) for _ in range(3))
+    g, beta, init = -torch.ones(2, 70, 2, device=dev), torch.full((2, 70, 2), 0.5, device=dev), torch.ones(2, 2, 16, 16, device=dev)
+    want, fin = gated_delta_forward(q, k, v, g, beta, state_init=init, return_state=True)
+    last, mine = init.clone(), v.clone()
+    gated_delta_forward(q, k, mine, g, beta, state_init=last, out=mine, return_state=True, state_out=last)
+    assert torch.equal(mine, want) and torch.equal(last, fin)
+    one = [t[:, 0].contiguous() for t in (q, k, v, g, beta)]
+    state, want = init.clone(), gated_delta_step(*one, init.clone())
+    assert torch.equal(gated_delta_step(*one, state, out=one[2]), want)
+    one[2] = v[:, 0].contiguous()
+    x, w, b = norm_inputs(dev)
+    store = torch.zeros(5, 40, device=dev)
+    for call in (lambda: gated_delta_forward(q, k, v, g, beta, out=q), lambda: gated_delta_forward(q, k, v, g, beta, out=k),
+                 lambda: gated_delta_forward(q, k, v, g, beta, state_out=q.view(-1)[:1024].view(2, 2, 16, 16)),
+                 lambda: gated_delta_step(*one, state, out=one[0]),
+                 lambda: gated_delta_step(*one, state, out=state.view(-1)[64:128].view(2, 2, 16)),
+                 lambda: layer_norm_forward(store[:4], w, b, out=store[1:]),
+                 lambda: layer_norm_forward(store[:1], store[1], b, out=store[1:2])):
+        with pytest.raises(ValueError, match="shares memory"):
+            call()
