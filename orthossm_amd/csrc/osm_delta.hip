@@ -247,11 +247,12 @@ __global__ void __launch_bounds__(64 * KT) delta_scan_kernel(const float* a, flo
 // Walks segment blockIdx.x % segs of a head.  MAP: the segment's state map, from
 // zero for the columns of v and from the identity's columns after them; else the
 // outputs.  KS: blocks of 32 rows of S; WAVES: of 16 columns each.
-// What bounds it: 512 chunks of 16 heads, bf16, d = 64, take 130 us for the maps and
-// 121 for the outputs, in which the vector instructions (the parts of X, U, S, Z, P)
-// fill a third to two fifths of the time, the matrix instructions a quarter, LDS two
-// fifths, and the two or three waves a SIMD has room for wait for each other in
-// between.  Tried without gain: products of two tiles in turn, a higher priority for
+// What bounds it: 256 chunks of 32 heads, bf16, d = 64, take 134 us for the maps and
+// 138 for the outputs, in which the vector instructions (the parts of X, U, S, Z, P)
+// fill a third of the time, the matrix instructions a quarter, LDS two fifths, and
+// the two or three waves a SIMD has room for wait for each other in between.  fp32
+// outputs take 101 KB of LDS (d = 64): four waves a CU, one a SIMD (three rows of up to
+// 5001 tokens, 8 heads, d = 50: 71 us, the maps at two waves a SIMD 46).  Tried without gain: products of two tiles in turn, a higher priority for
 // waves in their products, 128 registers for twice the waves, and LDS rows 160 bytes
 // apart, whose 16-byte reads meet no bank twice (their writes meet more: 144 us).
 template <typename T, int KS, int WAVES, bool MAP>
@@ -519,8 +520,10 @@ void launch_walk(const DeltaParams& p, hipStream_t stream) {
   // holds two such workgroups or more, wait less for each other.  Measured with four
   // and eight, B=1 S=8192 H=16: maps of bf16 dk=64 dv=128 148 and 165 us (the whole
   // forward), dk=dv=128 290 and 286, of fp32 dk=64 223 and 234, but dk=dv=128, one
-  // workgroup a CU, 567 and 478; outputs of bf16 dk=64 dv=128 171 and 165, dk=dv=128
-  // 393 and 285, of fp32 dk=64 285 and 234.
+  // workgroup a CU, 567 and 478; outputs of bf16 dk=64 dv=128 168 and 159, dk=dv=128
+  // 387 and 296, of fp32 dk=64 285 and 234.  With dv=64 four waves hold every column:
+  // bf16 dk=32 97 and 110, dk=64 121 and 136, but dk=96 194 and 178, dk=128 266 and 253;
+  // fp32 dk=64 198 and 192, dk=128 408 and 454.
   constexpr bool kFour = MAP && (sizeof(T) == 2 || KS <= 2);
   if constexpr (kFour)
     go(std::integral_constant<int, 4>{});
@@ -560,14 +563,14 @@ hipError_t forward_by_size(const DeltaParams& p, hipStream_t stream) {
 
 // Chunks a segment.  A segmented row is walked twice, on top of a scan, but by many
 // workgroups: worth it for up to 128 heads (bf16, d = 64, whole rows against
-// segments: 128 heads x 64 chunks 349 and 299 us, 160 x 51 289 and 298, 192 x 42 249
-// and 312; 16 x 512 2318 and 297) and from 4 chunks (8 heads x 4 32.1 and 30.5 us,
-// x 8 49.8 and 33.7).  At most as many segments as give every CU two workgroups: one
-// more and a third round of them begins (96 heads x 85 chunks: 5 segments 305 us, 6
-// 380).  Below that a walk costs its segment's length and the scan their number, so
+// segments: 128 heads x 64 chunks 382 and 303 us, 160 x 51 317 and 376, 192 x 42 273
+// and 324; 16 x 512 2609 and 335) and from 4 chunks (8 heads x 4 34.8 and 31.3 us,
+// x 8 54.8 and 35.7).  At most as many segments as give every CU two workgroups: one
+// more and a third round of them begins (96 heads x 85 chunks: 5 segments 306 us, 6
+// 366).  Below that a walk costs its segment's length and the scan their number, so
 // the best length goes with the root of the row's: with 1, 2, 3, 4 chunks a segment
-// 8 heads x 16 chunks take 41.8, 41.3, 45.9, 52.1 us, x 47 73.6, 59.4, 57.2, 60.9,
-// x 128 163, 109, 96, 87 (8: 95); fp32 and d = 128 have theirs at the same lengths.
+// 8 heads x 16 chunks take 43.9, 44.6, 49.1, 55.3 us, x 47 76.5, 62.7, 60.2, 64.8,
+// x 128 165, 113, 99, 90 (8: 101); fp32 and d = 128 have theirs at the same lengths.
 int delta_segment(int64_t heads, int64_t chunks) {
   if (heads > 128 || chunks < 4) return (int)std::max<int64_t>(chunks, 1);
   const int64_t most = 512 / std::max<int64_t>(heads, 1);

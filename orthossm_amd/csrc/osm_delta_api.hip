@@ -15,8 +15,8 @@ using osm::ok;
 
 // Sequences up to this many tokens walk the state token by token in one launch
 // (the step kernel) when nothing is saved for a backward.  Tokens against chunks,
-// bf16, d = 64: 8 heads of 4 tokens 10.3 and 18.8 us, of 8 17.2 and 18.9, of 16 30.7
-// and 18.9; 512 heads of 8 22.0 and 24.5, of 16 38.7 and 24.5.
+// bf16, d = 64: 8 heads of 4 tokens 11.2 and 20.3 us, of 8 17.9 and 20.3, of 16 31.8
+// and 20.5; 512 heads of 8 23.9 and 26.2, of 16 39.7 and 25.5.
 constexpr int64_t kShort = 8;
 
 constexpr int64_t kMaxDim = (int64_t(1) << 31) - 1;

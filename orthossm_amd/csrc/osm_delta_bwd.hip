@@ -633,7 +633,10 @@ __device__ __forceinline__ f32x4 wide(bf16x4 v) { return f32x4{(float)v[0], (flo
 // LDS: K by rows, then columns; dO; Q by rows, then Y and R, then C and dKw; Z,
 // its transpose and P's, then S and D (one after the other for more than 64 rows)
 // and Q by columns.  ONE: dv <= 64, so that what part 2 adds up need not live
-// through part 1 (where it does, registers spill).
+// through part 1.  Where it does, 94, 172, 229 and 334 registers spill for KS = 1 to 4:
+// 2048 chunks of dv = 64 take 170 us with ONE and 386 without for dk = 64, 227 and 708
+// for dk = 128, and of dv = 128, which has two slices, 262, 388 and 717 for dk = 32, 64,
+// 128.
 // What bounds it: 2048 chunks of d = 64 take 166 us, where their bytes take 37.  With
 // one workgroup a CU nothing covers a chunk's first loads (a fifth of its 41000
 // cycles) and the waits at the nine barriers; the two waves of a SIMD issue vector

@@ -8,7 +8,7 @@
 // rows that are added through a wave's shuffles and LDS: one barrier a token.  A
 // thread holds NC neighbouring columns: four (16-byte accesses) where the rows'
 // alignment allows it and there are more than 32 rows, one else (1024 states of 128 by
-// 128: 35.7 us with one, 29.7 with four).
+// 128: 35.7 us with one, 29.5 with four).
 // One token is bound by the state's bytes (read and written once, 128-byte
 // pieces of rows; the 1024 states at 4.5 TB/s), or by the launch when there are few
 // rows (8 states of 64 by 64: 5.2 us).
