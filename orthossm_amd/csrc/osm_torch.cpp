@@ -1262,18 +1262,17 @@ PyObject* run_clip(PyObject* const* p) {
   std::vector<void*> ptr(n);
   std::vector<int64_t> size(n);
   std::vector<int32_t> dtype(n);
-  std::vector<at::Tensor> scaled;   // (the list may change while the lock is released)
-  const at::Tensor* first = nullptr;
+  std::vector<at::Tensor> held;   // (the list may change while the lock is released)
+  held.reserve(n);
   for (Py_ssize_t i = 0; i < n; ++i) {
     const at::Tensor* const t = plain(PySequence_Fast_GET_ITEM(p[0], i));
     if (!t || !t->is_cuda() || !(is_f32(*t) || is_bf16(*t)) || !t->is_contiguous() || (scale && t->requires_grad()))
       Py_RETURN_NONE;
-    if (!first) first = t;
-    if (t->device() != first->device()) Py_RETURN_NONE;
+    if (i > 0 && t->device() != held[0].device()) Py_RETURN_NONE;
+    held.push_back(*t);
     ptr[i] = t->data_ptr();
     size[i] = t->numel();
     dtype[i] = code(*t);
-    if (scale) scaled.push_back(*t);
   }
   osm_clip_args a{};
   a.abi_version = OSM_ABI_VERSION;
@@ -1286,20 +1285,22 @@ PyObject* run_clip(PyObject* const* p) {
   a.eps = eps;
   Ref s_obj;
   void* stream;
-  const c10::DeviceGuard guard(first->device());
-  if (!stream_of(*first, &s_obj, &stream)) return nullptr;
+  const at::Tensor& first = held[0];
+  const c10::DeviceGuard guard(first.device());
+  if (!stream_of(first, &s_obj, &stream)) return nullptr;
   at::Tensor norm, ws;
   int rc;
   {
     const NoGil nogil;
-    norm = empty({}, *first, at::kFloat);
+    norm = empty({}, first, at::kFloat);
     a.norm = fptr(norm);
-    ws = scratch(lib.clip_bytes(&a), *first);
+    ws = scratch(lib.clip_bytes(&a), first);
     rc = lib.clip(&a, ws.data_ptr(), (size_t)ws.numel(), stream);
   }
   if (rc == OSM_E_LAYOUT) Py_RETURN_NONE;   // tensors that share memory: the Python path says so
   if (rc != OSM_OK) return fail_rc(rc);
-  for (const at::Tensor& t : scaled) written(t);
+  if (scale)
+    for (const at::Tensor& t : held) written(t);
   return THPVariable_Wrap(norm);
 }
 

@@ -342,7 +342,6 @@ def gated_delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
         out = torch.empty((B, H, dv), dtype=v.dtype, device=dev)
     else:
         _dest(out, (B, H, dv), v.dtype, dev, "out")
-    if given is not None:
         apart("out", out, dict(q=q, k=k, v=v, g=g, beta=beta, state=state, slots=slots), "v")
     a = nat.DeltaStepArgs()
     a.abi_version, a.dtype = nat.ABI_VERSION, _dtype_code(q.dtype)

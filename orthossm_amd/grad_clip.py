@@ -4,10 +4,9 @@
 ``clip_grad_norm``  the same, and every tensor times min(1, max_norm / (norm + eps)) in place.
 
 Tensors are fp32 or bf16 in any mix, of any sizes, on one device; those that are
-clipped share no memory.  Sums are
-held in double; the norm stays on the device, so nothing synchronises the host.
-A NaN norm makes every element NaN, an infinite one makes finite elements 0 and
-infinite ones NaN.  There is no CPU path.
+clipped share no memory.  Sums are held in double; the norm stays on the device,
+so nothing synchronises the host.  A NaN norm makes every element NaN, an
+infinite one makes finite elements 0 and infinite ones NaN.  There is no CPU path.
 """
 from __future__ import annotations
 
