@@ -460,6 +460,134 @@ typedef struct osm_clip_args {
   float* norm;                  /* device scalar */
 } osm_clip_args;
 
+/* ---------------------------------------------------------------------------
+ * The EMA with a learned gate for every channel and token:
+ *
+ *   h_t = a_t h_{t-1} + (1 - a_t) x_t,   a_t = sigmoid(gate_t)
+ *
+ * fp32 arithmetic and states, out rounded once.  Tokens at and past lengths[b]
+ * are not read, leave the state as it is and give zeros (outputs and gradients).
+ * A NaN or infinity in a token may reach the outputs of its whole tile of 128
+ * tokens, and those after it.  Outputs lie in no argument's memory.  No counterpart
+ * in the reference, whose decays are per head and constants of the backward. */
+typedef struct osm_seq {
+  void* p;                      /* element (b, t, d) at b*stride_b + t*stride_s + d */
+  int64_t stride_b, stride_s;   /* elements, >= 0; stride_s is unused where S = 1 */
+} osm_seq;
+
+typedef struct osm_ema_args {
+  int32_t abi_version;          /* = OSM_ABI_VERSION */
+  int32_t dtype;                /* osm_dtype of x, gate, out and their gradients */
+  int64_t B, S, D;
+  osm_seq x, gate, out;         /* [B,S,D]; out's rows must not overlap */
+  const int32_t* lengths;       /* [B], or NULL: every row has S tokens */
+  const float* state_init;      /* [B,D] contiguous, or NULL: zeros */
+  float* state_out;             /* [B,D] contiguous, or NULL; may be state_init */
+  float* saved;                 /* osm_gated_ema_saved_bytes for the backward, or NULL */
+} osm_ema_args;
+
+typedef struct osm_ema_bwd_args {
+  osm_seq grad_out, grad_x, grad_gate;   /* [B,S,D] of `dtype` */
+  const float* grad_state;      /* dL/d state_out [B,D] contiguous, or NULL */
+  float* grad_init;             /* [B,D] contiguous, or NULL; may be grad_state */
+} osm_ema_bwd_args;
+
+/* One token a row (stride_s unused), the states in a pool. */
+typedef struct osm_ema_step_args {
+  int32_t abi_version;          /* = OSM_ABI_VERSION */
+  int32_t dtype;                /* osm_dtype of x, gate and out */
+  int64_t B, D;
+  osm_seq x, gate, out;         /* [B,D] */
+  float* state;                 /* [n_slots,D], slots state_stride elements apart; updated in place */
+  int64_t state_stride, n_slots;
+  const int64_t* slots;         /* as osm_delta_step_args' */
+} osm_ema_step_args;
+
+/* ---------------------------------------------------------------------------
+ * A block's residual update between its two norms, over rows of D elements:
+ *
+ *   r = x + scale sigmoid(gate) N(y),   n = N'(r) weight + bias
+ *
+ * N' is the layer norm without parameters or, with OSM_RESNORM_RMS, v / sqrt(mean(v^2)
+ * + eps); N the same norm, or the identity without OSM_RESNORM_NORM_Y.  fp32
+ * arithmetic, n from r as it is before its rounding.  No counterpart in the reference. */
+#define OSM_RESNORM_NORM_Y 0x1
+#define OSM_RESNORM_RMS 0x2
+
+typedef struct osm_resnorm_args {
+  int32_t abi_version;          /* = OSM_ABI_VERSION */
+  int32_t flags;
+  int32_t stream_dtype;         /* osm_dtype of x, r and their gradients; OSM_F32 if block_dtype is */
+  int32_t block_dtype;          /* osm_dtype of y, gate, n and their gradients */
+  int64_t rows, D;
+  float eps;
+  const void* x;                /* each matrix: rows a stride apart, elements contiguous */
+  int64_t x_stride;
+  const void* y;
+  int64_t y_stride;
+  const void* gate;             /* or NULL: no factor */
+  int64_t gate_stride;
+  const float* scale;           /* [D], or NULL: ones */
+  const float* weight;          /* [D], or NULL: ones */
+  const float* bias;            /* [D], or NULL: zeros */
+  void* r;                      /* rows of outputs must not overlap; r may be x, n may be y */
+  int64_t r_stride;
+  void* n;
+  int64_t n_stride;
+  float* stats;                 /* [rows][4]: mean and 1 / spread of y (0, 1 without NORM_Y) and of r; NULL, or
+                                 * written by the forward and read by the backward */
+} osm_resnorm_args;
+
+typedef struct osm_resnorm_bwd_args {
+  const void* grad_r;           /* or NULL: zeros */
+  int64_t grad_r_stride;
+  const void* grad_n;           /* or NULL: zeros */
+  int64_t grad_n_stride;
+  void* grad_x;                 /* every gradient: or NULL */
+  int64_t grad_x_stride;
+  void* grad_y;
+  int64_t grad_y_stride;
+  void* grad_gate;
+  int64_t grad_gate_stride;
+  float* grad_scale;            /* [D] */
+  float* grad_weight;
+  float* grad_bias;
+} osm_resnorm_bwd_args;
+
+/* ---------------------------------------------------------------------------
+ * The cross entropy of a projection to a vocabulary, without its logits:
+ *
+ *   loss_n = log sum_v exp(hidden_n . weight_v) - hidden_n . weight_{targets_n}
+ *
+ * for tokens n with targets_n != ignore_index; the others count for nothing, their
+ * hidden rows are not read, and their loss and gradients are 0.  A target outside
+ * [0, V) gives NaN (the loss, and every gradient that the token has a part in).
+ * Products are at fp32's accuracy for fp32 inputs (three bf16 parts an operand) and
+ * exact for bf16 ones, sums in fp32.  No counterpart in the reference. */
+typedef struct osm_loss_args {
+  int32_t abi_version;          /* = OSM_ABI_VERSION */
+  int32_t dtype;                /* osm_dtype of hidden, weight and their gradients */
+  int64_t N, D, V;
+  const void* hidden;           /* [N,D], rows a stride apart, elements contiguous */
+  int64_t hidden_stride;
+  const void* weight;           /* [V,D] */
+  int64_t weight_stride;
+  const int64_t* targets;       /* [N] */
+  int64_t ignore_index;
+  float* losses;                /* [N], or NULL */
+  float* lse;                   /* [N]: log sum exp of each token that counts (0 of the others); written by the
+                                 * forward, read by the backward */
+  float* total;                 /* [2], or NULL: the sum of the losses, and the tokens that count (at least 1) */
+} osm_loss_args;
+
+typedef struct osm_loss_bwd_args {
+  const float* grad;            /* device scalar: the gradient of each token's loss, divided by total[1] if that is given */
+  const float* grad_losses;     /* [N], or NULL: further factors by token */
+  const float* total;           /* what the forward wrote, or NULL */
+  void* grad_hidden;            /* [N,D] contiguous, or NULL */
+  void* grad_weight;            /* [V,D] contiguous, or NULL */
+} osm_loss_bwd_args;
+
 /* Which entry point a workspace is sized for. */
 typedef enum osm_op { OSM_OP_FWD = 0, OSM_OP_TTT = 1, OSM_OP_BWD = 2 } osm_op;
 
@@ -583,6 +711,39 @@ int osm_layer_norm_bwd(const osm_norm_args* args, const osm_norm_bwd_args* bwd, 
  * (as many more for every further 150).  Workspace as above. */
 size_t osm_clip_workspace_bytes(const osm_clip_args* args);
 int osm_clip_grad_norm(const osm_clip_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The gated EMA over sequences.  `saved` and the workspace need no initialisation
+ * and 256-byte alignment; nothing is kept in the workspace between calls.  One
+ * launch, two where S is above 128 (backward: 64). */
+size_t osm_gated_ema_saved_bytes(const osm_ema_args* args);
+size_t osm_gated_ema_workspace_bytes(const osm_ema_args* args);
+int osm_gated_ema_fwd(const osm_ema_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Its backward, from the inputs and what osm_gated_ema_fwd saved of them (out and
+ * state_out of `args` are not used). */
+size_t osm_gated_ema_bwd_workspace_bytes(const osm_ema_args* args);
+int osm_gated_ema_bwd(const osm_ema_args* args, const osm_ema_bwd_args* bwd, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/* One token a row, in one launch. */
+int osm_gated_ema_step(const osm_ema_step_args* args, void* stream);
+
+/* The residual norm and its backward (from x, y, gate, scale, weight and stats; r,
+ * n and bias are not used), whose workspace needs no initialisation and 256-byte
+ * alignment. */
+int osm_residual_norm_fwd(const osm_resnorm_args* args, void* stream);
+size_t osm_residual_norm_bwd_workspace_bytes(const osm_resnorm_args* args);
+int osm_residual_norm_bwd(const osm_resnorm_args* args, const osm_resnorm_bwd_args* bwd, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* The cross entropy and its backward (from hidden, weight, targets and lse; losses
+ * and total of `args` are not used).  Workspaces as above.  The backward forms the
+ * probabilities of a piece of the vocabulary at a time. */
+size_t osm_linear_ce_workspace_bytes(const osm_loss_args* args);
+int osm_linear_ce_fwd(const osm_loss_args* args, void* workspace, size_t workspace_bytes, void* stream);
+size_t osm_linear_ce_bwd_workspace_bytes(const osm_loss_args* args);
+int osm_linear_ce_bwd(const osm_loss_args* args, const osm_loss_bwd_args* bwd, void* workspace, size_t workspace_bytes,
+                      void* stream);
 
 #ifdef __cplusplus
 }

@@ -40,6 +40,8 @@ ENGINE_MAX_D = 1024   # row length of osm_engine_prologue
 DELTA_MAX_DK = 128    # rows of the gated delta rule's state
 DELTA_MAX_STRIDE = 1 << 22   # elements from token to token
 CLIP_SCALE = 0x1
+RESNORM_NORM_Y = 0x1
+RESNORM_RMS = 0x2
 
 STATUS = {
     0: "OSM_OK",
@@ -84,6 +86,19 @@ EXPORTS = (
     "osm_layer_norm_bwd",
     "osm_clip_workspace_bytes",
     "osm_clip_grad_norm",
+    "osm_gated_ema_saved_bytes",
+    "osm_gated_ema_workspace_bytes",
+    "osm_gated_ema_fwd",
+    "osm_gated_ema_bwd_workspace_bytes",
+    "osm_gated_ema_bwd",
+    "osm_gated_ema_step",
+    "osm_residual_norm_fwd",
+    "osm_residual_norm_bwd_workspace_bytes",
+    "osm_residual_norm_bwd",
+    "osm_linear_ce_workspace_bytes",
+    "osm_linear_ce_fwd",
+    "osm_linear_ce_bwd_workspace_bytes",
+    "osm_linear_ce_bwd",
 )
 
 
@@ -414,6 +429,146 @@ class ClipArgs(ctypes.Structure):
     ]
 
 
+class Seq(ctypes.Structure):
+    """Mirror of ``osm_seq``."""
+
+    _fields_ = [
+        ("p", ctypes.c_void_p),
+        ("stride_b", ctypes.c_int64),
+        ("stride_s", ctypes.c_int64),
+    ]
+
+
+class EmaArgs(ctypes.Structure):
+    """Mirror of ``osm_ema_args``."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("B", ctypes.c_int64),
+        ("S", ctypes.c_int64),
+        ("D", ctypes.c_int64),
+        ("x", Seq),
+        ("gate", Seq),
+        ("out", Seq),
+        ("lengths", ctypes.c_void_p),
+        ("state_init", ctypes.c_void_p),
+        ("state_out", ctypes.c_void_p),
+        ("saved", ctypes.c_void_p),
+    ]
+
+
+class EmaBwdArgs(ctypes.Structure):
+    """Mirror of ``osm_ema_bwd_args``."""
+
+    _fields_ = [
+        ("grad_out", Seq),
+        ("grad_x", Seq),
+        ("grad_gate", Seq),
+        ("grad_state", ctypes.c_void_p),
+        ("grad_init", ctypes.c_void_p),
+    ]
+
+
+class EmaStepArgs(ctypes.Structure):
+    """Mirror of ``osm_ema_step_args``."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("B", ctypes.c_int64),
+        ("D", ctypes.c_int64),
+        ("x", Seq),
+        ("gate", Seq),
+        ("out", Seq),
+        ("state", ctypes.c_void_p),
+        ("state_stride", ctypes.c_int64),
+        ("n_slots", ctypes.c_int64),
+        ("slots", ctypes.c_void_p),
+    ]
+
+
+class ResnormArgs(ctypes.Structure):
+    """Mirror of ``osm_resnorm_args``."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("flags", ctypes.c_int32),
+        ("stream_dtype", ctypes.c_int32),
+        ("block_dtype", ctypes.c_int32),
+        ("rows", ctypes.c_int64),
+        ("D", ctypes.c_int64),
+        ("eps", ctypes.c_float),
+        ("x", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("y", ctypes.c_void_p),
+        ("y_stride", ctypes.c_int64),
+        ("gate", ctypes.c_void_p),
+        ("gate_stride", ctypes.c_int64),
+        ("scale", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("r", ctypes.c_void_p),
+        ("r_stride", ctypes.c_int64),
+        ("n", ctypes.c_void_p),
+        ("n_stride", ctypes.c_int64),
+        ("stats", ctypes.c_void_p),
+    ]
+
+
+class ResnormBwdArgs(ctypes.Structure):
+    """Mirror of ``osm_resnorm_bwd_args``."""
+
+    _fields_ = [
+        ("grad_r", ctypes.c_void_p),
+        ("grad_r_stride", ctypes.c_int64),
+        ("grad_n", ctypes.c_void_p),
+        ("grad_n_stride", ctypes.c_int64),
+        ("grad_x", ctypes.c_void_p),
+        ("grad_x_stride", ctypes.c_int64),
+        ("grad_y", ctypes.c_void_p),
+        ("grad_y_stride", ctypes.c_int64),
+        ("grad_gate", ctypes.c_void_p),
+        ("grad_gate_stride", ctypes.c_int64),
+        ("grad_scale", ctypes.c_void_p),
+        ("grad_weight", ctypes.c_void_p),
+        ("grad_bias", ctypes.c_void_p),
+    ]
+
+
+class LossArgs(ctypes.Structure):
+    """Mirror of ``osm_loss_args``."""
+
+    _fields_ = [
+        ("abi_version", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("N", ctypes.c_int64),
+        ("D", ctypes.c_int64),
+        ("V", ctypes.c_int64),
+        ("hidden", ctypes.c_void_p),
+        ("hidden_stride", ctypes.c_int64),
+        ("weight", ctypes.c_void_p),
+        ("weight_stride", ctypes.c_int64),
+        ("targets", ctypes.c_void_p),
+        ("ignore_index", ctypes.c_int64),
+        ("losses", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("total", ctypes.c_void_p),
+    ]
+
+
+class LossBwdArgs(ctypes.Structure):
+    """Mirror of ``osm_loss_bwd_args``."""
+
+    _fields_ = [
+        ("grad", ctypes.c_void_p),
+        ("grad_losses", ctypes.c_void_p),
+        ("total", ctypes.c_void_p),
+        ("grad_hidden", ctypes.c_void_p),
+        ("grad_weight", ctypes.c_void_p),
+    ]
+
+
 class OsmError(RuntimeError):
     def __init__(self, code: int, msg: str):
         super().__init__(f"{STATUS.get(code, code)}: {msg}")
@@ -494,6 +649,26 @@ def load() -> ctypes.CDLL:
         lib.osm_clip_workspace_bytes.argtypes = [ctypes.POINTER(ClipArgs)]
         lib.osm_clip_grad_norm.restype = ctypes.c_int
         lib.osm_clip_grad_norm.argtypes = [ctypes.POINTER(ClipArgs), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+        for name, args, bwd in (("gated_ema", EmaArgs, EmaBwdArgs), ("linear_ce", LossArgs, LossBwdArgs)):
+            for size in ("", "_bwd"):
+                f = getattr(lib, f"osm_{name}{size}_workspace_bytes")
+                f.restype, f.argtypes = ctypes.c_size_t, [ctypes.POINTER(args)]
+            f = getattr(lib, f"osm_{name}_fwd")
+            f.restype, f.argtypes = ctypes.c_int, [ctypes.POINTER(args), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+            f = getattr(lib, f"osm_{name}_bwd")
+            f.restype, f.argtypes = ctypes.c_int, [ctypes.POINTER(args), ctypes.POINTER(bwd), ctypes.c_void_p,
+                                                   ctypes.c_size_t, ctypes.c_void_p]
+        lib.osm_gated_ema_saved_bytes.restype = ctypes.c_size_t
+        lib.osm_gated_ema_saved_bytes.argtypes = [ctypes.POINTER(EmaArgs)]
+        lib.osm_gated_ema_step.restype = ctypes.c_int
+        lib.osm_gated_ema_step.argtypes = [ctypes.POINTER(EmaStepArgs), ctypes.c_void_p]
+        lib.osm_residual_norm_fwd.restype = ctypes.c_int
+        lib.osm_residual_norm_fwd.argtypes = [ctypes.POINTER(ResnormArgs), ctypes.c_void_p]
+        lib.osm_residual_norm_bwd_workspace_bytes.restype = ctypes.c_size_t
+        lib.osm_residual_norm_bwd_workspace_bytes.argtypes = [ctypes.POINTER(ResnormArgs)]
+        lib.osm_residual_norm_bwd.restype = ctypes.c_int
+        lib.osm_residual_norm_bwd.argtypes = [ctypes.POINTER(ResnormArgs), ctypes.POINTER(ResnormBwdArgs), ctypes.c_void_p,
+                                              ctypes.c_size_t, ctypes.c_void_p]
         got = lib.osm_abi_version()
         if got != ABI_VERSION:
             raise ImportError(f"orthossm_amd: library ABI {got} != binding ABI {ABI_VERSION}; rebuild")

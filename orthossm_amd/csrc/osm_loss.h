@@ -1,0 +1,64 @@
+// Parameters of the vocabulary's cross entropy (osm_loss.hip).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace osm {
+
+constexpr int kLossPad = 256;      // rows of compacted tokens, columns of a piece: multiples of this
+
+// The tokens that count, one after the other.
+struct LossTokens {
+  int* rows;                       // [N]: the token of each place
+  int* places;                     // [N]: the place of each token, -1: does not count
+  int* count;                      // device scalar
+};
+
+struct LossParams {
+  int64_t N, D, V;
+  int Npad, Dpad, parts;           // parts: 1 (bf16), 3 (fp32)
+  const void* hidden;
+  int64_t hidden_s;
+  const void* weight;
+  int64_t weight_s;
+  const int64_t* targets;
+  int64_t ignore;
+  LossTokens tok;
+  __bf16* h;                       // [parts][Npad][Dpad]: the hidden rows that count, zeros after them
+  __bf16* ht;                      // [parts][Dpad][Npad]: the same by column
+  // a piece of the vocabulary
+  int64_t v0;
+  int vn, vpad;                    // its classes; columns of p
+  const __bf16* w;                 // [parts][vn][w_ld], w_part apart
+  int64_t w_ld, w_part;
+  __bf16* wt;                      // [parts][Dpad][vpad]
+  __bf16* p;                       // [parts][Npad][vpad]: probabilities less the targets'
+  __bf16* pt;                      // [parts][vpad][Npad]
+  float* dh;                       // [splits][Npad][Dpad]
+  int splits, first;               // first: dh is written, not added to
+  // statistics
+  float2* stat;                    // [tiles of the vocabulary][Npad]: largest logit, sum of exp of what is below it
+  int tile0;                       // the piece's first tile
+  float* own;                      // [Npad]: the target's logit
+  float *losses, *lse, *total;
+  const float *grad, *grad_losses, *total_in;
+  void *grad_h, *grad_w;
+};
+
+hipError_t launch_loss_tokens(const LossParams& p, hipStream_t stream);                     // tok
+hipError_t launch_loss_rows(const LossParams& p, int dtype, hipStream_t stream);            // h
+hipError_t launch_loss_weight(const LossParams& p, __bf16* to, int dtype, hipStream_t stream);   // parts of the piece's rows
+hipError_t launch_loss_transpose(const __bf16* from, int64_t ld, int64_t from_part, int rows, int cols, __bf16* to, int to_ld,
+                                 int64_t to_part, int parts, hipStream_t stream);
+int loss_tile_rows(const LossParams& p);                                                    // classes of a tile of the logits
+hipError_t launch_loss_logits(const LossParams& p, hipStream_t stream);                     // stat, own
+hipError_t launch_loss_join(const LossParams& p, int tiles, hipStream_t stream);            // losses, lse
+hipError_t launch_loss_total(const LossParams& p, hipStream_t stream);
+hipError_t launch_loss_probs(const LossParams& p, hipStream_t stream);                      // p, pt
+hipError_t launch_loss_dh(const LossParams& p, hipStream_t stream);
+hipError_t launch_loss_dw(const LossParams& p, int dtype, hipStream_t stream);
+hipError_t launch_loss_zero(void* to, int64_t n, int dtype, hipStream_t stream);
+hipError_t launch_loss_finish(const LossParams& p, int dtype, hipStream_t stream);          // grad_h
+
+}  // namespace osm

@@ -1,0 +1,584 @@
+// The cross entropy of a projection to a vocabulary on gfx950, without its logits.
+//
+//   l = W h,  lse = log sum_v e^{l_v},  loss = lse - l_target
+//   P = (e^{l - lse} - [v = target]) g,   dH = P W,   dW = P^T H
+//
+// Forward: a workgroup forms a tile of logits by classes and tokens in its
+// accumulators and leaves of it, for every token, the largest and the sum of
+// exponentials below it; a second kernel joins the tiles.  Backward, a piece of the
+// vocabulary at a time: the logits again, from them P (to bf16, or three bf16 parts of
+// an fp32 result), by rows and by columns, then the two products.  What counts for
+// all of them: the products' operations on the matrix instruction (osm_gemm.h); the
+// tokens that do not count are left out first, so they cost nothing.
+#include <algorithm>
+#include <type_traits>
+
+#include "osm_gemm.h"
+#include "osm_loss.h"
+#include "osm_wide_store.h"
+
+namespace osm {
+namespace {
+
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.44269504f, kInf = __builtin_inff();
+
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+
+// ---- the tokens that count ----
+
+constexpr int kScanThreads = 1024;
+
+// One workgroup over all targets, in order.
+__global__ void __launch_bounds__(kScanThreads) loss_tokens_kernel(const LossParams p) {
+  __shared__ int sums[kScanThreads / 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int base = 0;
+  for (int64_t i0 = 0; i0 < p.N; i0 += kScanThreads) {
+    const int64_t i = i0 + threadIdx.x;
+    const bool in = i < p.N && p.targets[i] != p.ignore;
+    const unsigned long long mask = __ballot(in);
+    if (lane == 0) sums[wave] = __popcll(mask);
+    __syncthreads();
+    int before = base;
+    for (int w = 0; w < kScanThreads / 64; ++w) {
+      const int s = sums[w];
+      if (w < wave) before += s;
+      base += s;
+    }
+    const int at = before + __popcll(mask & ((1ull << lane) - 1));
+    if (in) p.tok.rows[at] = (int)i;
+    if (i < p.N) p.tok.places[i] = in ? at : -1;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *p.tok.count = base;
+}
+
+// ---- operands ----
+
+// The bf16 parts of x: part k is what rounding leaves of the parts before it.
+template <int PARTS>
+__device__ __forceinline__ void split(float x, __bf16 (&to)[PARTS]) {
+#pragma unroll
+  for (int k = 0; k < PARTS; ++k) {
+    to[k] = (__bf16)x;
+    x -= (float)to[k];
+  }
+}
+
+// Rows of `from` (with `rows`: those it names, zeros past *count) in units of 8
+// columns, zeros past the D-th, to [PARTS][n][ld].
+template <typename T, int PARTS>
+__global__ void __launch_bounds__(256) loss_pack_kernel(const T* from, int64_t stride, int D, int64_t n, int ld, const int* rows,
+                                                        const int* count, __bf16* to) {
+  const int units = ld / 8;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n * units) return;
+  const int64_t r = i / units;
+  const int c = (int)(i - r * units) * 8;
+  bf16x8 out[PARTS] = {};
+  if (!rows || r < *count) {
+    const T* const src = from + (rows ? rows[r] : r) * stride + c;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (c + k < D) {
+        __bf16 s[PARTS];
+        split<PARTS>((float)src[k], s);
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q) out[q][k] = s[q];
+      }
+  }
+#pragma unroll
+  for (int q = 0; q < PARTS; ++q) {
+    *reinterpret_cast<bf16x8*>(to + ((int64_t)q * n + r) * ld + c) = out[q];
+    wide_store_wait();
+  }
+}
+
+// 64 x 64 of a matrix by its columns: to[c][r] = from[r][c], zeros for r past `rows`
+// (up to to_ld).
+__global__ void __launch_bounds__(256) loss_transpose_kernel(const __bf16* from, int64_t ld, int64_t from_part, int rows, int cols,
+                                                             __bf16* to, int to_ld, int64_t to_part) {
+  __shared__ __bf16 t[64][66];
+  from += blockIdx.z * from_part;
+  to += blockIdx.z * to_part;
+  const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
+  for (int i = threadIdx.x; i < 64 * 8; i += 256) {
+    const int r = i / 8, c = i % 8 * 8;
+    bf16x8 v = {};
+    if (r0 + r < rows && c0 + c + 8 <= cols) {
+      v = *reinterpret_cast<const bf16x8*>(from + (int64_t)(r0 + r) * ld + c0 + c);
+    } else if (r0 + r < rows) {
+      for (int k = 0; k < 8; ++k)
+        if (c0 + c + k < cols) v[k] = from[(int64_t)(r0 + r) * ld + c0 + c + k];
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t[r][c + k] = v[k];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 64 * 8; i += 256) {
+    const int c = i / 8, r = i % 8 * 8;
+    if (c0 + c >= cols || r0 + r >= to_ld) continue;
+    bf16x8 v;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = t[r + k][c];
+    *reinterpret_cast<bf16x8*>(to + (int64_t)(c0 + c) * to_ld + r0 + r) = v;
+    wide_store_wait();
+  }
+}
+
+// ---- products ----
+
+// A block's tile (m, n) of tm by tn: the XCDs, to which blocks go in turn, take
+// contiguous shares of an order that walks bands of 8 columns by rows, so that what is
+// at work on an XCD at a time shares rows and columns in its L2.  False: no tile.
+__device__ __forceinline__ bool tile_of(int tm, int tn, int& m, int& n) {
+  const int total = tm * tn, share = (total + 7) / 8, id = (blockIdx.x & 7) * share + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= share || id >= total) return false;
+  const int band = id / (8 * tm), rest = id - band * 8 * tm, width = min(8, tn - band * 8);
+  m = rest / width;
+  n = band * 8 + rest - m * width;
+  return true;
+}
+unsigned grid_of(int64_t tm, int64_t tn) { return (unsigned)((tm * tn + 7) / 8 * 8); }
+
+GemmSide side(const __bf16* p, int64_t ld, int64_t part, int rows) { return {p, ld, part, rows}; }
+
+struct Product {
+  GemmSide a, b;
+  int tm, tn;
+};
+
+// Logits of a tile: A the piece's classes, B the tokens that count.  BWD false: the
+// tile's largest logit and sum of exponentials for each token, and the target's logit.
+// BWD true: P and its transpose.
+template <class G, int PARTS, bool BWD>
+__global__ void __launch_bounds__(G::kThreads) loss_logits_kernel(const LossParams p, const Product g) {
+  __shared__ __attribute__((aligned(16))) __bf16 lds[G::kLds];
+  int tm, tn;
+  if (!tile_of(g.tm, g.tn, tm, tn)) return;
+  const int count = *p.tok.count, m0 = tm * G::TM, n0 = tn * G::TN;
+  if (n0 >= count) return;
+  f32x16 acc[G::FM][G::FN];
+  gemm<G>(g.a, g.b, m0, n0, 0, p.Dpad / kStep, PARTS, lds, acc);
+  const GemmPlace<G> q;
+  if constexpr (!BWD) {
+    float2* const red = reinterpret_cast<float2*>(lds);   // [WM][TN]
+#pragma unroll
+    for (int j = 0; j < G::FN; ++j) {
+      const int n = n0 + q.col(j);
+      const int64_t target = n < count ? p.targets[p.tok.rows[n]] - p.v0 : -1;
+      float top = -kInf, sum = 0.0f;
+#pragma unroll
+      for (int f = 0; f < G::FM; ++f)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int m = m0 + q.row(f, i);
+          if (m == target && m < p.vn) p.own[n] = acc[f][j][i];
+          top = m < p.vn ? __builtin_fmaxf(top, acc[f][j][i]) : top;
+        }
+      const float base = top == -kInf ? 0.0f : top;
+#pragma unroll
+      for (int f = 0; f < G::FM; ++f)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum += m0 + q.row(f, i) < p.vn ? exp_of(acc[f][j][i] - base) : 0.0f;
+      // the other half's rows
+      const float top2 = __shfl_xor(top, 32), sum2 = __shfl_xor(sum, 32), both = __builtin_fmaxf(top, top2);
+      const float b2 = both == -kInf ? 0.0f : both;
+      sum = sum * exp_of(top - b2) + sum2 * exp_of(top2 - b2);
+      if (q.lane < 32) red[q.m / (G::TM / G::WM) * G::TN + q.col(j)] = make_float2(both, sum);
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < G::TN; c += G::kThreads) {
+      float top = -kInf, sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < G::WM; ++w) top = __builtin_fmaxf(top, red[w * G::TN + c].x);
+      const float b = top == -kInf ? 0.0f : top;
+#pragma unroll
+      for (int w = 0; w < G::WM; ++w) sum += red[w * G::TN + c].y * exp_of(red[w * G::TN + c].x - b);
+      p.stat[(int64_t)(p.tile0 + tm) * p.Npad + n0 + c] = make_float2(top, sum);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < G::FN; ++j) {
+      const int n = n0 + q.col(j);
+      const bool in = n < count;
+      const int token = in ? p.tok.rows[n] : 0;
+      const int64_t target = in ? p.targets[token] - p.v0 : -1;
+      const float lse = in ? p.lse[token] : 0.0f, f0 = in ? (p.grad_losses ? p.grad_losses[token] : 1.0f) : 0.0f;
+#pragma unroll
+      for (int f = 0; f < G::FM; ++f)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int m = m0 + q.row(f, i);
+          const float e = exp_of(acc[f][j][i] - lse) - (m == target ? 1.0f : 0.0f);
+          acc[f][j][i] = in && m < p.vn ? e * f0 : 0.0f;
+        }
+    }
+    constexpr int kRowUnits = G::TM / 8, kColUnits = G::TN / 8;
+    static_assert(G::TM * G::TN <= G::kLds, "a tile of P fits");
+#pragma unroll 1
+    for (int part = 0; part < PARTS; ++part) {
+      // by tokens: a lane's four neighbouring classes are half a 16-byte unit, which lies
+      // at its index xor its row's
+#pragma unroll
+      for (int j = 0; j < G::FN; ++j)
+#pragma unroll
+        for (int f = 0; f < G::FM; ++f)
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            const int c = q.col(j), r = q.row(f, i);
+            bf16x4 v;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = (__bf16)acc[f][j][i + k];
+            *reinterpret_cast<bf16x4*>(lds + c * G::TM + ((r / 8) ^ (c % kRowUnits)) * 8 + r % 8) = v;
+          }
+      __syncthreads();
+      for (int u = threadIdx.x; u < G::TN * kRowUnits; u += G::kThreads) {
+        const int c = u / kRowUnits, r = u % kRowUnits;
+        const bf16x8 v = *reinterpret_cast<const bf16x8*>(lds + c * G::TM + (r ^ (c % kRowUnits)) * 8);
+        if (m0 + r * 8 < p.vpad) {
+          *reinterpret_cast<bf16x8*>(p.p + ((int64_t)part * p.Npad + n0 + c) * p.vpad + m0 + r * 8) = v;
+          wide_store_wait();
+        }
+      }
+      __syncthreads();
+      // by classes; what the next part is made of stays in acc
+#pragma unroll
+      for (int j = 0; j < G::FN; ++j)
+#pragma unroll
+        for (int f = 0; f < G::FM; ++f)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int c = q.col(j), r = q.row(f, i);
+            const __bf16 v = (__bf16)acc[f][j][i];
+            lds[r * G::TN + ((c / 8) ^ (r % kColUnits)) * 8 + c % 8] = v;
+            if (PARTS > 1) acc[f][j][i] -= (float)v;
+          }
+      __syncthreads();
+      for (int u = threadIdx.x; u < G::TM * kColUnits; u += G::kThreads) {
+        const int r = u / kColUnits, c = u % kColUnits;
+        const bf16x8 v = *reinterpret_cast<const bf16x8*>(lds + r * G::TN + (c ^ (r % kColUnits)) * 8);
+        if (m0 + r < p.vpad) {
+          *reinterpret_cast<bf16x8*>(p.pt + ((int64_t)part * p.vpad + m0 + r) * p.Npad + n0 + c * 8) = v;
+          wide_store_wait();
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// dH of a piece: A the weights by column, B P; a split takes a share of the classes and
+// adds to sums of its own.
+template <class G, int PARTS>
+__global__ void __launch_bounds__(G::kThreads) loss_dh_kernel(const LossParams p, const Product g) {
+  __shared__ __attribute__((aligned(16))) __bf16 lds[G::kLds];
+  int tm, tn;
+  if (!tile_of(g.tm, g.tn, tm, tn)) return;
+  const int count = *p.tok.count, m0 = tm * G::TM, n0 = tn * G::TN;
+  if (n0 >= count) return;
+  const int all = p.vpad / kStep, each = (all + p.splits - 1) / p.splits, s0 = min((int)blockIdx.y * each, all);
+  f32x16 acc[G::FM][G::FN];
+  gemm<G>(g.a, g.b, m0, n0, (int64_t)s0 * kStep, min(each, all - s0), PARTS, lds, acc);
+  const GemmPlace<G> q;
+#pragma unroll
+  for (int j = 0; j < G::FN; ++j) {
+    float* const to = p.dh + ((int64_t)blockIdx.y * p.Npad + n0 + q.col(j)) * p.Dpad;
+#pragma unroll
+    for (int f = 0; f < G::FM; ++f)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const int m = m0 + q.row(f, i);
+        if (m >= p.Dpad) continue;
+        f32x4 v = {acc[f][j][i], acc[f][j][i + 1], acc[f][j][i + 2], acc[f][j][i + 3]};
+        if (!p.first) v += *reinterpret_cast<const f32x4*>(to + m);
+        *reinterpret_cast<f32x4*>(to + m) = v;
+        wide_store_wait();
+      }
+  }
+}
+
+__device__ __forceinline__ float factor(const LossParams& p) {
+  return (p.grad ? *p.grad : 1.0f) / (p.total_in ? p.total_in[1] : 1.0f);
+}
+
+// dW of a piece: A the hidden rows by column, B P by classes.
+template <class G, int PARTS, typename T>
+__global__ void __launch_bounds__(G::kThreads) loss_dw_kernel(const LossParams p, const Product g) {
+  __shared__ __attribute__((aligned(16))) __bf16 lds[G::kLds];
+  int tm, tn;
+  if (!tile_of(g.tm, g.tn, tm, tn)) return;
+  const int m0 = tm * G::TM, n0 = tn * G::TN;
+  f32x16 acc[G::FM][G::FN];
+  gemm<G>(g.a, g.b, m0, n0, 0, (*p.tok.count + kStep - 1) / kStep, PARTS, lds, acc);
+  const float s = factor(p);
+  const GemmPlace<G> q;
+  typedef T V4 __attribute__((ext_vector_type(4)));
+  const bool vec = p.D % 4 == 0;
+#pragma unroll
+  for (int j = 0; j < G::FN; ++j) {
+    const int n = n0 + q.col(j);
+    if (n >= p.vn) continue;
+    T* const to = static_cast<T*>(p.grad_w) + (p.v0 + n) * p.D;
+#pragma unroll
+    for (int f = 0; f < G::FM; ++f)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const int m = m0 + q.row(f, i);
+        V4 v;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = (T)(acc[f][j][i + k] * s);
+        if (vec) {
+          if (m < p.D) {
+            *reinterpret_cast<V4*>(to + m) = v;
+            if (sizeof(V4) > 8) wide_store_wait();
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (m + k < p.D) to[m + k] = v[k];
+        }
+      }
+  }
+}
+
+// ---- joins ----
+
+constexpr int kJoinTokens = 16, kJoinSlices = 16;
+
+// A place's statistics over the vocabulary's tiles, 16 threads a place.
+__global__ void __launch_bounds__(kJoinTokens * kJoinSlices) loss_join_kernel(const LossParams p, int tiles) {
+  __shared__ float2 red[kJoinSlices][kJoinTokens];
+  const int c = threadIdx.x % kJoinTokens, s = threadIdx.x / kJoinTokens, at = blockIdx.x * kJoinTokens + c;
+  if (blockIdx.x * kJoinTokens >= *p.tok.count) return;
+  float top = -kInf, sum = 0.0f;
+  for (int t = s; t < tiles; t += kJoinSlices) {
+    const float2 v = p.stat[(int64_t)t * p.Npad + at];
+    const float both = __builtin_fmaxf(top, v.x), b = both == -kInf ? 0.0f : both;
+    sum = sum * exp_of(top - b) + v.y * exp_of(v.x - b);
+    top = both;
+  }
+  red[s][c] = make_float2(top, sum);
+  __syncthreads();
+  if (s > 0 || at >= *p.tok.count) return;
+  for (int k = 1; k < kJoinSlices; ++k) top = __builtin_fmaxf(top, red[k][c].x);
+  const float b = top == -kInf ? 0.0f : top;
+  sum = 0.0f;
+  for (int k = 0; k < kJoinSlices; ++k) sum += red[k][c].y * exp_of(red[k][c].x - b);
+  const int token = p.tok.rows[at];
+  const int64_t target = p.targets[token];
+  const bool known = target >= 0 && target < p.V;
+  const float l = logf(sum);
+  p.lse[token] = known ? b + l : __builtin_nanf("");
+  if (p.losses) p.losses[token] = known ? l - (p.own[at] - b) : __builtin_nanf("");
+}
+
+// Zeros of the tokens that do not count.
+__global__ void __launch_bounds__(256) loss_blank_kernel(const LossParams p) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= p.N || p.tok.places[i] >= 0) return;
+  p.lse[i] = 0.0f;
+  if (p.losses) p.losses[i] = 0.0f;
+}
+
+// The sum of the losses in double, one workgroup, in an order that does not depend on timing.
+__global__ void __launch_bounds__(1024) loss_total_kernel(const LossParams p) {
+  __shared__ double red[1024];
+  double s = 0.0;
+  for (int64_t i = threadIdx.x; i < p.N; i += 1024) s += p.losses[i];
+  red[threadIdx.x] = s;
+  for (int w = 512; w > 0; w >>= 1) {
+    __syncthreads();
+    if ((int)threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
+  }
+  if (threadIdx.x == 0) {
+    p.total[0] = (float)red[0];
+    p.total[1] = p.tok.count ? (float)max(*p.tok.count, 1) : 1.0f;
+  }
+}
+
+// grad_h of every token from its place's sums, zeros where it does not count.
+template <typename T>
+__global__ void __launch_bounds__(256) loss_finish_kernel(const LossParams p) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int per = ((int)p.D + 3) / 4;
+  if (i >= p.N * per) return;
+  const int64_t n = i / per;
+  const int d = (int)(i - n * per) * 4, at = p.tok.places[n];
+  f32x4 v = {};
+  if (at >= 0) {
+    for (int s = 0; s < p.splits; ++s) v += *reinterpret_cast<const f32x4*>(p.dh + ((int64_t)s * p.Npad + at) * p.Dpad + d);
+    v *= factor(p);
+  }
+  T* const to = static_cast<T*>(p.grad_h) + n * p.D + d;
+  typedef T V4 __attribute__((ext_vector_type(4)));
+  V4 o;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) o[k] = (T)v[k];
+  if (p.D % 4 == 0) {
+    *reinterpret_cast<V4*>(to) = o;
+    if (sizeof(V4) > 8) wide_store_wait();
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (d + k < p.D) to[k] = o[k];
+  }
+}
+
+// Zeros of a gradient that no token has a part in.
+template <typename T>
+__global__ void __launch_bounds__(256) loss_zero_kernel(T* to, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) to[i] = (T)0.0f;
+}
+
+using Big = GemmTile<256, 256, 2, 4>;
+using Middle = GemmTile<128, 128, 2, 2>;
+using Small = GemmTile<128, 64, 2, 2>;
+constexpr int kCUs = 256;
+
+// The largest tile that still gives every CU one, else the smallest.
+template <typename F>
+void by_size(int64_t M, int64_t N, F f) {
+  auto tiles = [&](int64_t tm, int64_t tn) { return (M + tm - 1) / tm * ((N + tn - 1) / tn); };
+  if (tiles(256, 256) >= kCUs * 3 / 4)
+    f(Big{});
+  else if (tiles(128, 128) >= kCUs * 3 / 4)
+    f(Middle{});
+  else
+    f(Small{});
+}
+
+template <class G>
+Product product(GemmSide a, GemmSide b, int64_t M, int64_t N) {
+  return {a, b, (int)((M + G::TM - 1) / G::TM), (int)((N + G::TN - 1) / G::TN)};
+}
+
+template <typename F>
+void by_parts(int parts, F f) {
+  if (parts == 1)
+    f(std::integral_constant<int, 1>{});
+  else
+    f(std::integral_constant<int, 3>{});
+}
+
+template <bool BWD>
+hipError_t logits(const LossParams& p, hipStream_t stream) {
+  by_size(BWD ? p.vpad : p.V, p.N, [&](auto g) {
+    using G = decltype(g);
+    const Product t = product<G>(side(p.w, p.w_ld, p.w_part, p.vn), side(p.h, p.Dpad, (int64_t)p.Npad * p.Dpad, p.Npad),
+                                 BWD ? p.vpad : p.vn, p.N);
+    by_parts(p.parts, [&](auto n) {
+      hipLaunchKernelGGL((loss_logits_kernel<G, decltype(n)::value, BWD>), dim3(grid_of(t.tm, t.tn)), dim3(G::kThreads), 0, stream, p, t);
+    });
+  });
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_loss_tokens(const LossParams& p, hipStream_t stream) {
+  hipLaunchKernelGGL(loss_tokens_kernel, dim3(1), dim3(kScanThreads), 0, stream, p);
+  return hipGetLastError();
+}
+
+namespace {
+template <typename T, int PARTS>
+void pack(const void* from, int64_t stride, int64_t D, int64_t n, int ld, const int* rows, const int* count, __bf16* to, hipStream_t stream) {
+  hipLaunchKernelGGL((loss_pack_kernel<T, PARTS>), dim3((unsigned)((n * (ld / 8) + 255) / 256)), dim3(256), 0, stream,
+                     static_cast<const T*>(from), stride, (int)D, n, ld, rows, count, to);
+}
+}  // namespace
+
+hipError_t launch_loss_rows(const LossParams& p, int dtype, hipStream_t stream) {
+  if (dtype == 0)
+    pack<float, 3>(p.hidden, p.hidden_s, p.D, p.Npad, p.Dpad, p.tok.rows, p.tok.count, p.h, stream);
+  else
+    pack<__bf16, 1>(p.hidden, p.hidden_s, p.D, p.Npad, p.Dpad, p.tok.rows, p.tok.count, p.h, stream);
+  return hipGetLastError();
+}
+
+hipError_t launch_loss_weight(const LossParams& p, __bf16* to, int dtype, hipStream_t stream) {
+  if (dtype == 0)
+    pack<float, 3>(static_cast<const float*>(p.weight) + p.v0 * p.weight_s, p.weight_s, p.D, p.vn, p.Dpad, nullptr, nullptr, to, stream);
+  else
+    pack<__bf16, 1>(static_cast<const __bf16*>(p.weight) + p.v0 * p.weight_s, p.weight_s, p.D, p.vn, p.Dpad, nullptr, nullptr, to, stream);
+  return hipGetLastError();
+}
+
+hipError_t launch_loss_transpose(const __bf16* from, int64_t ld, int64_t from_part, int rows, int cols, __bf16* to, int to_ld,
+                                 int64_t to_part, int parts, hipStream_t stream) {
+  hipLaunchKernelGGL(loss_transpose_kernel, dim3((unsigned)((to_ld + 63) / 64), (unsigned)((cols + 63) / 64), parts), dim3(256), 0, stream,
+                     from, ld, from_part, rows, cols, to, to_ld, to_part);
+  return hipGetLastError();
+}
+
+int loss_tile_rows(const LossParams& p) {
+  int rows = 0;
+  by_size(p.V, p.N, [&](auto g) { rows = decltype(g)::TM; });
+  return rows;
+}
+
+hipError_t launch_loss_logits(const LossParams& p, hipStream_t stream) { return logits<false>(p, stream); }
+hipError_t launch_loss_probs(const LossParams& p, hipStream_t stream) { return logits<true>(p, stream); }
+
+hipError_t launch_loss_join(const LossParams& p, int tiles, hipStream_t stream) {
+  hipLaunchKernelGGL(loss_join_kernel, dim3((unsigned)((p.N + kJoinTokens - 1) / kJoinTokens)), dim3(kJoinTokens * kJoinSlices), 0, stream,
+                     p, tiles);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(loss_blank_kernel, dim3((unsigned)((p.N + 255) / 256)), dim3(256), 0, stream, p);
+  return hipGetLastError();
+}
+
+hipError_t launch_loss_total(const LossParams& p, hipStream_t stream) {
+  hipLaunchKernelGGL(loss_total_kernel, dim3(1), dim3(1024), 0, stream, p);
+  return hipGetLastError();
+}
+
+hipError_t launch_loss_dh(const LossParams& p, hipStream_t stream) {
+  by_size((int64_t)p.Dpad * p.splits, p.N, [&](auto g) {
+    using G = decltype(g);
+    const Product t = product<G>(side(p.wt, p.vpad, (int64_t)p.Dpad * p.vpad, (int)p.D), side(p.p, p.vpad, (int64_t)p.Npad * p.vpad, p.Npad),
+                                 p.D, p.N);
+    by_parts(p.parts, [&](auto n) {
+      hipLaunchKernelGGL((loss_dh_kernel<G, decltype(n)::value>), dim3(grid_of(t.tm, t.tn), p.splits), dim3(G::kThreads), 0, stream, p, t);
+    });
+  });
+  return hipGetLastError();
+}
+
+hipError_t launch_loss_dw(const LossParams& p, int dtype, hipStream_t stream) {
+  by_size(p.D, p.vn, [&](auto g) {
+    using G = decltype(g);
+    const Product t = product<G>(side(p.ht, p.Npad, (int64_t)p.Dpad * p.Npad, (int)p.D), side(p.pt, p.Npad, (int64_t)p.vpad * p.Npad, p.vpad),
+                                 p.D, p.vn);
+    if (dtype == 0)
+      hipLaunchKernelGGL((loss_dw_kernel<G, 3, float>), dim3(grid_of(t.tm, t.tn)), dim3(G::kThreads), 0, stream, p, t);
+    else
+      hipLaunchKernelGGL((loss_dw_kernel<G, 1, __bf16>), dim3(grid_of(t.tm, t.tn)), dim3(G::kThreads), 0, stream, p, t);
+  });
+  return hipGetLastError();
+}
+
+hipError_t launch_loss_zero(void* to, int64_t n, int dtype, hipStream_t stream) {
+  const dim3 grid((unsigned)std::min<int64_t>((n + 255) / 256, 4096));
+  if (dtype == 0)
+    hipLaunchKernelGGL((loss_zero_kernel<float>), grid, dim3(256), 0, stream, static_cast<float*>(to), n);
+  else
+    hipLaunchKernelGGL((loss_zero_kernel<__bf16>), grid, dim3(256), 0, stream, static_cast<__bf16*>(to), n);
+  return hipGetLastError();
+}
+
+hipError_t launch_loss_finish(const LossParams& p, int dtype, hipStream_t stream) {
+  const dim3 grid((unsigned)((p.N * ((p.D + 3) / 4) + 255) / 256));
+  if (dtype == 0)
+    hipLaunchKernelGGL((loss_finish_kernel<float>), grid, dim3(256), 0, stream, p);
+  else
+    hipLaunchKernelGGL((loss_finish_kernel<__bf16>), grid, dim3(256), 0, stream, p);
+  return hipGetLastError();
+}
+
+}  // namespace osm

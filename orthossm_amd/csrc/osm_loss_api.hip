@@ -1,0 +1,267 @@
+// C ABI of the vocabulary's cross entropy: argument checks, memory layout and
+// dispatch.  Declared in include/osm.h.
+#include <algorithm>
+
+#include "osm.h"
+#include "osm_kernels.h"
+#include "osm_loss.h"
+
+namespace {
+
+using osm::fail;
+using osm::kLossPad;
+using osm::LossParams;
+using osm::ok;
+
+constexpr int64_t kMaxRow = int64_t(1) << 21;   // elements of an operand's row
+
+int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+int check_args(const osm_loss_args* a) {
+  if (!a) return fail(OSM_E_ARG, "args is NULL");
+  if (a->abi_version != OSM_ABI_VERSION)
+    return fail(OSM_E_ARG, "abi_version %d does not match library ABI %d", a->abi_version, OSM_ABI_VERSION);
+  if (a->dtype != OSM_F32 && a->dtype != OSM_BF16) return fail(OSM_E_DTYPE, "dtype %d unsupported", a->dtype);
+  if (a->N < 0 || a->N > kMaxRow - kLossPad || a->D < 1 || a->D > (int64_t(1) << 17) || a->V < 1 || a->V > (int64_t(1) << 28))
+    return fail(OSM_E_SHAPE, "N=%lld outside [0, 2^21 - 256], D=%lld outside [1, 2^17] or V=%lld outside [1, 2^28]", (long long)a->N,
+                (long long)a->D, (long long)a->V);
+  return OSM_OK;
+}
+
+int check_matrix(const void* p, int64_t stride, int64_t least, int esize, const char* name) {
+  if (!p) return fail(OSM_E_ARG, "%s is NULL", name);
+  if ((uintptr_t)p % esize) return fail(OSM_E_LAYOUT, "%s is not aligned to its elements", name);
+  if (stride < least) return fail(OSM_E_LAYOUT, "%s: row stride %lld below %lld", name, (long long)stride, (long long)least);
+  return OSM_OK;
+}
+
+int check_inputs(const osm_loss_args* a) {
+  const int es = a->dtype == OSM_F32 ? 4 : 2;
+  int rc;
+  if ((rc = check_matrix(a->hidden, a->hidden_stride, 0, es, "hidden")) != OSM_OK ||
+      (rc = check_matrix(a->weight, a->weight_stride, 0, es, "weight")) != OSM_OK)
+    return rc;
+  if (!a->targets || (uintptr_t)a->targets % 8) return fail(OSM_E_ARG, "targets is NULL or not 8-byte aligned");
+  if (!a->lse || (uintptr_t)a->lse % 4) return fail(OSM_E_ARG, "lse is NULL or not 4-byte aligned");
+  return OSM_OK;
+}
+
+// Whether the weights are read where they are.
+bool direct(const osm_loss_args* a) {
+  return a->dtype == OSM_BF16 && a->D % 64 == 0 && (uintptr_t)a->weight % 16 == 0 && a->weight_stride % 8 == 0 &&
+         a->weight_stride < kMaxRow;
+}
+
+// What a launch works on: the compacted hidden rows, and pieces of the vocabulary.
+struct Plan {
+  int64_t Npad, Dpad, parts, piece;   // piece: classes, a multiple of kLossPad
+  int splits;
+  bool direct;
+};
+
+// Pieces of about the same size, each of at most `most` classes.
+int64_t piece_of(int64_t V, int64_t most) {
+  most = std::max<int64_t>(kLossPad, std::min(most, kMaxRow - kLossPad) / kLossPad * kLossPad);
+  const int64_t n = (V + most - 1) / most;
+  return up((V + n - 1) / n, kLossPad);
+}
+
+Plan plan_of(const osm_loss_args* a, bool bwd) {
+  Plan n;
+  n.parts = a->dtype == OSM_F32 ? 3 : 1;
+  n.Npad = up(std::max<int64_t>(a->N, 1), kLossPad);
+  n.Dpad = up(a->D, 64);
+  n.direct = direct(a);
+  // Backward: 2^27 elements of P.  Forward: as many of the weights' parts, or all classes at once.
+  n.piece = bwd ? piece_of(a->V, (int64_t(1) << 27) / (n.Npad * n.parts))
+                : n.direct ? up(a->V, kLossPad) : piece_of(a->V, (int64_t(1) << 27) / (n.Dpad * n.parts));
+  const int64_t tiles = ((a->D + 255) / 256) * (n.Npad / 256);
+  n.splits = (int)std::max<int64_t>(1, std::min<int64_t>({256 / std::max<int64_t>(1, tiles), n.piece / 1024, 8}));
+  return n;
+}
+
+// The regions of a workspace, each at a multiple of 256 bytes.
+struct Regions {
+  size_t total = 0;
+  size_t add(size_t bytes) {
+    const size_t at = total;
+    total += (bytes + 255) / 256 * 256;
+    return at;
+  }
+};
+struct Layout {
+  size_t rows, places, count, h, w, own, stat, ht, wt, p, pt, dh, total;
+};
+Layout layout_of(const osm_loss_args* a, const Plan& n, bool bwd) {
+  Regions r;
+  Layout l{};
+  l.rows = r.add(a->N * 4);
+  l.places = r.add(a->N * 4);
+  l.count = r.add(4);
+  const size_t hidden = (size_t)n.parts * n.Npad * n.Dpad * 2;
+  l.h = r.add(hidden);
+  l.w = r.add(n.direct ? 0 : (size_t)n.parts * n.piece * n.Dpad * 2);
+  if (!bwd) {
+    l.own = r.add(n.Npad * 4);
+    l.stat = r.add((size_t)(up(a->V, kLossPad) / 64) * n.Npad * 8);
+  } else {
+    l.ht = r.add(hidden);
+    l.wt = r.add((size_t)n.parts * n.Dpad * n.piece * 2);
+    l.p = r.add((size_t)n.parts * n.Npad * n.piece * 2);
+    l.pt = r.add((size_t)n.parts * n.Npad * n.piece * 2);
+    l.dh = r.add((size_t)n.splits * n.Npad * n.Dpad * 4);
+  }
+  l.total = r.total;
+  return l;
+}
+
+int check_workspace(const void* w, size_t have, size_t need) {
+  if (!w || (uintptr_t)w % 256 || have < need)
+    return fail(OSM_E_WORKSPACE, "the workspace must be 256-byte aligned and have %zu bytes (it has %zu)", need, w ? have : 0);
+  return OSM_OK;
+}
+
+LossParams params_of(const osm_loss_args* a, const Plan& n, const Layout& l, void* workspace) {
+  char* const w = static_cast<char*>(workspace);
+  LossParams p{};
+  p.N = a->N;
+  p.D = a->D;
+  p.V = a->V;
+  p.Npad = (int)n.Npad;
+  p.Dpad = (int)n.Dpad;
+  p.parts = (int)n.parts;
+  p.hidden = a->hidden;
+  p.hidden_s = a->hidden_stride;
+  p.weight = a->weight;
+  p.weight_s = a->weight_stride;
+  p.targets = a->targets;
+  p.ignore = a->ignore_index;
+  p.tok = {reinterpret_cast<int*>(w + l.rows), reinterpret_cast<int*>(w + l.places), reinterpret_cast<int*>(w + l.count)};
+  p.h = reinterpret_cast<__bf16*>(w + l.h);
+  p.lse = a->lse;
+  return p;
+}
+
+// The piece of `n` classes from v0 on, and its weights' parts where they are not read in place.
+hipError_t set_piece(LossParams& p, const osm_loss_args* a, const Plan& n, const Layout& l, char* w, int64_t v0, hipStream_t st) {
+  p.v0 = v0;
+  p.vn = (int)std::min(n.piece, a->V - v0);
+  p.vpad = (int)up(p.vn, kLossPad);
+  if (n.direct) {
+    p.w = static_cast<const __bf16*>(a->weight) + v0 * a->weight_stride;
+    p.w_ld = a->weight_stride;
+    p.w_part = 0;
+    return hipSuccess;
+  }
+  __bf16* const to = reinterpret_cast<__bf16*>(w + l.w);
+  p.w = to;
+  p.w_ld = n.Dpad;
+  p.w_part = (int64_t)p.vn * n.Dpad;
+  return osm::launch_loss_weight(p, to, a->dtype, st);
+}
+
+int hip_rc(hipError_t e) { return e == hipSuccess ? ok() : fail(OSM_E_HIP, "cross entropy launch: %s", hipGetErrorString(e)); }
+
+hipError_t forward(const osm_loss_args* a, const Plan& n, const Layout& l, void* workspace, hipStream_t st) {
+  char* const w = static_cast<char*>(workspace);
+  LossParams p = params_of(a, n, l, workspace);
+  p.own = reinterpret_cast<float*>(w + l.own);
+  p.stat = reinterpret_cast<float2*>(w + l.stat);
+  p.losses = a->losses;
+  p.total = a->total;
+  hipError_t e;
+  if ((e = osm::launch_loss_tokens(p, st)) != hipSuccess || (e = osm::launch_loss_rows(p, a->dtype, st)) != hipSuccess) return e;
+  const int rows = osm::loss_tile_rows(p);
+  for (int64_t v0 = 0; v0 < a->V; v0 += n.piece) {
+    p.tile0 = (int)(v0 / rows);
+    if ((e = set_piece(p, a, n, l, w, v0, st)) != hipSuccess || (e = osm::launch_loss_logits(p, st)) != hipSuccess) return e;
+  }
+  if ((e = osm::launch_loss_join(p, (int)((a->V + rows - 1) / rows), st)) != hipSuccess) return e;
+  return a->total ? osm::launch_loss_total(p, st) : hipSuccess;
+}
+
+hipError_t backward(const osm_loss_args* a, const osm_loss_bwd_args* b, const Plan& n, const Layout& l, void* workspace, hipStream_t st) {
+  char* const w = static_cast<char*>(workspace);
+  LossParams p = params_of(a, n, l, workspace);
+  p.ht = reinterpret_cast<__bf16*>(w + l.ht);
+  p.wt = reinterpret_cast<__bf16*>(w + l.wt);
+  p.p = reinterpret_cast<__bf16*>(w + l.p);
+  p.pt = reinterpret_cast<__bf16*>(w + l.pt);
+  p.dh = reinterpret_cast<float*>(w + l.dh);
+  p.splits = n.splits;
+  p.grad = b->grad;
+  p.grad_losses = b->grad_losses;
+  p.total_in = b->total;
+  p.grad_h = b->grad_hidden;
+  p.grad_w = b->grad_weight;
+  hipError_t e;
+  if ((e = osm::launch_loss_tokens(p, st)) != hipSuccess || (e = osm::launch_loss_rows(p, a->dtype, st)) != hipSuccess) return e;
+  if (b->grad_weight && (e = osm::launch_loss_transpose(p.h, n.Dpad, (int64_t)n.Npad * n.Dpad, (int)n.Npad, (int)a->D, p.ht, (int)n.Npad,
+                                                        (int64_t)n.Dpad * n.Npad, (int)n.parts, st)) != hipSuccess)
+    return e;
+  for (int64_t v0 = 0; v0 < a->V; v0 += n.piece) {
+    p.first = v0 == 0;
+    if ((e = set_piece(p, a, n, l, w, v0, st)) != hipSuccess || (e = osm::launch_loss_probs(p, st)) != hipSuccess) return e;
+    if (b->grad_hidden &&
+        ((e = osm::launch_loss_transpose(p.w, p.w_ld, p.w_part, p.vn, (int)a->D, p.wt, p.vpad, (int64_t)n.Dpad * p.vpad, (int)n.parts,
+                                         st)) != hipSuccess ||
+         (e = osm::launch_loss_dh(p, st)) != hipSuccess))
+      return e;
+    if (b->grad_weight && (e = osm::launch_loss_dw(p, a->dtype, st)) != hipSuccess) return e;
+  }
+  return b->grad_hidden ? osm::launch_loss_finish(p, a->dtype, st) : hipSuccess;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t osm_linear_ce_workspace_bytes(const osm_loss_args* a) {
+  return check_args(a) == OSM_OK && a->N > 0 ? layout_of(a, plan_of(a, false), false).total : 0;
+}
+
+int osm_linear_ce_fwd(const osm_loss_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_args(a);
+  if (rc != OSM_OK) return rc;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if ((uintptr_t)a->losses % 4 || (uintptr_t)a->total % 4) return fail(OSM_E_LAYOUT, "losses and total must be 4-byte aligned");
+  if (a->total && !a->losses && a->N > 0) return fail(OSM_E_ARG, "total without losses");
+  if (a->N == 0) {
+    if (!a->total) return ok();
+    osm::LossParams p{};
+    p.total = a->total;
+    return hip_rc(osm::launch_loss_total(p, st));
+  }
+  if ((rc = check_inputs(a)) != OSM_OK) return rc;
+  const Plan n = plan_of(a, false);
+  const Layout l = layout_of(a, n, false);
+  if ((rc = check_workspace(workspace, workspace_bytes, l.total)) != OSM_OK) return rc;
+  return hip_rc(forward(a, n, l, workspace, st));
+}
+
+size_t osm_linear_ce_bwd_workspace_bytes(const osm_loss_args* a) {
+  return check_args(a) == OSM_OK && a->N > 0 ? layout_of(a, plan_of(a, true), true).total : 0;
+}
+
+int osm_linear_ce_bwd(const osm_loss_args* a, const osm_loss_bwd_args* b, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_args(a);
+  if (rc != OSM_OK) return rc;
+  if (!b) return fail(OSM_E_ARG, "bwd is NULL");
+  const void* words[3] = {b->grad, b->grad_losses, b->total};
+  for (const void* w : words)
+    if ((uintptr_t)w % 4) return fail(OSM_E_LAYOUT, "grad, grad_losses and total must be 4-byte aligned");
+  // (rows of whole 4-element units are written by them)
+  const int es = a->dtype == OSM_F32 ? 4 : 2, unit = a->D % 4 == 0 ? 4 * es : es;
+  if ((uintptr_t)b->grad_hidden % unit || (uintptr_t)b->grad_weight % unit)
+    return fail(OSM_E_LAYOUT, "grad_hidden and grad_weight must be aligned to %d bytes", unit);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (a->N == 0)
+    return b->grad_weight ? hip_rc(osm::launch_loss_zero(b->grad_weight, a->V * a->D, a->dtype, st)) : ok();
+  if ((rc = check_inputs(a)) != OSM_OK) return rc;
+  const Plan n = plan_of(a, true);
+  const Layout l = layout_of(a, n, true);
+  if ((rc = check_workspace(workspace, workspace_bytes, l.total)) != OSM_OK) return rc;
+  return hip_rc(backward(a, b, n, l, workspace, st));
+}
+
+}  // extern "C"
