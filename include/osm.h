@@ -564,8 +564,11 @@ typedef struct osm_resnorm_bwd_args {
  * [0, V) gives NaN (the loss, and every gradient that the token has a part in).
  * Products are at fp32's accuracy for fp32 inputs (three bf16 parts an operand) and
  * exact for bf16 ones, sums in fp32.  No counterpart in the reference. */
+#define OSM_LOSS_MEAN 0x1
+
 typedef struct osm_loss_args {
   int32_t abi_version;          /* = OSM_ABI_VERSION */
+  int32_t flags;
   int32_t dtype;                /* osm_dtype of hidden, weight and their gradients */
   int64_t N, D, V;
   const void* hidden;           /* [N,D], rows a stride apart, elements contiguous */
@@ -577,13 +580,14 @@ typedef struct osm_loss_args {
   float* losses;                /* [N], or NULL */
   float* lse;                   /* [N]: log sum exp of each token that counts (0 of the others); written by the
                                  * forward, read by the backward */
-  float* total;                 /* [2], or NULL: the sum of the losses, and the tokens that count (at least 1) */
+  float* loss;                  /* device scalar, or NULL: the sum of the losses; with OSM_LOSS_MEAN divided by *count */
+  float* count;                 /* device scalar, or NULL: the tokens that count, at least 1 */
 } osm_loss_args;
 
 typedef struct osm_loss_bwd_args {
-  const float* grad;            /* device scalar: the gradient of each token's loss, divided by total[1] if that is given */
-  const float* grad_losses;     /* [N], or NULL: further factors by token */
-  const float* total;           /* what the forward wrote, or NULL */
+  const float* grad;            /* device scalar, or NULL (1): the gradient of every token's loss, */
+  const float* count;           /* device scalar, or NULL (1): divided by this */
+  const float* grad_losses;     /* [N], or NULL: and times its token's */
   void* grad_hidden;            /* [N,D] contiguous, or NULL */
   void* grad_weight;            /* [V,D] contiguous, or NULL */
 } osm_loss_bwd_args;
@@ -737,7 +741,8 @@ int osm_residual_norm_bwd(const osm_resnorm_args* args, const osm_resnorm_bwd_ar
                           size_t workspace_bytes, void* stream);
 
 /* The cross entropy and its backward (from hidden, weight, targets and lse; losses
- * and total of `args` are not used).  Workspaces as above.  The backward forms the
+, loss and
+ * count of `args` are not used).  Workspaces as above.  The backward forms the
  * probabilities of a piece of the vocabulary at a time. */
 size_t osm_linear_ce_workspace_bytes(const osm_loss_args* args);
 int osm_linear_ce_fwd(const osm_loss_args* args, void* workspace, size_t workspace_bytes, void* stream);

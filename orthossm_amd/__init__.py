@@ -18,8 +18,8 @@ from .delta import gated_delta, gated_delta_backward, gated_delta_forward, gated
 from .norm import layer_norm, layer_norm_backward, layer_norm_forward
 from .grad_clip import clip_grad_norm, grad_norm
 from .delta_layer import GatedDeltaLayer
-from .gated_ema import gated_ema, gated_ema_backward, gated_ema_forward, gated_ema_step
-from .residual_norm import residual_norm, residual_norm_backward, residual_norm_forward
+from .ema import gated_ema, gated_ema_backward, gated_ema_forward, gated_ema_step
+from .block_norm import residual_norm, residual_norm_backward, residual_norm_forward
 from .linear_loss import linear_cross_entropy, linear_cross_entropy_backward, linear_cross_entropy_forward
 
 __all__ = ["cheby_ema", "cheby_ema_forward", "cheby_ema_backward", "cheby_ema_ttt", "apply_cheby_rkv_v10",

@@ -42,6 +42,7 @@ DELTA_MAX_STRIDE = 1 << 22   # elements from token to token
 CLIP_SCALE = 0x1
 RESNORM_NORM_Y = 0x1
 RESNORM_RMS = 0x2
+LOSS_MEAN = 0x1
 
 STATUS = {
     0: "OSM_OK",
@@ -541,6 +542,7 @@ class LossArgs(ctypes.Structure):
 
     _fields_ = [
         ("abi_version", ctypes.c_int32),
+        ("flags", ctypes.c_int32),
         ("dtype", ctypes.c_int32),
         ("N", ctypes.c_int64),
         ("D", ctypes.c_int64),
@@ -553,7 +555,8 @@ class LossArgs(ctypes.Structure):
         ("ignore_index", ctypes.c_int64),
         ("losses", ctypes.c_void_p),
         ("lse", ctypes.c_void_p),
-        ("total", ctypes.c_void_p),
+        ("loss", ctypes.c_void_p),
+        ("count", ctypes.c_void_p),
     ]
 
 
@@ -562,8 +565,8 @@ class LossBwdArgs(ctypes.Structure):
 
     _fields_ = [
         ("grad", ctypes.c_void_p),
+        ("count", ctypes.c_void_p),
         ("grad_losses", ctypes.c_void_p),
-        ("total", ctypes.c_void_p),
         ("grad_hidden", ctypes.c_void_p),
         ("grad_weight", ctypes.c_void_p),
     ]
@@ -717,7 +720,12 @@ EXT_FUNCTIONS = ("osm_workspace_bytes", "osm_cheby_ema_fwd", "osm_cheby_ema_ttt"
                  "osm_engine_scratch_bytes", "osm_engine_prologue", "hipStreamIsCapturing", "osm_delta_saved_bytes",
                  "osm_delta_workspace_bytes", "osm_delta_fwd", "osm_delta_bwd_workspace_bytes", "osm_delta_bwd",
                  "osm_delta_step", "osm_layer_norm_fwd", "osm_layer_norm_bwd_workspace_bytes", "osm_layer_norm_bwd",
-                 "osm_clip_workspace_bytes", "osm_clip_grad_norm")
+                 "osm_clip_workspace_bytes", "osm_clip_grad_norm",
+                 "osm_gated_ema_saved_bytes", "osm_gated_ema_workspace_bytes", "osm_gated_ema_fwd",
+                 "osm_gated_ema_bwd_workspace_bytes", "osm_gated_ema_bwd", "osm_gated_ema_step",
+                 "osm_residual_norm_fwd", "osm_residual_norm_bwd_workspace_bytes", "osm_residual_norm_bwd",
+                 "osm_linear_ce_workspace_bytes", "osm_linear_ce_fwd", "osm_linear_ce_bwd_workspace_bytes",
+                 "osm_linear_ce_bwd")
 
 
 def check(rc: int) -> None:

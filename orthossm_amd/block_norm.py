@@ -35,6 +35,10 @@ from .ops import _current_stream, _dtype_code, _fast
 _TYPES = (torch.float32, torch.bfloat16)
 
 
+def _flags(norm_y, rms) -> int:
+    return (nat.RESNORM_NORM_Y if norm_y else 0) | (nat.RESNORM_RMS if rms else 0)
+
+
 def _prepare(x, y, gate, scale, weight, bias, norm_y, rms, eps):
     if not isinstance(x, torch.Tensor) or x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError("x must be a [..., D] tensor with D >= 1")
@@ -54,7 +58,7 @@ def _prepare(x, y, gate, scale, weight, bias, norm_y, rms, eps):
     mx, my, mg = _matrix(x), _matrix(y), None if gate is None else _matrix(gate)
     a = nat.ResnormArgs()
     a.abi_version = nat.ABI_VERSION
-    a.flags = (nat.RESNORM_NORM_Y if norm_y else 0) | (nat.RESNORM_RMS if rms else 0)
+    a.flags = _flags(norm_y, rms)
     a.stream_dtype, a.block_dtype = _dtype_code(x.dtype), _dtype_code(y.dtype)
     a.rows, a.D, a.eps = mx.shape[0], D, float(eps)
     a.x, a.x_stride = mx.data_ptr(), mx.stride(0)
@@ -159,6 +163,11 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, weight: torch.Tensor | None 
                   rms: bool = False, eps: float = 1e-5):
     """(r, n): the residual stream after a block's output y, and its norm,
     differentiable in x, y, gate, scale, weight and bias."""
+    fast = _fast()
+    if fast is not None:
+        res = fast.residual_norm(x, y, gate, scale, weight, bias, _flags(norm_y, rms), eps)
+        if res is not None:
+            return res
     if differentiable(x, y, gate, scale, weight, bias):
         return _ResidualNormFunction.apply(x, y, gate, scale, weight, bias, bool(norm_y), bool(rms), eps)
     return _forward(x, y, gate, scale, weight, bias, norm_y, rms, eps, False)[:2]

@@ -12,7 +12,7 @@ constexpr int kLossPad = 256;      // rows of compacted tokens, columns of a pie
 struct LossTokens {
   int* rows;                       // [N]: the token of each place
   int* places;                     // [N]: the place of each token, -1: does not count
-  int* count;                      // device scalar
+  int* count;                      // [2]: how many; a counter of the join's
 };
 
 struct LossParams {
@@ -25,8 +25,8 @@ struct LossParams {
   const int64_t* targets;
   int64_t ignore;
   LossTokens tok;
-  __bf16* h;                       // [parts][Npad][Dpad]: the hidden rows that count, zeros after them
-  __bf16* ht;                      // [parts][Dpad][Npad]: the same by column
+  __bf16* h;                       // [parts][Npad][Dpad]: the hidden rows that count (nothing is written after them)
+  __bf16* ht;                      // [parts][Dpad][Npad]: the same by column, zeros after them up to a whole step
   // a piece of the vocabulary
   int64_t v0;
   int vn, vpad;                    // its classes; columns of p
@@ -41,20 +41,20 @@ struct LossParams {
   float2* stat;                    // [tiles of the vocabulary][Npad]: largest logit, sum of exp of what is below it
   int tile0;                       // the piece's first tile
   float* own;                      // [Npad]: the target's logit
-  float *losses, *lse, *total;
-  const float *grad, *grad_losses, *total_in;
+  float *losses, *lse, *loss, *count;
+  int mean;
+  const float *grad, *grad_losses, *count_in;
   void *grad_h, *grad_w;
 };
 
-hipError_t launch_loss_tokens(const LossParams& p, hipStream_t stream);                     // tok
-hipError_t launch_loss_rows(const LossParams& p, int dtype, hipStream_t stream);            // h
+hipError_t launch_loss_rows(const LossParams& p, int dtype, hipStream_t stream);            // tok, h
 hipError_t launch_loss_weight(const LossParams& p, __bf16* to, int dtype, hipStream_t stream);   // parts of the piece's rows
-hipError_t launch_loss_transpose(const __bf16* from, int64_t ld, int64_t from_part, int rows, int cols, __bf16* to, int to_ld,
-                                 int64_t to_part, int parts, hipStream_t stream);
+hipError_t launch_loss_transpose(const __bf16* from, int64_t ld, int64_t from_part, int rows, const int* count, int cols, __bf16* to,
+                                 int to_ld, int64_t to_part, int parts, hipStream_t stream);
 int loss_tile_rows(const LossParams& p);                                                    // classes of a tile of the logits
 hipError_t launch_loss_logits(const LossParams& p, hipStream_t stream);                     // stat, own
-hipError_t launch_loss_join(const LossParams& p, int tiles, hipStream_t stream);            // losses, lse
-hipError_t launch_loss_total(const LossParams& p, hipStream_t stream);
+hipError_t launch_loss_join(const LossParams& p, int tiles, hipStream_t stream);            // losses, lse, loss, count
+hipError_t launch_loss_none(float* loss, float* count, hipStream_t stream);
 hipError_t launch_loss_probs(const LossParams& p, hipStream_t stream);                      // p, pt
 hipError_t launch_loss_dh(const LossParams& p, hipStream_t stream);
 hipError_t launch_loss_dw(const LossParams& p, int dtype, hipStream_t stream);

@@ -27,35 +27,6 @@ constexpr float kLog2e = 1.44269504f, kInf = __builtin_inff();
 
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
-// ---- the tokens that count ----
-
-constexpr int kScanThreads = 1024;
-
-// One workgroup over all targets, in order.
-__global__ void __launch_bounds__(kScanThreads) loss_tokens_kernel(const LossParams p) {
-  __shared__ int sums[kScanThreads / 64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int base = 0;
-  for (int64_t i0 = 0; i0 < p.N; i0 += kScanThreads) {
-    const int64_t i = i0 + threadIdx.x;
-    const bool in = i < p.N && p.targets[i] != p.ignore;
-    const unsigned long long mask = __ballot(in);
-    if (lane == 0) sums[wave] = __popcll(mask);
-    __syncthreads();
-    int before = base;
-    for (int w = 0; w < kScanThreads / 64; ++w) {
-      const int s = sums[w];
-      if (w < wave) before += s;
-      base += s;
-    }
-    const int at = before + __popcll(mask & ((1ull << lane) - 1));
-    if (in) p.tok.rows[at] = (int)i;
-    if (i < p.N) p.tok.places[i] = in ? at : -1;
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) *p.tok.count = base;
-}
-
 // ---- operands ----
 
 // The bf16 parts of x: part k is what rounding leaves of the parts before it.
@@ -68,28 +39,99 @@ __device__ __forceinline__ void split(float x, __bf16 (&to)[PARTS]) {
   }
 }
 
-// Rows of `from` (with `rows`: those it names, zeros past *count) in units of 8
-// columns, zeros past the D-th, to [PARTS][n][ld].
+// 8 columns from c on of a row of D, zeros past them, as parts.
 template <typename T, int PARTS>
-__global__ void __launch_bounds__(256) loss_pack_kernel(const T* from, int64_t stride, int D, int64_t n, int ld, const int* rows,
-                                                        const int* count, __bf16* to) {
+__device__ __forceinline__ void split_unit(const T* row, int c, int D, bool vec, bf16x8 (&out)[PARTS]) {
+  typedef T V8 __attribute__((ext_vector_type(8)));
+  V8 v = {};
+  if (vec) {   // (rows of whole units at multiples of 16 bytes)
+    if (c < D) v = *reinterpret_cast<const V8*>(row + c);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (c + k < D) v[k] = row[c + k];
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    __bf16 s[PARTS];
+    split<PARTS>((float)v[k], s);
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q) out[q][k] = s[q];
+  }
+}
+
+template <typename T>
+bool whole_units(const void* p, int64_t stride, int64_t D) {
+  return (uintptr_t)p % 16 == 0 && stride * sizeof(T) % 16 == 0 && D % 8 == 0;
+}
+
+// The tokens that count, one after the other: a block takes `each` tokens, counts those
+// before them, and writes where its own go, and their hidden rows.
+template <typename T, int PARTS>
+__global__ void __launch_bounds__(256) loss_rows_kernel(const LossParams p, int64_t each, bool vec) {
+  __shared__ int sums[4];
+  __shared__ int rows[256];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  auto in_order = [&](bool in, int& base) {   // this thread's place from `base` on; base: after all of them
+    const unsigned long long mask = __ballot(in);
+    __syncthreads();
+    if (lane == 0) sums[wave] = __popcll(mask);
+    __syncthreads();
+    int at = base + __popcll(mask & ((1ull << lane) - 1));
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) at += sums[w];
+      base += sums[w];
+    }
+    return at;
+  };
+  const int64_t t0 = blockIdx.x * each, t1 = min(t0 + each, p.N);
+  int before = 0;
+  for (int64_t i = threadIdx.x; i < t0; i += 256) before += p.targets[i] != p.ignore;
+#pragma unroll
+  for (int w = 32; w > 0; w >>= 1) before += __shfl_xor(before, w);
+  if (lane == 0) sums[wave] = before;
+  __syncthreads();
+  int base = sums[0] + sums[1] + sums[2] + sums[3];
+  const int units = p.Dpad / 8;
+  for (int64_t i0 = t0; i0 < t1; i0 += 256) {
+    const int64_t i = i0 + threadIdx.x;
+    const bool in = i < t1 && p.targets[i] != p.ignore;
+    const int first = base, at = in_order(in, base);
+    if (in) {
+      p.tok.rows[at] = (int)i;
+      rows[at - first] = (int)i;
+    }
+    if (i < t1) p.tok.places[i] = in ? at : -1;
+    __syncthreads();
+    const int n = base - first;
+    for (int u = threadIdx.x; u < n * units; u += 256) {
+      const int r = u / units, c = u - r * units;
+      bf16x8 out[PARTS];
+      split_unit<T, PARTS>(static_cast<const T*>(p.hidden) + rows[r] * p.hidden_s, 8 * c, (int)p.D, vec, out);
+#pragma unroll
+      for (int q = 0; q < PARTS; ++q) {
+        *reinterpret_cast<bf16x8*>(p.h + ((int64_t)q * p.Npad + first + r) * p.Dpad + 8 * c) = out[q];
+        wide_store_wait();
+      }
+    }
+  }
+  if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) {
+    p.tok.count[0] = base;
+    p.tok.count[1] = 0;   // blocks of the join that are done
+  }
+}
+
+// Rows of weights to [PARTS][n][ld].
+template <typename T, int PARTS>
+__global__ void __launch_bounds__(256) loss_pack_kernel(const T* from, int64_t stride, int D, int64_t n, int ld, bool vec, __bf16* to) {
   const int units = ld / 8;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= n * units) return;
   const int64_t r = i / units;
   const int c = (int)(i - r * units) * 8;
-  bf16x8 out[PARTS] = {};
-  if (!rows || r < *count) {
-    const T* const src = from + (rows ? rows[r] : r) * stride + c;
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (c + k < D) {
-        __bf16 s[PARTS];
-        split<PARTS>((float)src[k], s);
-#pragma unroll
-        for (int q = 0; q < PARTS; ++q) out[q][k] = s[q];
-      }
-  }
+  bf16x8 out[PARTS];
+  split_unit<T, PARTS>(from + r * stride, c, D, vec, out);
 #pragma unroll
   for (int q = 0; q < PARTS; ++q) {
     *reinterpret_cast<bf16x8*>(to + ((int64_t)q * n + r) * ld + c) = out[q];
@@ -98,10 +140,14 @@ __global__ void __launch_bounds__(256) loss_pack_kernel(const T* from, int64_t s
 }
 
 // 64 x 64 of a matrix by its columns: to[c][r] = from[r][c], zeros for r past `rows`
-// (up to to_ld).
-__global__ void __launch_bounds__(256) loss_transpose_kernel(const __bf16* from, int64_t ld, int64_t from_part, int rows, int cols,
-                                                             __bf16* to, int to_ld, int64_t to_part) {
+// (with `count`: past that), up to to_ld.
+__global__ void __launch_bounds__(256) loss_transpose_kernel(const __bf16* from, int64_t ld, int64_t from_part, int rows,
+                                                             const int* count, int cols, __bf16* to, int to_ld, int64_t to_part) {
   __shared__ __bf16 t[64][66];
+  if (count) {
+    rows = *count;
+    if ((int)blockIdx.x * 64 >= rows) return;   // (nothing reads past the last step that holds a row)
+  }
   from += blockIdx.z * from_part;
   to += blockIdx.z * to_part;
   const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
@@ -302,7 +348,7 @@ __global__ void __launch_bounds__(G::kThreads) loss_dh_kernel(const LossParams p
 }
 
 __device__ __forceinline__ float factor(const LossParams& p) {
-  return (p.grad ? *p.grad : 1.0f) / (p.total_in ? p.total_in[1] : 1.0f);
+  return (p.grad ? *p.grad : 1.0f) / (p.count_in ? *p.count_in : 1.0f);
 }
 
 // dW of a piece: A the hidden rows by column, B P by classes.
@@ -349,55 +395,68 @@ __global__ void __launch_bounds__(G::kThreads) loss_dw_kernel(const LossParams p
 
 constexpr int kJoinTokens = 16, kJoinSlices = 16;
 
-// A place's statistics over the vocabulary's tiles, 16 threads a place.
+// A token's statistics over the vocabulary's tiles, 16 threads a token; zeros of those
+// that do not count.  With `loss`: the block that is done last adds the losses, in double
+// and in an order that does not depend on timing.
 __global__ void __launch_bounds__(kJoinTokens * kJoinSlices) loss_join_kernel(const LossParams p, int tiles) {
   __shared__ float2 red[kJoinSlices][kJoinTokens];
-  const int c = threadIdx.x % kJoinTokens, s = threadIdx.x / kJoinTokens, at = blockIdx.x * kJoinTokens + c;
-  if (blockIdx.x * kJoinTokens >= *p.tok.count) return;
+  const int c = threadIdx.x % kJoinTokens, s = threadIdx.x / kJoinTokens;
+  const int64_t token = (int64_t)blockIdx.x * kJoinTokens + c;
+  const int at = token < p.N ? p.tok.places[token] : -1;
   float top = -kInf, sum = 0.0f;
-  for (int t = s; t < tiles; t += kJoinSlices) {
-    const float2 v = p.stat[(int64_t)t * p.Npad + at];
-    const float both = __builtin_fmaxf(top, v.x), b = both == -kInf ? 0.0f : both;
-    sum = sum * exp_of(top - b) + v.y * exp_of(v.x - b);
-    top = both;
-  }
+  if (at >= 0)
+    for (int t = s; t < tiles; t += kJoinSlices) {
+      const float2 v = p.stat[(int64_t)t * p.Npad + at];
+      const float both = __builtin_fmaxf(top, v.x), b = both == -kInf ? 0.0f : both;
+      sum = sum * exp_of(top - b) + v.y * exp_of(v.x - b);
+      top = both;
+    }
   red[s][c] = make_float2(top, sum);
   __syncthreads();
-  if (s > 0 || at >= *p.tok.count) return;
-  for (int k = 1; k < kJoinSlices; ++k) top = __builtin_fmaxf(top, red[k][c].x);
-  const float b = top == -kInf ? 0.0f : top;
-  sum = 0.0f;
-  for (int k = 0; k < kJoinSlices; ++k) sum += red[k][c].y * exp_of(red[k][c].x - b);
-  const int token = p.tok.rows[at];
-  const int64_t target = p.targets[token];
-  const bool known = target >= 0 && target < p.V;
-  const float l = logf(sum);
-  p.lse[token] = known ? b + l : __builtin_nanf("");
-  if (p.losses) p.losses[token] = known ? l - (p.own[at] - b) : __builtin_nanf("");
-}
-
-// Zeros of the tokens that do not count.
-__global__ void __launch_bounds__(256) loss_blank_kernel(const LossParams p) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= p.N || p.tok.places[i] >= 0) return;
-  p.lse[i] = 0.0f;
-  if (p.losses) p.losses[i] = 0.0f;
-}
-
-// The sum of the losses in double, one workgroup, in an order that does not depend on timing.
-__global__ void __launch_bounds__(1024) loss_total_kernel(const LossParams p) {
-  __shared__ double red[1024];
-  double s = 0.0;
-  for (int64_t i = threadIdx.x; i < p.N; i += 1024) s += p.losses[i];
-  red[threadIdx.x] = s;
-  for (int w = 512; w > 0; w >>= 1) {
+  if (s == 0 && token < p.N) {
+    float loss = 0.0f, lse = 0.0f;
+    if (at >= 0) {
+      for (int k = 1; k < kJoinSlices; ++k) top = __builtin_fmaxf(top, red[k][c].x);
+      const float b = top == -kInf ? 0.0f : top;
+      sum = 0.0f;
+      for (int k = 0; k < kJoinSlices; ++k) sum += red[k][c].y * exp_of(red[k][c].x - b);
+      const int64_t target = p.targets[token];
+      const bool known = target >= 0 && target < p.V;
+      const float l = logf(sum);
+      lse = known ? b + l : __builtin_nanf("");
+      loss = known ? l - (p.own[at] - b) : __builtin_nanf("");   // (small losses keep their digits)
+    }
+    p.lse[token] = lse;
+    if (p.losses) __hip_atomic_store(p.losses + token, loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if (!p.loss) return;
+  __shared__ int is_last;
+  __shared__ double part[kJoinTokens * kJoinSlices];
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) is_last = atomicAdd(p.tok.count + 1, 1) == (int)gridDim.x - 1;
+  __syncthreads();
+  if (!is_last) return;
+  __threadfence();
+  double d = 0.0;
+  for (int64_t i = threadIdx.x; i < p.N; i += kJoinTokens * kJoinSlices)
+    d += __hip_atomic_load(p.losses + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  part[threadIdx.x] = d;
+  for (int w = kJoinTokens * kJoinSlices / 2; w > 0; w >>= 1) {
     __syncthreads();
-    if ((int)threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
+    if ((int)threadIdx.x < w) part[threadIdx.x] += part[threadIdx.x + w];
   }
   if (threadIdx.x == 0) {
-    p.total[0] = (float)red[0];
-    p.total[1] = p.tok.count ? (float)max(*p.tok.count, 1) : 1.0f;
+    const float n = (float)max(p.tok.count[0], 1);
+    *p.loss = (float)(p.mean ? part[0] / n : part[0]);
+    if (p.count) *p.count = n;
   }
+}
+
+// The loss of no tokens.
+__global__ void loss_none_kernel(float* loss, float* count) {
+  if (loss) *loss = 0.0f;
+  if (count) *count = 1.0f;
 }
 
 // grad_h of every token from its place's sums, zeros where it does not count.
@@ -479,39 +538,38 @@ hipError_t logits(const LossParams& p, hipStream_t stream) {
 
 }  // namespace
 
-hipError_t launch_loss_tokens(const LossParams& p, hipStream_t stream) {
-  hipLaunchKernelGGL(loss_tokens_kernel, dim3(1), dim3(kScanThreads), 0, stream, p);
+hipError_t launch_loss_rows(const LossParams& p, int dtype, hipStream_t stream) {
+  // (blocks count what is before their tokens: at most 512 of them where there are many)
+  const int64_t each = std::max<int64_t>(16, (p.N + 511) / 512);
+  const dim3 grid((unsigned)((p.N + each - 1) / each));
+  if (dtype == 0)
+    hipLaunchKernelGGL((loss_rows_kernel<float, 3>), grid, dim3(256), 0, stream, p, each, whole_units<float>(p.hidden, p.hidden_s, p.D));
+  else
+    hipLaunchKernelGGL((loss_rows_kernel<__bf16, 1>), grid, dim3(256), 0, stream, p, each, whole_units<__bf16>(p.hidden, p.hidden_s, p.D));
   return hipGetLastError();
 }
 
 namespace {
 template <typename T, int PARTS>
-void pack(const void* from, int64_t stride, int64_t D, int64_t n, int ld, const int* rows, const int* count, __bf16* to, hipStream_t stream) {
-  hipLaunchKernelGGL((loss_pack_kernel<T, PARTS>), dim3((unsigned)((n * (ld / 8) + 255) / 256)), dim3(256), 0, stream,
-                     static_cast<const T*>(from), stride, (int)D, n, ld, rows, count, to);
+void pack(const LossParams& p, __bf16* to, hipStream_t stream) {
+  const T* const from = static_cast<const T*>(p.weight) + p.v0 * p.weight_s;
+  hipLaunchKernelGGL((loss_pack_kernel<T, PARTS>), dim3((unsigned)(((int64_t)p.vn * (p.Dpad / 8) + 255) / 256)), dim3(256), 0, stream, from,
+                     p.weight_s, (int)p.D, (int64_t)p.vn, p.Dpad, whole_units<T>(from, p.weight_s, p.D), to);
 }
 }  // namespace
 
-hipError_t launch_loss_rows(const LossParams& p, int dtype, hipStream_t stream) {
-  if (dtype == 0)
-    pack<float, 3>(p.hidden, p.hidden_s, p.D, p.Npad, p.Dpad, p.tok.rows, p.tok.count, p.h, stream);
-  else
-    pack<__bf16, 1>(p.hidden, p.hidden_s, p.D, p.Npad, p.Dpad, p.tok.rows, p.tok.count, p.h, stream);
-  return hipGetLastError();
-}
-
 hipError_t launch_loss_weight(const LossParams& p, __bf16* to, int dtype, hipStream_t stream) {
   if (dtype == 0)
-    pack<float, 3>(static_cast<const float*>(p.weight) + p.v0 * p.weight_s, p.weight_s, p.D, p.vn, p.Dpad, nullptr, nullptr, to, stream);
+    pack<float, 3>(p, to, stream);
   else
-    pack<__bf16, 1>(static_cast<const __bf16*>(p.weight) + p.v0 * p.weight_s, p.weight_s, p.D, p.vn, p.Dpad, nullptr, nullptr, to, stream);
+    pack<__bf16, 1>(p, to, stream);
   return hipGetLastError();
 }
 
-hipError_t launch_loss_transpose(const __bf16* from, int64_t ld, int64_t from_part, int rows, int cols, __bf16* to, int to_ld,
-                                 int64_t to_part, int parts, hipStream_t stream) {
+hipError_t launch_loss_transpose(const __bf16* from, int64_t ld, int64_t from_part, int rows, const int* count, int cols, __bf16* to,
+                                 int to_ld, int64_t to_part, int parts, hipStream_t stream) {
   hipLaunchKernelGGL(loss_transpose_kernel, dim3((unsigned)((to_ld + 63) / 64), (unsigned)((cols + 63) / 64), parts), dim3(256), 0, stream,
-                     from, ld, from_part, rows, cols, to, to_ld, to_part);
+                     from, ld, from_part, rows, count, cols, to, to_ld, to_part);
   return hipGetLastError();
 }
 
@@ -527,14 +585,11 @@ hipError_t launch_loss_probs(const LossParams& p, hipStream_t stream) { return l
 hipError_t launch_loss_join(const LossParams& p, int tiles, hipStream_t stream) {
   hipLaunchKernelGGL(loss_join_kernel, dim3((unsigned)((p.N + kJoinTokens - 1) / kJoinTokens)), dim3(kJoinTokens * kJoinSlices), 0, stream,
                      p, tiles);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(loss_blank_kernel, dim3((unsigned)((p.N + 255) / 256)), dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 
-hipError_t launch_loss_total(const LossParams& p, hipStream_t stream) {
-  hipLaunchKernelGGL(loss_total_kernel, dim3(1), dim3(1024), 0, stream, p);
+hipError_t launch_loss_none(float* loss, float* count, hipStream_t stream) {
+  hipLaunchKernelGGL(loss_none_kernel, dim3(1), dim3(1), 0, stream, loss, count);
   return hipGetLastError();
 }
 

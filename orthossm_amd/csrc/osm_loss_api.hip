@@ -21,6 +21,7 @@ int check_args(const osm_loss_args* a) {
   if (!a) return fail(OSM_E_ARG, "args is NULL");
   if (a->abi_version != OSM_ABI_VERSION)
     return fail(OSM_E_ARG, "abi_version %d does not match library ABI %d", a->abi_version, OSM_ABI_VERSION);
+  if (a->flags & ~OSM_LOSS_MEAN) return fail(OSM_E_ARG, "unknown flag bits 0x%x", a->flags);
   if (a->dtype != OSM_F32 && a->dtype != OSM_BF16) return fail(OSM_E_DTYPE, "dtype %d unsupported", a->dtype);
   if (a->N < 0 || a->N > kMaxRow - kLossPad || a->D < 1 || a->D > (int64_t(1) << 17) || a->V < 1 || a->V > (int64_t(1) << 28))
     return fail(OSM_E_SHAPE, "N=%lld outside [0, 2^21 - 256], D=%lld outside [1, 2^17] or V=%lld outside [1, 2^28]", (long long)a->N,
@@ -97,7 +98,7 @@ Layout layout_of(const osm_loss_args* a, const Plan& n, bool bwd) {
   Layout l{};
   l.rows = r.add(a->N * 4);
   l.places = r.add(a->N * 4);
-  l.count = r.add(4);
+  l.count = r.add(8);
   const size_t hidden = (size_t)n.parts * n.Npad * n.Dpad * 2;
   l.h = r.add(hidden);
   l.w = r.add(n.direct ? 0 : (size_t)n.parts * n.piece * n.Dpad * 2);
@@ -168,16 +169,17 @@ hipError_t forward(const osm_loss_args* a, const Plan& n, const Layout& l, void*
   p.own = reinterpret_cast<float*>(w + l.own);
   p.stat = reinterpret_cast<float2*>(w + l.stat);
   p.losses = a->losses;
-  p.total = a->total;
-  hipError_t e;
-  if ((e = osm::launch_loss_tokens(p, st)) != hipSuccess || (e = osm::launch_loss_rows(p, a->dtype, st)) != hipSuccess) return e;
+  p.loss = a->loss;
+  p.count = a->count;
+  p.mean = (a->flags & OSM_LOSS_MEAN) != 0;
+  hipError_t e = osm::launch_loss_rows(p, a->dtype, st);
+  if (e != hipSuccess) return e;
   const int rows = osm::loss_tile_rows(p);
   for (int64_t v0 = 0; v0 < a->V; v0 += n.piece) {
     p.tile0 = (int)(v0 / rows);
     if ((e = set_piece(p, a, n, l, w, v0, st)) != hipSuccess || (e = osm::launch_loss_logits(p, st)) != hipSuccess) return e;
   }
-  if ((e = osm::launch_loss_join(p, (int)((a->V + rows - 1) / rows), st)) != hipSuccess) return e;
-  return a->total ? osm::launch_loss_total(p, st) : hipSuccess;
+  return osm::launch_loss_join(p, (int)((a->V + rows - 1) / rows), st);
 }
 
 hipError_t backward(const osm_loss_args* a, const osm_loss_bwd_args* b, const Plan& n, const Layout& l, void* workspace, hipStream_t st) {
@@ -191,19 +193,19 @@ hipError_t backward(const osm_loss_args* a, const osm_loss_bwd_args* b, const Pl
   p.splits = n.splits;
   p.grad = b->grad;
   p.grad_losses = b->grad_losses;
-  p.total_in = b->total;
+  p.count_in = b->count;
   p.grad_h = b->grad_hidden;
   p.grad_w = b->grad_weight;
-  hipError_t e;
-  if ((e = osm::launch_loss_tokens(p, st)) != hipSuccess || (e = osm::launch_loss_rows(p, a->dtype, st)) != hipSuccess) return e;
-  if (b->grad_weight && (e = osm::launch_loss_transpose(p.h, n.Dpad, (int64_t)n.Npad * n.Dpad, (int)n.Npad, (int)a->D, p.ht, (int)n.Npad,
-                                                        (int64_t)n.Dpad * n.Npad, (int)n.parts, st)) != hipSuccess)
+  hipError_t e = osm::launch_loss_rows(p, a->dtype, st);
+  if (e != hipSuccess) return e;
+  if (b->grad_weight && (e = osm::launch_loss_transpose(p.h, n.Dpad, (int64_t)n.Npad * n.Dpad, (int)n.Npad, p.tok.count, (int)a->D, p.ht,
+                                                        (int)n.Npad, (int64_t)n.Dpad * n.Npad, (int)n.parts, st)) != hipSuccess)
     return e;
   for (int64_t v0 = 0; v0 < a->V; v0 += n.piece) {
     p.first = v0 == 0;
     if ((e = set_piece(p, a, n, l, w, v0, st)) != hipSuccess || (e = osm::launch_loss_probs(p, st)) != hipSuccess) return e;
     if (b->grad_hidden &&
-        ((e = osm::launch_loss_transpose(p.w, p.w_ld, p.w_part, p.vn, (int)a->D, p.wt, p.vpad, (int64_t)n.Dpad * p.vpad, (int)n.parts,
+        ((e = osm::launch_loss_transpose(p.w, p.w_ld, p.w_part, p.vn, nullptr, (int)a->D, p.wt, p.vpad, (int64_t)n.Dpad * p.vpad, (int)n.parts,
                                          st)) != hipSuccess ||
          (e = osm::launch_loss_dh(p, st)) != hipSuccess))
       return e;
@@ -224,14 +226,11 @@ int osm_linear_ce_fwd(const osm_loss_args* a, void* workspace, size_t workspace_
   int rc = check_args(a);
   if (rc != OSM_OK) return rc;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if ((uintptr_t)a->losses % 4 || (uintptr_t)a->total % 4) return fail(OSM_E_LAYOUT, "losses and total must be 4-byte aligned");
-  if (a->total && !a->losses && a->N > 0) return fail(OSM_E_ARG, "total without losses");
-  if (a->N == 0) {
-    if (!a->total) return ok();
-    osm::LossParams p{};
-    p.total = a->total;
-    return hip_rc(osm::launch_loss_total(p, st));
-  }
+  const void* words[3] = {a->losses, a->loss, a->count};
+  for (const void* w : words)
+    if ((uintptr_t)w % 4) return fail(OSM_E_LAYOUT, "losses, loss and count must be 4-byte aligned");
+  if ((a->loss && !a->losses && a->N > 0) || (a->count && !a->loss)) return fail(OSM_E_ARG, "loss without losses, or count without loss");
+  if (a->N == 0) return a->loss ? hip_rc(osm::launch_loss_none(a->loss, a->count, st)) : ok();
   if ((rc = check_inputs(a)) != OSM_OK) return rc;
   const Plan n = plan_of(a, false);
   const Layout l = layout_of(a, n, false);
@@ -247,9 +246,9 @@ int osm_linear_ce_bwd(const osm_loss_args* a, const osm_loss_bwd_args* b, void* 
   int rc = check_args(a);
   if (rc != OSM_OK) return rc;
   if (!b) return fail(OSM_E_ARG, "bwd is NULL");
-  const void* words[3] = {b->grad, b->grad_losses, b->total};
+  const void* words[3] = {b->grad, b->grad_losses, b->count};
   for (const void* w : words)
-    if ((uintptr_t)w % 4) return fail(OSM_E_LAYOUT, "grad, grad_losses and total must be 4-byte aligned");
+    if ((uintptr_t)w % 4) return fail(OSM_E_LAYOUT, "grad, grad_losses and count must be 4-byte aligned");
   // (rows of whole 4-element units are written by them)
   const int es = a->dtype == OSM_F32 ? 4 : 2, unit = a->D % 4 == 0 ? 4 * es : es;
   if ((uintptr_t)b->grad_hidden % unit || (uintptr_t)b->grad_weight % unit)

@@ -53,8 +53,21 @@ struct Lib {
   decltype(&osm_layer_norm_bwd) norm_bwd;
   decltype(&osm_clip_workspace_bytes) clip_bytes;
   decltype(&osm_clip_grad_norm) clip;
+  decltype(&osm_gated_ema_saved_bytes) ema_saved;
+  decltype(&osm_gated_ema_workspace_bytes) ema_bytes;
+  decltype(&osm_gated_ema_fwd) ema_fwd;
+  decltype(&osm_gated_ema_bwd_workspace_bytes) ema_bwd_bytes;
+  decltype(&osm_gated_ema_bwd) ema_bwd;
+  decltype(&osm_gated_ema_step) ema_step;
+  decltype(&osm_residual_norm_fwd) block_fwd;
+  decltype(&osm_residual_norm_bwd_workspace_bytes) block_bwd_bytes;
+  decltype(&osm_residual_norm_bwd) block_bwd;
+  decltype(&osm_linear_ce_workspace_bytes) loss_bytes;
+  decltype(&osm_linear_ce_fwd) loss_fwd;
+  decltype(&osm_linear_ce_bwd_workspace_bytes) loss_bwd_bytes;
+  decltype(&osm_linear_ce_bwd) loss_bwd;
 } lib;
-constexpr int kFunctions = 22;
+constexpr int kFunctions = 35;
 PyObject* raw_stream = nullptr;   // device index -> raw stream handle
 PyObject* ws_cache = nullptr;     // {(device index, stream, op): uint8 tensor}
 PyObject* workspace = nullptr;    // (device, stream, bytes, op) -> uint8 tensor
@@ -1304,6 +1317,501 @@ PyObject* run_clip(PyObject* const* p) {
   return THPVariable_Wrap(norm);
 }
 
+// ---- gated EMA, residual norm, the vocabulary's cross entropy (orthossm_amd/ema.py,
+// block_norm.py, linear_loss.py): as above.
+
+osm_seq seq_of(const at::Tensor& t) { return {t.data_ptr(), t.stride(0), t.dim() == 3 ? t.stride(1) : 0}; }
+
+// Rows of contiguous elements that the kernels address, of one float type.
+bool ema_tensor(const at::Tensor& t, int64_t dim) {
+  if (!t.is_cuda() || !(is_f32(t) || is_bf16(t)) || t.dim() != dim || t.size(dim - 1) < 1 || (t.stride(dim - 1) != 1 && t.size(dim - 1) > 1))
+    return false;
+  for (int64_t i = 0; i < dim - 1; ++i)
+    if (t.stride(i) < 0) return false;
+  return true;
+}
+bool alike(const at::Tensor& t, const at::Tensor& x) {
+  return t.scalar_type() == x.scalar_type() && t.sizes() == x.sizes() && t.device() == x.device();
+}
+
+bool ema_lengths(const at::Tensor& t, const at::Tensor& x) {
+  return t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == x.size(0) && t.is_contiguous() && t.device() == x.device();
+}
+
+bool ema_state(const at::Tensor& t, const at::Tensor& x) {
+  return t.dim() == 2 && t.size(0) == x.size(0) && t.size(1) == x.size(2) && f32_flat(t, t.numel(), x);
+}
+
+void ema_args(const at::Tensor& x, const at::Tensor& gate, osm_ema_args* a) {
+  a->abi_version = OSM_ABI_VERSION;
+  a->dtype = code(x);
+  a->B = x.size(0);
+  a->S = x.size(1);
+  a->D = x.size(2);
+  a->x = seq_of(x);
+  a->gate = seq_of(gate);
+}
+
+// args: x, gate, lengths, state_init.
+bool ema_common(PyObject* const* p, osm_ema_args* a, const at::Tensor** x, const at::Tensor** gate) {
+  *x = plain(p[0]);
+  *gate = plain(p[1]);
+  if (!*x || !*gate || !ema_tensor(**x, 3) || !ema_tensor(**gate, 3) || !alike(**gate, **x)) return false;
+  ema_args(**x, **gate, a);
+  if (p[2] != Py_None) {
+    const at::Tensor* t = plain(p[2]);
+    if (!t || !ema_lengths(*t, **x)) return false;
+    a->lengths = static_cast<const int32_t*>(t->data_ptr());
+  }
+  if (p[3] != Py_None) {
+    const at::Tensor* t = plain(p[3]);
+    if (!t || !ema_state(*t, **x)) return false;
+    a->state_init = fptr(*t);
+  }
+  return true;
+}
+
+// The forward into new tensors, those of `fin` and `saved` where wanted.
+int ema_forward(osm_ema_args& a, const at::Tensor& x, bool want_state, bool save, void* stream, at::Tensor* out, at::Tensor* fin,
+                at::Tensor* saved) {
+  *out = empty(x.sizes(), x, x.scalar_type());
+  a.out = seq_of(*out);
+  if (want_state) {
+    *fin = empty({a.B, a.D}, x, at::kFloat);
+    a.state_out = fptr(*fin);
+  }
+  if (save) {
+    *saved = scratch(lib.ema_saved(&a), x);
+    a.saved = static_cast<float*>(saved->data_ptr());
+  }
+  const at::Tensor ws = scratch(lib.ema_bytes(&a), x);
+  return lib.ema_fwd(&a, ws.data_ptr(), (size_t)ws.numel(), stream);
+}
+
+// ema_forward(<common 4>, want_state): None, or (out, state | None).
+PyObject* run_ema_forward(PyObject* const* p) {
+  osm_ema_args a{};
+  const at::Tensor *x, *gate;
+  if (!ema_common(p, &a, &x, &gate)) Py_RETURN_NONE;
+  const bool want_state = PyObject_IsTrue(p[4]) == 1;
+  if (PyErr_Occurred()) return nullptr;
+  Ref s_obj;
+  void* stream;
+  const c10::DeviceGuard guard(x->device());
+  if (!stream_of(*x, &s_obj, &stream)) return nullptr;
+  at::Tensor out, fin, saved;
+  int rc;
+  {
+    const NoGil nogil;
+    rc = ema_forward(a, *x, want_state, false, stream, &out, &fin, &saved);
+  }
+  if (rc != OSM_OK) return fail_rc(rc);
+  return Py_BuildValue("(NN)", THPVariable_Wrap(out), wrap_or_none(fin));
+}
+
+struct EmaCall {
+  osm_ema_args* a;
+  void* stream;
+  int rc;
+};
+struct EmaGrad : torch::autograd::Function<EmaGrad> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& gate,
+                                                const std::optional<at::Tensor>& init, const std::optional<at::Tensor>& lengths,
+                                                EmaCall* c) {
+    ctx->set_materialize_grads(false);   // an unused output's gradient stays undefined
+    at::Tensor out, fin, saved;
+    c->rc = ema_forward(*c->a, x, true, true, c->stream, &out, &fin, &saved);
+    ctx->save_for_backward({x, gate, lengths ? *lengths : at::Tensor(), saved});
+    ctx->saved_data["need"] =
+        (int64_t)(x.requires_grad() | gate.requires_grad() << 1 | (init && init->requires_grad()) << 2);
+    return {out, fin};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto t = ctx->get_saved_variables();
+    const int64_t need = ctx->saved_data["need"].toInt();
+    at::Tensor gr[3];
+    {
+      const at::NoGradGuard no_grad;
+      const at::Tensor &x = t[0], &saved = t[3];
+      TORCH_CHECK(ema_tensor(x, 3) && ema_tensor(t[1], 3) && alike(t[1], x) && (!t[2].defined() || ema_lengths(t[2], x)), kAnotherForm,
+                  "gated_ema");
+      osm_ema_args a{};
+      ema_args(x, t[1], &a);
+      TORCH_CHECK(saved.scalar_type() == at::kByte && (size_t)saved.numel() == lib.ema_saved(&a) && saved.is_contiguous() &&
+                      saved.device() == x.device(),
+                  kAnotherForm, "gated_ema");
+      if (t[2].defined()) a.lengths = static_cast<const int32_t*>(t[2].data_ptr());
+      a.saved = static_cast<float*>(saved.data_ptr());
+      const c10::DeviceGuard guard(x.device());
+      at::Tensor go = grads[0].defined() ? grads[0] : at::zeros_like(x);
+      if (!ema_tensor(go, 3) || !alike(go, x)) go = go.to(x.options()).contiguous();
+      const at::Tensor gs = grads[1].defined() ? grads[1].to(at::kFloat).contiguous() : at::Tensor();
+      TORCH_CHECK(ema_tensor(go, 3) && alike(go, x) && (!gs.defined() || ema_state(gs, x)), kAnotherForm, "gated_ema");
+      osm_ema_bwd_args b{};
+      b.grad_out = seq_of(go);
+      if (gs.defined()) b.grad_state = fptr(gs);
+      for (int i = 0; i < 2; ++i) gr[i] = empty(x.sizes(), x, x.scalar_type());
+      b.grad_x = seq_of(gr[0]);
+      b.grad_gate = seq_of(gr[1]);
+      if (need & 4) {
+        gr[2] = empty({a.B, a.D}, x, at::kFloat);
+        b.grad_init = fptr(gr[2]);
+      }
+      const at::Tensor ws = scratch(lib.ema_bwd_bytes(&a), x);
+      throw_rc(lib.ema_bwd(&a, &b, ws.data_ptr(), (size_t)ws.numel(), engine_stream(x)));
+    }
+    torch::autograd::variable_list res(5);
+    for (int i = 0; i < 3; ++i)
+      if (need >> i & 1) res[i] = gr[i];
+    return once(std::move(res), {grads[0], grads[1], t[0], t[1]});
+  }
+};
+
+// gated_ema(<common 4>): None, or (out, state) with their gradient's function; without one (out, state).
+PyObject* run_gated_ema(PyObject* const* p) {
+  osm_ema_args a{};
+  const at::Tensor *x, *gate;
+  if (!ema_common(p, &a, &x, &gate)) Py_RETURN_NONE;
+  const std::optional<at::Tensor> lengths = optional_tensor(p[2]), init = optional_tensor(p[3]);
+  if (has_tangent(*x) || has_tangent(*gate) || (init && has_tangent(*init))) Py_RETURN_NONE;
+  Ref s_obj;
+  void* stream;
+  const c10::DeviceGuard guard(x->device());
+  if (!stream_of(*x, &s_obj, &stream)) return nullptr;
+  const bool grad = x->requires_grad() || gate->requires_grad() || (init && init->requires_grad());
+  at::Tensor out, fin, saved;
+  int rc;
+  {
+    const NoGil nogil;
+    if (grad && at::GradMode::is_enabled()) {
+      EmaCall c{&a, stream, OSM_OK};
+      const torch::autograd::variable_list res = EmaGrad::apply(*x, *gate, init, lengths, &c);
+      out = res[0];
+      fin = res[1];
+      rc = c.rc;
+    } else {
+      rc = ema_forward(a, *x, true, false, stream, &out, &fin, &saved);
+    }
+  }
+  if (rc != OSM_OK) return fail_rc(rc);
+  return Py_BuildValue("(NN)", THPVariable_Wrap(out), THPVariable_Wrap(fin));
+}
+
+// ema_step(x, gate, state, slots): None, or out.
+PyObject* run_ema_step(PyObject* const* p) {
+  const at::Tensor *x = plain(p[0]), *gate = plain(p[1]), *state = plain(p[2]);
+  if (!x || !gate || !state || !ema_tensor(*x, 2) || !ema_tensor(*gate, 2) || !alike(*gate, *x) || state->dim() != 2 || !is_f32(*state) ||
+      state->device() != x->device() || state->size(1) != x->size(1) || (state->stride(1) != 1 && state->size(1) > 1) ||
+      state->stride(0) < state->size(1) || state->requires_grad())
+    Py_RETURN_NONE;
+  osm_ema_step_args a{};
+  a.abi_version = OSM_ABI_VERSION;
+  a.dtype = code(*x);
+  a.B = x->size(0);
+  a.D = x->size(1);
+  a.x = seq_of(*x);
+  a.gate = seq_of(*gate);
+  a.state = fptr(*state);
+  a.state_stride = state->stride(0);
+  a.n_slots = state->size(0);
+  if (p[3] == Py_None) {
+    if (a.n_slots < a.B) Py_RETURN_NONE;
+  } else {
+    const at::Tensor* s = plain(p[3]);
+    if (!s || s->scalar_type() != at::kLong || s->dim() != 1 || s->size(0) != a.B || !s->is_contiguous() || s->device() != x->device())
+      Py_RETURN_NONE;
+    a.slots = static_cast<const int64_t*>(s->data_ptr());
+  }
+  Ref s_obj;
+  void* stream;
+  const c10::DeviceGuard guard(x->device());
+  if (!stream_of(*x, &s_obj, &stream)) return nullptr;
+  at::Tensor out;
+  int rc;
+  {
+    const NoGil nogil;
+    out = empty({a.B, a.D}, *x, x->scalar_type());
+    a.out = seq_of(out);
+    rc = lib.ema_step(&a, stream);
+  }
+  if (rc != OSM_OK) return fail_rc(rc);
+  written(*state);
+  return THPVariable_Wrap(out);
+}
+
+// The residual norm's tensors: x, y, gate (or none), scale, weight, bias (or none).
+struct Block {
+  const at::Tensor* t[6];
+  osm_resnorm_args a{};
+};
+
+bool block_tensors(Block* k) {
+  const at::Tensor *const xp = k->t[0], *const yp = k->t[1], *const gp = k->t[2];
+  if (!norm_rows(xp) || !norm_rows(yp) || yp->sizes() != xp->sizes() || yp->device() != xp->device() || (is_f32(*yp) && !is_f32(*xp)) ||
+      (gp && (!norm_rows(gp) || !alike(*gp, *yp))))
+    return false;
+  osm_resnorm_args& a = k->a;
+  a.abi_version = OSM_ABI_VERSION;
+  a.stream_dtype = code(*xp);
+  a.block_dtype = code(*yp);
+  a.D = xp->size(xp->dim() - 1);
+  a.rows = xp->numel() / a.D;
+  a.x = xp->data_ptr();
+  a.y = yp->data_ptr();
+  a.gate = gp ? gp->data_ptr() : nullptr;
+  a.x_stride = a.y_stride = a.gate_stride = a.D;
+  const float** to[3] = {&a.scale, &a.weight, &a.bias};
+  for (int i = 0; i < 3; ++i) {
+    const at::Tensor* w = k->t[3 + i];
+    if (!w) continue;
+    if (!f32_vec(w, a.D, *xp)) return false;
+    *to[i] = fptr(*w);
+  }
+  return true;
+}
+
+at::DimVector stats_size(const at::Tensor& x) {
+  at::DimVector s(x.sizes().begin(), x.sizes().end());
+  s.back() = 4;
+  return s;
+}
+
+int block_forward(Block& k, bool stats, void* stream, at::Tensor* r, at::Tensor* n, at::Tensor* st) {
+  const at::Tensor &x = *k.t[0], &y = *k.t[1];
+  *r = empty(x.sizes(), x, x.scalar_type());
+  *n = empty(x.sizes(), x, y.scalar_type());
+  k.a.r = r->data_ptr();
+  k.a.n = n->data_ptr();
+  k.a.r_stride = k.a.n_stride = k.a.D;
+  if (stats) {
+    *st = empty(stats_size(x), x, at::kFloat);
+    k.a.stats = fptr(*st);
+  }
+  return lib.block_fwd(&k.a, stream);
+}
+
+struct BlockCall {
+  Block* k;
+  void* stream;
+  int rc;
+};
+struct BlockGrad : torch::autograd::Function<BlockGrad> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& y,
+                                                const std::optional<at::Tensor>& gate, const std::optional<at::Tensor>& scale,
+                                                const std::optional<at::Tensor>& weight, const std::optional<at::Tensor>& bias,
+                                                BlockCall* c) {
+    ctx->set_materialize_grads(false);   // an unused output's gradient stays undefined
+    at::Tensor r, n, st;
+    c->rc = block_forward(*c->k, true, c->stream, &r, &n, &st);
+    const at::Tensor none;
+    ctx->save_for_backward({x, y, gate ? *gate : none, scale ? *scale : none, weight ? *weight : none, st});
+    int64_t need = x.requires_grad() | y.requires_grad() << 1;
+    const std::optional<at::Tensor>* rest[4] = {&gate, &scale, &weight, &bias};
+    for (int i = 0; i < 4; ++i) need |= (int64_t)(*rest[i] && (*rest[i])->requires_grad()) << (2 + i);
+    ctx->saved_data["need"] = need;
+    ctx->saved_data["flags"] = (int64_t)c->k->a.flags;
+    return {r, n};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto t = ctx->get_saved_variables();
+    const int64_t need = ctx->saved_data["need"].toInt();
+    torch::autograd::variable_list res(7);
+    {
+      const at::NoGradGuard no_grad;
+      Block k;
+      for (int i = 0; i < 5; ++i) k.t[i] = t[i].defined() ? &t[i] : nullptr;
+      k.t[5] = nullptr;
+      const bool inputs = block_tensors(&k);
+      TORCH_CHECK(inputs && f32_flat(t[5], 4 * k.a.rows, t[0]), kAnotherForm, "residual_norm");
+      const at::Tensor &x = t[0], &y = t[1];
+      k.a.flags = (int32_t)ctx->saved_data["flags"].toInt();
+      k.a.stats = fptr(t[5]);
+      const c10::DeviceGuard guard(x.device());
+      osm_resnorm_bwd_args b{};
+      at::Tensor g[2];
+      const void** const at_g[2] = {&b.grad_r, &b.grad_n};
+      for (int i = 0; i < 2; ++i) {
+        if (!grads[i].defined()) continue;
+        const at::Tensor& like = i ? y : x;
+        g[i] = norm_grad_form(grads[i], like) ? grads[i] : grads[i].to(like.options()).contiguous();
+        TORCH_CHECK(norm_grad_form(g[i], like), kAnotherForm, "residual_norm");
+        *at_g[i] = g[i].data_ptr();
+      }
+      b.grad_r_stride = b.grad_n_stride = b.grad_x_stride = b.grad_y_stride = b.grad_gate_stride = k.a.D;
+      void** const rows[3] = {&b.grad_x, &b.grad_y, &b.grad_gate};
+      float** const sums[3] = {&b.grad_scale, &b.grad_weight, &b.grad_bias};
+      for (int i = 0; i < 3; ++i) {
+        if (need >> i & 1) {
+          res[i] = empty(x.sizes(), x, t[i].scalar_type());
+          *rows[i] = res[i].data_ptr();
+        }
+        if (need >> (3 + i) & 1) {
+          res[3 + i] = empty({k.a.D}, x, at::kFloat);
+          *sums[i] = fptr(res[3 + i]);
+        }
+      }
+      const at::Tensor ws = scratch(lib.block_bwd_bytes(&k.a), x);
+      throw_rc(lib.block_bwd(&k.a, &b, ws.data_ptr(), (size_t)ws.numel(), engine_stream(x)));
+    }
+    return once(std::move(res), {grads[0], grads[1], t[0], t[1], t[2], t[3], t[4]});
+  }
+};
+
+// residual_norm(x, y, gate, scale, weight, bias, flags, eps): None, or (r, n) with their gradient's function.
+PyObject* run_residual_norm(PyObject* const* p) {
+  Block k;
+  for (int i = 0; i < 6; ++i) {
+    k.t[i] = p[i] == Py_None ? nullptr : plain(p[i]);
+    if (!k.t[i] && (i < 2 || p[i] != Py_None)) Py_RETURN_NONE;
+  }
+  if (!block_tensors(&k) || !as_float(p[7], &k.a.eps)) Py_RETURN_NONE;
+  k.a.flags = (int32_t)PyLong_AsLong(p[6]);
+  if (PyErr_Occurred()) return nullptr;
+  bool grad = false;
+  for (const at::Tensor* t : k.t) {
+    if (t && has_tangent(*t)) Py_RETURN_NONE;
+    grad = grad || (t && t->requires_grad());
+  }
+  const at::Tensor &x = *k.t[0], &y = *k.t[1];
+  Ref s_obj;
+  void* stream;
+  const c10::DeviceGuard guard(x.device());
+  if (!stream_of(x, &s_obj, &stream)) return nullptr;
+  at::Tensor r, n, st;
+  int rc;
+  {
+    const NoGil nogil;
+    if (grad && at::GradMode::is_enabled()) {
+      BlockCall c{&k, stream, OSM_OK};
+      const torch::autograd::variable_list res =
+          BlockGrad::apply(x, y, optional_tensor(p[2]), optional_tensor(p[3]), optional_tensor(p[4]), optional_tensor(p[5]), &c);
+      r = res[0];
+      n = res[1];
+      rc = c.rc;
+    } else {
+      rc = block_forward(k, false, stream, &r, &n, &st);
+    }
+  }
+  if (rc != OSM_OK) return fail_rc(rc);
+  return Py_BuildValue("(NN)", THPVariable_Wrap(r), THPVariable_Wrap(n));
+}
+
+// The cross entropy's tensors: hidden [.., D], weight [V,D], targets.
+bool loss_tensors(const at::Tensor& h, const at::Tensor& w, const at::Tensor& t, osm_loss_args* a) {
+  if (!norm_rows(&h) || !w.is_cuda() || w.dim() != 2 || w.scalar_type() != h.scalar_type() || w.device() != h.device() ||
+      w.size(0) < 1 || w.size(1) != h.size(h.dim() - 1) || !w.is_contiguous() || t.scalar_type() != at::kLong || t.device() != h.device() ||
+      !t.is_contiguous() || t.sizes() != h.sizes().slice(0, h.dim() - 1))
+    return false;
+  a->abi_version = OSM_ABI_VERSION;
+  a->dtype = code(h);
+  a->D = w.size(1);
+  a->V = w.size(0);
+  a->N = t.numel();
+  a->hidden = h.data_ptr();
+  a->weight = w.data_ptr();
+  a->hidden_stride = a->weight_stride = a->D;
+  a->targets = static_cast<const int64_t*>(t.data_ptr());
+  return true;
+}
+
+// 0: every token's loss, 1: their sum, 2: their mean
+int loss_forward(osm_loss_args& a, const at::Tensor& h, const at::Tensor& t, int64_t how, void* stream, at::Tensor* loss, at::Tensor* lse,
+                 at::Tensor* count) {
+  at::Tensor losses = empty(t.sizes(), h, at::kFloat);
+  *lse = empty(t.sizes(), h, at::kFloat);
+  a.losses = fptr(losses);
+  a.lse = fptr(*lse);
+  if (how == 0) {
+    *loss = losses;
+  } else {
+    *loss = empty({}, h, at::kFloat);
+    a.loss = fptr(*loss);
+  }
+  if (how == 2) {
+    a.flags = OSM_LOSS_MEAN;
+    *count = empty({}, h, at::kFloat);
+    a.count = fptr(*count);
+  }
+  const at::Tensor ws = scratch(lib.loss_bytes(&a), h);
+  return lib.loss_fwd(&a, ws.data_ptr(), (size_t)ws.numel(), stream);
+}
+
+struct LossCall {
+  osm_loss_args* a;
+  int64_t how;
+  void* stream;
+  int rc;
+};
+struct LossGrad : torch::autograd::Function<LossGrad> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& h, const at::Tensor& w, const at::Tensor& t,
+                            LossCall* c) {
+    at::Tensor loss, lse, count;
+    c->rc = loss_forward(*c->a, h, t, c->how, c->stream, &loss, &lse, &count);
+    ctx->save_for_backward({h, w, t, lse, count});
+    ctx->saved_data["need"] = (int64_t)(h.requires_grad() | w.requires_grad() << 1);
+    ctx->saved_data["each"] = c->how == 0;
+    ctx->saved_data["ignore"] = c->a->ignore_index;
+    return loss;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto t = ctx->get_saved_variables();
+    const int64_t need = ctx->saved_data["need"].toInt();
+    const bool each = ctx->saved_data["each"].toBool();
+    torch::autograd::variable_list res(4);
+    {
+      const at::NoGradGuard no_grad;
+      const at::Tensor &h = t[0], &w = t[1], &lse = t[3];
+      osm_loss_args a{};
+      TORCH_CHECK(loss_tensors(h, w, t[2], &a) && f32_flat(lse, a.N, h) && (!t[4].defined() || f32_flat(t[4], 1, h)), kAnotherForm,
+                  "linear_cross_entropy");
+      a.ignore_index = ctx->saved_data["ignore"].toInt();
+      a.lse = fptr(lse);
+      const c10::DeviceGuard guard(h.device());
+      const at::Tensor g = grads[0].to(at::kFloat).contiguous();
+      TORCH_CHECK(f32_flat(g, each ? a.N : 1, h), kAnotherForm, "linear_cross_entropy");
+      osm_loss_bwd_args b{};
+      (each ? b.grad_losses : b.grad) = fptr(g);
+      if (t[4].defined()) b.count = fptr(t[4]);
+      void** const to[2] = {&b.grad_hidden, &b.grad_weight};
+      for (int i = 0; i < 2; ++i)
+        if (need >> i & 1) {
+          res[i] = empty(t[i].sizes(), h, h.scalar_type());
+          *to[i] = res[i].data_ptr();
+        }
+      const at::Tensor ws = scratch(lib.loss_bwd_bytes(&a), h);
+      throw_rc(lib.loss_bwd(&a, &b, ws.data_ptr(), (size_t)ws.numel(), engine_stream(h)));
+    }
+    return once(std::move(res), {grads[0], t[0], t[1]});
+  }
+};
+
+// linear_cross_entropy(hidden, weight, targets, ignore_index, how): None, or the loss with its gradient's function.
+PyObject* run_linear_loss(PyObject* const* p) {
+  const at::Tensor *h = plain(p[0]), *w = plain(p[1]), *t = plain(p[2]);
+  osm_loss_args a{};
+  int64_t how;
+  if (!h || !w || !t || !loss_tensors(*h, *w, *t, &a) || !as_int(p[3], &a.ignore_index) || !as_int(p[4], &how)) Py_RETURN_NONE;
+  if (has_tangent(*h) || has_tangent(*w)) Py_RETURN_NONE;
+  Ref s_obj;
+  void* stream;
+  const c10::DeviceGuard guard(h->device());
+  if (!stream_of(*h, &s_obj, &stream)) return nullptr;
+  at::Tensor loss, lse, count;
+  int rc;
+  {
+    const NoGil nogil;
+    if ((h->requires_grad() || w->requires_grad()) && at::GradMode::is_enabled()) {
+      LossCall c{&a, how, stream, OSM_OK};
+      loss = LossGrad::apply(*h, *w, *t, &c);
+      rc = c.rc;
+    } else {
+      rc = loss_forward(a, *h, *t, how, stream, &loss, &lse, &count);
+    }
+  }
+  if (rc != OSM_OK) return fail_rc(rc);
+  return THPVariable_Wrap(loss);
+}
+
 // Runs a function under the argument count and the C++ exceptions of ATen.
 template <int N, typename F>
 PyObject* guarded(PyObject* const* args, Py_ssize_t n, F f) {
@@ -1340,6 +1848,11 @@ PyObject* py_norm_forward(PyObject*, PyObject* const* a, Py_ssize_t n) { return 
 PyObject* py_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded<8>(a, n, run_norm_backward); }
 PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded<4>(a, n, run_layer_norm); }
 PyObject* py_clip(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded<4>(a, n, run_clip); }
+PyObject* py_ema_forward(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded<5>(a, n, run_ema_forward); }
+PyObject* py_gated_ema(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded<4>(a, n, run_gated_ema); }
+PyObject* py_ema_step(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded<4>(a, n, run_ema_step); }
+PyObject* py_residual_norm(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded<8>(a, n, run_residual_norm); }
+PyObject* py_linear_loss(PyObject*, PyObject* const* a, Py_ssize_t n) { return guarded<5>(a, n, run_linear_loss); }
 
 // init(addresses of the library's functions in the order of Lib, raw_stream, ws_cache, workspace, check)
 PyObject* py_init(PyObject*, PyObject* args) {
@@ -1374,6 +1887,19 @@ PyObject* py_init(PyObject*, PyObject* args) {
   lib.norm_bwd = reinterpret_cast<decltype(lib.norm_bwd)>(f[19]);
   lib.clip_bytes = reinterpret_cast<decltype(lib.clip_bytes)>(f[20]);
   lib.clip = reinterpret_cast<decltype(lib.clip)>(f[21]);
+  lib.ema_saved = reinterpret_cast<decltype(lib.ema_saved)>(f[22]);
+  lib.ema_bytes = reinterpret_cast<decltype(lib.ema_bytes)>(f[23]);
+  lib.ema_fwd = reinterpret_cast<decltype(lib.ema_fwd)>(f[24]);
+  lib.ema_bwd_bytes = reinterpret_cast<decltype(lib.ema_bwd_bytes)>(f[25]);
+  lib.ema_bwd = reinterpret_cast<decltype(lib.ema_bwd)>(f[26]);
+  lib.ema_step = reinterpret_cast<decltype(lib.ema_step)>(f[27]);
+  lib.block_fwd = reinterpret_cast<decltype(lib.block_fwd)>(f[28]);
+  lib.block_bwd_bytes = reinterpret_cast<decltype(lib.block_bwd_bytes)>(f[29]);
+  lib.block_bwd = reinterpret_cast<decltype(lib.block_bwd)>(f[30]);
+  lib.loss_bytes = reinterpret_cast<decltype(lib.loss_bytes)>(f[31]);
+  lib.loss_fwd = reinterpret_cast<decltype(lib.loss_fwd)>(f[32]);
+  lib.loss_bwd_bytes = reinterpret_cast<decltype(lib.loss_bwd_bytes)>(f[33]);
+  lib.loss_bwd = reinterpret_cast<decltype(lib.loss_bwd)>(f[34]);
   PyObject** slots[4] = {&raw_stream, &ws_cache, &workspace, &check};
   PyObject* vals[4] = {rs, wc, wf, ck};
   for (int i = 0; i < 4; ++i) {
@@ -1407,6 +1933,11 @@ PyMethodDef methods[] = {
     {"norm_backward", fast(py_norm_backward), METH_FASTCALL, nullptr},
     {"layer_norm", fast(py_layer_norm), METH_FASTCALL, nullptr},
     {"clip", fast(py_clip), METH_FASTCALL, nullptr},
+    {"ema_forward", fast(py_ema_forward), METH_FASTCALL, nullptr},
+    {"gated_ema", fast(py_gated_ema), METH_FASTCALL, nullptr},
+    {"ema_step", fast(py_ema_step), METH_FASTCALL, nullptr},
+    {"residual_norm", fast(py_residual_norm), METH_FASTCALL, nullptr},
+    {"linear_loss", fast(py_linear_loss), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "osm_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -109,6 +109,11 @@ def gated_ema_forward(x: torch.Tensor, gate: torch.Tensor, *, state_init: torch.
     fp32 when ``return_state``.  ``out`` and ``state_out`` (contiguous; state_out
     may be state_init, else they lie in no argument's memory) receive the results
     instead of new tensors."""
+    fast = _fast()
+    if fast is not None and out is None and state_out is None:
+        res = fast.ema_forward(x, gate, lengths, state_init, return_state)
+        if res is not None:
+            return res if return_state else res[0]
     out, fin, _, _ = _forward(x, gate, state_init, lengths, out, return_state, state_out, False)
     return (out, fin) if return_state else out
 
@@ -179,6 +184,11 @@ def gated_ema(x: torch.Tensor, gate: torch.Tensor, *, state_init: torch.Tensor |
     """``gated_ema_forward`` as a differentiable op: gradients flow to x, gate
     and state_init, from the output and the final state.  Returns h, or (h,
     final state) when ``return_state``."""
+    fast = _fast()
+    if fast is not None:
+        res = fast.gated_ema(x, gate, lengths, state_init)
+        if res is not None:
+            return res if return_state else res[0]
     if differentiable(x, gate, state_init):
         out, fin = _GatedEmaFunction.apply(x, gate, state_init, lengths)
         return (out, fin) if return_state else out
@@ -192,6 +202,11 @@ def gated_ema_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, *, 
     device, no slot twice): a negative one marks an idle row, whose output is 0;
     one past the pool gives NaN; neither touches a state.  Returns h [B,D] in x's
     type, in ``out`` (contiguous, in no argument's memory) if given."""
+    fast = _fast()
+    if fast is not None and out is None:
+        res = fast.ema_step(x, gate, state, slots)
+        if res is not None:
+            return res
     lib = nat.load()
     x, gate = _check(x, gate, 2, "[B,D]")
     dev = x.device

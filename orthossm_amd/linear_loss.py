@@ -33,6 +33,8 @@ from .delta import _scratch, differentiable, on_device
 from .norm import _matrix
 from .ops import _current_stream, _dtype_code, _fast
 
+_HOW = {"none": 0, "sum": 1, "mean": 2}
+
 
 def _prepare(hidden, weight, targets, ignore_index):
     if not isinstance(hidden, torch.Tensor) or hidden.dim() < 1 or hidden.shape[-1] < 1:
@@ -59,29 +61,36 @@ def _prepare(hidden, weight, targets, ignore_index):
     return a, (hidden, weight, targets), (rows, w)
 
 
-def _forward(hidden, weight, targets, ignore_index, total: bool):
+def _forward(hidden, weight, targets, ignore_index, reduction="none"):
+    """(losses, or their sum or mean; lse; the count that a mean divided by;
+    the inputs as the kernels read them)."""
     lib = nat.load()
     a, ins, keep = _prepare(hidden, weight, targets, ignore_index)
     dev, shape = ins[0].device, ins[2].shape
     losses, lse = (torch.empty(shape, dtype=torch.float32, device=dev) for _ in range(2))
-    tot = torch.empty(2, dtype=torch.float32, device=dev) if total else None
-    a.losses, a.lse, a.total = losses.data_ptr(), lse.data_ptr(), tot.data_ptr() if total else None
+    a.losses, a.lse, loss, count = losses.data_ptr(), lse.data_ptr(), losses, None
+    if reduction != "none":
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        a.loss = loss.data_ptr()
+    if reduction == "mean":
+        a.flags, count = nat.LOSS_MEAN, torch.empty((), dtype=torch.float32, device=dev)
+        a.count = count.data_ptr()
     ws = _scratch(lib.osm_linear_ce_workspace_bytes(ctypes.byref(a)), dev)
     with on_device(dev):
         nat.check(lib.osm_linear_ce_fwd(ctypes.byref(a), ctypes.c_void_p(ws.data_ptr()), ws.numel(),
                                         ctypes.c_void_p(_current_stream(dev))))
     del keep
-    return losses, lse, tot, ins
+    return loss, lse, count, ins
 
 
 def linear_cross_entropy_forward(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *,
                                  ignore_index: int = -100):
     """(losses, lse) fp32 of targets' shape: each token's loss and the logarithm
     of its sum of exponentials, 0 for tokens that do not count."""
-    return _forward(hidden, weight, targets, ignore_index, False)[:2]
+    return _forward(hidden, weight, targets, ignore_index)[:2]
 
 
-def _backward(hidden, weight, targets, lse, ignore_index, grad, grad_losses, total, need_hidden, need_weight):
+def _backward(hidden, weight, targets, lse, ignore_index, grad, count, grad_losses, need_hidden, need_weight):
     lib = nat.load()
     a, (hidden, weight, targets), keep = _prepare(hidden, weight, targets, ignore_index)
     dev = hidden.device
@@ -98,7 +107,7 @@ def _backward(hidden, weight, targets, lse, ignore_index, grad, grad_losses, tot
             raise ValueError(f"grad_losses must be a tensor of shape {tuple(targets.shape)}")
         grad_losses = grad_losses.to(device=dev, dtype=torch.float32).contiguous()
         b.grad_losses = grad_losses.data_ptr()
-    b.total = total.data_ptr() if total is not None else None
+    b.count = count.data_ptr() if count is not None else None
     gh = torch.empty(hidden.shape, dtype=hidden.dtype, device=dev) if need_hidden else None
     gw = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if need_weight else None
     b.grad_hidden, b.grad_weight = (None if t is None else t.data_ptr() for t in (gh, gw))
@@ -115,7 +124,7 @@ def linear_cross_entropy_backward(grad_losses: torch.Tensor, hidden: torch.Tenso
                                   need_hidden: bool = True, need_weight: bool = True):
     """(grad_hidden, grad_weight) in the inputs' type, None for what is not
     needed, from dL/d losses and what the forward gave."""
-    return _backward(hidden, weight, targets, lse, ignore_index, None, grad_losses, None, need_hidden, need_weight)
+    return _backward(hidden, weight, targets, lse, ignore_index, None, None, grad_losses, need_hidden, need_weight)
 
 
 class _LinearCrossEntropyFunction(torch.autograd.Function):
@@ -123,23 +132,19 @@ class _LinearCrossEntropyFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, hidden, weight, targets, ignore_index, reduction):
-        losses, lse, total, ins = _forward(hidden, weight, targets, ignore_index, reduction != "none")
-        ctx.save_for_backward(*ins, lse, total if reduction == "mean" else None)
+        loss, lse, count, ins = _forward(hidden, weight, targets, ignore_index, reduction)
+        ctx.save_for_backward(*ins, lse, count)
         ctx.ignore_index, ctx.reduction, ctx.types = ignore_index, reduction, (hidden.dtype, weight.dtype)
-        return _reduced(losses, total, reduction)
+        return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        hidden, weight, targets, lse, total = ctx.saved_tensors
+        hidden, weight, targets, lse, count = ctx.saved_tensors
         each = ctx.reduction == "none"
-        grads = _backward(hidden, weight, targets, lse, ctx.ignore_index, None if each else grad, grad if each else None,
-                          total, *ctx.needs_input_grad[:2])
+        grads = _backward(hidden, weight, targets, lse, ctx.ignore_index, None if each else grad, count, grad if each else None,
+                          *ctx.needs_input_grad[:2])
         return (*(None if t is None else t.to(dt) for t, dt in zip(grads, ctx.types)), None, None, None)
-
-
-def _reduced(losses, total, reduction):
-    return losses if reduction == "none" else total[0] / total[1] if reduction == "mean" else total[0].clone()
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, ignore_index: int = -100,
@@ -147,9 +152,13 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     """The cross entropy of softmax(hidden weight^T) against targets, fp32,
     differentiable in hidden and weight: the mean over the tokens that count (0
     where none does), their sum, or (``"none"``) every token's."""
-    if reduction not in ("mean", "sum", "none"):
+    if reduction not in _HOW:
         raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
+    fast = _fast()
+    if fast is not None:
+        loss = fast.linear_loss(hidden, weight, targets, ignore_index, _HOW[reduction])
+        if loss is not None:
+            return loss
     if differentiable(hidden, weight):
         return _LinearCrossEntropyFunction.apply(hidden, weight, targets, int(ignore_index), reduction)
-    losses, _, total, _ = _forward(hidden, weight, targets, ignore_index, reduction != "none")
-    return _reduced(losses, total, reduction)
+    return _forward(hidden, weight, targets, ignore_index, reduction)[0]

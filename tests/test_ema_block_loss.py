@@ -145,13 +145,14 @@ LOSS_ERRORS = COMMON + [(dict(N=-1), -2), (dict(N=1 << 21), -2), (dict(D=0), -2)
                         (dict(targets=None), -1), (dict(targets=P + 4), -1), (dict(lse=None), -1), (dict(lse=P + 2), -1)]
 
 
-@pytest.mark.parametrize("kw,code", LOSS_ERRORS + [(dict(losses=P + 2), -4), (dict(total=P + 2), -4), (dict(losses=None, total=P), -1)])
+@pytest.mark.parametrize("kw,code", LOSS_ERRORS + [(dict(losses=P + 2), -4), (dict(loss=P + 2), -4), (dict(count=P + 1), -4), (dict(losses=None, loss=P), -1),
+                                                   (dict(count=P), -1), (dict(flags=2), -1)])
 def test_loss_errors(kw, code):
     assert nat.load().osm_linear_ce_fwd(ctypes.byref(loss(**kw)), ctypes.c_void_p(P), 1 << 40, None) == code
 
 
 @pytest.mark.parametrize("kw,bwd,code", [(kw, {}, code) for kw, code in LOSS_ERRORS] + [
-    ({}, dict(grad=P + 2), -4), ({}, dict(grad_losses=P + 2), -4), ({}, dict(total=P + 1), -4), ({}, dict(grad_hidden=P + 4), -4),
+    ({}, dict(grad=P + 2), -4), ({}, dict(grad_losses=P + 2), -4), ({}, dict(count=P + 1), -4), ({}, dict(grad_hidden=P + 4), -4),
     ({}, dict(grad_weight=P + 8), -4), (dict(D=63), dict(grad_weight=P + 2), -4)])
 def test_loss_backward_errors(kw, bwd, code):
     b = nat.LossBwdArgs()
