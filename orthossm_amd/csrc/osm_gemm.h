@@ -1,13 +1,15 @@
-// A tile of a product of two bf16 matrices with contiguous rows, C = A B^T, on
-// gfx950's matrix instruction: what the vocabulary's cross entropy is built on.
+// A tile of a product of two bf16 matrices on gfx950's matrix instruction, C[n][m] =
+// sum_k A(m, k) B(n, k): what the vocabulary's cross entropy is built on.
 //
-// A workgroup forms TM x TN of C.  64 columns of both operands' rows at a time go
-// from memory to LDS without passing through registers, into one of two buffers
-// while the other is multiplied.  A row's 16-byte units lie in LDS at their index
-// xor half the row's, so that the 32 rows of a matrix instruction are read from
-// different banks; the order is made by the addresses that are read from memory.
-// An fp32 operand is three bf16 matrices whose sum it is (its parts), and the
-// product the sum of the six products of parts that are not below 2^-24.
+// Each operand lies by rows (a row holds the k of one m or n) or by columns (a row
+// holds the m or n of one k).  A workgroup forms TM x TN of C.  64 k of both operands at a
+// time go from memory to LDS without passing through registers, into one of two buffers
+// while the other is multiplied.  By rows, a row's 16-byte units lie in LDS at their index
+// xor half the row's, so that the 32 rows of a matrix instruction are read from different
+// banks; by columns, a row's 32-byte units lie at theirs xor the row's, so that the 4 rows
+// of a transposing read are.  The order is made by the addresses that are read from memory.
+// An fp32 operand is three bf16 matrices whose sum it is (its parts), and the product the
+// sum of the six products of parts that are not below 2^-24.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -18,24 +20,36 @@ namespace osm {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int kStep = 64;        // columns of a step
-constexpr int kUnits = kStep / 8;
+constexpr int kStep = 64;        // k come in multiples of this
+
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
 
 struct GemmSide {
   const __bf16* p;               // rows ld apart, a multiple of 8; 16-byte aligned
   int64_t ld, part;              // elements from row to row (below 2^21), from part to part
   int rows;                      // rows to read (past them: the last one again)
+  int cols;                      // by columns: elements of a row to read, a multiple of 8 (past them: the last ones again)
 };
 
-template <int TM_, int TN_, int WM_, int WN_>
+template <int TM_, int TN_, int WM_, int WN_, int KS_ = 64, int ST_ = 2>
 struct GemmTile {
   static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_;   // tile; waves along each
+  static constexpr int KS = KS_, ST = ST_;                       // k of a step; buffers
   static constexpr int kThreads = 64 * WM * WN;
   static constexpr int FM = TM / WM / 32, FN = TN / WN / 32;     // 32 x 32 squares of a wave
-  static constexpr int kBuffer = (TM + TN) * kStep;              // elements of a buffer
-  static constexpr int kLds = 2 * kBuffer;
-  static_assert(TM * kUnits % kThreads == 0 && TN * kUnits % kThreads == 0, "whole loads");
+  static constexpr int kBuffer = (TM + TN) * KS;                 // elements of a buffer
+  static constexpr int kLds = ST * kBuffer;
+  static constexpr int kLoads = kBuffer / 8 / kThreads;          // of a thread and step
+  static_assert(TM * KS / 8 % kThreads == 0 && TN * KS / 8 % kThreads == 0 && kStep % KS == 0, "whole loads and steps");
 };
+
+// Waits until at most `n` of this wave's loads are on their way.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N < 64, "6 bits");
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4) << 14);
+}
 
 // Where a thread's accumulators lie in C's tile: row(i) of column col, i in [0, 16).
 template <class G>
@@ -52,50 +66,105 @@ struct GemmPlace {
   __device__ __forceinline__ int col(int fn) const { return n + 32 * fn + (lane & 31); }
 };
 
-__device__ __forceinline__ void to_lds(const __bf16* from, __bf16* to) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16,
-                                   0, 0);
+// 16 bytes a lane from memory to LDS, to the 1024 bytes from `to` (the same in every lane)
+// on in the order of the lanes.  It has no result to wait for: who reads them waits for
+// vmcnt himself.  (In place of the compiler's builtin, ahead of whose effects it would
+// wait at the next transposing read, which is of the other buffer.)
+__device__ __forceinline__ void to_lds(const __bf16* from, unsigned to) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory");
+}
+__device__ __forceinline__ unsigned lds_address(const __bf16* p) {
+  return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) __bf16*)p;
 }
 
-// acc = the rows from m0 of A times the rows from n0 of B over `steps` steps of
-// columns from column k0 (a multiple of kStep).  parts: 1, or 3 for each side.
-template <class G>
-__device__ __forceinline__ void gemm(const GemmSide& A, const GemmSide& B, int m0, int n0, int64_t k0, int steps, int parts,
+// One operand of a tile, T of its m or n: where a thread's share of a step comes from, and
+// where a lane's share of a matrix instruction lies in LDS.
+template <class G, int T, bool COLS>
+struct GemmOperand {
+  static constexpr int KS = G::KS, kRow = COLS ? T : KS, kRowUnits = kRow / 8;   // elements, 16-byte units of a row in LDS
+  static constexpr int N = T * KS / 8 / G::kThreads;
+  // (rows of 128 bytes: two of them go through the banks; of 64 bytes: four)
+  static __device__ __forceinline__ int turn(int row) { return KS == 64 ? row >> 1 & 7 : row >> 2 & 3; }
+  int from[N];             // elements from the step's first
+  const __bf16 *first, *at;
+  int64_t ld, part;
+  int rows, k;             // by columns: rows in all, and ahead of the step
+
+  static __device__ __forceinline__ int row_of(int i) { return ((int)threadIdx.x + i * G::kThreads) / kRowUnits; }
+  static __device__ __forceinline__ int col_of(int i) {
+    const int u = (int)threadIdx.x + i * G::kThreads, r = u / kRowUnits, c = u % kRowUnits;
+    return 8 * (COLS ? (c ^ ((r & 3) << 1)) : (c ^ turn(r)));
+  }
+  __device__ __forceinline__ GemmOperand(const GemmSide& s, int m0, int64_t k0) {
+    ld = s.ld;
+    part = s.part;
+    rows = s.rows;
+    k = (int)k0;
+    first = s.p + (COLS ? k0 * ld + m0 : m0 * ld + k0);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      from[i] = COLS ? row_of(i) * (int)ld + min(col_of(i), s.cols - 8 - m0) : min(row_of(i), rows - 1 - m0) * (int)ld + col_of(i);
+  }
+  __device__ __forceinline__ void start(int index, int64_t k0) {
+    at = first + index * part;
+    k = (int)k0;
+  }
+  // The next step to LDS.
+  __device__ __forceinline__ void fetch(unsigned to) {
+    to += __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
+    if (!COLS || k + KS <= rows) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) to_lds(at + from[i], to + i * G::kThreads * 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int r = row_of(i), over = max(r + k - (rows - 1), 0);
+        to_lds(at + from[i] - (int64_t)over * ld, to + i * G::kThreads * 16);
+      }
+    }
+    at += COLS ? KS * ld : KS;
+    k += KS;
+  }
+  // A lane's 8 elements of the 32 from `m` on, in the s-th 16 k of the step.
+  static __device__ __forceinline__ bf16x8 read(const __bf16* lds, int m, int s, int lane) {
+    if constexpr (!COLS) {
+      const int r = lane & 31;
+      return *reinterpret_cast<const bf16x8*>(lds + (m + r) * KS + (((2 * s + (lane >> 5)) ^ turn(r)) * 8));
+    } else {
+      // (a group of 16 lanes reads 4 rows of 16 elements and gets them by columns)
+      const int i = lane & 15, g = lane >> 4, r = 16 * s + 8 * (g >> 1) + (i >> 2);
+      const __bf16* const p = lds + r * kRow + (((m >> 4) + (g & 1)) ^ (i >> 2)) * 16 + (i & 3) * 4;
+      typedef __attribute__((address_space(3))) i16x4* Lds;
+      const bf16x4 lo = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(p)));
+      const bf16x4 hi = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(p + 4 * kRow)));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+};
+
+// acc = the m from m0 of A times the n from n0 of B over `steps` times kStep k from k0 on (a
+// multiple of kStep).  parts: 1, or 3 for each side.
+template <class G, bool ACOLS, bool BCOLS>
+__device__ __forceinline__ void gemm(const GemmSide& A, const GemmSide& B, int m0, int n0, int64_t k0, int n_steps, int parts,
                                      __bf16* lds, f32x16 (&acc)[G::FM][G::FN]) {
-  constexpr int NA = G::TM * kUnits / G::kThreads, NB = G::TN * kUnits / G::kThreads;
+  using OA = GemmOperand<G, G::TM, ACOLS>;
+  using OB = GemmOperand<G, G::TN, BCOLS>;
   const GemmPlace<G> q;
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int oa[NA], ob[NB];   // elements from the first row, column k0
-#pragma unroll
-  for (int i = 0; i < NA; ++i) {
-    const int u = tid + i * G::kThreads, r = u / kUnits, c = (u % kUnits) ^ ((r >> 1) & 7);
-    oa[i] = min(r, A.rows - 1 - m0) * (int)A.ld + 8 * c;
-  }
-#pragma unroll
-  for (int i = 0; i < NB; ++i) {
-    const int u = tid + i * G::kThreads, r = u / kUnits, c = (u % kUnits) ^ ((r >> 1) & 7);
-    ob[i] = min(r, B.rows - 1 - n0) * (int)B.ld + 8 * c;
-  }
-  const __bf16* const a0 = A.p + m0 * A.ld + k0;
-  const __bf16* const b0 = B.p + n0 * B.ld + k0;
-  const int segments = parts == 1 ? 1 : 6, total = steps * segments;
+  OA a(A, m0, k0);
+  OB b(B, n0, k0);
+  const int steps = n_steps * (kStep / G::KS), segments = parts == 1 ? 1 : 6, total = steps * segments;
   // (parts i of A and j of B in order: 2 0, 1 1, 0 2, 1 0, 0 1, 0 0, the small ones first)
   int seg = 0, at = 0;
-  const __bf16 *pa, *pb;
   auto point = [&] {
-    const int i = segments == 1 ? 0 : (0x001012 >> (4 * seg)) & 15, j = segments == 1 ? 0 : (0x010210 >> (4 * seg)) & 15;
-    pa = a0 + i * A.part;
-    pb = b0 + j * B.part;
+    a.start(segments == 1 ? 0 : (0x001012 >> (4 * seg)) & 15, k0);
+    b.start(segments == 1 ? 0 : (0x010210 >> (4 * seg)) & 15, k0);
   };
   point();
+  const unsigned base = __builtin_amdgcn_readfirstlane(lds_address(lds));
   auto fetch = [&](int buf) {
-    __bf16* const to = lds + buf * G::kBuffer + wave * 512;
-#pragma unroll
-    for (int i = 0; i < NA; ++i) to_lds(pa + oa[i], to + i * G::kThreads * 8);
-#pragma unroll
-    for (int i = 0; i < NB; ++i) to_lds(pb + ob[i], to + G::TM * kStep + i * G::kThreads * 8);
-    pa += kStep;
-    pb += kStep;
+    const unsigned to = base + buf * G::kBuffer * 2;
+    a.fetch(to);
+    b.fetch(to + G::TM * G::KS * 2);
     if (++at == steps) {
       at = 0;
       ++seg;
@@ -106,23 +175,29 @@ __device__ __forceinline__ void gemm(const GemmSide& A, const GemmSide& B, int m
   for (int i = 0; i < G::FM; ++i)
 #pragma unroll
     for (int j = 0; j < G::FN; ++j) acc[i][j] = (f32x16)0.0f;
-  // a lane's row of a square and its unit in each half step
-  const int r = q.lane & 31, half = q.lane >> 5, x = (r >> 1) & 7;   // (squares start at multiples of 32 rows: x is the same)
-  if (total > 0) fetch(0);
-  for (int t = 0; t < total; ++t) {
-    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this step's units are in LDS
-    __syncthreads();                      // everyone's are, and the other buffer has been read
-    if (t + 1 < total) fetch((t + 1) & 1);
-    const __bf16* const la = lds + (t & 1) * G::kBuffer;
-    const __bf16* const lb = la + G::TM * kStep;
+  // Step t is multiplied while the ST - 1 after it are on their way; the last of those goes
+  // where step t - 1 was, which everyone has read by the barrier.
 #pragma unroll
-    for (int s = 0; s < kStep / 16; ++s) {
-      const int unit = ((2 * s + half) ^ x) * 8;
+  for (int t = 0; t < G::ST - 1; ++t)
+    if (t < total) fetch(t);
+  int buf = 0;
+  for (int t = 0; t < total; ++t) {
+    if (t + G::ST - 2 < total)
+      wait_loads<(G::ST - 2) * G::kLoads>();
+    else
+      wait_loads<0>();
+    __syncthreads();
+    if (t + G::ST - 1 < total) fetch(buf == 0 ? G::ST - 1 : buf - 1);
+    const __bf16* const la = lds + buf * G::kBuffer;
+    const __bf16* const lb = la + G::TM * G::KS;
+    buf = buf == G::ST - 1 ? 0 : buf + 1;
+#pragma unroll
+    for (int s = 0; s < G::KS / 16; ++s) {
       bf16x8 fa[G::FM], fb[G::FN];
 #pragma unroll
-      for (int i = 0; i < G::FM; ++i) fa[i] = *reinterpret_cast<const bf16x8*>(la + (q.m + 32 * i + r) * kStep + unit);
+      for (int i = 0; i < G::FM; ++i) fa[i] = OA::read(la, q.m + 32 * i, s, q.lane);
 #pragma unroll
-      for (int j = 0; j < G::FN; ++j) fb[j] = *reinterpret_cast<const bf16x8*>(lb + (q.n + 32 * j + r) * kStep + unit);
+      for (int j = 0; j < G::FN; ++j) fb[j] = OB::read(lb, q.n + 32 * j, s, q.lane);
 #pragma unroll
       for (int i = 0; i < G::FM; ++i)
 #pragma unroll

@@ -10,9 +10,10 @@ constexpr int kLossPad = 256;      // rows of compacted tokens, columns of a pie
 
 // The tokens that count, one after the other.
 struct LossTokens {
-  int* rows;                       // [N]: the token of each place
+  int* targets;                    // [N]: by place, -1: outside the vocabulary
+  float2* factors;                 // [N]: by place, log2(e) lse and grad_losses (1 without); the backward's
   int* places;                     // [N]: the place of each token, -1: does not count
-  int* count;                      // [2]: how many; a counter of the join's
+  int* count;                      // device scalar: how many
 };
 
 struct LossParams {
@@ -25,16 +26,13 @@ struct LossParams {
   const int64_t* targets;
   int64_t ignore;
   LossTokens tok;
-  __bf16* h;                       // [parts][Npad][Dpad]: the hidden rows that count (nothing is written after them)
-  __bf16* ht;                      // [parts][Dpad][Npad]: the same by column, zeros after them up to a whole step
+  __bf16* h;                       // [parts][Npad][Dpad]: the hidden rows that count, zeros after them up to a whole step
   // a piece of the vocabulary
   int64_t v0;
   int vn, vpad;                    // its classes; columns of p
   const __bf16* w;                 // [parts][vn][w_ld], w_part apart
   int64_t w_ld, w_part;
-  __bf16* wt;                      // [parts][Dpad][vpad]
   __bf16* p;                       // [parts][Npad][vpad]: probabilities less the targets'
-  __bf16* pt;                      // [parts][vpad][Npad]
   float* dh;                       // [splits][Npad][Dpad]
   int splits, first;               // first: dh is written, not added to
   // statistics
@@ -47,15 +45,13 @@ struct LossParams {
   void *grad_h, *grad_w;
 };
 
-hipError_t launch_loss_rows(const LossParams& p, int dtype, hipStream_t stream);            // tok, h
+hipError_t launch_loss_rows(const LossParams& p, int dtype, bool bwd, hipStream_t stream);  // tok, h
 hipError_t launch_loss_weight(const LossParams& p, __bf16* to, int dtype, hipStream_t stream);   // parts of the piece's rows
-hipError_t launch_loss_transpose(const __bf16* from, int64_t ld, int64_t from_part, int rows, const int* count, int cols, __bf16* to,
-                                 int to_ld, int64_t to_part, int parts, hipStream_t stream);
 int loss_tile_rows(const LossParams& p);                                                    // classes of a tile of the logits
 hipError_t launch_loss_logits(const LossParams& p, hipStream_t stream);                     // stat, own
 hipError_t launch_loss_join(const LossParams& p, int tiles, hipStream_t stream);            // losses, lse, loss, count
 hipError_t launch_loss_none(float* loss, float* count, hipStream_t stream);
-hipError_t launch_loss_probs(const LossParams& p, hipStream_t stream);                      // p, pt
+hipError_t launch_loss_probs(const LossParams& p, hipStream_t stream);                      // p
 hipError_t launch_loss_dh(const LossParams& p, hipStream_t stream);
 hipError_t launch_loss_dw(const LossParams& p, int dtype, hipStream_t stream);
 hipError_t launch_loss_zero(void* to, int64_t n, int dtype, hipStream_t stream);

@@ -7,9 +7,11 @@
 // accumulators and leaves of it, for every token, the largest and the sum of
 // exponentials below it; a second kernel joins the tiles.  Backward, a piece of the
 // vocabulary at a time: the logits again, from them P (to bf16, or three bf16 parts of
-// an fp32 result), by rows and by columns, then the two products.  What counts for
-// all of them: the products' operations on the matrix instruction (osm_gemm.h); the
-// tokens that do not count are left out first, so they cost nothing.
+// an fp32 result), then the two products, which read W, P and H by columns where they
+// have to.  What counts for all of them: the products' operations on the matrix
+// instruction (osm_gemm.h); the tokens that do not count are left out first, so they
+// cost nothing.  Exponentials and logarithms are those of 2: l log2(e) less the largest
+// is one fused operation, and what its rounding leaves out cancels in the loss.
 #include <algorithm>
 #include <type_traits>
 
@@ -20,12 +22,11 @@
 namespace osm {
 namespace {
 
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr float kLog2e = 1.44269504f, kInf = __builtin_inff();
+constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f, kInf = __builtin_inff();
 
-__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // ---- operands ----
 
@@ -68,7 +69,7 @@ bool whole_units(const void* p, int64_t stride, int64_t D) {
 // The tokens that count, one after the other: a block takes `each` tokens, counts those
 // before them, and writes where its own go, and their hidden rows.
 template <typename T, int PARTS>
-__global__ void __launch_bounds__(256) loss_rows_kernel(const LossParams p, int64_t each, bool vec) {
+__global__ void __launch_bounds__(256) loss_rows_kernel(const LossParams p, int64_t each, bool vec, bool bwd) {
   __shared__ int sums[4];
   __shared__ int rows[256];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -99,7 +100,9 @@ __global__ void __launch_bounds__(256) loss_rows_kernel(const LossParams p, int6
     const bool in = i < t1 && p.targets[i] != p.ignore;
     const int first = base, at = in_order(in, base);
     if (in) {
-      p.tok.rows[at] = (int)i;
+      const int64_t target = p.targets[i];
+      p.tok.targets[at] = target >= 0 && target < p.V ? (int)target : -1;
+      if (bwd) p.tok.factors[at] = make_float2(p.lse[i] * kLog2e, p.grad_losses ? p.grad_losses[i] : 1.0f);
       rows[at - first] = (int)i;
     }
     if (i < t1) p.tok.places[i] = in ? at : -1;
@@ -116,9 +119,14 @@ __global__ void __launch_bounds__(256) loss_rows_kernel(const LossParams p, int6
       }
     }
   }
-  if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) {
-    p.tok.count[0] = base;
-    p.tok.count[1] = 0;   // blocks of the join that are done
+  if (blockIdx.x < gridDim.x - 1) return;
+  if (threadIdx.x == 0) *p.tok.count = base;
+  // zeros up to a whole step of the products over tokens
+  const int over = (base + kStep - 1) / kStep * kStep - base;
+  for (int u = threadIdx.x; u < PARTS * over * units; u += 256) {
+    const int q = u / (over * units), r = u - q * over * units;
+    *reinterpret_cast<bf16x8*>(p.h + ((int64_t)q * p.Npad + base) * p.Dpad + 8 * (int64_t)r) = bf16x8{};
+    wide_store_wait();
   }
 }
 
@@ -139,42 +147,6 @@ __global__ void __launch_bounds__(256) loss_pack_kernel(const T* from, int64_t s
   }
 }
 
-// 64 x 64 of a matrix by its columns: to[c][r] = from[r][c], zeros for r past `rows`
-// (with `count`: past that), up to to_ld.
-__global__ void __launch_bounds__(256) loss_transpose_kernel(const __bf16* from, int64_t ld, int64_t from_part, int rows,
-                                                             const int* count, int cols, __bf16* to, int to_ld, int64_t to_part) {
-  __shared__ __bf16 t[64][66];
-  if (count) {
-    rows = *count;
-    if ((int)blockIdx.x * 64 >= rows) return;   // (nothing reads past the last step that holds a row)
-  }
-  from += blockIdx.z * from_part;
-  to += blockIdx.z * to_part;
-  const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
-  for (int i = threadIdx.x; i < 64 * 8; i += 256) {
-    const int r = i / 8, c = i % 8 * 8;
-    bf16x8 v = {};
-    if (r0 + r < rows && c0 + c + 8 <= cols) {
-      v = *reinterpret_cast<const bf16x8*>(from + (int64_t)(r0 + r) * ld + c0 + c);
-    } else if (r0 + r < rows) {
-      for (int k = 0; k < 8; ++k)
-        if (c0 + c + k < cols) v[k] = from[(int64_t)(r0 + r) * ld + c0 + c + k];
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) t[r][c + k] = v[k];
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < 64 * 8; i += 256) {
-    const int c = i / 8, r = i % 8 * 8;
-    if (c0 + c >= cols || r0 + r >= to_ld) continue;
-    bf16x8 v;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = t[r + k][c];
-    *reinterpret_cast<bf16x8*>(to + (int64_t)(c0 + c) * to_ld + r0 + r) = v;
-    wide_store_wait();
-  }
-}
-
 // ---- products ----
 
 // A block's tile (m, n) of tm by tn: the XCDs, to which blocks go in turn, take
@@ -190,7 +162,7 @@ __device__ __forceinline__ bool tile_of(int tm, int tn, int& m, int& n) {
 }
 unsigned grid_of(int64_t tm, int64_t tn) { return (unsigned)((tm * tn + 7) / 8 * 8); }
 
-GemmSide side(const __bf16* p, int64_t ld, int64_t part, int rows) { return {p, ld, part, rows}; }
+GemmSide side(const __bf16* p, int64_t ld, int64_t part, int rows, int cols) { return {p, ld, part, rows, cols}; }
 
 struct Product {
   GemmSide a, b;
@@ -199,7 +171,7 @@ struct Product {
 
 // Logits of a tile: A the piece's classes, B the tokens that count.  BWD false: the
 // tile's largest logit and sum of exponentials for each token, and the target's logit.
-// BWD true: P and its transpose.
+// BWD true: P.
 template <class G, int PARTS, bool BWD>
 __global__ void __launch_bounds__(G::kThreads) loss_logits_kernel(const LossParams p, const Product g) {
   __shared__ __attribute__((aligned(16))) __bf16 lds[G::kLds];
@@ -207,34 +179,46 @@ __global__ void __launch_bounds__(G::kThreads) loss_logits_kernel(const LossPara
   if (!tile_of(g.tm, g.tn, tm, tn)) return;
   const int count = *p.tok.count, m0 = tm * G::TM, n0 = tn * G::TN;
   if (n0 >= count) return;
-  f32x16 acc[G::FM][G::FN];
-  gemm<G>(g.a, g.b, m0, n0, 0, p.Dpad / kStep, PARTS, lds, acc);
   const GemmPlace<G> q;
+  const int rows = p.vn - m0;   // of the tile that are classes
+  // Of column j's token: its target as a row of the tile, -1 if it is none that this wave
+  // holds, and its factors.  (Read here: after the product nothing would hide the way.)
+  int aim[G::FN];
+  float2 factors[G::FN];
+#pragma unroll
+  for (int j = 0; j < G::FN; ++j) {
+    const int n = min(n0 + q.col(j), count - 1), t = p.tok.targets[n] - (int)p.v0 - m0;
+    aim[j] = n0 + q.col(j) < count && t >= q.m && t < min(q.m + G::TM / G::WM, rows) ? t : -1;
+    if (BWD) factors[j] = p.tok.factors[n];
+  }
+  f32x16 acc[G::FM][G::FN];
+  gemm<G, false, false>(g.a, g.b, m0, n0, 0, p.Dpad / kStep, PARTS, lds, acc);
+  // f(value, row) for the rows that a lane holds of column j; change: what it gives takes the value's place
+  auto each = [&](int j, auto f) {
+#pragma unroll
+    for (int s = 0; s < G::FM; ++s)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) f(acc[s][j][i], q.row(s, i));
+  };
+  auto change = [&](int j, auto f) {
+#pragma unroll
+    for (int s = 0; s < G::FM; ++s)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[s][j][i] = f(acc[s][j][i], q.row(s, i));
+  };
   if constexpr (!BWD) {
     float2* const red = reinterpret_cast<float2*>(lds);   // [WM][TN]
 #pragma unroll
     for (int j = 0; j < G::FN; ++j) {
-      const int n = n0 + q.col(j);
-      const int64_t target = n < count ? p.targets[p.tok.rows[n]] - p.v0 : -1;
+      if (rows < G::TM) change(j, [&](float l, int m) { return m < rows ? l : -kInf; });
+      if (__any(aim[j] >= 0)) each(j, [&](float l, int m) { if (m == aim[j]) p.own[n0 + q.col(j)] = l; });
       float top = -kInf, sum = 0.0f;
-#pragma unroll
-      for (int f = 0; f < G::FM; ++f)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int m = m0 + q.row(f, i);
-          if (m == target && m < p.vn) p.own[n] = acc[f][j][i];
-          top = m < p.vn ? __builtin_fmaxf(top, acc[f][j][i]) : top;
-        }
+      each(j, [&](float l, int) { top = __builtin_fmaxf(top, l); });
+      top = __builtin_fmaxf(top, __shfl_xor(top, 32)) * kLog2e;   // (the other half's rows)
       const float base = top == -kInf ? 0.0f : top;
-#pragma unroll
-      for (int f = 0; f < G::FM; ++f)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sum += m0 + q.row(f, i) < p.vn ? exp_of(acc[f][j][i] - base) : 0.0f;
-      // the other half's rows
-      const float top2 = __shfl_xor(top, 32), sum2 = __shfl_xor(sum, 32), both = __builtin_fmaxf(top, top2);
-      const float b2 = both == -kInf ? 0.0f : both;
-      sum = sum * exp_of(top - b2) + sum2 * exp_of(top2 - b2);
-      if (q.lane < 32) red[q.m / (G::TM / G::WM) * G::TN + q.col(j)] = make_float2(both, sum);
+      each(j, [&](float l, int) { sum += exp2_of(__builtin_fmaf(l, kLog2e, -base)); });
+      sum += __shfl_xor(sum, 32);
+      if (q.lane < 32) red[q.m / (G::TM / G::WM) * G::TN + q.col(j)] = make_float2(top, sum);
     }
     __syncthreads();
     for (int c = threadIdx.x; c < G::TN; c += G::kThreads) {
@@ -243,32 +227,24 @@ __global__ void __launch_bounds__(G::kThreads) loss_logits_kernel(const LossPara
       for (int w = 0; w < G::WM; ++w) top = __builtin_fmaxf(top, red[w * G::TN + c].x);
       const float b = top == -kInf ? 0.0f : top;
 #pragma unroll
-      for (int w = 0; w < G::WM; ++w) sum += red[w * G::TN + c].y * exp_of(red[w * G::TN + c].x - b);
+      for (int w = 0; w < G::WM; ++w) sum += red[w * G::TN + c].y * exp2_of(red[w * G::TN + c].x - b);
       p.stat[(int64_t)(p.tile0 + tm) * p.Npad + n0 + c] = make_float2(top, sum);
     }
   } else {
 #pragma unroll
     for (int j = 0; j < G::FN; ++j) {
       const int n = n0 + q.col(j);
-      const bool in = n < count;
-      const int token = in ? p.tok.rows[n] : 0;
-      const int64_t target = in ? p.targets[token] - p.v0 : -1;
-      const float lse = in ? p.lse[token] : 0.0f, f0 = in ? (p.grad_losses ? p.grad_losses[token] : 1.0f) : 0.0f;
-#pragma unroll
-      for (int f = 0; f < G::FM; ++f)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int m = m0 + q.row(f, i);
-          const float e = exp_of(acc[f][j][i] - lse) - (m == target ? 1.0f : 0.0f);
-          acc[f][j][i] = in && m < p.vn ? e * f0 : 0.0f;
-        }
+      change(j, [&](float l, int) { return exp2_of(__builtin_fmaf(l, kLog2e, -factors[j].x)); });
+      if (__any(aim[j] >= 0)) change(j, [&](float e, int m) { return m == aim[j] ? e - 1.0f : e; });
+      if (p.grad_losses) change(j, [&](float e, int) { return e * factors[j].y; });
+      if (rows < G::TM || n0 + G::TN > count) change(j, [&](float e, int m) { return n < count && m < rows ? e : 0.0f; });
     }
-    constexpr int kRowUnits = G::TM / 8, kColUnits = G::TN / 8;
+    constexpr int kRowUnits = G::TM / 8;
     static_assert(G::TM * G::TN <= G::kLds, "a tile of P fits");
 #pragma unroll 1
     for (int part = 0; part < PARTS; ++part) {
-      // by tokens: a lane's four neighbouring classes are half a 16-byte unit, which lies
-      // at its index xor its row's
+      // a lane's four neighbouring classes are half a 16-byte unit, which lies at its index
+      // xor its token's; what the next part is made of stays in acc
 #pragma unroll
       for (int j = 0; j < G::FN; ++j)
 #pragma unroll
@@ -278,10 +254,14 @@ __global__ void __launch_bounds__(G::kThreads) loss_logits_kernel(const LossPara
             const int c = q.col(j), r = q.row(f, i);
             bf16x4 v;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = (__bf16)acc[f][j][i + k];
+            for (int k = 0; k < 4; ++k) {
+              v[k] = (__bf16)acc[f][j][i + k];
+              if (PARTS > 1) acc[f][j][i + k] -= (float)v[k];
+            }
             *reinterpret_cast<bf16x4*>(lds + c * G::TM + ((r / 8) ^ (c % kRowUnits)) * 8 + r % 8) = v;
           }
       __syncthreads();
+#pragma unroll 4
       for (int u = threadIdx.x; u < G::TN * kRowUnits; u += G::kThreads) {
         const int c = u / kRowUnits, r = u % kRowUnits;
         const bf16x8 v = *reinterpret_cast<const bf16x8*>(lds + c * G::TM + (r ^ (c % kRowUnits)) * 8);
@@ -290,34 +270,12 @@ __global__ void __launch_bounds__(G::kThreads) loss_logits_kernel(const LossPara
           wide_store_wait();
         }
       }
-      __syncthreads();
-      // by classes; what the next part is made of stays in acc
-#pragma unroll
-      for (int j = 0; j < G::FN; ++j)
-#pragma unroll
-        for (int f = 0; f < G::FM; ++f)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int c = q.col(j), r = q.row(f, i);
-            const __bf16 v = (__bf16)acc[f][j][i];
-            lds[r * G::TN + ((c / 8) ^ (r % kColUnits)) * 8 + c % 8] = v;
-            if (PARTS > 1) acc[f][j][i] -= (float)v;
-          }
-      __syncthreads();
-      for (int u = threadIdx.x; u < G::TM * kColUnits; u += G::kThreads) {
-        const int r = u / kColUnits, c = u % kColUnits;
-        const bf16x8 v = *reinterpret_cast<const bf16x8*>(lds + r * G::TN + (c ^ (r % kColUnits)) * 8);
-        if (m0 + r < p.vpad) {
-          *reinterpret_cast<bf16x8*>(p.pt + ((int64_t)part * p.vpad + m0 + r) * p.Npad + n0 + c * 8) = v;
-          wide_store_wait();
-        }
-      }
-      __syncthreads();
+      if (part + 1 < PARTS) __syncthreads();
     }
   }
 }
 
-// dH of a piece: A the weights by column, B P; a split takes a share of the classes and
+// dH of a piece: A the weights by columns, B P; a split takes a share of the classes and
 // adds to sums of its own.
 template <class G, int PARTS>
 __global__ void __launch_bounds__(G::kThreads) loss_dh_kernel(const LossParams p, const Product g) {
@@ -328,7 +286,7 @@ __global__ void __launch_bounds__(G::kThreads) loss_dh_kernel(const LossParams p
   if (n0 >= count) return;
   const int all = p.vpad / kStep, each = (all + p.splits - 1) / p.splits, s0 = min((int)blockIdx.y * each, all);
   f32x16 acc[G::FM][G::FN];
-  gemm<G>(g.a, g.b, m0, n0, (int64_t)s0 * kStep, min(each, all - s0), PARTS, lds, acc);
+  gemm<G, true, false>(g.a, g.b, m0, n0, (int64_t)s0 * kStep, min(each, all - s0), PARTS, lds, acc);
   const GemmPlace<G> q;
 #pragma unroll
   for (int j = 0; j < G::FN; ++j) {
@@ -351,7 +309,7 @@ __device__ __forceinline__ float factor(const LossParams& p) {
   return (p.grad ? *p.grad : 1.0f) / (p.count_in ? *p.count_in : 1.0f);
 }
 
-// dW of a piece: A the hidden rows by column, B P by classes.
+// dW of a piece: A the hidden rows, B P, both by columns.
 template <class G, int PARTS, typename T>
 __global__ void __launch_bounds__(G::kThreads) loss_dw_kernel(const LossParams p, const Product g) {
   __shared__ __attribute__((aligned(16))) __bf16 lds[G::kLds];
@@ -359,7 +317,7 @@ __global__ void __launch_bounds__(G::kThreads) loss_dw_kernel(const LossParams p
   if (!tile_of(g.tm, g.tn, tm, tn)) return;
   const int m0 = tm * G::TM, n0 = tn * G::TN;
   f32x16 acc[G::FM][G::FN];
-  gemm<G>(g.a, g.b, m0, n0, 0, (*p.tok.count + kStep - 1) / kStep, PARTS, lds, acc);
+  gemm<G, true, true>(g.a, g.b, m0, n0, 0, (*p.tok.count + kStep - 1) / kStep, PARTS, lds, acc);
   const float s = factor(p);
   const GemmPlace<G> q;
   typedef T V4 __attribute__((ext_vector_type(4)));
@@ -396,59 +354,55 @@ __global__ void __launch_bounds__(G::kThreads) loss_dw_kernel(const LossParams p
 constexpr int kJoinTokens = 16, kJoinSlices = 16;
 
 // A token's statistics over the vocabulary's tiles, 16 threads a token; zeros of those
-// that do not count.  With `loss`: the block that is done last adds the losses, in double
-// and in an order that does not depend on timing.
+// that do not count.
 __global__ void __launch_bounds__(kJoinTokens * kJoinSlices) loss_join_kernel(const LossParams p, int tiles) {
   __shared__ float2 red[kJoinSlices][kJoinTokens];
   const int c = threadIdx.x % kJoinTokens, s = threadIdx.x / kJoinTokens;
   const int64_t token = (int64_t)blockIdx.x * kJoinTokens + c;
   const int at = token < p.N ? p.tok.places[token] : -1;
   float top = -kInf, sum = 0.0f;
-  if (at >= 0)
+  if (at >= 0) {
+#pragma unroll 4
     for (int t = s; t < tiles; t += kJoinSlices) {
       const float2 v = p.stat[(int64_t)t * p.Npad + at];
       const float both = __builtin_fmaxf(top, v.x), b = both == -kInf ? 0.0f : both;
-      sum = sum * exp_of(top - b) + v.y * exp_of(v.x - b);
+      sum = sum * exp2_of(top - b) + v.y * exp2_of(v.x - b);
       top = both;
     }
+  }
   red[s][c] = make_float2(top, sum);
   __syncthreads();
-  if (s == 0 && token < p.N) {
-    float loss = 0.0f, lse = 0.0f;
-    if (at >= 0) {
-      for (int k = 1; k < kJoinSlices; ++k) top = __builtin_fmaxf(top, red[k][c].x);
-      const float b = top == -kInf ? 0.0f : top;
-      sum = 0.0f;
-      for (int k = 0; k < kJoinSlices; ++k) sum += red[k][c].y * exp_of(red[k][c].x - b);
-      const int64_t target = p.targets[token];
-      const bool known = target >= 0 && target < p.V;
-      const float l = logf(sum);
-      lse = known ? b + l : __builtin_nanf("");
-      loss = known ? l - (p.own[at] - b) : __builtin_nanf("");   // (small losses keep their digits)
-    }
-    p.lse[token] = lse;
-    if (p.losses) __hip_atomic_store(p.losses + token, loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (s > 0 || token >= p.N) return;
+  float loss = 0.0f, lse = 0.0f;
+  if (at >= 0) {
+    for (int k = 1; k < kJoinSlices; ++k) top = __builtin_fmaxf(top, red[k][c].x);
+    const float b = top == -kInf ? 0.0f : top;
+    sum = 0.0f;
+    for (int k = 0; k < kJoinSlices; ++k) sum += red[k][c].y * exp2_of(red[k][c].x - b);
+    const int64_t target = p.targets[token];
+    const bool known = target >= 0 && target < p.V;
+    const float l = log2f(sum);
+    lse = known ? (b + l) * kLn2 : __builtin_nanf("");
+    // (small losses keep their digits)
+    loss = known ? (l - __builtin_fmaf(p.own[at], kLog2e, -b)) * kLn2 : __builtin_nanf("");
   }
-  if (!p.loss) return;
-  __shared__ int is_last;
-  __shared__ double part[kJoinTokens * kJoinSlices];
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) is_last = atomicAdd(p.tok.count + 1, 1) == (int)gridDim.x - 1;
-  __syncthreads();
-  if (!is_last) return;
-  __threadfence();
-  double d = 0.0;
-  for (int64_t i = threadIdx.x; i < p.N; i += kJoinTokens * kJoinSlices)
-    d += __hip_atomic_load(p.losses + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  part[threadIdx.x] = d;
-  for (int w = kJoinTokens * kJoinSlices / 2; w > 0; w >>= 1) {
+  p.lse[token] = lse;
+  if (p.losses) p.losses[token] = loss;
+}
+
+// The sum of the losses in double, one workgroup, in an order that does not depend on timing.
+__global__ void __launch_bounds__(1024) loss_total_kernel(const LossParams p) {
+  __shared__ double red[1024];
+  double s = 0.0;
+  for (int64_t i = threadIdx.x; i < p.N; i += 1024) s += p.losses[i];
+  red[threadIdx.x] = s;
+  for (int w = 512; w > 0; w >>= 1) {
     __syncthreads();
-    if ((int)threadIdx.x < w) part[threadIdx.x] += part[threadIdx.x + w];
+    if ((int)threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
   }
   if (threadIdx.x == 0) {
-    const float n = (float)max(p.tok.count[0], 1);
-    *p.loss = (float)(p.mean ? part[0] / n : part[0]);
+    const float n = (float)max(*p.tok.count, 1);
+    *p.loss = (float)(p.mean ? red[0] / n : red[0]);
     if (p.count) *p.count = n;
   }
 }
@@ -493,18 +447,19 @@ __global__ void __launch_bounds__(256) loss_zero_kernel(T* to, int64_t n) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) to[i] = (T)0.0f;
 }
 
-using Big = GemmTile<256, 256, 2, 4>;
+using Big = GemmTile<256, 256, 4, 2>;
 using Middle = GemmTile<128, 128, 2, 2>;
 using Small = GemmTile<128, 64, 2, 2>;
 constexpr int kCUs = 256;
 
-// The largest tile that still gives every CU one, else the smallest.
-template <typename F>
+// The largest tile that still gives most CUs one, else the smallest.  (BIG false: without
+// the largest, whose accumulators leave no registers for what is made of them.)
+template <bool BIG = true, typename F>
 void by_size(int64_t M, int64_t N, F f) {
   auto tiles = [&](int64_t tm, int64_t tn) { return (M + tm - 1) / tm * ((N + tn - 1) / tn); };
-  if (tiles(256, 256) >= kCUs * 3 / 4)
-    f(Big{});
-  else if (tiles(128, 128) >= kCUs * 3 / 4)
+  if constexpr (BIG)
+    if (tiles(256, 256) >= kCUs * 3 / 4) return f(Big{});
+  if (tiles(128, 128) >= kCUs * 3 / 4)
     f(Middle{});
   else
     f(Small{});
@@ -525,12 +480,13 @@ void by_parts(int parts, F f) {
 
 template <bool BWD>
 hipError_t logits(const LossParams& p, hipStream_t stream) {
-  by_size(BWD ? p.vpad : p.V, p.N, [&](auto g) {
-    using G = decltype(g);
-    const Product t = product<G>(side(p.w, p.w_ld, p.w_part, p.vn), side(p.h, p.Dpad, (int64_t)p.Npad * p.Dpad, p.Npad),
-                                 BWD ? p.vpad : p.vn, p.N);
-    by_parts(p.parts, [&](auto n) {
-      hipLaunchKernelGGL((loss_logits_kernel<G, decltype(n)::value, BWD>), dim3(grid_of(t.tm, t.tn)), dim3(G::kThreads), 0, stream, p, t);
+  by_parts(p.parts, [&](auto n) {
+    constexpr int PARTS = decltype(n)::value;
+    by_size<!BWD || PARTS == 1>(BWD ? p.vpad : p.V, p.N, [&](auto g) {
+      using G = decltype(g);
+      const Product t = product<G>(side(p.w, p.w_ld, p.w_part, p.vn, 0), side(p.h, p.Dpad, (int64_t)p.Npad * p.Dpad, p.Npad, 0),
+                                   BWD ? p.vpad : p.vn, p.N);
+      hipLaunchKernelGGL((loss_logits_kernel<G, PARTS, BWD>), dim3(grid_of(t.tm, t.tn)), dim3(G::kThreads), 0, stream, p, t);
     });
   });
   return hipGetLastError();
@@ -538,14 +494,14 @@ hipError_t logits(const LossParams& p, hipStream_t stream) {
 
 }  // namespace
 
-hipError_t launch_loss_rows(const LossParams& p, int dtype, hipStream_t stream) {
+hipError_t launch_loss_rows(const LossParams& p, int dtype, bool bwd, hipStream_t stream) {
   // (blocks count what is before their tokens: at most 512 of them where there are many)
   const int64_t each = std::max<int64_t>(16, (p.N + 511) / 512);
   const dim3 grid((unsigned)((p.N + each - 1) / each));
   if (dtype == 0)
-    hipLaunchKernelGGL((loss_rows_kernel<float, 3>), grid, dim3(256), 0, stream, p, each, whole_units<float>(p.hidden, p.hidden_s, p.D));
+    hipLaunchKernelGGL((loss_rows_kernel<float, 3>), grid, dim3(256), 0, stream, p, each, whole_units<float>(p.hidden, p.hidden_s, p.D), bwd);
   else
-    hipLaunchKernelGGL((loss_rows_kernel<__bf16, 1>), grid, dim3(256), 0, stream, p, each, whole_units<__bf16>(p.hidden, p.hidden_s, p.D));
+    hipLaunchKernelGGL((loss_rows_kernel<__bf16, 1>), grid, dim3(256), 0, stream, p, each, whole_units<__bf16>(p.hidden, p.hidden_s, p.D), bwd);
   return hipGetLastError();
 }
 
@@ -566,13 +522,6 @@ hipError_t launch_loss_weight(const LossParams& p, __bf16* to, int dtype, hipStr
   return hipGetLastError();
 }
 
-hipError_t launch_loss_transpose(const __bf16* from, int64_t ld, int64_t from_part, int rows, const int* count, int cols, __bf16* to,
-                                 int to_ld, int64_t to_part, int parts, hipStream_t stream) {
-  hipLaunchKernelGGL(loss_transpose_kernel, dim3((unsigned)((to_ld + 63) / 64), (unsigned)((cols + 63) / 64), parts), dim3(256), 0, stream,
-                     from, ld, from_part, rows, count, cols, to, to_ld, to_part);
-  return hipGetLastError();
-}
-
 int loss_tile_rows(const LossParams& p) {
   int rows = 0;
   by_size(p.V, p.N, [&](auto g) { rows = decltype(g)::TM; });
@@ -585,6 +534,9 @@ hipError_t launch_loss_probs(const LossParams& p, hipStream_t stream) { return l
 hipError_t launch_loss_join(const LossParams& p, int tiles, hipStream_t stream) {
   hipLaunchKernelGGL(loss_join_kernel, dim3((unsigned)((p.N + kJoinTokens - 1) / kJoinTokens)), dim3(kJoinTokens * kJoinSlices), 0, stream,
                      p, tiles);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !p.loss) return e;
+  hipLaunchKernelGGL(loss_total_kernel, dim3(1), dim3(1024), 0, stream, p);
   return hipGetLastError();
 }
 
@@ -596,7 +548,7 @@ hipError_t launch_loss_none(float* loss, float* count, hipStream_t stream) {
 hipError_t launch_loss_dh(const LossParams& p, hipStream_t stream) {
   by_size((int64_t)p.Dpad * p.splits, p.N, [&](auto g) {
     using G = decltype(g);
-    const Product t = product<G>(side(p.wt, p.vpad, (int64_t)p.Dpad * p.vpad, (int)p.D), side(p.p, p.vpad, (int64_t)p.Npad * p.vpad, p.Npad),
+    const Product t = product<G>(side(p.w, p.w_ld, p.w_part, p.vn, p.Dpad), side(p.p, p.vpad, (int64_t)p.Npad * p.vpad, p.Npad, 0),
                                  p.D, p.N);
     by_parts(p.parts, [&](auto n) {
       hipLaunchKernelGGL((loss_dh_kernel<G, decltype(n)::value>), dim3(grid_of(t.tm, t.tn), p.splits), dim3(G::kThreads), 0, stream, p, t);
@@ -608,8 +560,8 @@ hipError_t launch_loss_dh(const LossParams& p, hipStream_t stream) {
 hipError_t launch_loss_dw(const LossParams& p, int dtype, hipStream_t stream) {
   by_size(p.D, p.vn, [&](auto g) {
     using G = decltype(g);
-    const Product t = product<G>(side(p.ht, p.Npad, (int64_t)p.Dpad * p.Npad, (int)p.D), side(p.pt, p.Npad, (int64_t)p.vpad * p.Npad, p.vpad),
-                                 p.D, p.vn);
+    const Product t = product<G>(side(p.h, p.Dpad, (int64_t)p.Npad * p.Dpad, p.Npad, p.Dpad),
+                                 side(p.p, p.vpad, (int64_t)p.Npad * p.vpad, p.Npad, p.vpad), p.D, p.vn);
     if (dtype == 0)
       hipLaunchKernelGGL((loss_dw_kernel<G, 3, float>), dim3(grid_of(t.tm, t.tn)), dim3(G::kThreads), 0, stream, p, t);
     else

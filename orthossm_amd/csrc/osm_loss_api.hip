@@ -60,11 +60,17 @@ struct Plan {
   bool direct;
 };
 
-// Pieces of about the same size, each of at most `most` classes.
-int64_t piece_of(int64_t V, int64_t most) {
-  most = std::max<int64_t>(kLossPad, std::min(most, kMaxRow - kLossPad) / kLossPad * kLossPad);
-  const int64_t n = (V + most - 1) / most;
-  return up((V + n - 1) / n, kLossPad);
+// Classes of a piece: its parts of P (or of the weights) are at most 2^28 elements.
+int64_t piece_of(int64_t V, int64_t rows) {
+  const int64_t most = std::min((int64_t(1) << 28) / rows, kMaxRow - 1) / kLossPad * kLossPad;
+  return std::min(std::max<int64_t>(most, kLossPad), up(V, kLossPad));
+}
+
+// The classes of the next of `left`: as many times 256 tiles of dW (a tile for every CU) as
+// a piece holds, then the rest.
+int64_t next_piece(int64_t left, int64_t piece, int64_t D) {
+  const int64_t wave = std::max<int64_t>(1, 256 / ((D + 255) / 256)) * 256, n = std::min(left, piece);
+  return n > wave ? n / wave * wave : n;
 }
 
 Plan plan_of(const osm_loss_args* a, bool bwd) {
@@ -73,10 +79,9 @@ Plan plan_of(const osm_loss_args* a, bool bwd) {
   n.Npad = up(std::max<int64_t>(a->N, 1), kLossPad);
   n.Dpad = up(a->D, 64);
   n.direct = direct(a);
-  // Backward: 2^27 elements of P.  Forward: as many of the weights' parts, or all classes at once.
-  n.piece = bwd ? piece_of(a->V, (int64_t(1) << 27) / (n.Npad * n.parts))
-                : n.direct ? up(a->V, kLossPad) : piece_of(a->V, (int64_t(1) << 27) / (n.Dpad * n.parts));
-  const int64_t tiles = ((a->D + 255) / 256) * (n.Npad / 256);
+  const int64_t across = (a->D + 255) / 256;
+  n.piece = bwd ? piece_of(a->V, n.Npad * n.parts) : n.direct ? up(a->V, kLossPad) : piece_of(a->V, n.Dpad * n.parts);
+  const int64_t tiles = across * (n.Npad / 256);
   n.splits = (int)std::max<int64_t>(1, std::min<int64_t>({256 / std::max<int64_t>(1, tiles), n.piece / 1024, 8}));
   return n;
 }
@@ -91,14 +96,15 @@ struct Regions {
   }
 };
 struct Layout {
-  size_t rows, places, count, h, w, own, stat, ht, wt, p, pt, dh, total;
+  size_t targets, factors, places, count, h, w, own, stat, p, dh, total;
 };
 Layout layout_of(const osm_loss_args* a, const Plan& n, bool bwd) {
   Regions r;
   Layout l{};
-  l.rows = r.add(a->N * 4);
+  l.targets = r.add(a->N * 4);
+  l.factors = r.add(bwd ? a->N * 8 : 0);
   l.places = r.add(a->N * 4);
-  l.count = r.add(8);
+  l.count = r.add(4);
   const size_t hidden = (size_t)n.parts * n.Npad * n.Dpad * 2;
   l.h = r.add(hidden);
   l.w = r.add(n.direct ? 0 : (size_t)n.parts * n.piece * n.Dpad * 2);
@@ -106,10 +112,7 @@ Layout layout_of(const osm_loss_args* a, const Plan& n, bool bwd) {
     l.own = r.add(n.Npad * 4);
     l.stat = r.add((size_t)(up(a->V, kLossPad) / 64) * n.Npad * 8);
   } else {
-    l.ht = r.add(hidden);
-    l.wt = r.add((size_t)n.parts * n.Dpad * n.piece * 2);
     l.p = r.add((size_t)n.parts * n.Npad * n.piece * 2);
-    l.pt = r.add((size_t)n.parts * n.Npad * n.piece * 2);
     l.dh = r.add((size_t)n.splits * n.Npad * n.Dpad * 4);
   }
   l.total = r.total;
@@ -137,16 +140,18 @@ LossParams params_of(const osm_loss_args* a, const Plan& n, const Layout& l, voi
   p.weight_s = a->weight_stride;
   p.targets = a->targets;
   p.ignore = a->ignore_index;
-  p.tok = {reinterpret_cast<int*>(w + l.rows), reinterpret_cast<int*>(w + l.places), reinterpret_cast<int*>(w + l.count)};
+  p.tok = {reinterpret_cast<int*>(w + l.targets), reinterpret_cast<float2*>(w + l.factors), reinterpret_cast<int*>(w + l.places),
+           reinterpret_cast<int*>(w + l.count)};
   p.h = reinterpret_cast<__bf16*>(w + l.h);
   p.lse = a->lse;
   return p;
 }
 
-// The piece of `n` classes from v0 on, and its weights' parts where they are not read in place.
-hipError_t set_piece(LossParams& p, const osm_loss_args* a, const Plan& n, const Layout& l, char* w, int64_t v0, hipStream_t st) {
+// The piece of vn classes from v0 on, and its weights' parts where they are not read in place.
+hipError_t set_piece(LossParams& p, const osm_loss_args* a, const Plan& n, const Layout& l, char* w, int64_t v0, int64_t vn,
+                     hipStream_t st) {
   p.v0 = v0;
-  p.vn = (int)std::min(n.piece, a->V - v0);
+  p.vn = (int)vn;
   p.vpad = (int)up(p.vn, kLossPad);
   if (n.direct) {
     p.w = static_cast<const __bf16*>(a->weight) + v0 * a->weight_stride;
@@ -172,12 +177,14 @@ hipError_t forward(const osm_loss_args* a, const Plan& n, const Layout& l, void*
   p.loss = a->loss;
   p.count = a->count;
   p.mean = (a->flags & OSM_LOSS_MEAN) != 0;
-  hipError_t e = osm::launch_loss_rows(p, a->dtype, st);
+  hipError_t e = osm::launch_loss_rows(p, a->dtype, false, st);
   if (e != hipSuccess) return e;
   const int rows = osm::loss_tile_rows(p);
   for (int64_t v0 = 0; v0 < a->V; v0 += n.piece) {
     p.tile0 = (int)(v0 / rows);
-    if ((e = set_piece(p, a, n, l, w, v0, st)) != hipSuccess || (e = osm::launch_loss_logits(p, st)) != hipSuccess) return e;
+    if ((e = set_piece(p, a, n, l, w, v0, std::min(n.piece, a->V - v0), st)) != hipSuccess ||
+        (e = osm::launch_loss_logits(p, st)) != hipSuccess)
+      return e;
   }
   return osm::launch_loss_join(p, (int)((a->V + rows - 1) / rows), st);
 }
@@ -185,10 +192,7 @@ hipError_t forward(const osm_loss_args* a, const Plan& n, const Layout& l, void*
 hipError_t backward(const osm_loss_args* a, const osm_loss_bwd_args* b, const Plan& n, const Layout& l, void* workspace, hipStream_t st) {
   char* const w = static_cast<char*>(workspace);
   LossParams p = params_of(a, n, l, workspace);
-  p.ht = reinterpret_cast<__bf16*>(w + l.ht);
-  p.wt = reinterpret_cast<__bf16*>(w + l.wt);
   p.p = reinterpret_cast<__bf16*>(w + l.p);
-  p.pt = reinterpret_cast<__bf16*>(w + l.pt);
   p.dh = reinterpret_cast<float*>(w + l.dh);
   p.splits = n.splits;
   p.grad = b->grad;
@@ -196,19 +200,13 @@ hipError_t backward(const osm_loss_args* a, const osm_loss_bwd_args* b, const Pl
   p.count_in = b->count;
   p.grad_h = b->grad_hidden;
   p.grad_w = b->grad_weight;
-  hipError_t e = osm::launch_loss_rows(p, a->dtype, st);
+  hipError_t e = osm::launch_loss_rows(p, a->dtype, true, st);
   if (e != hipSuccess) return e;
-  if (b->grad_weight && (e = osm::launch_loss_transpose(p.h, n.Dpad, (int64_t)n.Npad * n.Dpad, (int)n.Npad, p.tok.count, (int)a->D, p.ht,
-                                                        (int)n.Npad, (int64_t)n.Dpad * n.Npad, (int)n.parts, st)) != hipSuccess)
-    return e;
-  for (int64_t v0 = 0; v0 < a->V; v0 += n.piece) {
+  for (int64_t v0 = 0, vn; v0 < a->V; v0 += vn) {
+    vn = next_piece(a->V - v0, n.piece, a->D);
     p.first = v0 == 0;
-    if ((e = set_piece(p, a, n, l, w, v0, st)) != hipSuccess || (e = osm::launch_loss_probs(p, st)) != hipSuccess) return e;
-    if (b->grad_hidden &&
-        ((e = osm::launch_loss_transpose(p.w, p.w_ld, p.w_part, p.vn, nullptr, (int)a->D, p.wt, p.vpad, (int64_t)n.Dpad * p.vpad, (int)n.parts,
-                                         st)) != hipSuccess ||
-         (e = osm::launch_loss_dh(p, st)) != hipSuccess))
-      return e;
+    if ((e = set_piece(p, a, n, l, w, v0, vn, st)) != hipSuccess || (e = osm::launch_loss_probs(p, st)) != hipSuccess) return e;
+    if (b->grad_hidden && (e = osm::launch_loss_dh(p, st)) != hipSuccess) return e;
     if (b->grad_weight && (e = osm::launch_loss_dw(p, a->dtype, st)) != hipSuccess) return e;
   }
   return b->grad_hidden ? osm::launch_loss_finish(p, a->dtype, st) : hipSuccess;
