@@ -66,9 +66,10 @@ int check_inputs(const osm_ema_args* a) {
   if (a->B > 0 && a->S > 0 &&
       ((rc = check_seq(a->x, es, a->S, "x")) != OSM_OK || (rc = check_seq(a->gate, es, a->S, "gate")) != OSM_OK))
     return rc;
-  const void* words[4] = {a->lengths, a->state_init, a->state_out, a->saved};
+  const void* words[3] = {a->lengths, a->state_init, a->state_out};
   for (const void* w : words)
-    if ((uintptr_t)w % 4) return fail(OSM_E_LAYOUT, "lengths, states and saved must be 4-byte aligned");
+    if ((uintptr_t)w % 4) return fail(OSM_E_LAYOUT, "lengths and states must be 4-byte aligned");
+  if ((uintptr_t)a->saved % 256) return fail(OSM_E_LAYOUT, "saved must be 256-byte aligned");
   return OSM_OK;
 }
 

@@ -107,15 +107,24 @@ __global__ void __launch_bounds__(256) loss_rows_kernel(const LossParams p, int6
     }
     if (i < t1) p.tok.places[i] = in ? at : -1;
     __syncthreads();
-    const int n = base - first;
-    for (int u = threadIdx.x; u < n * units; u += 256) {
-      const int r = u / units, c = u - r * units;
-      bf16x8 out[PARTS];
-      split_unit<T, PARTS>(static_cast<const T*>(p.hidden) + rows[r] * p.hidden_s, 8 * c, (int)p.D, vec, out);
+    const int n = (base - first) * units;
+    constexpr int kAtOnce = 4;   // (loads on their way)
+    for (int u0 = threadIdx.x; u0 < n; u0 += 256 * kAtOnce) {
+      bf16x8 out[kAtOnce][PARTS];
 #pragma unroll
-      for (int q = 0; q < PARTS; ++q) {
-        *reinterpret_cast<bf16x8*>(p.h + ((int64_t)q * p.Npad + first + r) * p.Dpad + 8 * c) = out[q];
-        wide_store_wait();
+      for (int k = 0; k < kAtOnce; ++k) {
+        const int u = min(u0 + 256 * k, n - 1), r = u / units;
+        split_unit<T, PARTS>(static_cast<const T*>(p.hidden) + rows[r] * p.hidden_s, 8 * (u - r * units), (int)p.D, vec, out[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const int u = u0 + 256 * k;
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q)
+          if (u < n) {
+            *reinterpret_cast<bf16x8*>(p.h + ((int64_t)q * p.Npad + first) * p.Dpad + 8 * (int64_t)u) = out[k][q];
+            wide_store_wait();
+          }
       }
     }
   }
@@ -452,14 +461,15 @@ using Middle = GemmTile<128, 128, 2, 2>;
 using Small = GemmTile<128, 64, 2, 2>;
 constexpr int kCUs = 256;
 
-// The largest tile that still gives most CUs one, else the smallest.  (BIG false: without
+// The largest tile of which most CUs get what they hold, one of the largest or two of the
+// next, else the smallest.  (BIG false: without
 // the largest, whose accumulators leave no registers for what is made of them.)
 template <bool BIG = true, typename F>
 void by_size(int64_t M, int64_t N, F f) {
   auto tiles = [&](int64_t tm, int64_t tn) { return (M + tm - 1) / tm * ((N + tn - 1) / tn); };
   if constexpr (BIG)
     if (tiles(256, 256) >= kCUs * 3 / 4) return f(Big{});
-  if (tiles(128, 128) >= kCUs * 3 / 4)
+  if (tiles(128, 128) >= kCUs * 3 / 2)
     f(Middle{});
   else
     f(Small{});
@@ -495,8 +505,8 @@ hipError_t logits(const LossParams& p, hipStream_t stream) {
 }  // namespace
 
 hipError_t launch_loss_rows(const LossParams& p, int dtype, bool bwd, hipStream_t stream) {
-  // (blocks count what is before their tokens: at most 512 of them where there are many)
-  const int64_t each = std::max<int64_t>(16, (p.N + 511) / 512);
+  // (a block counts what is before its tokens, so that there are at most 1024 of them)
+  const int64_t each = std::max<int64_t>(4, (p.N + 1023) / 1024);
   const dim3 grid((unsigned)((p.N + each - 1) / each));
   if (dtype == 0)
     hipLaunchKernelGGL((loss_rows_kernel<float, 3>), grid, dim3(256), 0, stream, p, each, whole_units<float>(p.hidden, p.hidden_s, p.D), bwd);

@@ -81,12 +81,13 @@ __device__ __forceinline__ void store_piece(T* p, const float (&f)[U], int c, in
   }
 }
 
-// e^-|v| once; both values to fp32's accuracy.
+// Both off by |v| 2^-24 and a few units of 2^-24 (the hardware's reciprocal: the exact
+// division takes twice the instructions of all the rest).
 struct Gate {
   float o, rest;   // sigmoid(v), sigmoid(-v)
 };
 __device__ __forceinline__ Gate gate_of(float v) {
-  const float e = __expf(-__builtin_fabsf(v)), r = 1.0f / (1.0f + e), s = e * r;
+  const float e = __builtin_amdgcn_exp2f(-1.44269504f * __builtin_fabsf(v)), r = __builtin_amdgcn_rcpf(1.0f + e), s = e * r;
   return v >= 0.0f ? Gate{r, s} : Gate{s, r};
 }
 
@@ -128,17 +129,46 @@ __device__ __forceinline__ void normalise(float (&v)[NV][U], int D, int u, float
     for (int i = 0; i < U; ++i) v[k][i] *= rs;
 }
 
-// fp32 parameters of a thread's columns; `fill` where there are none, zeros past the row's end.
-template <int TPR, int NV, int U>
-__device__ __forceinline__ void param(float (&v)[NV][U], const float* w, float fill, int D, int u) {
+// COUNT fp32 parameters of a row's columns, in LDS while that leaves room for two
+// workgroups a CU (rows up to 4096), else in registers; `fill` where there are none, zeros
+// past the row's end.
+template <int TPR, int NV, int U, int COUNT>
+struct Params {
+  static constexpr int kCols = TPR * NV * U;
+  static constexpr bool kShared = kCols <= 4096;
+  typedef float Four __attribute__((ext_vector_type(4)));
+  float own[kShared ? 1 : COUNT][NV][U];
+  float* lds;
+  int u;
+  static constexpr int kLds = kShared ? COUNT * kCols : 1;
+  __device__ __forceinline__ Params(float* s, int thread) : lds(s), u(thread) {}
+  __device__ __forceinline__ void set(int which, const float* w, float fill, int D) {
+    if constexpr (kShared) {
+      for (int c = threadIdx.x; c < kCols; c += blockDim.x) lds[which * kCols + c] = c < D ? (w ? w[c] : fill) : 0.0f;
+    } else {
 #pragma unroll
-  for (int k = 0; k < NV; ++k)
+      for (int k = 0; k < NV; ++k)
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int c = (u + k * TPR) * U + i;
-      v[k][i] = c < D ? (w ? w[c] : fill) : 0.0f;
+        for (int i = 0; i < U; ++i) {
+          const int c = (u + k * TPR) * U + i;
+          own[which][k][i] = c < D ? (w ? w[c] : fill) : 0.0f;
+        }
     }
-}
+  }
+  __device__ __forceinline__ void get(int which, int k, float (&v)[U]) const {
+    if constexpr (kShared) {
+#pragma unroll
+      for (int i = 0; i < U; i += 4) {
+        const Four f = *reinterpret_cast<const Four*>(lds + which * kCols + (u + k * TPR) * U + i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[i + j] = f[j];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < U; ++i) v[i] = own[which][k][i];
+    }
+  }
+};
 
 // TX: the residual stream's type, TY: the block's; TPR threads a row, max(TPR, 256)
 // a workgroup, units of U columns.
@@ -146,14 +176,12 @@ template <typename TX, typename TY, int U, int TPR, int NV>
 __global__ void __launch_bounds__(RowThreads<TPR>::kThreads) resnorm_fwd_kernel(const ResnormParams p) {
   constexpr int kRows = RowThreads<TPR>::kRows;
   __shared__ float red[2][16][1];
+  using P = Params<TPR, NV, U, 3>;
+  __shared__ __attribute__((aligned(16))) float shared[P::kLds];
   const int u = threadIdx.x % TPR, D = (int)p.D;
-  float w[NV][U], b[NV][U], sc[NV][U];
-  param<TPR>(w, p.weight, 1.0f, D, u);
-  param<TPR>(b, p.bias, 0.0f, D, u);
-  param<TPR>(sc, p.scale, 1.0f, D, u);
   const int64_t step = (int64_t)gridDim.x * kRows;
   int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
-  int par = 0;
+  int half = 0;
   Piece<TX, U> rx[NV];
   Piece<TY, U> ry[NV], rg[NV];
   auto fetch = [&](int64_t at) {
@@ -166,27 +194,34 @@ __global__ void __launch_bounds__(RowThreads<TPR>::kThreads) resnorm_fwd_kernel(
     }
   };
   if (row < p.rows) fetch(row);
+  P par(shared, u);
+  par.set(0, p.weight, 1.0f, D);
+  par.set(1, p.bias, 0.0f, D);
+  par.set(2, p.scale, 1.0f, D);
+  __syncthreads();
   // (every thread of a workgroup runs the same trips: kRows is 1 where row_sum has barriers)
   for (; row < p.rows; row += step) {
     float x[NV][U], y[NV][U], o[NV][U];
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
+    for (int k = 0; k < NV; ++k) {
+      par.get(2, k, o[k]);
 #pragma unroll
       for (int i = 0; i < U; ++i) {
         x[k][i] = rx[k].get(i);
         y[k][i] = ry[k].get(i);
-        o[k][i] = sc[k][i] * (p.gate ? gate_of(rg[k].get(i)).o : 1.0f);
+        if (p.gate) o[k][i] *= gate_of(rg[k].get(i)).o;
       }
+    }
     if (row + step < p.rows) fetch(row + step);
     float my = 0.0f, sy = 1.0f, mr, sr;
-    if (p.norm_y) normalise<TPR>(y, D, u, p.eps, p.rms, red, par, my, sy);
+    if (p.norm_y) normalise<TPR>(y, D, u, p.eps, p.rms, red, half, my, sy);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
 #pragma unroll
       for (int i = 0; i < U; ++i) x[k][i] = __builtin_fmaf(o[k][i], y[k][i], x[k][i]);
       store_piece<TX, U>(static_cast<TX*>(p.r) + row * p.r_s, x[k], (u + k * TPR) * U, D, p.vec);
     }
-    normalise<TPR>(x, D, u, p.eps, p.rms, red, par, mr, sr);
+    normalise<TPR>(x, D, u, p.eps, p.rms, red, half, mr, sr);
     if (p.stats && u == 0) {
       float* const st = p.stats + 4 * row;
       st[0] = my;
@@ -196,30 +231,33 @@ __global__ void __launch_bounds__(RowThreads<TPR>::kThreads) resnorm_fwd_kernel(
     }
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
+      float w[U], b[U];
+      par.get(0, k, w);
+      par.get(1, k, b);
 #pragma unroll
-      for (int i = 0; i < U; ++i) x[k][i] = __builtin_fmaf(x[k][i], w[k][i], b[k][i]);
+      for (int i = 0; i < U; ++i) x[k][i] = __builtin_fmaf(x[k][i], w[i], b[i]);
       store_piece<TY, U>(static_cast<TY*>(p.n) + row * p.n_s, x[k], (u + k * TPR) * U, D, p.vec);
     }
   }
 }
 
 template <typename TX, typename TY, int U, int TPR, int NV>
-__global__ void __launch_bounds__(RowThreads<TPR>::kThreads) resnorm_bwd_kernel(const ResnormParams p) {
+__global__ void __launch_bounds__(RowThreads<TPR>::kThreads, 2) resnorm_bwd_kernel(const ResnormParams p) {
   constexpr int kRows = RowThreads<TPR>::kRows;
+  using P = Params<TPR, NV, U, 2>;
   __shared__ float red[2][16][2];
+  __shared__ __attribute__((aligned(16))) float shared[P::kLds];
   const int u = threadIdx.x % TPR, D = (int)p.D;
-  float w[NV][U], sc[NV][U], dw[NV][U], db[NV][U], ds[NV][U];
-  param<TPR>(w, p.weight, 1.0f, D, u);
-  param<TPR>(sc, p.scale, 1.0f, D, u);
+  float dw[NV][U], db[NV][U], ds[NV][U];
 #pragma unroll
   for (int k = 0; k < NV; ++k)
 #pragma unroll
     for (int i = 0; i < U; ++i) dw[k][i] = db[k][i] = ds[k][i] = 0.0f;
   const int64_t step = (int64_t)gridDim.x * kRows;
   int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
-  int par = 0;
-  Piece<TX, U> rx[NV], rr[NV] = {};
-  Piece<TY, U> ry[NV], rg[NV] = {}, rn[NV] = {};
+  int half = 0;
+  Piece<TX, U> next_x[NV], next_r[NV] = {};
+  Piece<TY, U> next_y[NV], next_g[NV] = {}, next_n[NV] = {};
   float st[4];
   auto fetch = [&](int64_t at) {
 #pragma unroll
@@ -227,71 +265,88 @@ __global__ void __launch_bounds__(RowThreads<TPR>::kThreads) resnorm_bwd_kernel(
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int c = (u + k * TPR) * U;
-      ry[k].load(static_cast<const TY*>(p.y) + at * p.y_s, c, D, p.vec);
-      if (p.gate) rg[k].load(static_cast<const TY*>(p.gate) + at * p.gate_s, c, D, p.vec);
-      rx[k].load(static_cast<const TX*>(p.x) + at * p.x_s, c, D, p.vec);
-      if (p.gn) rn[k].load(static_cast<const TY*>(p.gn) + at * p.gn_s, c, D, p.vec);
-      if (p.gr) rr[k].load(static_cast<const TX*>(p.gr) + at * p.gr_s, c, D, p.vec);
+      next_y[k].load(static_cast<const TY*>(p.y) + at * p.y_s, c, D, p.vec);
+      if (p.gate) next_g[k].load(static_cast<const TY*>(p.gate) + at * p.gate_s, c, D, p.vec);
+      next_x[k].load(static_cast<const TX*>(p.x) + at * p.x_s, c, D, p.vec);
+      if (p.gn) next_n[k].load(static_cast<const TY*>(p.gn) + at * p.gn_s, c, D, p.vec);
+      if (p.gr) next_r[k].load(static_cast<const TX*>(p.gr) + at * p.gr_s, c, D, p.vec);
     }
   };
   if (row < p.rows) fetch(row);
+  P par(shared, u);
+  par.set(0, p.weight, 1.0f, D);
+  par.set(1, p.scale, 1.0f, D);
+  __syncthreads();
   for (; row < p.rows; row += step) {
-    float yh[NV][U], rh[NV][U], o[NV][U], rest[NV][U], g[NV][U], dr[NV][U];
+    // What the second pass takes again stays as it was loaded: its values are formed twice,
+    // in fewer registers.
+    Piece<TY, U> y[NV], gate[NV], n[NV];
+    Piece<TX, U> gr[NV];
+    float rh[NV][U], dr[NV][U];
     const float sy = st[1], sr = st[3], my = st[0], mr = st[2];
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
+    for (int k = 0; k < NV; ++k) {
+      y[k] = next_y[k];
+      gate[k] = next_g[k];
+      n[k] = next_n[k];
+      gr[k] = next_r[k];
+      float w[U], sc[U];
+      par.get(0, k, w);
+      par.get(1, k, sc);
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        const Gate q = p.gate ? gate_of(rg[k].get(i)) : Gate{1.0f, 0.0f};
-        o[k][i] = q.o;
-        rest[k][i] = q.rest;
-        yh[k][i] = (ry[k].get(i) - my) * sy;
+        const float o = p.gate ? gate_of(gate[k].get(i)).o : 1.0f, dn = n[k].get(i);
         // (the forward's r, to the last bit)
-        const float r = __builtin_fmaf(sc[k][i] * q.o, yh[k][i], rx[k].get(i));
+        const float r = __builtin_fmaf(sc[i] * o, (y[k].get(i) - my) * sy, next_x[k].get(i));
         rh[k][i] = (r - mr) * sr;
-        const float dn = rn[k].get(i);
         dw[k][i] = __builtin_fmaf(dn, rh[k][i], dw[k][i]);
         db[k][i] += dn;
-        g[k][i] = dn * w[k][i];          // zeros past the row's end: dn and w are
-        dr[k][i] = rr[k].get(i);
-        s[0] += g[k][i];
-        s[1] = __builtin_fmaf(g[k][i], rh[k][i], s[1]);
+        const float g = dn * w[i];       // zeros past the row's end: dn and w are
+        s[0] += g;
+        s[1] = __builtin_fmaf(g, rh[k][i], s[1]);
       }
+    }
     if (row + step < p.rows) fetch(row + step);
-    row_sum<TPR>(s, red[par]);
-    par ^= 1;
+    row_sum<TPR>(s, red[half]);
+    half ^= 1;
     float a = p.rms ? 0.0f : s[0] / (float)D, c = s[1] / (float)D;
     s[0] = s[1] = 0.0f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
+      float w[U], sc[U], dg[U];
+      par.get(0, k, w);
+      par.get(1, k, sc);
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        dr[k][i] += sr * (g[k][i] - a - rh[k][i] * c);
-        ds[k][i] = __builtin_fmaf(dr[k][i], yh[k][i] * o[k][i], ds[k][i]);
-        const float du = dr[k][i] * sc[k][i];   // zero past the row's end: sc is
-        g[k][i] = du * o[k][i];
-        rest[k][i] *= g[k][i] * yh[k][i];
-        s[0] += g[k][i];
-        s[1] = __builtin_fmaf(g[k][i], yh[k][i], s[1]);
+        const Gate q = p.gate ? gate_of(gate[k].get(i)) : Gate{1.0f, 0.0f};
+        const float yh = (y[k].get(i) - my) * sy;
+        dr[k][i] = gr[k].get(i) + sr * (n[k].get(i) * w[i] - a - rh[k][i] * c);
+        ds[k][i] = __builtin_fmaf(dr[k][i], yh * q.o, ds[k][i]);
+        const float e = dr[k][i] * sc[i] * q.o;   // zero past the row's end: sc is
+        dg[i] = q.rest * (e * yh);
+        s[0] += e;
+        s[1] = __builtin_fmaf(e, yh, s[1]);
+        rh[k][i] = e;
       }
       const int at = (u + k * TPR) * U;
       if (p.gx) store_piece<TX, U>(static_cast<TX*>(p.gx) + row * p.gx_s, dr[k], at, D, p.vec);
-      if (p.gg) store_piece<TY, U>(static_cast<TY*>(p.gg) + row * p.gg_s, rest[k], at, D, p.vec);
+      if (p.gg) store_piece<TY, U>(static_cast<TY*>(p.gg) + row * p.gg_s, dg, at, D, p.vec);
     }
     a = c = 0.0f;
     if (p.norm_y) {
-      row_sum<TPR>(s, red[par]);
-      par ^= 1;
+      row_sum<TPR>(s, red[half]);
+      half ^= 1;
       a = p.rms ? 0.0f : s[0] / (float)D;
       c = s[1] / (float)D;
     }
     if (p.gy)
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
+        float dy[U];
 #pragma unroll
-        for (int i = 0; i < U; ++i) g[k][i] = sy * (g[k][i] - a - yh[k][i] * c);
-        store_piece<TY, U>(static_cast<TY*>(p.gy) + row * p.gy_s, g[k], (u + k * TPR) * U, D, p.vec);
+        for (int i = 0; i < U; ++i) dy[i] = sy * (rh[k][i] - a - (y[k].get(i) - my) * sy * c);
+        store_piece<TY, U>(static_cast<TY*>(p.gy) + row * p.gy_s, dy, (u + k * TPR) * U, D, p.vec);
       }
   }
   // This workgroup's line of sums: its row groups in order.
@@ -523,15 +578,17 @@ void by_length(int64_t D, Go go, Long long_rows) {
     long_rows();
 }
 
-constexpr int kMaxGroups = 2048;
+constexpr int kMaxGroups = 8192;
 constexpr int kLastFwd = 16, kLastBwd = 8;   // elements of a thread where 1024 hold a row
 
-template <typename TY>
-constexpr int kUnit = 16 / (int)sizeof(TY);
+// Columns of a unit: 16 bytes of the wider type, so that a wave's accesses to either are
+// without gaps.
+template <typename TX>
+constexpr int kUnit = 16 / (int)sizeof(TX);
 
 template <typename TX, typename TY>
 hipError_t forward(const ResnormParams& p, hipStream_t stream) {
-  constexpr int U = kUnit<TY>;
+  constexpr int U = kUnit<TX>;
   by_length<U, kLastFwd>(
       p.D,
       [&](auto tpr, auto nv) {
@@ -549,7 +606,7 @@ hipError_t forward(const ResnormParams& p, hipStream_t stream) {
 
 template <typename TX, typename TY>
 hipError_t backward(const ResnormParams& p, float* dw, float* db, float* ds, hipStream_t stream) {
-  constexpr int U = kUnit<TY>;
+  constexpr int U = kUnit<TX>;
   const int lines = norm_lines(p.rows, p.D);
   hipError_t e = hipSuccess;
   by_length<U, kLastBwd>(
