@@ -559,8 +559,8 @@ typedef struct osm_resnorm_bwd_args {
  *
  *   loss_n = log sum_v exp(hidden_n . weight_v) - hidden_n . weight_{targets_n}
  *
- * for tokens n with targets_n != ignore_index; the others count for nothing, their
- * hidden rows are not read, and their loss and gradients are 0.  A target outside
+ * for tokens n with targets_n != ignore_index; the others count for nothing, whatever
+ * their hidden rows hold, and their loss and gradients are 0.  A target outside
  * [0, V) gives NaN (the loss, and every gradient that the token has a part in).
  * Products are at fp32's accuracy for fp32 inputs (three bf16 parts an operand) and
  * exact for bf16 ones, sums in fp32.  No counterpart in the reference. */

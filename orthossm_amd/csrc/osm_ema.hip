@@ -112,6 +112,10 @@ __device__ __forceinline__ void put2(float* p, int64_t at, int c, int D, F2 v) {
   if (c + 1 < D) p[at + c + 1] = v.y;
 }
 
+// Until these are in registers.  (A state may lie where another block writes the one it
+// hands on: that block waits for what is posted after this.)
+__device__ __forceinline__ void arrive(F2 v) { asm volatile("" ::"v"(v.x), "v"(v.y)); }
+
 // Waits for a word to be published (they are never 0): its producer has been running
 // since before this block drew its tile.
 __device__ __forceinline__ unsigned long long await(const unsigned long long* at) {
@@ -272,6 +276,7 @@ __global__ void __launch_bounds__(kThreads, 4) ema_fwd_kernel(const EmaParams p)
   }
   L.a[q.wave][q.lane] = floor2(A);
   L.b[q.wave][q.lane] = B;
+  arrive(start);
   __syncthreads();
   F2 h = carry_in(p, L, q, q.tile, (q.tile + 1) * kTile >= len, false, start);
   if (!live) return;
@@ -338,6 +343,7 @@ __global__ void __launch_bounds__(kThreads, 4) ema_bwd_kernel(const EmaParams p)
   L.a[q.wave][q.lane] = floor2(A);
   L.b[q.wave][q.lane] = Q;
   fb[q.wave][q.lane] = B;
+  arrive(start);
   __syncthreads();
   const int used = (len + kTile - 1) / kTile;
   F2 g = carry_in(p, L, q, used - 1 - q.tile, q.tile == 0, true, start);

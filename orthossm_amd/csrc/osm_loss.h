@@ -8,7 +8,8 @@ namespace osm {
 
 constexpr int kLossPad = 256;      // rows of compacted tokens, columns of a piece: multiples of this
 
-// The tokens that count, one after the other.
+// The tokens that count, one after the other.  All NULL in a short forward, whose tokens
+// are all in their own places, those that do not count too.
 struct LossTokens {
   int* targets;                    // [N]: by place, -1: outside the vocabulary
   float2* factors;                 // [N]: by place, log2(e) lse and grad_losses (1 without); the backward's
@@ -26,7 +27,9 @@ struct LossParams {
   const int64_t* targets;
   int64_t ignore;
   LossTokens tok;
-  __bf16* h;                       // [parts][Npad][Dpad]: the hidden rows that count, zeros after them up to a whole step
+  const __bf16* h;                 // [parts][h_rows][h_ld], h_part apart: the hidden rows that count, zeros after them up to a whole step
+  int64_t h_ld, h_part;
+  int h_rows;
   // a piece of the vocabulary
   int64_t v0;
   int vn, vpad;                    // its classes; columns of p
@@ -45,7 +48,7 @@ struct LossParams {
   void *grad_h, *grad_w;
 };
 
-hipError_t launch_loss_rows(const LossParams& p, int dtype, bool bwd, hipStream_t stream);  // tok, h
+hipError_t launch_loss_rows(const LossParams& p, __bf16* h, int dtype, bool bwd, hipStream_t stream);   // tok, h
 hipError_t launch_loss_weight(const LossParams& p, __bf16* to, int dtype, hipStream_t stream);   // parts of the piece's rows
 int loss_tile_rows(const LossParams& p);                                                    // classes of a tile of the logits
 hipError_t launch_loss_logits(const LossParams& p, hipStream_t stream);                     // stat, own

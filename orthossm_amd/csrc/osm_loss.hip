@@ -69,7 +69,7 @@ bool whole_units(const void* p, int64_t stride, int64_t D) {
 // The tokens that count, one after the other: a block takes `each` tokens, counts those
 // before them, and writes where its own go, and their hidden rows.
 template <typename T, int PARTS>
-__global__ void __launch_bounds__(256) loss_rows_kernel(const LossParams p, int64_t each, bool vec, bool bwd) {
+__global__ void __launch_bounds__(256) loss_rows_kernel(const LossParams p, __bf16* to, int64_t each, bool vec, bool bwd) {
   __shared__ int sums[4];
   __shared__ int rows[256];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(256) loss_rows_kernel(const LossParams p, int6
 #pragma unroll
         for (int q = 0; q < PARTS; ++q)
           if (u < n) {
-            *reinterpret_cast<bf16x8*>(p.h + ((int64_t)q * p.Npad + first) * p.Dpad + 8 * (int64_t)u) = out[k][q];
+            *reinterpret_cast<bf16x8*>(to + ((int64_t)q * p.Npad + first) * p.Dpad + 8 * (int64_t)u) = out[k][q];
             wide_store_wait();
           }
       }
@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(256) loss_rows_kernel(const LossParams p, int6
   const int over = (base + kStep - 1) / kStep * kStep - base;
   for (int u = threadIdx.x; u < PARTS * over * units; u += 256) {
     const int q = u / (over * units), r = u - q * over * units;
-    *reinterpret_cast<bf16x8*>(p.h + ((int64_t)q * p.Npad + base) * p.Dpad + 8 * (int64_t)r) = bf16x8{};
+    *reinterpret_cast<bf16x8*>(to + ((int64_t)q * p.Npad + base) * p.Dpad + 8 * (int64_t)r) = bf16x8{};
     wide_store_wait();
   }
 }
@@ -186,7 +186,8 @@ __global__ void __launch_bounds__(G::kThreads) loss_logits_kernel(const LossPara
   __shared__ __attribute__((aligned(16))) __bf16 lds[G::kLds];
   int tm, tn;
   if (!tile_of(g.tm, g.tn, tm, tn)) return;
-  const int count = *p.tok.count, m0 = tm * G::TM, n0 = tn * G::TN;
+  const bool all = !BWD && !p.tok.count;
+  const int count = all ? (int)p.N : *p.tok.count, m0 = tm * G::TM, n0 = tn * G::TN;
   if (n0 >= count) return;
   const GemmPlace<G> q;
   const int rows = p.vn - m0;   // of the tile that are classes
@@ -196,8 +197,10 @@ __global__ void __launch_bounds__(G::kThreads) loss_logits_kernel(const LossPara
   float2 factors[G::FN];
 #pragma unroll
   for (int j = 0; j < G::FN; ++j) {
-    const int n = min(n0 + q.col(j), count - 1), t = p.tok.targets[n] - (int)p.v0 - m0;
-    aim[j] = n0 + q.col(j) < count && t >= q.m && t < min(q.m + G::TM / G::WM, rows) ? t : -1;
+    const int n = min(n0 + q.col(j), count - 1);
+    int64_t t = all ? p.targets[n] : p.tok.targets[n];
+    t = t < p.V ? t - p.v0 - m0 : -1;
+    aim[j] = n0 + q.col(j) < count && t >= q.m && t < min(q.m + G::TM / G::WM, rows) ? (int)t : -1;
     if (BWD) factors[j] = p.tok.factors[n];
   }
   f32x16 acc[G::FM][G::FN];
@@ -362,13 +365,26 @@ __global__ void __launch_bounds__(G::kThreads) loss_dw_kernel(const LossParams p
 
 constexpr int kJoinTokens = 16, kJoinSlices = 16;
 
+// The sum of d over a workgroup of T threads in its first, in an order that does not depend
+// on timing.
+template <int T>
+__device__ __forceinline__ double block_sum(double d, double* red) {
+  red[threadIdx.x] = d;
+  for (int w = T / 2; w > 0; w >>= 1) {
+    __syncthreads();
+    if ((int)threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
+  }
+  return red[0];
+}
+
 // A token's statistics over the vocabulary's tiles, 16 threads a token; zeros of those
 // that do not count.
 __global__ void __launch_bounds__(kJoinTokens * kJoinSlices) loss_join_kernel(const LossParams p, int tiles) {
   __shared__ float2 red[kJoinSlices][kJoinTokens];
   const int c = threadIdx.x % kJoinTokens, s = threadIdx.x / kJoinTokens;
   const int64_t token = (int64_t)blockIdx.x * kJoinTokens + c;
-  const int at = token < p.N ? p.tok.places[token] : -1;
+  int at = -1;
+  if (token < p.N) at = p.tok.places ? p.tok.places[token] : p.targets[token] != p.ignore ? (int)token : -1;
   float top = -kInf, sum = 0.0f;
   if (at >= 0) {
 #pragma unroll 4
@@ -401,18 +417,18 @@ __global__ void __launch_bounds__(kJoinTokens * kJoinSlices) loss_join_kernel(co
 
 // The sum of the losses in double, one workgroup, in an order that does not depend on timing.
 __global__ void __launch_bounds__(1024) loss_total_kernel(const LossParams p) {
-  __shared__ double red[1024];
-  double s = 0.0;
-  for (int64_t i = threadIdx.x; i < p.N; i += 1024) s += p.losses[i];
-  red[threadIdx.x] = s;
-  for (int w = 512; w > 0; w >>= 1) {
-    __syncthreads();
-    if ((int)threadIdx.x < w) red[threadIdx.x] += red[threadIdx.x + w];
+  __shared__ double red[1024], counts[1024];
+  double s = 0.0, n = 0.0;
+  for (int64_t i = threadIdx.x; i < p.N; i += 1024) {
+    s += p.losses[i];
+    if (!p.tok.count) n += p.targets[i] != p.ignore;
   }
+  s = block_sum<1024>(s, red);
+  n = p.tok.count ? *p.tok.count : block_sum<1024>(n, counts);
   if (threadIdx.x == 0) {
-    const float n = (float)max(*p.tok.count, 1);
-    *p.loss = (float)(p.mean ? red[0] / n : red[0]);
-    if (p.count) *p.count = n;
+    n = n < 1.0 ? 1.0 : n;
+    *p.loss = (float)(p.mean ? s / n : s);
+    if (p.count) *p.count = (float)n;
   }
 }
 
@@ -425,28 +441,29 @@ __global__ void loss_none_kernel(float* loss, float* count) {
 // grad_h of every token from its place's sums, zeros where it does not count.
 template <typename T>
 __global__ void __launch_bounds__(256) loss_finish_kernel(const LossParams p) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int per = ((int)p.D + 3) / 4;
-  if (i >= p.N * per) return;
-  const int64_t n = i / per;
-  const int d = (int)(i - n * per) * 4, at = p.tok.places[n];
-  f32x4 v = {};
-  if (at >= 0) {
-    for (int s = 0; s < p.splits; ++s) v += *reinterpret_cast<const f32x4*>(p.dh + ((int64_t)s * p.Npad + at) * p.Dpad + d);
-    v *= factor(p);
-  }
-  T* const to = static_cast<T*>(p.grad_h) + n * p.D + d;
-  typedef T V4 __attribute__((ext_vector_type(4)));
-  V4 o;
+  const int64_t per = (p.D + 3) / 4, all = p.N * per;
+  const float s = factor(p);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t n = i / per;
+    const int d = (int)(i - n * per) * 4, at = p.tok.places[n];
+    f32x4 v = {};
+    if (at >= 0) {
+      for (int k = 0; k < p.splits; ++k) v += *reinterpret_cast<const f32x4*>(p.dh + ((int64_t)k * p.Npad + at) * p.Dpad + d);
+      v *= s;
+    }
+    T* const to = static_cast<T*>(p.grad_h) + n * p.D + d;
+    typedef T V4 __attribute__((ext_vector_type(4)));
+    V4 o;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) o[k] = (T)v[k];
-  if (p.D % 4 == 0) {
-    *reinterpret_cast<V4*>(to) = o;
-    if (sizeof(V4) > 8) wide_store_wait();
-  } else {
+    for (int k = 0; k < 4; ++k) o[k] = (T)v[k];
+    if (p.D % 4 == 0) {
+      *reinterpret_cast<V4*>(to) = o;
+      if (sizeof(V4) > 8) wide_store_wait();
+    } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (d + k < p.D) to[k] = o[k];
+      for (int k = 0; k < 4; ++k)
+        if (d + k < p.D) to[k] = o[k];
+    }
   }
 }
 
@@ -494,7 +511,7 @@ hipError_t logits(const LossParams& p, hipStream_t stream) {
     constexpr int PARTS = decltype(n)::value;
     by_size<!BWD || PARTS == 1>(BWD ? p.vpad : p.V, p.N, [&](auto g) {
       using G = decltype(g);
-      const Product t = product<G>(side(p.w, p.w_ld, p.w_part, p.vn, 0), side(p.h, p.Dpad, (int64_t)p.Npad * p.Dpad, p.Npad, 0),
+      const Product t = product<G>(side(p.w, p.w_ld, p.w_part, p.vn, 0), side(p.h, p.h_ld, p.h_part, p.h_rows, 0),
                                    BWD ? p.vpad : p.vn, p.N);
       hipLaunchKernelGGL((loss_logits_kernel<G, PARTS, BWD>), dim3(grid_of(t.tm, t.tn)), dim3(G::kThreads), 0, stream, p, t);
     });
@@ -504,14 +521,14 @@ hipError_t logits(const LossParams& p, hipStream_t stream) {
 
 }  // namespace
 
-hipError_t launch_loss_rows(const LossParams& p, int dtype, bool bwd, hipStream_t stream) {
+hipError_t launch_loss_rows(const LossParams& p, __bf16* h, int dtype, bool bwd, hipStream_t stream) {
   // (a block counts what is before its tokens, so that there are at most 1024 of them)
   const int64_t each = std::max<int64_t>(4, (p.N + 1023) / 1024);
   const dim3 grid((unsigned)((p.N + each - 1) / each));
   if (dtype == 0)
-    hipLaunchKernelGGL((loss_rows_kernel<float, 3>), grid, dim3(256), 0, stream, p, each, whole_units<float>(p.hidden, p.hidden_s, p.D), bwd);
+    hipLaunchKernelGGL((loss_rows_kernel<float, 3>), grid, dim3(256), 0, stream, p, h, each, whole_units<float>(p.hidden, p.hidden_s, p.D), bwd);
   else
-    hipLaunchKernelGGL((loss_rows_kernel<__bf16, 1>), grid, dim3(256), 0, stream, p, each, whole_units<__bf16>(p.hidden, p.hidden_s, p.D), bwd);
+    hipLaunchKernelGGL((loss_rows_kernel<__bf16, 1>), grid, dim3(256), 0, stream, p, h, each, whole_units<__bf16>(p.hidden, p.hidden_s, p.D), bwd);
   return hipGetLastError();
 }
 
@@ -570,7 +587,7 @@ hipError_t launch_loss_dh(const LossParams& p, hipStream_t stream) {
 hipError_t launch_loss_dw(const LossParams& p, int dtype, hipStream_t stream) {
   by_size(p.D, p.vn, [&](auto g) {
     using G = decltype(g);
-    const Product t = product<G>(side(p.h, p.Dpad, (int64_t)p.Npad * p.Dpad, p.Npad, p.Dpad),
+    const Product t = product<G>(side(p.h, p.h_ld, p.h_part, p.h_rows, p.Dpad),
                                  side(p.p, p.vpad, (int64_t)p.Npad * p.vpad, p.Npad, p.vpad), p.D, p.vn);
     if (dtype == 0)
       hipLaunchKernelGGL((loss_dw_kernel<G, 3, float>), dim3(grid_of(t.tm, t.tn)), dim3(G::kThreads), 0, stream, p, t);
@@ -590,7 +607,7 @@ hipError_t launch_loss_zero(void* to, int64_t n, int dtype, hipStream_t stream) 
 }
 
 hipError_t launch_loss_finish(const LossParams& p, int dtype, hipStream_t stream) {
-  const dim3 grid((unsigned)((p.N * ((p.D + 3) / 4) + 255) / 256));
+  const dim3 grid((unsigned)std::min<int64_t>((p.N * ((p.D + 3) / 4) + 255) / 256, 1 << 16));
   if (dtype == 0)
     hipLaunchKernelGGL((loss_finish_kernel<float>), grid, dim3(256), 0, stream, p);
   else

@@ -53,6 +53,14 @@ bool direct(const osm_loss_args* a) {
          a->weight_stride < kMaxRow;
 }
 
+// Whether a forward takes all tokens where they are: few, of rows that can be read there.
+// (64 tokens of 256 over 1000 classes: two launches for three, SHORT us.  With more tokens, what
+// the others cost is worth leaving out, and the launch is a small part.)
+bool in_place(const osm_loss_args* a) {
+  return a->N <= 512 && a->dtype == OSM_BF16 && a->D % 64 == 0 && (uintptr_t)a->hidden % 16 == 0 && a->hidden_stride % 8 == 0 &&
+         a->hidden_stride < kMaxRow;
+}
+
 // What a launch works on: the compacted hidden rows, and pieces of the vocabulary.
 struct Plan {
   int64_t Npad, Dpad, parts, piece;   // piece: classes, a multiple of kLossPad
@@ -143,6 +151,9 @@ LossParams params_of(const osm_loss_args* a, const Plan& n, const Layout& l, voi
   p.tok = {reinterpret_cast<int*>(w + l.targets), reinterpret_cast<float2*>(w + l.factors), reinterpret_cast<int*>(w + l.places),
            reinterpret_cast<int*>(w + l.count)};
   p.h = reinterpret_cast<__bf16*>(w + l.h);
+  p.h_ld = n.Dpad;
+  p.h_part = n.Npad * n.Dpad;
+  p.h_rows = (int)n.Npad;
   p.lse = a->lse;
   return p;
 }
@@ -177,7 +188,15 @@ hipError_t forward(const osm_loss_args* a, const Plan& n, const Layout& l, void*
   p.loss = a->loss;
   p.count = a->count;
   p.mean = (a->flags & OSM_LOSS_MEAN) != 0;
-  hipError_t e = osm::launch_loss_rows(p, a->dtype, false, st);
+  hipError_t e = hipSuccess;
+  if (in_place(a)) {
+    p.tok = {};
+    p.h = static_cast<const __bf16*>(a->hidden);
+    p.h_ld = a->hidden_stride;
+    p.h_rows = (int)a->N;
+  } else {
+    e = osm::launch_loss_rows(p, reinterpret_cast<__bf16*>(w + l.h), a->dtype, false, st);
+  }
   if (e != hipSuccess) return e;
   const int rows = osm::loss_tile_rows(p);
   for (int64_t v0 = 0; v0 < a->V; v0 += n.piece) {
@@ -200,7 +219,7 @@ hipError_t backward(const osm_loss_args* a, const osm_loss_bwd_args* b, const Pl
   p.count_in = b->count;
   p.grad_h = b->grad_hidden;
   p.grad_w = b->grad_weight;
-  hipError_t e = osm::launch_loss_rows(p, a->dtype, true, st);
+  hipError_t e = osm::launch_loss_rows(p, reinterpret_cast<__bf16*>(w + l.h), a->dtype, true, st);
   if (e != hipSuccess) return e;
   for (int64_t v0 = 0, vn; v0 < a->V; v0 += vn) {
     vn = next_piece(a->V - v0, n.piece, a->D);

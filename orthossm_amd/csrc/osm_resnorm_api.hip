@@ -21,8 +21,8 @@ int check_args(const osm_resnorm_args* a) {
   const int s = a->stream_dtype, b = a->block_dtype;
   if ((s != OSM_F32 && s != OSM_BF16) || (b != OSM_F32 && b != OSM_BF16) || (b == OSM_F32 && s != OSM_F32))
     return fail(OSM_E_DTYPE, "stream_dtype %d with block_dtype %d unsupported", s, b);
-  if (a->rows < 0 || a->D < 1 || a->D >= (int64_t(1) << 31))
-    return fail(OSM_E_SHAPE, "rows=%lld must be >= 0 and D=%lld in [1, 2^31)", (long long)a->rows, (long long)a->D);
+  if (a->rows < 0 || a->D < 1 || a->D > (int64_t(1) << 25))   // (threads of the sums' launch: 96 D)
+    return fail(OSM_E_SHAPE, "rows=%lld must be >= 0 and D=%lld in [1, 2^25]", (long long)a->rows, (long long)a->D);
   if (!(a->eps >= 0.0f)) return fail(OSM_E_ARG, "eps=%g must be >= 0", (double)a->eps);
   const void* words[4] = {a->scale, a->weight, a->bias, a->stats};
   for (const void* w : words)

@@ -11,7 +11,7 @@ on gfx950), without its logits.
 hidden [..., D] and weight [V,D] fp32 or bf16 (mixed or other types go to fp32)
 with contiguous rows (others are copied first), targets whole numbers of
 hidden's shape without D.  Tokens whose target is ``ignore_index`` count for
-nothing: their hidden rows are not read, their losses and gradients are 0.  A
+nothing, whatever their hidden rows hold: their losses and gradients are 0.  A
 target outside [0, V) gives NaN: that token's loss, and every gradient that it
 has a part in.  Logits, sums and losses are fp32; the gradients' factors
 softmax - onehot are rounded to bf16 for bf16 inputs.

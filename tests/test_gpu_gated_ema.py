@@ -180,6 +180,18 @@ def test_layouts(dev):
     assert all(torch.equal(p, q) for p, q in zip(gated_ema_backward(x, gate, one)[:2], gated_ema_backward(x, gate, one.contiguous())[:2]))
 
 
+def test_states_in_place(dev):
+    """The final state where the first was, and the gradients likewise, over several tiles
+    and groups of them."""
+    for S in (100, 400, 3000):
+        x, gate, init, go, gs = (t.to(dev) for t in make(4, S, 384, seed=S))
+        want, last = gated_ema_forward(x, gate, state_init=init, return_state=True)
+        for _ in range(5):
+            state = init.clone()
+            got = gated_ema_forward(x, gate, state_init=state, state_out=state)
+            assert torch.equal(got, want) and torch.equal(state, last)
+
+
 def test_types(dev):
     x, gate, init, go, _ = (t.to(dev) for t in make(2, 50, 8, seed=6))
     leaves = x.half().requires_grad_(), gate.bfloat16().requires_grad_(), init.double().requires_grad_()

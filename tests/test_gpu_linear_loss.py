@@ -103,10 +103,11 @@ def test_widths(dev, D, dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("ignored", [0.02, 0.5, 0.95, 1.1])
-def test_ignored_tokens_are_not_read(dev, ignored, dtype):
-    hidden, weight, targets = make(300, 80, 400, dtype, seed=1, ignored=ignored)
-    hidden[targets == IGNORE] = float("nan")
-    check(dev, hidden, weight, targets)
+def test_ignored_tokens_may_hold_anything(dev, ignored, dtype):
+    for N, D in ((300, 80), (300, 64), (600, 64)):
+        hidden, weight, targets = make(N, D, 400, dtype, seed=1, ignored=ignored)
+        hidden[targets == IGNORE] = float("nan")
+        check(dev, hidden, weight, targets)
 
 
 # The three tile sizes of each product, several pieces of the vocabulary.
