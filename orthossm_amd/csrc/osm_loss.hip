@@ -476,11 +476,16 @@ __global__ void __launch_bounds__(256) loss_zero_kernel(T* to, int64_t n) {
 using Big = GemmTile<256, 256, 4, 2>;
 using Middle = GemmTile<128, 128, 2, 2>;
 using Small = GemmTile<128, 64, 2, 2>;
+using Tiny = GemmTile<64, 64, 2, 2>;
 constexpr int kCUs = 256;
 
 // The largest tile of which most CUs get what they hold, one of the largest or two of the
-// next, else the smallest.  (BIG false: without
-// the largest, whose accumulators leave no registers for what is made of them.)
+// next, else the third, and the least where few CUs get one.  Measured in us, larger and
+// smaller: 5003 classes x 981 tokens x 448, three parts each, the logits with 320 of the
+// second or 640 of the third 49 and 59 (P 56 and 66); 1000 x 64 x 256, 8 of the third or 16 of
+// the least 7.2 and 5.7; the products alone, 50176 x 8192 x 1024, first and second 740 and 836.
+// (BIG false: without the largest, whose accumulators leave no registers for what is made of
+// them.)
 template <bool BIG = true, typename F>
 void by_size(int64_t M, int64_t N, F f) {
   auto tiles = [&](int64_t tm, int64_t tn) { return (M + tm - 1) / tm * ((N + tn - 1) / tn); };
@@ -488,8 +493,10 @@ void by_size(int64_t M, int64_t N, F f) {
     if (tiles(256, 256) >= kCUs * 3 / 4) return f(Big{});
   if (tiles(128, 128) >= kCUs * 3 / 2)
     f(Middle{});
-  else
+  else if (tiles(128, 64) >= kCUs / 2)
     f(Small{});
+  else
+    f(Tiny{});
 }
 
 template <class G>
