@@ -2,14 +2,17 @@
 // sum_k A(m, k) B(n, k): what the vocabulary's cross entropy is built on.
 //
 // Each operand lies by rows (a row holds the k of one m or n) or by columns (a row
-// holds the m or n of one k).  A workgroup forms TM x TN of C.  64 k of both operands at a
-// time go from memory to LDS without passing through registers, into one of two buffers
-// while the other is multiplied.  By rows, a row's 16-byte units lie in LDS at their index
+// holds the m or n of one k).  A workgroup forms TM x TN of C.  64 k (32 of
+// operands in parts) of both operands at a time go from memory to LDS without passing
+// through registers, into one of two buffers while the other is multiplied.  By rows, a row's 16-byte units lie in LDS at their index
 // xor half the row's, so that the 32 rows of a matrix instruction are read from different
 // banks; by columns, a row's 32-byte units lie at theirs xor the row's, so that the 4 rows
 // of a transposing read are.  The order is made by the addresses that are read from memory.
 // An fp32 operand is three bf16 matrices whose sum it is (its parts), and the product the
-// sum of the six products of parts that are not below 2^-24.
+// sum of the six products of parts that are not below 2^-24: the product of the first
+// parts, and in accumulators of their own the five small ones.  All parts of a step lie in
+// LDS together: they come from memory and are read once for the six products (5003 x 981 x
+// 448: 34 us; with a walk over k for each product 49).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -32,24 +35,20 @@ struct GemmSide {
   int cols;                      // by columns: elements of a row to read, a multiple of 8 (past them: the last ones again)
 };
 
-template <int TM_, int TN_, int WM_, int WN_, int KS_ = 64, int ST_ = 2>
+template <int TM_, int TN_, int WM_, int WN_, int PARTS_ = 1>
 struct GemmTile {
   static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_;   // tile; waves along each
-  static constexpr int KS = KS_, ST = ST_;                       // k of a step; buffers
+  static constexpr int PARTS = PARTS_;                           // of an operand
+  static constexpr int KS = PARTS == 1 ? 64 : 32;                // k of a step
   static constexpr int kThreads = 64 * WM * WN;
   static constexpr int FM = TM / WM / 32, FN = TN / WN / 32;     // 32 x 32 squares of a wave
-  static constexpr int kBuffer = (TM + TN) * KS;                 // elements of a buffer
-  static constexpr int kLds = ST * kBuffer;
-  static constexpr int kLoads = kBuffer / 8 / kThreads;          // of a thread and step
+  static constexpr int kBuffer = PARTS * (TM + TN) * KS;         // elements of a buffer: A's parts, then B's
+  static constexpr int kLds = 2 * kBuffer;
   static_assert(TM * KS / 8 % kThreads == 0 && TN * KS / 8 % kThreads == 0 && kStep % KS == 0, "whole loads and steps");
 };
 
-// Waits until at most `n` of this wave's loads are on their way.
-template <int N>
-__device__ __forceinline__ void wait_loads() {
-  static_assert(N < 64, "6 bits");
-  __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4) << 14);
-}
+// Waits until none of this wave's loads is on its way.
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
 
 // Where a thread's accumulators lie in C's tile: row(i) of column col, i in [0, 16).
 template <class G>
@@ -86,7 +85,7 @@ struct GemmOperand {
   // (rows of 128 bytes: two of them go through the banks; of 64 bytes: four)
   static __device__ __forceinline__ int turn(int row) { return KS == 64 ? row >> 1 & 7 : row >> 2 & 3; }
   int from[N];             // elements from the step's first
-  const __bf16 *first, *at;
+  const __bf16* first;     // the next step's
   int64_t ld, part;
   int rows, k;             // by columns: rows in all, and ahead of the step
 
@@ -105,24 +104,26 @@ struct GemmOperand {
     for (int i = 0; i < N; ++i)
       from[i] = COLS ? row_of(i) * (int)ld + min(col_of(i), s.cols - 8 - m0) : min(row_of(i), rows - 1 - m0) * (int)ld + col_of(i);
   }
-  __device__ __forceinline__ void start(int index, int64_t k0) {
-    at = first + index * part;
-    k = (int)k0;
-  }
   // The next step to LDS.
   __device__ __forceinline__ void fetch(unsigned to) {
     to += __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
-    if (!COLS || k + KS <= rows) {
+    const bool whole = !COLS || k + KS <= rows;
 #pragma unroll
-      for (int i = 0; i < N; ++i) to_lds(at + from[i], to + i * G::kThreads * 16);
-    } else {
+    for (int q = 0; q < G::PARTS; ++q) {
+      const __bf16* const at = first + q * part;
+      const unsigned there = to + q * T * KS * 2;
+      if (whole) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int r = row_of(i), over = max(r + k - (rows - 1), 0);
-        to_lds(at + from[i] - (int64_t)over * ld, to + i * G::kThreads * 16);
+        for (int i = 0; i < N; ++i) to_lds(at + from[i], there + i * G::kThreads * 16);
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int r = row_of(i), over = max(r + k - (rows - 1), 0);
+          to_lds(at + from[i] - (int64_t)over * ld, there + i * G::kThreads * 16);
+        }
       }
     }
-    at += COLS ? KS * ld : KS;
+    first += COLS ? KS * ld : KS;
     k += KS;
   }
   // A lane's 8 elements of the 32 from `m` on, in the s-th 16 k of the step.
@@ -142,66 +143,55 @@ struct GemmOperand {
   }
 };
 
-// acc = the m from m0 of A times the n from n0 of B over `steps` times kStep k from k0 on (a
-// multiple of kStep).  parts: 1, or 3 for each side.
+// acc = the m from m0 of A times the n from n0 of B over n_steps times kStep k from k0 on (a
+// multiple of kStep).
 template <class G, bool ACOLS, bool BCOLS>
-__device__ __forceinline__ void gemm(const GemmSide& A, const GemmSide& B, int m0, int n0, int64_t k0, int n_steps, int parts,
-                                     __bf16* lds, f32x16 (&acc)[G::FM][G::FN]) {
+__device__ __forceinline__ void gemm(const GemmSide& A, const GemmSide& B, int m0, int n0, int64_t k0, int n_steps, __bf16* lds,
+                                     f32x16 (&acc)[G::FM][G::FN]) {
   using OA = GemmOperand<G, G::TM, ACOLS>;
   using OB = GemmOperand<G, G::TN, BCOLS>;
+  constexpr int P = G::PARTS;
   const GemmPlace<G> q;
   OA a(A, m0, k0);
   OB b(B, n0, k0);
-  const int steps = n_steps * (kStep / G::KS), segments = parts == 1 ? 1 : 6, total = steps * segments;
-  // (parts i of A and j of B in order: 2 0, 1 1, 0 2, 1 0, 0 1, 0 0, the small ones first)
-  int seg = 0, at = 0;
-  auto point = [&] {
-    a.start(segments == 1 ? 0 : (0x001012 >> (4 * seg)) & 15, k0);
-    b.start(segments == 1 ? 0 : (0x010210 >> (4 * seg)) & 15, k0);
-  };
-  point();
+  const int steps = n_steps * (kStep / G::KS);
   const unsigned base = __builtin_amdgcn_readfirstlane(lds_address(lds));
   auto fetch = [&](int buf) {
     const unsigned to = base + buf * G::kBuffer * 2;
     a.fetch(to);
-    b.fetch(to + G::TM * G::KS * 2);
-    if (++at == steps) {
-      at = 0;
-      ++seg;
-      point();
-    }
+    b.fetch(to + P * G::TM * G::KS * 2);
   };
+  f32x16 small[P == 1 ? 1 : G::FM][G::FN];
 #pragma unroll
   for (int i = 0; i < G::FM; ++i)
 #pragma unroll
-    for (int j = 0; j < G::FN; ++j) acc[i][j] = (f32x16)0.0f;
-  // Step t is multiplied while the ST - 1 after it are on their way; the last of those goes
-  // where step t - 1 was, which everyone has read by the barrier.
-#pragma unroll
-  for (int t = 0; t < G::ST - 1; ++t)
-    if (t < total) fetch(t);
-  int buf = 0;
-  for (int t = 0; t < total; ++t) {
-    if (t + G::ST - 2 < total)
-      wait_loads<(G::ST - 2) * G::kLoads>();
-    else
-      wait_loads<0>();
+    for (int j = 0; j < G::FN; ++j) {
+      acc[i][j] = (f32x16)0.0f;
+      if (P > 1) small[i][j] = (f32x16)0.0f;
+    }
+  // Step t is multiplied while the next one is on its way to where step t - 1 was, which
+  // everyone has read by the barrier.
+  if (steps > 0) fetch(0);
+  for (int t = 0; t < steps; ++t) {
+    wait_loads();
     __syncthreads();
-    if (t + G::ST - 1 < total) fetch(buf == 0 ? G::ST - 1 : buf - 1);
-    const __bf16* const la = lds + buf * G::kBuffer;
-    const __bf16* const lb = la + G::TM * G::KS;
-    buf = buf == G::ST - 1 ? 0 : buf + 1;
+    if (t + 1 < steps) fetch((t + 1) & 1);
+    const __bf16* const la = lds + (t & 1) * G::kBuffer;
+    const __bf16* const lb = la + P * G::TM * G::KS;
     // By rows, what the next 16 k take is read while these are multiplied, a read after each
     // matrix instruction (50176 x 8192 x 1024: 735 us without, 695 with; transposing reads,
     // twice as many, are better left to the compiler: 231 and 237 us for 1024 x 16384 x 8192).
     constexpr bool kAhead = !ACOLS && !BCOLS;
     constexpr int kParts = G::KS / 16, kHeld = kAhead ? 2 : 1;
-    bf16x8 fa[kHeld][G::FM], fb[kHeld][G::FN];
+    bf16x8 fa[kHeld][P][G::FM], fb[kHeld][P][G::FN];
     auto read = [&](int s) {
 #pragma unroll
-      for (int i = 0; i < G::FM; ++i) fa[s % kHeld][i] = OA::read(la, q.m + 32 * i, s, q.lane);
+      for (int p = 0; p < P; ++p) {
 #pragma unroll
-      for (int j = 0; j < G::FN; ++j) fb[s % kHeld][j] = OB::read(lb, q.n + 32 * j, s, q.lane);
+        for (int i = 0; i < G::FM; ++i) fa[s % kHeld][p][i] = OA::read(la + p * G::TM * G::KS, q.m + 32 * i, s, q.lane);
+#pragma unroll
+        for (int j = 0; j < G::FN; ++j) fb[s % kHeld][p][j] = OB::read(lb + p * G::TN * G::KS, q.n + 32 * j, s, q.lane);
+      }
     };
     if (kAhead) read(0);
 #pragma unroll
@@ -210,20 +200,35 @@ __device__ __forceinline__ void gemm(const GemmSide& A, const GemmSide& B, int m
         read(s);
       else if (s + 1 < kParts)
         read(s + 1);
+      auto multiply = [&](int pa, int pb, f32x16 (&to)[G::FM][G::FN]) {
 #pragma unroll
-      for (int i = 0; i < G::FM; ++i)
+        for (int i = 0; i < G::FM; ++i)
 #pragma unroll
-        for (int j = 0; j < G::FN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[s % kHeld][i], fb[s % kHeld][j], acc[i][j], 0, 0, 0);
+          for (int j = 0; j < G::FN; ++j)
+            to[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[s % kHeld][pa][i], fb[s % kHeld][pb][j], to[i][j], 0, 0, 0);
+      };
+      if constexpr (P > 1) {
+        multiply(2, 0, small);
+        multiply(0, 2, small);
+        multiply(1, 1, small);
+        multiply(1, 0, small);
+        multiply(0, 1, small);
+      }
+      multiply(0, 0, acc);
       if constexpr (kAhead) {
 #pragma unroll
-        for (int i = 0; i < G::FM * G::FN; ++i) {
+        for (int i = 0; i < G::FM * G::FN * (P > 1 ? 6 : 1); ++i) {
           __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // a matrix instruction
           __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);   // an LDS read
         }
       }
     }
   }
+  if constexpr (P > 1)
+#pragma unroll
+    for (int i = 0; i < G::FM; ++i)
+#pragma unroll
+      for (int j = 0; j < G::FN; ++j) acc[i][j] += small[i][j];
   __syncthreads();   // the buffers are free
 }
 

@@ -56,7 +56,7 @@ hipError_t launch_loss_join(const LossParams& p, int tiles, hipStream_t stream);
 hipError_t launch_loss_none(float* loss, float* count, hipStream_t stream);
 hipError_t launch_loss_probs(const LossParams& p, hipStream_t stream);                      // p
 hipError_t launch_loss_dh(const LossParams& p, hipStream_t stream);
-hipError_t launch_loss_dw(const LossParams& p, int dtype, hipStream_t stream);
+hipError_t launch_loss_dw(LossParams p, int from, int n, hipStream_t stream);                // of n of the piece's classes
 hipError_t launch_loss_zero(void* to, int64_t n, int dtype, hipStream_t stream);
 hipError_t launch_loss_finish(const LossParams& p, int dtype, hipStream_t stream);          // grad_h
 

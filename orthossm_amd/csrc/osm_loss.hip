@@ -181,7 +181,7 @@ struct Product {
 // Logits of a tile: A the piece's classes, B the tokens that count.  BWD false: the
 // tile's largest logit and sum of exponentials for each token, and the target's logit.
 // BWD true: P.
-template <class G, int PARTS, bool BWD>
+template <class G, bool BWD>
 __global__ void __launch_bounds__(G::kThreads) loss_logits_kernel(const LossParams p, const Product g) {
   __shared__ __attribute__((aligned(16))) __bf16 lds[G::kLds];
   int tm, tn;
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(G::kThreads) loss_logits_kernel(const LossPara
     if (BWD) factors[j] = p.tok.factors[n];
   }
   f32x16 acc[G::FM][G::FN];
-  gemm<G, false, false>(g.a, g.b, m0, n0, 0, p.Dpad / kStep, PARTS, lds, acc);
+  gemm<G, false, false>(g.a, g.b, m0, n0, 0, p.Dpad / kStep, lds, acc);
   // f(value, row) for the rows that a lane holds of column j; change: what it gives takes the value's place
   auto each = [&](int j, auto f) {
 #pragma unroll
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(G::kThreads) loss_logits_kernel(const LossPara
       if (p.grad_losses) change(j, [&](float e, int) { return e * factors[j].y; });
       if (rows < G::TM || n0 + G::TN > count) change(j, [&](float e, int m) { return n < count && m < rows ? e : 0.0f; });
     }
-    constexpr int kRowUnits = G::TM / 8;
+    constexpr int PARTS = G::PARTS, kRowUnits = G::TM / 8;
     static_assert(G::TM * G::TN <= G::kLds, "a tile of P fits");
 #pragma unroll 1
     for (int part = 0; part < PARTS; ++part) {
@@ -289,20 +289,20 @@ __global__ void __launch_bounds__(G::kThreads) loss_logits_kernel(const LossPara
 
 // dH of a piece: A the weights by columns, B P; a split takes a share of the classes and
 // adds to sums of its own.
-template <class G, int PARTS>
+template <class G>
 __global__ void __launch_bounds__(G::kThreads) loss_dh_kernel(const LossParams p, const Product g) {
   __shared__ __attribute__((aligned(16))) __bf16 lds[G::kLds];
   int tm, tn;
-  if (!tile_of(g.tm, g.tn, tm, tn)) return;
-  const int count = *p.tok.count, m0 = tm * G::TM, n0 = tn * G::TN;
+  if (!tile_of(g.tm, g.tn * p.splits, tm, tn)) return;   // (a split beside the other: an XCD's tiles are of few of them)
+  const int split = tn / g.tn, count = *p.tok.count, m0 = tm * G::TM, n0 = (tn - split * g.tn) * G::TN;
   if (n0 >= count) return;
-  const int all = p.vpad / kStep, each = (all + p.splits - 1) / p.splits, s0 = min((int)blockIdx.y * each, all);
+  const int all = p.vpad / kStep, each = (all + p.splits - 1) / p.splits, s0 = min(split * each, all);
   f32x16 acc[G::FM][G::FN];
-  gemm<G, true, false>(g.a, g.b, m0, n0, (int64_t)s0 * kStep, min(each, all - s0), PARTS, lds, acc);
+  gemm<G, true, false>(g.a, g.b, m0, n0, (int64_t)s0 * kStep, min(each, all - s0), lds, acc);
   const GemmPlace<G> q;
 #pragma unroll
   for (int j = 0; j < G::FN; ++j) {
-    float* const to = p.dh + ((int64_t)blockIdx.y * p.Npad + n0 + q.col(j)) * p.Dpad;
+    float* const to = p.dh + ((int64_t)split * p.Npad + n0 + q.col(j)) * p.Dpad;
 #pragma unroll
     for (int f = 0; f < G::FM; ++f)
 #pragma unroll
@@ -322,14 +322,14 @@ __device__ __forceinline__ float factor(const LossParams& p) {
 }
 
 // dW of a piece: A the hidden rows, B P, both by columns.
-template <class G, int PARTS, typename T>
+template <class G, typename T>
 __global__ void __launch_bounds__(G::kThreads) loss_dw_kernel(const LossParams p, const Product g) {
   __shared__ __attribute__((aligned(16))) __bf16 lds[G::kLds];
   int tm, tn;
   if (!tile_of(g.tm, g.tn, tm, tn)) return;
   const int m0 = tm * G::TM, n0 = tn * G::TN;
   f32x16 acc[G::FM][G::FN];
-  gemm<G, true, true>(g.a, g.b, m0, n0, 0, (*p.tok.count + kStep - 1) / kStep, PARTS, lds, acc);
+  gemm<G, true, true>(g.a, g.b, m0, n0, 0, (*p.tok.count + kStep - 1) / kStep, lds, acc);
   const float s = factor(p);
   const GemmPlace<G> q;
   typedef T V4 __attribute__((ext_vector_type(4)));
@@ -473,30 +473,42 @@ __global__ void __launch_bounds__(256) loss_zero_kernel(T* to, int64_t n) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) to[i] = (T)0.0f;
 }
 
-using Big = GemmTile<256, 256, 4, 2>;
-using Middle = GemmTile<128, 128, 2, 2>;
-using Small = GemmTile<128, 64, 2, 2>;
-using Tiny = GemmTile<64, 64, 2, 2>;
 constexpr int kCUs = 256;
 
-// The largest tile of which most CUs get what they hold, one of the largest or two of the
-// next, else the third, and the least where few CUs get one.  Measured in us, larger and
-// smaller: 5003 classes x 981 tokens x 448, three parts each, the logits with 320 of the
-// second or 640 of the third 49 and 59 (P 56 and 66); 1000 x 64 x 256, 8 of the third or 16 of
-// the least 7.2 and 5.7; the products alone, 50176 x 8192 x 1024, first and second 740 and 836.
-// (BIG false: without the largest, whose accumulators leave no registers for what is made of
-// them.)
-template <bool BIG = true, typename F>
+// The largest tile of which the CUs get as many as they hold, or nearly, else the next.
+// One part: of the largest a CU holds one, of the second two, and the least is taken where
+// few CUs get one.  Measured in us: 50176 classes x 8192 tokens x 1024, the first and the
+// second 740 and 836; 1000 x 64 x 256, 8 of the third or 16 of the least 7.2 and 5.7.
+// Three parts: 16384 x 4096 x 1024, the three 694, 776 and 918; 5003 x 981 x 448, 320, 640
+// and 1264 tiles 35, 34 and 34; 448 x 5003 x 1024, 160, 316 and 553 tiles 46, 44 and 40.
+template <int PARTS, typename F>
 void by_size(int64_t M, int64_t N, F f) {
   auto tiles = [&](int64_t tm, int64_t tn) { return (M + tm - 1) / tm * ((N + tn - 1) / tn); };
-  if constexpr (BIG)
-    if (tiles(256, 256) >= kCUs * 3 / 4) return f(Big{});
-  if (tiles(128, 128) >= kCUs * 3 / 2)
-    f(Middle{});
-  else if (tiles(128, 64) >= kCUs / 2)
-    f(Small{});
+  if constexpr (PARTS == 1) {
+    if (tiles(256, 256) >= kCUs * 3 / 4)
+      f(GemmTile<256, 256, 4, 2>{});
+    else if (tiles(128, 128) >= kCUs * 3 / 2)
+      f(GemmTile<128, 128, 2, 2>{});
+    else if (tiles(128, 64) >= kCUs / 2)
+      f(GemmTile<128, 64, 2, 2>{});
+    else
+      f(GemmTile<64, 64, 2, 2>{});
+  } else {
+    if (tiles(128, 128) >= kCUs * 3)
+      f(GemmTile<128, 128, 4, 2, 3>{});
+    else if (tiles(128, 64) >= kCUs * 2)
+      f(GemmTile<128, 64, 2, 2, 3>{});
+    else
+      f(GemmTile<64, 64, 2, 2, 3>{});
+  }
+}
+// f of the tile that M x N takes
+template <typename F>
+void by_size(int parts, int64_t M, int64_t N, F f) {
+  if (parts == 1)
+    by_size<1>(M, N, f);
   else
-    f(Tiny{});
+    by_size<3>(M, N, f);
 }
 
 template <class G>
@@ -504,24 +516,13 @@ Product product(GemmSide a, GemmSide b, int64_t M, int64_t N) {
   return {a, b, (int)((M + G::TM - 1) / G::TM), (int)((N + G::TN - 1) / G::TN)};
 }
 
-template <typename F>
-void by_parts(int parts, F f) {
-  if (parts == 1)
-    f(std::integral_constant<int, 1>{});
-  else
-    f(std::integral_constant<int, 3>{});
-}
-
 template <bool BWD>
 hipError_t logits(const LossParams& p, hipStream_t stream) {
-  by_parts(p.parts, [&](auto n) {
-    constexpr int PARTS = decltype(n)::value;
-    by_size<!BWD || PARTS == 1>(BWD ? p.vpad : p.V, p.N, [&](auto g) {
-      using G = decltype(g);
-      const Product t = product<G>(side(p.w, p.w_ld, p.w_part, p.vn, 0), side(p.h, p.h_ld, p.h_part, p.h_rows, 0),
-                                   BWD ? p.vpad : p.vn, p.N);
-      hipLaunchKernelGGL((loss_logits_kernel<G, PARTS, BWD>), dim3(grid_of(t.tm, t.tn)), dim3(G::kThreads), 0, stream, p, t);
-    });
+  by_size(p.parts, BWD ? p.vpad : p.V, p.N, [&](auto g) {
+    using G = decltype(g);
+    const Product t = product<G>(side(p.w, p.w_ld, p.w_part, p.vn, 0), side(p.h, p.h_ld, p.h_part, p.h_rows, 0),
+                                 BWD ? p.vpad : p.vn, p.N);
+    hipLaunchKernelGGL((loss_logits_kernel<G, BWD>), dim3(grid_of(t.tm, t.tn)), dim3(G::kThreads), 0, stream, p, t);
   });
   return hipGetLastError();
 }
@@ -558,7 +559,7 @@ hipError_t launch_loss_weight(const LossParams& p, __bf16* to, int dtype, hipStr
 
 int loss_tile_rows(const LossParams& p) {
   int rows = 0;
-  by_size(p.V, p.N, [&](auto g) { rows = decltype(g)::TM; });
+  by_size(p.parts, p.V, p.N, [&](auto g) { rows = decltype(g)::TM; });
   return rows;
 }
 
@@ -580,26 +581,24 @@ hipError_t launch_loss_none(float* loss, float* count, hipStream_t stream) {
 }
 
 hipError_t launch_loss_dh(const LossParams& p, hipStream_t stream) {
-  by_size((int64_t)p.Dpad * p.splits, p.N, [&](auto g) {
+  by_size(p.parts, (int64_t)p.Dpad * p.splits, p.N, [&](auto g) {
     using G = decltype(g);
     const Product t = product<G>(side(p.w, p.w_ld, p.w_part, p.vn, p.Dpad), side(p.p, p.vpad, (int64_t)p.Npad * p.vpad, p.Npad, 0),
                                  p.D, p.N);
-    by_parts(p.parts, [&](auto n) {
-      hipLaunchKernelGGL((loss_dh_kernel<G, decltype(n)::value>), dim3(grid_of(t.tm, t.tn), p.splits), dim3(G::kThreads), 0, stream, p, t);
-    });
+    hipLaunchKernelGGL((loss_dh_kernel<G>), dim3(grid_of(t.tm, t.tn * p.splits)), dim3(G::kThreads), 0, stream, p, t);
   });
   return hipGetLastError();
 }
 
-hipError_t launch_loss_dw(const LossParams& p, int dtype, hipStream_t stream) {
-  by_size(p.D, p.vn, [&](auto g) {
+hipError_t launch_loss_dw(LossParams p, int from, int n, hipStream_t stream) {
+  p.v0 += from;
+  p.vn = n;
+  by_size(p.parts, p.D, n, [&](auto g) {
     using G = decltype(g);
+    using T = std::conditional_t<G::PARTS == 1, __bf16, float>;
     const Product t = product<G>(side(p.h, p.h_ld, p.h_part, p.h_rows, p.Dpad),
-                                 side(p.p, p.vpad, (int64_t)p.Npad * p.vpad, p.Npad, p.vpad), p.D, p.vn);
-    if (dtype == 0)
-      hipLaunchKernelGGL((loss_dw_kernel<G, 3, float>), dim3(grid_of(t.tm, t.tn)), dim3(G::kThreads), 0, stream, p, t);
-    else
-      hipLaunchKernelGGL((loss_dw_kernel<G, 1, __bf16>), dim3(grid_of(t.tm, t.tn)), dim3(G::kThreads), 0, stream, p, t);
+                                 side(p.p + from, p.vpad, (int64_t)p.Npad * p.vpad, p.Npad, p.vpad - from), p.D, n);
+    hipLaunchKernelGGL((loss_dw_kernel<G, T>), dim3(grid_of(t.tm, t.tn)), dim3(G::kThreads), 0, stream, p, t);
   });
   return hipGetLastError();
 }

@@ -54,7 +54,7 @@ bool direct(const osm_loss_args* a) {
 }
 
 // Whether a forward takes all tokens where they are: few, of rows that can be read there.
-// (64 tokens of 256 over 1000 classes: two launches for three, SHORT us.  With more tokens, what
+// (64 tokens of 256 over 1000 classes: two launches for three, 9.7 us for 13.4.  With more tokens, what
 // the others cost is worth leaving out, and the launch is a small part.)
 bool in_place(const osm_loss_args* a) {
   return a->N <= 512 && a->dtype == OSM_BF16 && a->D % 64 == 0 && (uintptr_t)a->hidden % 16 == 0 && a->hidden_stride % 8 == 0 &&
@@ -68,18 +68,21 @@ struct Plan {
   bool direct;
 };
 
-// Classes of a piece: its parts of P (or of the weights) are at most 2^27 elements (2^26: too few for 256
-// tiles of dW at 8192 tokens of 1024, 8% slower; 2^28 and 2^29: the same).
+// Classes of a piece: its parts of P (or of the weights) are at most 9 2^24 elements (less than
+// 2^27: too few for 256 tiles of dW at 8192 tokens of 1024, 8% slower; twice and four times as
+// many: the same; the ninth is for a last piece that is a little longer).
 int64_t piece_of(int64_t V, int64_t rows) {
-  const int64_t most = std::min((int64_t(1) << 27) / rows, kMaxRow - 1) / kLossPad * kLossPad;
+  const int64_t most = std::min((int64_t(9) << 24) / rows, kMaxRow - 1) / kLossPad * kLossPad;
   return std::min(std::max<int64_t>(most, kLossPad), up(V, kLossPad));
 }
 
-// The classes of the next of `left`: as many times 256 tiles of dW (a tile for every CU) as
-// a piece holds, then the rest.
+// Classes of 256 tiles of dW, a tile for every CU.
+int64_t wave_of(int64_t D) { return std::max<int64_t>(1, 256 / ((D + 255) / 256)) * 256; }
+
+// The classes of the next of `left`: all, or as many times 256 tiles of dW as a piece holds.
 int64_t next_piece(int64_t left, int64_t piece, int64_t D) {
-  const int64_t wave = std::max<int64_t>(1, 256 / ((D + 255) / 256)) * 256, n = std::min(left, piece);
-  return n > wave ? n / wave * wave : n;
+  const int64_t wave = wave_of(D);
+  return left <= piece ? left : piece > wave ? piece / wave * wave : piece;
 }
 
 Plan plan_of(const osm_loss_args* a, bool bwd) {
@@ -227,7 +230,11 @@ hipError_t backward(const osm_loss_args* a, const osm_loss_bwd_args* b, const Pl
     p.first = v0 == 0;
     if ((e = set_piece(p, a, n, l, w, v0, vn, st)) != hipSuccess || (e = osm::launch_loss_probs(p, st)) != hipSuccess) return e;
     if (b->grad_hidden && (e = osm::launch_loss_dh(p, st)) != hipSuccess) return e;
-    if (b->grad_weight && (e = osm::launch_loss_dw(p, a->dtype, st)) != hipSuccess) return e;
+    if (!b->grad_weight) continue;
+    // (what is over 256 tiles of dW, in tiles of its own)
+    const int64_t wave = wave_of(a->D), whole = n.parts == 1 && vn > wave ? vn / wave * wave : vn;
+    if ((e = osm::launch_loss_dw(p, 0, (int)whole, st)) != hipSuccess) return e;
+    if (whole < vn && (e = osm::launch_loss_dw(p, (int)whole, (int)(vn - whole), st)) != hipSuccess) return e;
   }
   return b->grad_hidden ? osm::launch_loss_finish(p, a->dtype, st) : hipSuccess;
 }
