@@ -4,7 +4,7 @@
 // Each operand lies by rows (a row holds the k of one m or n) or by columns (a row
 // holds the m or n of one k).  A workgroup forms TM x TN of C.  64 k (32 of
 // operands in parts) of both operands at a time go from memory to LDS without passing
-// through registers, into one of two buffers while the other is multiplied.  By rows, a row's 16-byte units lie in LDS at their index
+// through registers, into one of two (or more) buffers while another is multiplied.  By rows, a row's 16-byte units lie in LDS at their index
 // xor half the row's, so that the 32 rows of a matrix instruction are read from different
 // banks; by columns, a row's 32-byte units lie at theirs xor the row's, so that the 4 rows
 // of a transposing read are.  The order is made by the addresses that are read from memory.
@@ -35,20 +35,25 @@ struct GemmSide {
   int cols;                      // by columns: elements of a row to read, a multiple of 8 (past them: the last ones again)
 };
 
-template <int TM_, int TN_, int WM_, int WN_, int PARTS_ = 1>
+template <int TM_, int TN_, int WM_, int WN_, int PARTS_ = 1, int ST_ = 2>
 struct GemmTile {
   static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_;   // tile; waves along each
-  static constexpr int PARTS = PARTS_;                           // of an operand
+  static constexpr int PARTS = PARTS_, ST = ST_;                 // of an operand; buffers
   static constexpr int KS = PARTS == 1 ? 64 : 32;                // k of a step
   static constexpr int kThreads = 64 * WM * WN;
   static constexpr int FM = TM / WM / 32, FN = TN / WN / 32;     // 32 x 32 squares of a wave
   static constexpr int kBuffer = PARTS * (TM + TN) * KS;         // elements of a buffer: A's parts, then B's
-  static constexpr int kLds = 2 * kBuffer;
+  static constexpr int kLds = ST * kBuffer;
+  static constexpr int kLoads = kBuffer / 8 / kThreads;          // of a thread and step
   static_assert(TM * KS / 8 % kThreads == 0 && TN * KS / 8 % kThreads == 0 && kStep % KS == 0, "whole loads and steps");
 };
 
-// Waits until none of this wave's loads is on its way.
-__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+// Waits until at most N of this wave's loads are on their way.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N < 64, "6 bits");
+  __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4) << 14);
+}
 
 // Where a thread's accumulators lie in C's tile: row(i) of column col, i in [0, 16).
 template <class G>
@@ -169,15 +174,22 @@ __device__ __forceinline__ void gemm(const GemmSide& A, const GemmSide& B, int m
       acc[i][j] = (f32x16)0.0f;
       if (P > 1) small[i][j] = (f32x16)0.0f;
     }
-  // Step t is multiplied while the next one is on its way to where step t - 1 was, which
-  // everyone has read by the barrier.
-  if (steps > 0) fetch(0);
+  // Step t is multiplied while the ST - 1 after it are on their way; the last of those goes
+  // where step t - 1 was, which everyone has read by the barrier.
+#pragma unroll
+  for (int t = 0; t < G::ST - 1; ++t)
+    if (t < steps) fetch(t);
+  int buf = 0;
   for (int t = 0; t < steps; ++t) {
-    wait_loads();
+    if (t + G::ST - 2 < steps)
+      wait_loads<(G::ST - 2) * G::kLoads>();
+    else
+      wait_loads<0>();
     __syncthreads();
-    if (t + 1 < steps) fetch((t + 1) & 1);
-    const __bf16* const la = lds + (t & 1) * G::kBuffer;
+    if (t + G::ST - 1 < steps) fetch(buf == 0 ? G::ST - 1 : buf - 1);
+    const __bf16* const la = lds + buf * G::kBuffer;
     const __bf16* const lb = la + P * G::TM * G::KS;
+    buf = buf == G::ST - 1 ? 0 : buf + 1;
     // By rows, what the next 16 k take is read while these are multiplied, a read after each
     // matrix instruction (50176 x 8192 x 1024: 735 us without, 695 with; transposing reads,
     // twice as many, are better left to the compiler: 231 and 237 us for 1024 x 16384 x 8192).

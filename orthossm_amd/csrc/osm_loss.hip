@@ -479,6 +479,8 @@ constexpr int kCUs = 256;
 // One part: of the largest a CU holds one, of the second two, and the least is taken where
 // few CUs get one.  Measured in us: 50176 classes x 8192 tokens x 1024, the first and the
 // second 740 and 836; 1000 x 64 x 256, 8 of the third or 16 of the least 7.2 and 5.7.
+// (The least, alone on its CU, has two steps on their way: 1024 x 849 x 8192, far apart in
+// memory, 54 for 94; the others gain nothing by it, or lose a workgroup's room.)
 // Three parts: 16384 x 4096 x 1024, the three 694, 776 and 918; 5003 x 981 x 448, 320, 640
 // and 1264 tiles 35, 34 and 34; 448 x 5003 x 1024, 160, 316 and 553 tiles 46, 44 and 40.
 template <int PARTS, typename F>
@@ -492,7 +494,7 @@ void by_size(int64_t M, int64_t N, F f) {
     else if (tiles(128, 64) >= kCUs / 2)
       f(GemmTile<128, 64, 2, 2>{});
     else
-      f(GemmTile<64, 64, 2, 2>{});
+      f(GemmTile<64, 64, 2, 2, 1, 3>{});
   } else {
     if (tiles(128, 128) >= kCUs * 3)
       f(GemmTile<128, 128, 4, 2, 3>{});
