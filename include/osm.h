@@ -562,8 +562,10 @@ typedef struct osm_resnorm_bwd_args {
  * for tokens n with targets_n != ignore_index; the others count for nothing, whatever
  * their hidden rows hold, and their loss and gradients are 0.  A target outside
  * [0, V) gives NaN (the loss, and every gradient that the token has a part in).
- * Products are at fp32's accuracy for fp32 inputs (three bf16 parts an operand) and
- * exact for bf16 ones, sums in fp32.  No counterpart in the reference. */
+ * Products are at fp32's accuracy for fp32 inputs (three bf16 parts an operand; a value
+ * that bf16 rounds to infinity, above 3.39e38, makes NaN) and exact for bf16 ones, sums in
+ * fp32; the backward's probabilities are rounded to bf16 for bf16 inputs (of more than 64
+ * tokens; of fewer to twice the bits).  No counterpart in the reference. */
 #define OSM_LOSS_MEAN 0x1
 
 typedef struct osm_loss_args {
@@ -740,10 +742,10 @@ size_t osm_residual_norm_bwd_workspace_bytes(const osm_resnorm_args* args);
 int osm_residual_norm_bwd(const osm_resnorm_args* args, const osm_resnorm_bwd_args* bwd, void* workspace,
                           size_t workspace_bytes, void* stream);
 
-/* The cross entropy and its backward (from hidden, weight, targets and lse; losses
-, loss and
- * count of `args` are not used).  Workspaces as above.  The backward forms the
- * probabilities of a piece of the vocabulary at a time. */
+/* The cross entropy and its backward (from hidden, weight, targets and lse; losses, loss
+ * and count of `args` are not used).  Workspaces as above.  The backward forms the
+ * probabilities of a piece of the vocabulary at a time: up to 302 MB of them (more only
+ * where 256 classes of all tokens are more). */
 size_t osm_linear_ce_workspace_bytes(const osm_loss_args* args);
 int osm_linear_ce_fwd(const osm_loss_args* args, void* workspace, size_t workspace_bytes, void* stream);
 size_t osm_linear_ce_bwd_workspace_bytes(const osm_loss_args* args);

@@ -2,17 +2,24 @@
 // sum_k A(m, k) B(n, k): what the vocabulary's cross entropy is built on.
 //
 // Each operand lies by rows (a row holds the k of one m or n) or by columns (a row
-// holds the m or n of one k).  A workgroup forms TM x TN of C.  64 k (32 of
-// operands in parts) of both operands at a time go from memory to LDS without passing
-// through registers, into one of two (or more) buffers while another is multiplied.  By rows, a row's 16-byte units lie in LDS at their index
-// xor half the row's, so that the 32 rows of a matrix instruction are read from different
-// banks; by columns, a row's 32-byte units lie at theirs xor the row's, so that the 4 rows
-// of a transposing read are.  The order is made by the addresses that are read from memory.
+// holds the m or n of one k).  A workgroup forms TM x TN of C.  64 k (32 of operands in
+// parts) of both operands at a time go from memory to LDS without passing through
+// registers, into one buffer while another is multiplied.  By rows, a row's 16-byte units
+// lie in LDS at their index xor half the row's, so that the 32 rows of a matrix
+// instruction are read from different banks; by columns, a row's 32-byte units lie at
+// theirs xor the row's, so that the 4 rows of a transposing read are.  The order is made by
+// the addresses that are read from memory.
+//
 // An fp32 operand is three bf16 matrices whose sum it is (its parts), and the product the
 // sum of the six products of parts that are not below 2^-24: the product of the first
 // parts, and in accumulators of their own the five small ones.  All parts of a step lie in
 // LDS together: they come from memory and are read once for the six products (5003 x 981 x
 // 448: 34 us; with a walk over k for each product 49).
+//
+// What bounds it: the matrix instructions, half of the time (50176 x 8192 x 1024 in tiles of
+// 256 x 256: 680 us, 1238 TFLOP/s, by columns both ways 1170; 16384 x 4096 x 1024 of three
+// parts 1172), and between them the barrier at a step's end, where all waves wait for the
+// next step's loads; 128 KB of LDS leave no room for a third buffer.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -41,6 +48,7 @@ struct GemmTile {
   static constexpr int PARTS = PARTS_, ST = ST_;                 // of an operand; buffers
   static constexpr int KS = PARTS == 1 ? 64 : 32;                // k of a step
   static constexpr int kThreads = 64 * WM * WN;
+  static constexpr bool kFew = PARTS == 1 && TM < 256;           // for few tokens too
   static constexpr int FM = TM / WM / 32, FN = TN / WN / 32;     // 32 x 32 squares of a wave
   static constexpr int kBuffer = PARTS * (TM + TN) * KS;         // elements of a buffer: A's parts, then B's
   static constexpr int kLds = ST * kBuffer;
@@ -148,7 +156,15 @@ struct GemmOperand {
   }
 };
 
-// acc = the m from m0 of A times the n from n0 of B over n_steps times kStep k from k0 on (a
+template <class G>
+__device__ __forceinline__ void zero(f32x16 (&acc)[G::FM][G::FN]) {
+#pragma unroll
+  for (int i = 0; i < G::FM; ++i)
+#pragma unroll
+    for (int j = 0; j < G::FN; ++j) acc[i][j] = (f32x16)0.0f;
+}
+
+// acc += the m from m0 of A times the n from n0 of B over n_steps times kStep k from k0 on (a
 // multiple of kStep).
 template <class G, bool ACOLS, bool BCOLS>
 __device__ __forceinline__ void gemm(const GemmSide& A, const GemmSide& B, int m0, int n0, int64_t k0, int n_steps, __bf16* lds,
@@ -167,13 +183,7 @@ __device__ __forceinline__ void gemm(const GemmSide& A, const GemmSide& B, int m
     b.fetch(to + P * G::TM * G::KS * 2);
   };
   f32x16 small[P == 1 ? 1 : G::FM][G::FN];
-#pragma unroll
-  for (int i = 0; i < G::FM; ++i)
-#pragma unroll
-    for (int j = 0; j < G::FN; ++j) {
-      acc[i][j] = (f32x16)0.0f;
-      if (P > 1) small[i][j] = (f32x16)0.0f;
-    }
+  if constexpr (P > 1) zero<G>(small);
   // Step t is multiplied while the ST - 1 after it are on their way; the last of those goes
   // where step t - 1 was, which everyone has read by the barrier.
 #pragma unroll

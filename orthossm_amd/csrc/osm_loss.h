@@ -19,7 +19,7 @@ struct LossTokens {
 
 struct LossParams {
   int64_t N, D, V;
-  int Npad, Dpad, parts;           // parts: 1 (bf16), 3 (fp32)
+  int Npad, Dpad, parts, p_parts;  // parts of hidden and weight: 1 (bf16), 3 (fp32); of p: 2 of few bf16 tokens
   const void* hidden;
   int64_t hidden_s;
   const void* weight;
@@ -35,7 +35,7 @@ struct LossParams {
   int vn, vpad;                    // its classes; columns of p
   const __bf16* w;                 // [parts][vn][w_ld], w_part apart
   int64_t w_ld, w_part;
-  __bf16* p;                       // [parts][Npad][vpad]: probabilities less the targets'
+  __bf16* p;                       // [p_parts][Npad][vpad]: probabilities less the targets'
   float* dh;                       // [splits][Npad][Dpad]
   int splits, first;               // first: dh is written, not added to
   // statistics

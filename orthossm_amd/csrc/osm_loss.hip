@@ -5,13 +5,19 @@
 //
 // Forward: a workgroup forms a tile of logits by classes and tokens in its
 // accumulators and leaves of it, for every token, the largest and the sum of
-// exponentials below it; a second kernel joins the tiles.  Backward, a piece of the
-// vocabulary at a time: the logits again, from them P (to bf16, or three bf16 parts of
-// an fp32 result), then the two products, which read W, P and H by columns where they
+// exponentials below it (an online softmax over tiles); a second kernel joins the tiles.  Backward, a piece of the
+// vocabulary at a time: the logits again, from them P (to bf16, of few tokens to two bf16
+// parts, of fp32 to three), then the two products, which read W, P and H by columns where they
 // have to.  What counts for all of them: the products' operations on the matrix
 // instruction (osm_gemm.h); the tokens that do not count are left out first, so they
 // cost nothing.  Exponentials and logarithms are those of 2: l log2(e) less the largest
 // is one fused operation, and what its rounding leaves out cancels in the loss.
+//
+// 8192 tokens, 50001 classes, 1024 columns, bf16: forward 890 us (943 TFLOP/s of 1213 that the
+// product alone reaches; its epilogue, which nothing overlaps, takes 12%, four fifths of it the
+// exponentials), P 975, dH 860, dW 860; a library's product of the logits alone takes 815, with
+// 1.6 GB of them written.  4096 tokens, 32768 classes of 1024, forward: 255 us, 1080 TFLOP/s.
+// 981 tokens, 5003 classes, 448 columns, fp32: 48, 55, 59, 47 us, 26 GFLOP in bf16 each.
 #include <algorithm>
 #include <type_traits>
 
@@ -204,6 +210,7 @@ __global__ void __launch_bounds__(G::kThreads) loss_logits_kernel(const LossPara
     if (BWD) factors[j] = p.tok.factors[n];
   }
   f32x16 acc[G::FM][G::FN];
+  zero<G>(acc);
   gemm<G, false, false>(g.a, g.b, m0, n0, 0, p.Dpad / kStep, lds, acc);
   // f(value, row) for the rows that a lane holds of column j; change: what it gives takes the value's place
   auto each = [&](int j, auto f) {
@@ -251,12 +258,13 @@ __global__ void __launch_bounds__(G::kThreads) loss_logits_kernel(const LossPara
       if (p.grad_losses) change(j, [&](float e, int) { return e * factors[j].y; });
       if (rows < G::TM || n0 + G::TN > count) change(j, [&](float e, int m) { return n < count && m < rows ? e : 0.0f; });
     }
-    constexpr int PARTS = G::PARTS, kRowUnits = G::TM / 8;
+    constexpr int kRowUnits = G::TM / 8;
+    const int parts = G::PARTS > 1 ? G::PARTS : G::kFew ? p.p_parts : 1;
     static_assert(G::TM * G::TN <= G::kLds, "a tile of P fits");
 #pragma unroll 1
-    for (int part = 0; part < PARTS; ++part) {
+    for (int part = 0; part < parts; ++part) {
       // a lane's four neighbouring classes are half a 16-byte unit, which lies at its index
-      // xor its token's; what the next part is made of stays in acc
+      // xor its token's; then the next part is what rounding left
 #pragma unroll
       for (int j = 0; j < G::FN; ++j)
 #pragma unroll
@@ -266,10 +274,7 @@ __global__ void __launch_bounds__(G::kThreads) loss_logits_kernel(const LossPara
             const int c = q.col(j), r = q.row(f, i);
             bf16x4 v;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              v[k] = (__bf16)acc[f][j][i + k];
-              if (PARTS > 1) acc[f][j][i + k] -= (float)v[k];
-            }
+            for (int k = 0; k < 4; ++k) v[k] = (__bf16)acc[f][j][i + k];
             *reinterpret_cast<bf16x4*>(lds + c * G::TM + ((r / 8) ^ (c % kRowUnits)) * 8 + r % 8) = v;
           }
       __syncthreads();
@@ -282,9 +287,21 @@ __global__ void __launch_bounds__(G::kThreads) loss_logits_kernel(const LossPara
           wide_store_wait();
         }
       }
-      if (part + 1 < PARTS) __syncthreads();
+      if (part + 1 == parts) break;
+#pragma unroll
+      for (int j = 0; j < G::FN; ++j) change(j, [&](float e, int) { return e - (float)(__bf16)e; });
+      __syncthreads();
     }
   }
+}
+
+// f of P, whose parts a product of three part operands takes by itself; where few tokens'
+// has two, each is a walk of its own.
+template <class G, typename F>
+__device__ __forceinline__ void over_parts(const LossParams& p, GemmSide b, F f) {
+  const int n = G::kFew ? p.p_parts : 1;
+#pragma unroll 1
+  for (int i = 0; i < n; ++i, b.p += b.part) f(b);
 }
 
 // dH of a piece: A the weights by columns, B P; a split takes a share of the classes and
@@ -298,7 +315,10 @@ __global__ void __launch_bounds__(G::kThreads) loss_dh_kernel(const LossParams p
   if (n0 >= count) return;
   const int all = p.vpad / kStep, each = (all + p.splits - 1) / p.splits, s0 = min(split * each, all);
   f32x16 acc[G::FM][G::FN];
-  gemm<G, true, false>(g.a, g.b, m0, n0, (int64_t)s0 * kStep, min(each, all - s0), lds, acc);
+  zero<G>(acc);
+  over_parts<G>(p, g.b, [&](const GemmSide& b) {
+    gemm<G, true, false>(g.a, b, m0, n0, (int64_t)s0 * kStep, min(each, all - s0), lds, acc);
+  });
   const GemmPlace<G> q;
 #pragma unroll
   for (int j = 0; j < G::FN; ++j) {
@@ -329,7 +349,10 @@ __global__ void __launch_bounds__(G::kThreads) loss_dw_kernel(const LossParams p
   if (!tile_of(g.tm, g.tn, tm, tn)) return;
   const int m0 = tm * G::TM, n0 = tn * G::TN;
   f32x16 acc[G::FM][G::FN];
-  gemm<G, true, true>(g.a, g.b, m0, n0, 0, (*p.tok.count + kStep - 1) / kStep, lds, acc);
+  zero<G>(acc);
+  over_parts<G>(p, g.b, [&](const GemmSide& b) {
+    gemm<G, true, true>(g.a, b, m0, n0, 0, (*p.tok.count + kStep - 1) / kStep, lds, acc);
+  });
   const float s = factor(p);
   const GemmPlace<G> q;
   typedef T V4 __attribute__((ext_vector_type(4)));
@@ -475,42 +498,41 @@ __global__ void __launch_bounds__(256) loss_zero_kernel(T* to, int64_t n) {
 
 constexpr int kCUs = 256;
 
-// The largest tile of which the CUs get as many as they hold, or nearly, else the next.
-// One part: of the largest a CU holds one, of the second two, and the least is taken where
-// few CUs get one.  Measured in us: 50176 classes x 8192 tokens x 1024, the first and the
-// second 740 and 836; 1000 x 64 x 256, 8 of the third or 16 of the least 7.2 and 5.7.
-// (The least, alone on its CU, has two steps on their way: 1024 x 849 x 8192, far apart in
-// memory, 54 for 94; the others gain nothing by it, or lose a workgroup's room.)
-// Three parts: 16384 x 4096 x 1024, the three 694, 776 and 918; 5003 x 981 x 448, 320, 640
-// and 1264 tiles 35, 34 and 34; 448 x 5003 x 1024, 160, 316 and 553 tiles 46, 44 and 40.
-template <int PARTS, typename F>
-void by_size(int64_t M, int64_t N, F f) {
+// The largest tile of which the CUs get as many as they hold, or nearly, else the next; none
+// that is more than twice as wide as the product.  Measured in us, the larger and the smaller:
+//   50176 classes x 8192 tokens x 1024, the first and the second: 680, 855
+//   64 tokens over 50001 classes of 1024, forward, the first and the third: 40, 27
+//   1000 x 64 x 256, 8 of the third or 16 of the least: 4.0, 3.3
+//   1024 x 849 x 8192, 56 of the second, 112 of the third, 224 of the least: 81, 71, 61
+// (The least, alone on its CU, has two steps on their way: 43 for those 61, and 54 for 94 where
+// rows lie 35 KB apart.  The others gain nothing by it, or lose a workgroup's room.)
+// Three parts, the three tiles:
+//   16384 x 4096 x 1024: 703, 791, 922
+//   5003 x 981 x 448, 320, 640 and 1264 tiles: 38, 36, 37
+//   448 x 5003 x 1024, 160, 316 and 553 tiles: 50, 47, 44
+// The gradient of few tokens' weights has no use for the first tile, which could not hold what
+// P's two parts take: it writes more than it multiplies.
+template <typename F>
+void by_size(const LossParams& p, int64_t M, int64_t N, F f) {
   auto tiles = [&](int64_t tm, int64_t tn) { return (M + tm - 1) / tm * ((N + tn - 1) / tn); };
-  if constexpr (PARTS == 1) {
-    if (tiles(256, 256) >= kCUs * 3 / 4)
+  const int64_t least = std::min(M, N);
+  if (p.parts == 1) {
+    if (tiles(256, 256) >= kCUs * 3 / 4 && least > 128 && p.p_parts == 1)
       f(GemmTile<256, 256, 4, 2>{});
-    else if (tiles(128, 128) >= kCUs * 3 / 2)
+    else if (tiles(128, 128) >= kCUs * 3 / 2 && least > 64)
       f(GemmTile<128, 128, 2, 2>{});
     else if (tiles(128, 64) >= kCUs / 2)
       f(GemmTile<128, 64, 2, 2>{});
     else
       f(GemmTile<64, 64, 2, 2, 1, 3>{});
   } else {
-    if (tiles(128, 128) >= kCUs * 3)
+    if (tiles(128, 128) >= kCUs * 3 && least > 64)
       f(GemmTile<128, 128, 4, 2, 3>{});
     else if (tiles(128, 64) >= kCUs * 2)
       f(GemmTile<128, 64, 2, 2, 3>{});
     else
       f(GemmTile<64, 64, 2, 2, 3>{});
   }
-}
-// f of the tile that M x N takes
-template <typename F>
-void by_size(int parts, int64_t M, int64_t N, F f) {
-  if (parts == 1)
-    by_size<1>(M, N, f);
-  else
-    by_size<3>(M, N, f);
 }
 
 template <class G>
@@ -520,7 +542,7 @@ Product product(GemmSide a, GemmSide b, int64_t M, int64_t N) {
 
 template <bool BWD>
 hipError_t logits(const LossParams& p, hipStream_t stream) {
-  by_size(p.parts, BWD ? p.vpad : p.V, p.N, [&](auto g) {
+  by_size(p, BWD ? p.vpad : p.V, p.N, [&](auto g) {
     using G = decltype(g);
     const Product t = product<G>(side(p.w, p.w_ld, p.w_part, p.vn, 0), side(p.h, p.h_ld, p.h_part, p.h_rows, 0),
                                  BWD ? p.vpad : p.vn, p.N);
@@ -561,7 +583,7 @@ hipError_t launch_loss_weight(const LossParams& p, __bf16* to, int dtype, hipStr
 
 int loss_tile_rows(const LossParams& p) {
   int rows = 0;
-  by_size(p.parts, p.V, p.N, [&](auto g) { rows = decltype(g)::TM; });
+  by_size(p, p.V, p.N, [&](auto g) { rows = decltype(g)::TM; });
   return rows;
 }
 
@@ -583,7 +605,7 @@ hipError_t launch_loss_none(float* loss, float* count, hipStream_t stream) {
 }
 
 hipError_t launch_loss_dh(const LossParams& p, hipStream_t stream) {
-  by_size(p.parts, (int64_t)p.Dpad * p.splits, p.N, [&](auto g) {
+  by_size(p, (int64_t)p.Dpad * p.splits, p.N, [&](auto g) {
     using G = decltype(g);
     const Product t = product<G>(side(p.w, p.w_ld, p.w_part, p.vn, p.Dpad), side(p.p, p.vpad, (int64_t)p.Npad * p.vpad, p.Npad, 0),
                                  p.D, p.N);
@@ -595,7 +617,7 @@ hipError_t launch_loss_dh(const LossParams& p, hipStream_t stream) {
 hipError_t launch_loss_dw(LossParams p, int from, int n, hipStream_t stream) {
   p.v0 += from;
   p.vn = n;
-  by_size(p.parts, p.D, n, [&](auto g) {
+  by_size(p, p.D, n, [&](auto g) {
     using G = decltype(g);
     using T = std::conditional_t<G::PARTS == 1, __bf16, float>;
     const Product t = product<G>(side(p.h, p.h_ld, p.h_part, p.h_rows, p.Dpad),

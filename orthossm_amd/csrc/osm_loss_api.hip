@@ -63,7 +63,7 @@ bool in_place(const osm_loss_args* a) {
 
 // What a launch works on: the compacted hidden rows, and pieces of the vocabulary.
 struct Plan {
-  int64_t Npad, Dpad, parts, piece;   // piece: classes, a multiple of kLossPad
+  int64_t Npad, Dpad, parts, p_parts, piece;   // piece: classes, a multiple of kLossPad
   int splits;
   bool direct;
 };
@@ -88,11 +88,15 @@ int64_t next_piece(int64_t left, int64_t piece, int64_t D) {
 Plan plan_of(const osm_loss_args* a, bool bwd) {
   Plan n;
   n.parts = a->dtype == OSM_F32 ? 3 : 1;
+  // (P rounded to bf16 adds as much to a gradient's error as the gradient's own rounding, and
+  // no more where many tokens' errors mean out: of few tokens, which cost little, it is held
+  // to twice the bits.)
+  n.p_parts = n.parts == 1 && a->N <= 64 ? 2 : n.parts;
   n.Npad = up(std::max<int64_t>(a->N, 1), kLossPad);
   n.Dpad = up(a->D, 64);
   n.direct = direct(a);
   const int64_t across = (a->D + 255) / 256;
-  n.piece = bwd ? piece_of(a->V, n.Npad * n.parts) : n.direct ? up(a->V, kLossPad) : piece_of(a->V, n.Dpad * n.parts);
+  n.piece = bwd ? piece_of(a->V, n.Npad * n.p_parts) : n.direct ? up(a->V, kLossPad) : piece_of(a->V, n.Dpad * n.parts);
   const int64_t tiles = across * (n.Npad / 256);
   n.splits = (int)std::max<int64_t>(1, std::min<int64_t>({256 / std::max<int64_t>(1, tiles), n.piece / 1024, 8}));
   return n;
@@ -124,7 +128,7 @@ Layout layout_of(const osm_loss_args* a, const Plan& n, bool bwd) {
     l.own = r.add(n.Npad * 4);
     l.stat = r.add((size_t)(up(a->V, kLossPad) / 64) * n.Npad * 8);
   } else {
-    l.p = r.add((size_t)n.parts * n.Npad * n.piece * 2);
+    l.p = r.add((size_t)n.p_parts * n.Npad * n.piece * 2);
     l.dh = r.add((size_t)n.splits * n.Npad * n.Dpad * 4);
   }
   l.total = r.total;
@@ -146,6 +150,7 @@ LossParams params_of(const osm_loss_args* a, const Plan& n, const Layout& l, voi
   p.Npad = (int)n.Npad;
   p.Dpad = (int)n.Dpad;
   p.parts = (int)n.parts;
+  p.p_parts = (int)n.p_parts;
   p.hidden = a->hidden;
   p.hidden_s = a->hidden_stride;
   p.weight = a->weight;

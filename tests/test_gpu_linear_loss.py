@@ -6,7 +6,8 @@ d = (D + 8) 2^-24 max_v sum |h w| (and another 2^-22 |logit| where logits are as
 16, for exp2's argument).  A loss is off by 2 d and the roundings of the sums of
 exponentials over up to 64 elements, their joins and the logarithm: 80 2^-24 of a factor,
 so 5e-6.  A probability less its target's one is off by 2 d + 5e-6 of the probability, and,
-for bf16 inputs, rounded to bf16: 2^-8 of the value, the sum of 3 parts for fp32: 3 2^-24.
+for bf16 inputs, rounded to bf16: 2^-8 of the value (up to 64 tokens: the sum of 2 parts,
+2^-16), the sum of 3 parts for fp32: 3 2^-24.
 The gradients add up terms P W and P H: (V + 16) 2^-24, (N + 16) 2^-24 of the sum of their
 sizes, and bf16 results half a unit in the last place, 2^-8.
 """
@@ -54,7 +55,7 @@ def check(dev, hidden, weight, targets, ignore=IGNORE):
     off = P * (2 * d + 5e-6)
     P[at, t] -= 1.0
     # rounded to bf16, once and (with each token's own gradient in it) as it is used
-    off = off + P.abs() * (2.0 ** -8 if bf else 4 * 2.0 ** -24)
+    off = off + P.abs() * ((2.0 ** -16 if N <= 64 else 2.0 ** -8) if bf else 4 * 2.0 ** -24)
     leaves = [hd.requires_grad_(), wd.requires_grad_()]
     for reduction, each_g in (("none", g[keep].double()), ("sum", torch.full((keep.numel(),), 0.75, dtype=torch.float64)),
                               ("mean", torch.full((keep.numel(),), 0.75 / max(1, keep.numel()), dtype=torch.float64))):
@@ -99,6 +100,13 @@ def test_vocabularies(dev, V, dtype):
 @pytest.mark.parametrize("D", [1, 3, 8, 31, 63, 64, 65, 100, 128, 200, 256, 257, 512, 1000])
 def test_widths(dev, D, dtype):
     check(dev, *make(40, D, 150, dtype, seed=D))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N", [1, 64, 65, 129])
+def test_few_tokens_over_many_classes(dev, N, dtype):
+    check(dev, *make(N, 64, 49400, dtype, seed=N, ignored=0.2 if N > 1 else 0.0))
+    check(dev, *make(N, 2100, 700, dtype, seed=N))
 
 
 @pytest.mark.parametrize("dtype", TYPES)
