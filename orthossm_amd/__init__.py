@@ -10,6 +10,12 @@ call sites in ``orthossm_amd.engine``.
 For layers that learn at test time with a matrix-valued state: the gated delta
 rule (chunked forward and backward, one-token step), layer norm and gradient
 clipping, and ``GatedDeltaLayer``, which runs them together.
+
+For models around either recurrence: an EMA whose decay is learned per channel
+and token (``gated_ema``, one-token step over a pool of states), a block's
+residual update between its two norms (``residual_norm``) and the cross entropy
+of a vocabulary without its logits (``linear_cross_entropy``), each with its
+gradients.
 """
 from .ops import cheby_ema, cheby_ema_backward, cheby_ema_forward, cheby_ema_ttt
 from .sdpc_kernel import apply_cheby_rkv_core, apply_cheby_rkv_v10

@@ -13,11 +13,12 @@
 // cost nothing.  Exponentials and logarithms are those of 2: l log2(e) less the largest
 // is one fused operation, and what its rounding leaves out cancels in the loss.
 //
-// 8192 tokens, 50001 classes, 1024 columns, bf16: forward 890 us (943 TFLOP/s of 1213 that the
-// product alone reaches; its epilogue, which nothing overlaps, takes 12%, four fifths of it the
-// exponentials), P 975, dH 860, dW 860; a library's product of the logits alone takes 815, with
-// 1.6 GB of them written.  4096 tokens, 32768 classes of 1024, forward: 255 us, 1080 TFLOP/s.
-// 981 tokens, 5003 classes, 448 columns, fp32: 48, 55, 59, 47 us, 26 GFLOP in bf16 each.
+// 8192 tokens, 50001 classes, 1024 columns, bf16: forward 813 to 900 us from GPU to GPU (1030 to
+// 930 TFLOP/s; the product alone 680; its epilogue, which nothing overlaps, takes 12%, most of it
+// the exponentials), P 930, dH 850, dW 820; a library's product for the logits alone takes 815,
+// with 0.8 GB of them written.  4096 tokens, 32768 classes, 1024 columns, forward: 255 us,
+// 1080 TFLOP/s.  981 tokens, 5003 classes, 400 columns, fp32: 48, 54, 59, 47 us, of 6 products
+// of 4 GFLOP each.
 #include <algorithm>
 #include <type_traits>
 
@@ -278,13 +279,24 @@ __global__ void __launch_bounds__(G::kThreads) loss_logits_kernel(const LossPara
             *reinterpret_cast<bf16x4*>(lds + c * G::TM + ((r / 8) ^ (c % kRowUnits)) * 8 + r % 8) = v;
           }
       __syncthreads();
-#pragma unroll 4
-      for (int u = threadIdx.x; u < G::TN * kRowUnits; u += G::kThreads) {
-        const int c = u / kRowUnits, r = u % kRowUnits;
-        const bf16x8 v = *reinterpret_cast<const bf16x8*>(lds + c * G::TM + (r ^ (c % kRowUnits)) * 8);
-        if (m0 + r * 8 < p.vpad) {
-          *reinterpret_cast<bf16x8*>(p.p + ((int64_t)part * p.Npad + n0 + c) * p.vpad + m0 + r * 8) = v;
-          wide_store_wait();
+      constexpr int kEach = G::TN * kRowUnits / G::kThreads, kAtOnce = kEach < 4 ? kEach : 4;   // units of a thread
+      static_assert(G::kThreads % kRowUnits == 0 && kEach % kAtOnce == 0, "a thread's units are of one class");
+      const int c0 = threadIdx.x / kRowUnits, r = threadIdx.x % kRowUnits;
+      if (m0 + r * 8 < p.vpad) {
+        __bf16* const to = p.p + ((int64_t)part * p.Npad + n0 + c0) * p.vpad + m0 + r * 8;
+#pragma unroll
+        for (int k = 0; k < kEach; k += kAtOnce) {
+          bf16x8 v[kAtOnce];
+#pragma unroll
+          for (int i = 0; i < kAtOnce; ++i) {
+            const int c = c0 + (k + i) * (G::kThreads / kRowUnits);
+            v[i] = *reinterpret_cast<const bf16x8*>(lds + c * G::TM + (r ^ (c % kRowUnits)) * 8);
+          }
+#pragma unroll
+          for (int i = 0; i < kAtOnce; ++i) {
+            *reinterpret_cast<bf16x8*>(to + (int64_t)(k + i) * (G::kThreads / kRowUnits) * p.vpad) = v[i];
+            wide_store_wait();
+          }
         }
       }
       if (part + 1 == parts) break;

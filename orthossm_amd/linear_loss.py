@@ -14,7 +14,8 @@ hidden's shape without D.  Tokens whose target is ``ignore_index`` count for
 nothing, whatever their hidden rows hold: their losses and gradients are 0.  A
 target outside [0, V) gives NaN: that token's loss, and every gradient that it
 has a part in.  Logits, sums and losses are fp32; the gradients' factors
-softmax - onehot are rounded to bf16 for bf16 inputs.
+softmax - onehot are rounded to bf16 for bf16 inputs (up to 64 tokens: to the
+sum of two bf16 numbers).
 
 The backward forms the logits of a piece of the vocabulary at a time: its
 memory is bounded by the pieces, not by the vocabulary.  All run on the current
