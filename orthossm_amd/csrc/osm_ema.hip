@@ -11,6 +11,11 @@
 // (which the group's last tile publishes), and runs its tokens from there.  The
 // order of composition is fixed, so results do not depend on timing.
 //
+// What bounds both: the bytes of x, gate, h (x, gate, dh, dx, dgate).  8x32768x1024 bf16:
+// forward 335 us, 4.8 TB/s, backward, in tiles of 64 tokens since it holds twice as much of
+// each, 605 us, 4.4 TB/s (groups of four tiles: 337 and 610).  Few lane-blocks: the chain
+// from group to group.
+//
 // The tiles that a block waits for are at work before it is: where the lane-blocks are a
 // multiple of 8, blocks take their tiles by index, and those of a lane-block are on one
 // XCD, to which blocks go in the order of their index; else a block draws its tile from

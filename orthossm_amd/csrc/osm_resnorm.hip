@@ -8,7 +8,9 @@
 //   dy = s_y (e - mean(e) - yh mean(e yh))
 //   dw = sum_rows dn rh,  db = sum_rows dn,  dscale = sum_rows dr u      (no mean(g), mean(e) with rms)
 //
-// What bounds both: the bytes of x, y, gate, r, n (x, y, gate, dr, dn, dx, dy, dgate).
+// What bounds both: the bytes of x, y, gate, r, n (x, y, gate, dr, dn, dx, dy, dgate);
+// 262144 rows of 1024, blocks in bf16 around an fp32 stream: forward 650 us, 5.8 TB/s,
+// backward 1210 us, 4.9 TB/s.
 // A row is held in the registers of a quarter of a wave, of one, of four or of
 // sixteen, so every input is read once, and the next row is on its way while one is
 // worked on.  The backward forms r again from x, y and gate and the saved statistics,
@@ -558,7 +560,8 @@ __global__ void __launch_bounds__(kFoldCols * kFoldGroups) resnorm_fold_kernel(c
 }
 
 // Calls go(TPR, NV) for the fewest threads that hold a row, up to 16 elements each
-// (LAST in the case of 1024 threads), or long_rows() past that.
+// (LAST in the case of 1024 threads), or long_rows() past that.  (Rows of 1024 columns around
+// an fp32 stream by 256 threads in place of 64: forward 841 us for 660, backward the same.)
 template <int U, int LAST, typename Go, typename Long>
 void by_length(int64_t D, Go go, Long long_rows) {
   const int64_t units = (D + U - 1) / U;
@@ -578,11 +581,13 @@ void by_length(int64_t D, Go go, Long long_rows) {
     long_rows();
 }
 
-constexpr int kMaxGroups = 8192;
+// Workgroups of a forward, each of which walks rows a grid apart (262144 rows of 1024 around an
+// fp32 stream: 2048, 8192 and 32768 take 678, 660 and 643 us).
+constexpr int kMaxGroups = 32768;
 constexpr int kLastFwd = 16, kLastBwd = 8;   // elements of a thread where 1024 hold a row
 
 // Columns of a unit: 16 bytes of the wider type, so that a wave's accesses to either are
-// without gaps.
+// without gaps (8 columns of an fp32 stream: 871 and 1368 us for 660 and 1317).
 template <typename TX>
 constexpr int kUnit = 16 / (int)sizeof(TX);
 
