@@ -247,6 +247,41 @@ def test_on_another_stream(dev, path, name):
     assert all(torch.equal(a, b) for a, b in zip(want, got))
 
 
+@pytest.mark.parametrize("name", ["ema", "block", "block rms", "loss", "loss sum", "loss none"])
+def test_a_captured_training_pass(dev, path, name, monkeypatch):
+    """Forward and backward in a graph, replayed between eager passes over the same leaves
+    (none of which is alive while the graph is captured)."""
+    make, call = CALLS[name]
+    goal = targets()
+    monkeypatch.setitem(globals(), "targets", lambda: goal)   # (made from the host)
+    leaves = [t.requires_grad_() for t in make()]
+    weights = [torch.full_like(o, 0.5) for o in call([t.detach() for t in leaves])]
+
+    def once():
+        outs = call(leaves)
+        grads = torch.autograd.grad(outs, leaves, weights, allow_unused=True)
+        return [o.detach() for o in outs] + [g for g in grads if g is not None]
+
+    want = [t.clone() for t in once()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        once()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = once()
+    for _ in range(3):
+        for t in held:
+            t.zero_()
+        graph.replay()
+        got = once()
+        torch.cuda.synchronize()
+        for a, b, c in zip(want, got, held):
+            assert torch.equal(a, b) and torch.equal(a, c)
+
+
 class Model(torch.nn.Module):
     """Layers of the gated EMA between residual norms, and the loss."""
 
