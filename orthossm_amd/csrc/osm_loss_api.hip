@@ -96,7 +96,10 @@ Plan plan_of(const osm_loss_args* a, bool bwd) {
   n.Dpad = up(a->D, 64);
   n.direct = direct(a);
   const int64_t across = (a->D + 255) / 256;
-  n.piece = bwd ? piece_of(a->V, n.Npad * n.p_parts) : n.direct ? up(a->V, kLossPad) : piece_of(a->V, n.Dpad * n.parts);
+  // (a forward's launch has at most 2^32 threads, 256 for 64 x 64)
+  const int64_t most = std::max<int64_t>((int64_t(1) << 36) / n.Npad / kLossPad * kLossPad - kLossPad, kLossPad);
+  n.piece = bwd ? piece_of(a->V, n.Npad * n.p_parts)
+                : std::min(most, n.direct ? up(a->V, kLossPad) : piece_of(a->V, n.Dpad * n.parts));
   const int64_t tiles = across * (n.Npad / 256);
   n.splits = (int)std::max<int64_t>(1, std::min<int64_t>({256 / std::max<int64_t>(1, tiles), n.piece / 1024, 8}));
   return n;

@@ -10,10 +10,13 @@ thread's rows, four row groups, an eighth of the lines of sums): 200 2^-24 of th
 the terms' sizes.  The gradients to rows are differences (for one or two elements a row
 nearly all of them cancels), so their bounds are relative to the size of their terms.
 """
+import ctypes
+
 import pytest
 import torch
 
-from orthossm_amd import layer_norm, residual_norm, residual_norm_backward, residual_norm_forward
+from orthossm_amd import _native as nat
+from orthossm_amd import block_norm, layer_norm, residual_norm, residual_norm_backward, residual_norm_forward
 
 pytestmark = pytest.mark.gpu
 FP32 = 1.6e-5
@@ -251,6 +254,18 @@ def test_empty(dev):
         r, n = residual_norm(x, x.detach(), wl, scale=sl)
         gx, gw, gs = torch.autograd.grad((r, n), (x, wl, sl), (torch.zeros(shape, device=dev),) * 2)
         assert r.shape == n.shape == gx.shape == shape and (gw == 0).all() and (gs == 0).all()
+
+
+@pytest.mark.parametrize("rows,D", [(70, 33), (300, 1024), (5, 9000), (9, 20000)])
+def test_outputs_in_the_inputs_memory(dev, rows, D):
+    """From C, r may be x and n may be y."""
+    t = {k: v.to(dev) for k, v in make((rows, D), seed=21).items()}
+    args = [t[k] for k in ("x", "y", "gate", "scale", "weight", "bias")]
+    r, n, _ = residual_norm_forward(args[0], args[1], args[4], args[5], gate=args[2], scale=args[3])
+    a, ins, keep = block_norm._prepare(*args, True, False, 1e-5)
+    a.r, a.r_stride, a.n, a.n_stride = a.x, a.x_stride, a.y, a.y_stride
+    nat.check(nat.load().osm_residual_norm_fwd(ctypes.byref(a), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)))
+    assert torch.equal(t["x"], r) and torch.equal(t["y"], n)
 
 
 def test_same_bits_on_every_run_and_graph(dev):
