@@ -48,8 +48,8 @@ struct LossParams {
   void *grad_h, *grad_w;
 };
 
-hipError_t launch_loss_rows(const LossParams& p, __bf16* h, int dtype, bool bwd, hipStream_t stream);   // tok, h
-hipError_t launch_loss_weight(const LossParams& p, __bf16* to, int dtype, hipStream_t stream);   // parts of the piece's rows
+hipError_t launch_loss_rows(const LossParams& p, __bf16* h, __bf16* w, int dtype, bool bwd, hipStream_t stream);   // tok, h; w: or NULL
+hipError_t launch_loss_weight(const LossParams& p, __bf16* w, int dtype, hipStream_t stream);   // parts of the piece's rows
 int loss_tile_rows(const LossParams& p);                                                    // classes of a tile of the logits
 hipError_t launch_loss_logits(const LossParams& p, hipStream_t stream);                     // stat, own
 hipError_t launch_loss_join(const LossParams& p, int tiles, hipStream_t stream);            // losses, lse, loss, count

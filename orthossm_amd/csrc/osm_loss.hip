@@ -17,7 +17,7 @@
 // 930 TFLOP/s; the product alone 680; its epilogue, which nothing overlaps, takes 12%, most of it
 // the exponentials), P 930, dH 850, dW 820; a library's product for the logits alone takes 815,
 // with 0.8 GB of them written.  4096 tokens, 32768 classes, 1024 columns, forward: 255 us,
-// 1080 TFLOP/s.  981 tokens of 1401, 5003 classes, 400 columns, fp32: 38, 43, 44, 46 us, of 6
+// 1080 TFLOP/s.  981 tokens of 1401, 5003 classes, 400 columns, fp32: 39, 43, 37, 46 us, of 6
 // products of 4 GFLOP each.
 #include <algorithm>
 #include <type_traits>
@@ -73,10 +73,38 @@ bool whole_units(const void* p, int64_t stride, int64_t D) {
   return (uintptr_t)p % 16 == 0 && stride * sizeof(T) % 16 == 0 && D % 8 == 0;
 }
 
-// The tokens that count, one after the other: a block takes `each` tokens, counts those
-// before them, and writes where its own go, and their hidden rows.
+// A piece's rows of weights to [PARTS][vn][Dpad].
 template <typename T, int PARTS>
-__global__ void __launch_bounds__(256) loss_rows_kernel(const LossParams p, __bf16* to, int64_t each, bool vec, bool bwd) {
+__device__ __forceinline__ void pack(const LossParams& p, __bf16* to, bool vec, int64_t block) {
+  const int units = p.Dpad / 8;
+  const int64_t i = block * 256 + threadIdx.x, n = p.vn;
+  if (i >= n * units) return;
+  const int64_t r = i / units;
+  const int c = (int)(i - r * units) * 8;
+  bf16x8 out[PARTS];
+  split_unit<T, PARTS>(static_cast<const T*>(p.weight) + (p.v0 + r) * p.weight_s, c, (int)p.D, vec, out);
+#pragma unroll
+  for (int q = 0; q < PARTS; ++q) {
+    *reinterpret_cast<bf16x8*>(to + (q * n + r) * p.Dpad + c) = out[q];
+    wide_store_wait();
+  }
+}
+template <typename T, int PARTS>
+__global__ void __launch_bounds__(256) loss_pack_kernel(const LossParams p, __bf16* to, bool vec) {
+  pack<T, PARTS>(p, to, vec, blockIdx.x);
+}
+
+// The tokens that count, one after the other: a block takes `each` tokens, counts those
+// before them, and writes where its own go, and their hidden rows.  The blocks after those take
+// the first piece's weights (981 tokens, 5003 classes, 400 columns, fp32: 10 us for
+// 7 and 6, and a launch less twice a step, 180 us for 196).
+template <typename T, int PARTS>
+__global__ void __launch_bounds__(256) loss_rows_kernel(const LossParams p, __bf16* to, int64_t each, int blocks, bool vec, __bf16* w,
+                                                          bool w_vec, bool bwd) {
+  if ((int)blockIdx.x >= blocks) {
+    pack<T, PARTS>(p, w, w_vec, (int)blockIdx.x - blocks);
+    return;
+  }
   __shared__ int sums[4];
   __shared__ int rows[256];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -135,30 +163,13 @@ __global__ void __launch_bounds__(256) loss_rows_kernel(const LossParams p, __bf
       }
     }
   }
-  if (blockIdx.x < gridDim.x - 1) return;
+  if ((int)blockIdx.x < blocks - 1) return;
   if (threadIdx.x == 0) *p.tok.count = base;
   // zeros up to a whole step of the products over tokens
   const int over = (base + kStep - 1) / kStep * kStep - base;
   for (int u = threadIdx.x; u < PARTS * over * units; u += 256) {
     const int q = u / (over * units), r = u - q * over * units;
     *reinterpret_cast<bf16x8*>(to + ((int64_t)q * p.Npad + base) * p.Dpad + 8 * (int64_t)r) = bf16x8{};
-    wide_store_wait();
-  }
-}
-
-// Rows of weights to [PARTS][n][ld].
-template <typename T, int PARTS>
-__global__ void __launch_bounds__(256) loss_pack_kernel(const T* from, int64_t stride, int D, int64_t n, int ld, bool vec, __bf16* to) {
-  const int units = ld / 8;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n * units) return;
-  const int64_t r = i / units;
-  const int c = (int)(i - r * units) * 8;
-  bf16x8 out[PARTS];
-  split_unit<T, PARTS>(from + r * stride, c, D, vec, out);
-#pragma unroll
-  for (int q = 0; q < PARTS; ++q) {
-    *reinterpret_cast<bf16x8*>(to + ((int64_t)q * n + r) * ld + c) = out[q];
     wide_store_wait();
   }
 }
@@ -572,31 +583,32 @@ hipError_t logits(const LossParams& p, hipStream_t stream) {
 
 }  // namespace
 
-hipError_t launch_loss_rows(const LossParams& p, __bf16* h, int dtype, bool bwd, hipStream_t stream) {
-  // (a block counts what is before its tokens, so that there are at most 1024 of them)
-  const int64_t each = std::max<int64_t>(4, (p.N + 1023) / 1024);
-  const dim3 grid((unsigned)((p.N + each - 1) / each));
-  if (dtype == 0)
-    hipLaunchKernelGGL((loss_rows_kernel<float, 3>), grid, dim3(256), 0, stream, p, h, each, whole_units<float>(p.hidden, p.hidden_s, p.D), bwd);
-  else
-    hipLaunchKernelGGL((loss_rows_kernel<__bf16, 1>), grid, dim3(256), 0, stream, p, h, each, whole_units<__bf16>(p.hidden, p.hidden_s, p.D), bwd);
-  return hipGetLastError();
-}
-
 namespace {
+int64_t pack_blocks(const LossParams& p) { return ((int64_t)p.vn * (p.Dpad / 8) + 255) / 256; }
+
 template <typename T, int PARTS>
-void pack(const LossParams& p, __bf16* to, hipStream_t stream) {
-  const T* const from = static_cast<const T*>(p.weight) + p.v0 * p.weight_s;
-  hipLaunchKernelGGL((loss_pack_kernel<T, PARTS>), dim3((unsigned)(((int64_t)p.vn * (p.Dpad / 8) + 255) / 256)), dim3(256), 0, stream, from,
-                     p.weight_s, (int)p.D, (int64_t)p.vn, p.Dpad, whole_units<T>(from, p.weight_s, p.D), to);
+void rows(const LossParams& p, __bf16* h, __bf16* w, bool bwd, hipStream_t stream) {
+  // (a block counts what is before its tokens, so that there are at most 1024 of them)
+  const int64_t each = std::max<int64_t>(4, (p.N + 1023) / 1024), blocks = (p.N + each - 1) / each;
+  hipLaunchKernelGGL((loss_rows_kernel<T, PARTS>), dim3((unsigned)(blocks + (w ? pack_blocks(p) : 0))), dim3(256), 0, stream, p, h, each,
+                     (int)blocks, whole_units<T>(p.hidden, p.hidden_s, p.D), w, whole_units<T>(p.weight, p.weight_s, p.D), bwd);
 }
 }  // namespace
 
-hipError_t launch_loss_weight(const LossParams& p, __bf16* to, int dtype, hipStream_t stream) {
+hipError_t launch_loss_rows(const LossParams& p, __bf16* h, __bf16* w, int dtype, bool bwd, hipStream_t stream) {
   if (dtype == 0)
-    pack<float, 3>(p, to, stream);
+    rows<float, 3>(p, h, w, bwd, stream);
   else
-    pack<__bf16, 1>(p, to, stream);
+    rows<__bf16, 1>(p, h, w, bwd, stream);
+  return hipGetLastError();
+}
+
+hipError_t launch_loss_weight(const LossParams& p, __bf16* to, int dtype, hipStream_t stream) {
+  const dim3 grid((unsigned)pack_blocks(p));
+  if (dtype == 0)
+    hipLaunchKernelGGL((loss_pack_kernel<float, 3>), grid, dim3(256), 0, stream, p, to, whole_units<float>(p.weight, p.weight_s, p.D));
+  else
+    hipLaunchKernelGGL((loss_pack_kernel<__bf16, 1>), grid, dim3(256), 0, stream, p, to, whole_units<__bf16>(p.weight, p.weight_s, p.D));
   return hipGetLastError();
 }
 

@@ -173,23 +173,14 @@ LossParams params_of(const osm_loss_args* a, const Plan& n, const Layout& l, voi
   return p;
 }
 
-// The piece of vn classes from v0 on, and its weights' parts where they are not read in place.
-hipError_t set_piece(LossParams& p, const osm_loss_args* a, const Plan& n, const Layout& l, char* w, int64_t v0, int64_t vn,
-                     hipStream_t st) {
+// The piece of vn classes from v0 on.
+void set_piece(LossParams& p, const osm_loss_args* a, const Plan& n, const Layout& l, char* w, int64_t v0, int64_t vn) {
   p.v0 = v0;
   p.vn = (int)vn;
   p.vpad = (int)up(p.vn, kLossPad);
-  if (n.direct) {
-    p.w = static_cast<const __bf16*>(a->weight) + v0 * a->weight_stride;
-    p.w_ld = a->weight_stride;
-    p.w_part = 0;
-    return hipSuccess;
-  }
-  __bf16* const to = reinterpret_cast<__bf16*>(w + l.w);
-  p.w = to;
-  p.w_ld = n.Dpad;
-  p.w_part = (int64_t)p.vn * n.Dpad;
-  return osm::launch_loss_weight(p, to, a->dtype, st);
+  p.w = n.direct ? static_cast<const __bf16*>(a->weight) + v0 * a->weight_stride : reinterpret_cast<const __bf16*>(w + l.w);
+  p.w_ld = n.direct ? a->weight_stride : n.Dpad;
+  p.w_part = n.direct ? 0 : (int64_t)p.vn * n.Dpad;
 }
 
 int hip_rc(hipError_t e) { return e == hipSuccess ? ok() : fail(OSM_E_HIP, "cross entropy launch: %s", hipGetErrorString(e)); }
@@ -203,21 +194,25 @@ hipError_t forward(const osm_loss_args* a, const Plan& n, const Layout& l, void*
   p.loss = a->loss;
   p.count = a->count;
   p.mean = (a->flags & OSM_LOSS_MEAN) != 0;
+  __bf16* const parts = n.direct ? nullptr : reinterpret_cast<__bf16*>(w + l.w);
   hipError_t e = hipSuccess;
+  bool packed = n.direct;
+  set_piece(p, a, n, l, w, 0, std::min(n.piece, a->V));
   if (in_place(a)) {
     p.tok = {};
     p.h = static_cast<const __bf16*>(a->hidden);
     p.h_ld = a->hidden_stride;
     p.h_rows = (int)a->N;
   } else {
-    e = osm::launch_loss_rows(p, reinterpret_cast<__bf16*>(w + l.h), a->dtype, false, st);
+    e = osm::launch_loss_rows(p, reinterpret_cast<__bf16*>(w + l.h), parts, a->dtype, false, st);
+    packed = true;
   }
   if (e != hipSuccess) return e;
   const int rows = osm::loss_tile_rows(p);
-  for (int64_t v0 = 0; v0 < a->V; v0 += n.piece) {
+  for (int64_t v0 = 0; v0 < a->V; v0 += n.piece, packed = n.direct) {
     p.tile0 = (int)(v0 / rows);
-    if ((e = set_piece(p, a, n, l, w, v0, std::min(n.piece, a->V - v0), st)) != hipSuccess ||
-        (e = osm::launch_loss_logits(p, st)) != hipSuccess)
+    set_piece(p, a, n, l, w, v0, std::min(n.piece, a->V - v0));
+    if ((!packed && (e = osm::launch_loss_weight(p, parts, a->dtype, st)) != hipSuccess) || (e = osm::launch_loss_logits(p, st)) != hipSuccess)
       return e;
   }
   return osm::launch_loss_join(p, (int)((a->V + rows - 1) / rows), st);
@@ -234,12 +229,17 @@ hipError_t backward(const osm_loss_args* a, const osm_loss_bwd_args* b, const Pl
   p.count_in = b->count;
   p.grad_h = b->grad_hidden;
   p.grad_w = b->grad_weight;
-  hipError_t e = osm::launch_loss_rows(p, reinterpret_cast<__bf16*>(w + l.h), a->dtype, true, st);
-  if (e != hipSuccess) return e;
+  __bf16* const parts = n.direct ? nullptr : reinterpret_cast<__bf16*>(w + l.w);
+  hipError_t e;
   for (int64_t v0 = 0, vn; v0 < a->V; v0 += vn) {
     vn = next_piece(a->V - v0, n.piece, a->D);
     p.first = v0 == 0;
-    if ((e = set_piece(p, a, n, l, w, v0, vn, st)) != hipSuccess || (e = osm::launch_loss_probs(p, st)) != hipSuccess) return e;
+    set_piece(p, a, n, l, w, v0, vn);
+    if (p.first)
+      e = osm::launch_loss_rows(p, reinterpret_cast<__bf16*>(w + l.h), parts, a->dtype, true, st);
+    else
+      e = n.direct ? hipSuccess : osm::launch_loss_weight(p, parts, a->dtype, st);
+    if (e != hipSuccess || (e = osm::launch_loss_probs(p, st)) != hipSuccess) return e;
     if (b->grad_hidden && (e = osm::launch_loss_dh(p, st)) != hipSuccess) return e;
     if (!b->grad_weight) continue;
     // (what is over 256 tiles of dW, in tiles of its own: 17233 classes, 8192 tokens, 1024 columns: 338 us in one launch
