@@ -81,10 +81,15 @@ struct GemmPlace {
 // 16 bytes a lane from memory to LDS, to the 1024 bytes from `to` (the same in every lane)
 // on in the order of the lanes.  It has no result to wait for: who reads them waits for
 // vmcnt himself.  (In place of the compiler's builtin, ahead of whose effects it would
-// wait at the next transposing read, which is of the other buffer.)
+// wait at the next transposing read, which is of the other buffer.)  What the compiler may
+// hold in M0 it sets again: the register is declared, though not one that it allocates, of
+// which it would warn.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void to_lds(const __bf16* from, unsigned to) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory", "m0");
 }
+#pragma clang diagnostic pop
 __device__ __forceinline__ unsigned lds_address(const __bf16* p) {
   return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) __bf16*)p;
 }
