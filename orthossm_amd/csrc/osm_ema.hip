@@ -392,6 +392,7 @@ __global__ void __launch_bounds__(256) ema_step_kernel(const EmaStepParams p) {
 #pragma unroll
     for (int k = 0; k < NC; ++k) h[k] = slot < 0 ? 0.0f : __builtin_nanf("");
     LaneVec<T, NC>::store(out, h);
+    wide_store_wait();
     return;
   }
   float* const s = p.state + slot * p.state_s + c;

@@ -83,6 +83,13 @@ __device__ __forceinline__ void store_piece(T* p, const float (&f)[U], int c, in
   }
 }
 
+// A row's statistics, in one store.
+__device__ __forceinline__ void store_stats(float* p, float my, float sy, float mr, float sr) {
+  typedef float Loose __attribute__((ext_vector_type(4), aligned(4)));
+  *reinterpret_cast<Loose*>(p) = Loose{my, sy, mr, sr};
+  wide_store_wait();
+}
+
 // Both off by |v| 2^-24 and a few units of 2^-24 (the hardware's reciprocal: the exact
 // division takes twice the instructions of all the rest).
 struct Gate {
@@ -224,13 +231,7 @@ __global__ void __launch_bounds__(RowThreads<TPR>::kThreads) resnorm_fwd_kernel(
       store_piece<TX, U>(static_cast<TX*>(p.r) + row * p.r_s, x[k], (u + k * TPR) * U, D, p.vec);
     }
     normalise<TPR>(x, D, u, p.eps, p.rms, red, half, mr, sr);
-    if (p.stats && u == 0) {
-      float* const st = p.stats + 4 * row;
-      st[0] = my;
-      st[1] = sy;
-      st[2] = mr;
-      st[3] = sr;
-    }
+    if (p.stats && u == 0) store_stats(p.stats + 4 * row, my, sy, mr, sr);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       float w[U], b[U];
@@ -444,13 +445,7 @@ __global__ void __launch_bounds__(kLongThreads) resnorm_fwd_long_kernel(const Re
     float my = 0.0f, sy = 1.0f, mr, sr;
     if (p.norm_y) long_stats(p, [&](int64_t c) { return (float)q.y[c]; }, red, par, my, sy);
     long_stats(p, [&](int64_t c) { return q.r(c, my, sy); }, red, par, mr, sr);
-    if (p.stats && threadIdx.x == 0) {
-      float* const st = p.stats + 4 * row;
-      st[0] = my;
-      st[1] = sy;
-      st[2] = mr;
-      st[3] = sr;
-    }
+    if (p.stats && threadIdx.x == 0) store_stats(p.stats + 4 * row, my, sy, mr, sr);
     for (int64_t c = threadIdx.x; c < p.D; c += kLongThreads) {
       const float r = q.r(c, my, sy);
       static_cast<TX*>(p.r)[row * p.r_s + c] = (TX)r;
