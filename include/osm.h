@@ -744,8 +744,10 @@ int osm_residual_norm_bwd(const osm_resnorm_args* args, const osm_resnorm_bwd_ar
 
 /* The cross entropy and its backward (from hidden, weight, targets and lse; losses, loss
  * and count of `args` are not used).  Workspaces as above.  The backward forms the
- * probabilities of a piece of the vocabulary at a time: up to 302 MB of them (more only
- * where 256 classes of all tokens are more). */
+ * probabilities of a piece of the vocabulary at a time: up to 302 MB of them, and of the
+ * piece's weights where they are copied as much again (more only where 256 classes are
+ * more).  They are read where they are in bf16 of D a multiple of 64, rows at multiples
+ * of 16 bytes. */
 size_t osm_linear_ce_workspace_bytes(const osm_loss_args* args);
 int osm_linear_ce_fwd(const osm_loss_args* args, void* workspace, size_t workspace_bytes, void* stream);
 size_t osm_linear_ce_bwd_workspace_bytes(const osm_loss_args* args);

@@ -68,9 +68,10 @@ struct Plan {
   bool direct;
 };
 
-// Classes of a piece: its parts of P (or of the weights) are at most 9 2^24 elements (less than
-// 2^27: too few for 256 tiles of dW at 8192 tokens of 1024, 8% slower; twice and four times as
-// many: the same; the ninth is for a last piece that is a little longer).
+// Classes of a piece: its parts of P, and of the weights where they are copied, are each at most
+// 9 2^24 elements, unless 256 classes are more (less than 2^27: too few for 256 tiles of dW at
+// 8192 tokens of 1024, 8% slower; twice and four times as many: the same; the ninth is for a last
+// piece that is a little longer).  `rows`: elements of a class.
 int64_t piece_of(int64_t V, int64_t rows) {
   const int64_t most = std::min((int64_t(9) << 24) / rows, kMaxRow - 1) / kLossPad * kLossPad;
   return std::min(std::max<int64_t>(most, kLossPad), up(V, kLossPad));
@@ -98,8 +99,8 @@ Plan plan_of(const osm_loss_args* a, bool bwd) {
   const int64_t across = (a->D + 255) / 256;
   // (a forward's launch has at most 2^32 threads, 256 for 64 x 64)
   const int64_t most = std::max<int64_t>((int64_t(1) << 36) / n.Npad / kLossPad * kLossPad - kLossPad, kLossPad);
-  n.piece = bwd ? piece_of(a->V, n.Npad * n.p_parts)
-                : std::min(most, n.direct ? up(a->V, kLossPad) : piece_of(a->V, n.Dpad * n.parts));
+  const int64_t copied = n.direct ? up(a->V, kLossPad) : piece_of(a->V, n.Dpad * n.parts);
+  n.piece = std::min(copied, bwd ? piece_of(a->V, n.Npad * n.p_parts) : most);
   // Splits of dH's classes: as many as leave each a product that is worth its sums, six times the
   // work a class in three parts.  (1024 and 512 classes: fp32, 1000 x 7000 x 400, a backward in 187
   // and 179 us, 300 x 2000 x 800 in 71 and 64; bf16, 1500 x 4000 x 1024, in 81 and 86.)

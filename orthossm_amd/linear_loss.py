@@ -18,9 +18,10 @@ softmax - onehot are rounded to bf16 for bf16 inputs (up to 64 tokens: to the
 sum of two bf16 numbers).
 
 The backward forms the logits of a piece of the vocabulary at a time: its
-memory is bounded by the pieces, not by the vocabulary.  All run on the current
-torch stream of hidden's device and never synchronise the host.  There is no CPU
-path.
+memory is bounded by the pieces (302 MB of P, and as much of the weights where
+they are copied: fp32, rows that are not whole units of 64 columns at multiples
+of 16 bytes), not by the vocabulary.  All run on the current torch stream of
+hidden's device and never synchronise the host.  There is no CPU path.
 """
 from __future__ import annotations
 
