@@ -50,7 +50,7 @@ struct LossParams {
 
 hipError_t launch_loss_rows(const LossParams& p, __bf16* h, __bf16* w, int dtype, bool bwd, hipStream_t stream);   // tok, h; w: or NULL
 hipError_t launch_loss_weight(const LossParams& p, __bf16* w, int dtype, hipStream_t stream);   // parts of the piece's rows
-int loss_tile_rows(const LossParams& p);                                                    // classes of a tile of the logits
+int loss_tile_rows(const LossParams& p);                                                    // classes of a forward's tile of logits, by N, V and parts
 hipError_t launch_loss_logits(const LossParams& p, hipStream_t stream);                     // stat, own
 hipError_t launch_loss_join(const LossParams& p, int tiles, hipStream_t stream);            // losses, lse, loss, count
 hipError_t launch_loss_none(float* loss, float* count, hipStream_t stream);

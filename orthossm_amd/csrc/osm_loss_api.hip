@@ -64,7 +64,7 @@ bool in_place(const osm_loss_args* a) {
 // What a launch works on: the compacted hidden rows, and pieces of the vocabulary.
 struct Plan {
   int64_t Npad, Dpad, parts, p_parts, piece;   // piece: classes, a multiple of kLossPad
-  int splits;
+  int splits, rows;                            // rows: classes of a forward's tile of logits
   bool direct;
 };
 
@@ -106,8 +106,17 @@ Plan plan_of(const osm_loss_args* a, bool bwd) {
   // and 179 us, 300 x 2000 x 800 in 71 and 64; bf16, 1500 x 4000 x 1024, in 81 and 86.)
   const int64_t tiles = across * (n.Npad / 256), least = n.parts == 1 ? 1024 : 512;
   n.splits = (int)std::max<int64_t>(1, std::min<int64_t>({256 / std::max<int64_t>(1, tiles), n.piece / least, 8}));
+  LossParams p{};
+  p.N = a->N;
+  p.V = a->V;
+  p.parts = (int)n.parts;
+  p.p_parts = (int)n.p_parts;
+  n.rows = osm::loss_tile_rows(p);
   return n;
 }
+
+// A forward's tiles along the vocabulary.
+int tiles_of(const osm_loss_args* a, const Plan& n) { return (int)((a->V + n.rows - 1) / n.rows); }
 
 // The regions of a workspace, each at a multiple of 256 bytes.
 struct Regions {
@@ -133,7 +142,7 @@ Layout layout_of(const osm_loss_args* a, const Plan& n, bool bwd) {
   l.w = r.add(n.direct ? 0 : (size_t)n.parts * n.piece * n.Dpad * 2);
   if (!bwd) {
     l.own = r.add(n.Npad * 4);
-    l.stat = r.add((size_t)(up(a->V, kLossPad) / 64) * n.Npad * 8);
+    l.stat = r.add((size_t)tiles_of(a, n) * n.Npad * 8);
   } else {
     l.p = r.add((size_t)n.p_parts * n.Npad * n.piece * 2);
     l.dh = r.add((size_t)n.splits * n.Npad * n.Dpad * 4);
@@ -209,14 +218,13 @@ hipError_t forward(const osm_loss_args* a, const Plan& n, const Layout& l, void*
     packed = true;
   }
   if (e != hipSuccess) return e;
-  const int rows = osm::loss_tile_rows(p);
   for (int64_t v0 = 0; v0 < a->V; v0 += n.piece, packed = n.direct) {
-    p.tile0 = (int)(v0 / rows);
+    p.tile0 = (int)(v0 / n.rows);
     set_piece(p, a, n, l, w, v0, std::min(n.piece, a->V - v0));
     if ((!packed && (e = osm::launch_loss_weight(p, parts, a->dtype, st)) != hipSuccess) || (e = osm::launch_loss_logits(p, st)) != hipSuccess)
       return e;
   }
-  return osm::launch_loss_join(p, (int)((a->V + rows - 1) / rows), st);
+  return osm::launch_loss_join(p, tiles_of(a, n), st);
 }
 
 hipError_t backward(const osm_loss_args* a, const osm_loss_bwd_args* b, const Plan& n, const Layout& l, void* workspace, hipStream_t st) {

@@ -54,3 +54,13 @@ def test_copies_are_of_fewer_threads_than_a_launch_may_have(form, N):
     for width in (1 << 14, 1 << 17):
         need = nat.load().osm_linear_ce_bwd_workspace_bytes(args(N, width - less, 1 << 28, dtype, shift, gap))
         assert 0 < need / (16 * (1 if dtype else 3)) < 1 << 32
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_statistics_are_of_the_tiles_that_there_are(dtype):
+    """8 bytes a token and tile: of 256 classes in bf16 and 128 in fp32 where there are many."""
+    N, D, V = 1 << 16, 64, 128000
+    n, parts, rows = N, 1 if dtype else 3, 256 if dtype else 128
+    copies = 2 * parts * n * D + (0 if dtype else 2 * parts * up(V, 256) * D)
+    need = nat.load().osm_linear_ce_workspace_bytes(args(N, D, V, dtype))
+    assert need <= 8 * n * (up(V, rows) // rows) + copies + 16 * n + (1 << 16)
