@@ -562,10 +562,12 @@ typedef struct osm_resnorm_bwd_args {
  * for tokens n with targets_n != ignore_index; the others count for nothing, whatever
  * their hidden rows hold, and their loss and gradients are 0.  A target outside
  * [0, V) gives NaN (the loss, and every gradient that the token has a part in).
- * Products are at fp32's accuracy for fp32 inputs (three bf16 parts an operand; a value
- * that bf16 rounds to infinity, above 3.39e38, makes NaN) and exact for bf16 ones, sums in
- * fp32; the backward's probabilities are rounded to bf16 for bf16 inputs (of more than 64
- * tokens; of fewer to twice the bits).  No counterpart in the reference. */
+ * Products are at fp32's accuracy for fp32 inputs (three bf16 parts an operand) and exact
+ * for bf16 ones, sums in fp32; the backward's probabilities are rounded to bf16 for bf16
+ * inputs (of more than 64 tokens; of fewer to twice the bits).  Infinities count as they are:
+ * weights of -inf leave a class out of the losses and of the weights' gradient (in
+ * grad_hidden 0 times infinity is NaN); a logit of +inf makes its token's loss NaN.  No
+ * counterpart in the reference. */
 #define OSM_LOSS_MEAN 0x1
 
 typedef struct osm_loss_args {

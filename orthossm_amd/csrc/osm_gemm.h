@@ -251,11 +251,15 @@ __device__ __forceinline__ void gemm(const GemmSide& A, const GemmSide& B, int m
       }
     }
   }
+  // (an infinite operand is so in its first part, and its other products are none)
   if constexpr (P > 1)
 #pragma unroll
     for (int i = 0; i < G::FM; ++i)
 #pragma unroll
-      for (int j = 0; j < G::FN; ++j) acc[i][j] += small[i][j];
+      for (int j = 0; j < G::FN; ++j)
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          if (__builtin_fabsf(acc[i][j][k]) < __builtin_inff()) acc[i][j][k] += small[i][j][k];
   __syncthreads();   // the buffers are free
 }
 

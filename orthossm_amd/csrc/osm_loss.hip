@@ -37,12 +37,17 @@ __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2
 
 // ---- operands ----
 
-// The bf16 parts of x: part k is what rounding leaves of the parts before it.
+constexpr float kMostBf16 = 0x1.fep127f;
+
+// The bf16 parts of x: part k is what rounding leaves of the parts before it.  (The first of
+// what bf16 would round to infinity is its largest; of an infinity it is one, and the others are
+// of no use.)
 template <int PARTS>
 __device__ __forceinline__ void split(float x, __bf16 (&to)[PARTS]) {
 #pragma unroll
   for (int k = 0; k < PARTS; ++k) {
-    to[k] = (__bf16)x;
+    const bool clamp = PARTS > 1 && k == 0 && __builtin_fabsf(x) < kInf;
+    to[k] = (__bf16)(clamp ? __builtin_fmaxf(__builtin_fminf(x, kMostBf16), -kMostBf16) : x);
     x -= (float)to[k];
   }
 }

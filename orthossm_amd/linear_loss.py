@@ -13,7 +13,8 @@ with contiguous rows (others are copied first), targets whole numbers of
 hidden's shape without D.  Tokens whose target is ``ignore_index`` count for
 nothing, whatever their hidden rows hold: their losses and gradients are 0.  A
 target outside [0, V) gives NaN: that token's loss, and every gradient that it
-has a part in.  Logits, sums and losses are fp32; the gradients' factors
+has a part in.  Infinities count as they are (a class whose weights are -inf is
+left out where hidden is positive), but a logit of +inf makes NaN.  Logits, sums and losses are fp32; the gradients' factors
 softmax - onehot are rounded to bf16 for bf16 inputs (up to 64 tokens: to the
 sum of two bf16 numbers).
 
