@@ -477,7 +477,7 @@ typedef struct osm_seq {
 
 typedef struct osm_ema_args {
   int32_t abi_version;          /* = OSM_ABI_VERSION */
-  int32_t dtype;                /* osm_dtype of x, gate, out and their gradients */
+  int32_t dtype;                /* osm_dtype of x, gate, out and their gradients; OSM_FLAG_POLL_LIMIT_ZERO may be beside it */
   int64_t B, S, D;
   osm_seq x, gate, out;         /* [B,S,D]; out's rows must not overlap */
   const int32_t* lengths;       /* [B], or NULL: every row has S tokens */
@@ -722,7 +722,9 @@ int osm_clip_grad_norm(const osm_clip_args* args, void* workspace, size_t worksp
 
 /* The gated EMA over sequences.  `saved` and the workspace need no initialisation
  * and 256-byte alignment; nothing is kept in the workspace between calls.  One
- * launch, two where S is above 128 (backward: 64). */
+ * launch, two where S is above 128 (backward: 64): then a tile's wait for those ahead
+ * of it that gives up makes NaN of what depends on it and sets the fault word, which
+ * osm_workspace_status reads until the next call (its launch counter is 0). */
 size_t osm_gated_ema_saved_bytes(const osm_ema_args* args);
 size_t osm_gated_ema_workspace_bytes(const osm_ema_args* args);
 int osm_gated_ema_fwd(const osm_ema_args* args, void* workspace, size_t workspace_bytes, void* stream);

@@ -12,7 +12,9 @@ constexpr int kEmaRun = 16;        // tokens of a group, forward
 constexpr int kEmaBwdRun = 8;      // backward, which holds twice as much of a token
 constexpr int kEmaTile = kEmaWaves * kEmaRun, kEmaBwdTile = kEmaWaves * kEmaBwdRun;
 constexpr int kEmaGroup = 8;       // tiles from checkpoint to checkpoint
-constexpr int kEmaTicketStride = 32;   // counters lie on lines of their own
+// A lane-block's line of the workspace: its counter at this word.  The first's holds the launch's
+// fault word too, where the headers of the other look-backs' workspaces do.
+constexpr int kEmaLine = 32, kEmaTicket = 1;
 
 struct EmaSeq {
   void* p;
@@ -30,9 +32,10 @@ struct EmaParams {
   float* ginit;                  // [B,D], or NULL
   unsigned long long* words;     // zeroed: [lane-blocks][tiles][kEmaLanes] tile maps
   unsigned long long* marks;     // zeroed: [lane-blocks][groups][kEmaLanes] states after whole groups
-  unsigned* tickets;             // zeroed: [lane-blocks], kEmaTicketStride apart
+  unsigned* lines;               // zeroed: [lane-blocks][kEmaLine]
   int B, S, D, n_lbd, n_lb, n_tiles, n_groups, n_saved;
   int vec;                       // rows and D in pairs of channels, aligned
+  unsigned poll_limit;           // of a wait: kSpinLimit, or 0 under OSM_FLAG_POLL_LIMIT_ZERO
 };
 
 struct EmaStepParams {

@@ -21,7 +21,7 @@
 // XCD, to which blocks go in the order of their index; else a block draws its tile from
 // its lane-block's counter when it starts (8x32768x1024 bf16, by index and drawn: 346 and
 // 368 us forward, 614 and 648 backward).  The waits are bounded all the same; one that
-// gives up makes NaN.
+// gives up makes NaN of what depends on it and sets the workspace's fault word.
 #include <algorithm>
 #include <type_traits>
 
@@ -122,14 +122,16 @@ __device__ __forceinline__ void put2(float* p, int64_t at, int c, int D, F2 v) {
 __device__ __forceinline__ void arrive(F2 v) { asm volatile("" ::"v"(v.x), "v"(v.y)); }
 
 // Waits for a word to be published (they are never 0): its producer has been running
-// since before this block drew its tile.
-__device__ __forceinline__ unsigned long long await(const unsigned long long* at) {
+// since before this block drew its tile.  A wait that gives up sets the fault word.
+__device__ __forceinline__ unsigned long long await(const unsigned long long* at, const EmaParams& p) {
   unsigned long long w = peek(at);
-  for (unsigned polls = 0; w == 0 && polls < kSpinLimit; ++polls) {
+  for (unsigned polls = 0; w == 0 && polls < p.poll_limit; ++polls) {
     __builtin_amdgcn_s_sleep(1);
     w = peek(at);
   }
-  return w ? w : 0x7fc000007fc00000ull;   // NaN, NaN
+  if (w) return w;
+  raise_fault(p.lines, kKindFault);
+  return 0x7fc000007fc00000ull;   // NaN, NaN
 }
 __device__ __forceinline__ unsigned long long word_of(float hi, float lo) {
   return (unsigned long long)__float_as_uint(hi) << 32 | __float_as_uint(lo);
@@ -161,7 +163,7 @@ __device__ __forceinline__ Place place(const EmaParams& p, Shared& L) {
     q.tile = blockIdx.x / p.n_lb;
   } else if (p.n_tiles > 1) {
     if (threadIdx.x == 0)
-      L.drawn = (int)__hip_atomic_fetch_add(p.tickets + (int64_t)q.lb * kEmaTicketStride, 1u, __ATOMIC_RELAXED,
+      L.drawn = (int)__hip_atomic_fetch_add(p.lines + (int64_t)q.lb * kEmaLine + kEmaTicket, 1u, __ATOMIC_RELAXED,
                                             __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
     q.tile = __builtin_amdgcn_readfirstlane(L.drawn);
@@ -195,12 +197,12 @@ __device__ __forceinline__ F2 carry_in(const EmaParams& p, Shared& L, const Plac
   if (j > 0) {
     if (q.wave < k) {
       const unsigned long long* const w = p.words + ((int64_t)q.lb * p.n_tiles + g * kEmaGroup + q.wave) * kEmaLanes + 2 * q.lane;
-      const unsigned long long u = await(w), v = await(w + 1);
+      const unsigned long long u = await(w, p), v = await(w + 1, p);
       L.pa[q.wave][q.lane] = F2{__uint_as_float((unsigned)(u >> 32)), __uint_as_float((unsigned)(v >> 32))};
       L.pb[q.wave][q.lane] = F2{__uint_as_float((unsigned)u), __uint_as_float((unsigned)v)};
     } else if (q.wave == kEmaGroup - 1 && g > 0) {
       const unsigned long long* const w = p.marks + ((int64_t)q.lb * p.n_groups + g - 1) * kEmaLanes + 2 * q.lane;
-      const unsigned long long u = await(w), v = await(w + 1);
+      const unsigned long long u = await(w, p), v = await(w + 1, p);
       L.pb[kEmaGroup - 1][q.lane] = F2{__uint_as_float((unsigned)u), __uint_as_float((unsigned)v)};
     }
     __syncthreads();

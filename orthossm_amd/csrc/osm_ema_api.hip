@@ -48,9 +48,13 @@ int check_out(const osm_seq& r, int esize, int64_t B, int64_t S, int64_t D, cons
   return by_row || by_token ? OSM_OK : fail(OSM_E_LAYOUT, "%s: rows overlap", name);
 }
 
+// (a test aid's bit may be beside the type)
+int32_t type_of(const osm_ema_args* a) { return a->dtype & ~OSM_FLAG_POLL_LIMIT_ZERO; }
+int esize_of(const osm_ema_args* a) { return type_of(a) == OSM_F32 ? 4 : 2; }
+
 int check_shape(const osm_ema_args* a) {
   if (!a) return fail(OSM_E_ARG, "args is NULL");
-  const int rc = check_common(a->abi_version, a->dtype, a->B, a->D);
+  const int rc = check_common(a->abi_version, type_of(a), a->B, a->D);
   if (rc != OSM_OK) return rc;
   if (a->S < 0 || a->S > kMaxDim - 255) return fail(OSM_E_SHAPE, "S=%lld outside [0, 2^31 - 256)", (long long)a->S);
   const int64_t lbd = div_up(a->D, kEmaLanes);
@@ -62,7 +66,7 @@ int check_shape(const osm_ema_args* a) {
 int check_inputs(const osm_ema_args* a) {
   int rc = check_shape(a);
   if (rc != OSM_OK) return rc;
-  const int es = a->dtype == OSM_F32 ? 4 : 2;
+  const int es = esize_of(a);
   if (a->B > 0 && a->S > 0 &&
       ((rc = check_seq(a->x, es, a->S, "x")) != OSM_OK || (rc = check_seq(a->gate, es, a->S, "gate")) != OSM_OK))
     return rc;
@@ -74,13 +78,13 @@ int check_inputs(const osm_ema_args* a) {
 }
 
 struct Sizes {
-  size_t words, marks, tickets;   // bytes, zeroed ahead of a launch; 0: one tile a row
-  size_t total() const { return words + marks + tickets; }
+  size_t lines, words, marks;   // bytes, in this order, zeroed ahead of a launch; 0: one tile a row
+  size_t total() const { return lines + words + marks; }
 };
 Sizes sizes_of(const osm_ema_args* a, int tile) {
   const size_t lb = (size_t)a->B * div_up(a->D, kEmaLanes), tiles = div_up(a->S, tile);
   if (tiles <= 1 || lb == 0) return {0, 0, 0};
-  return {lb * tiles * kEmaLanes * 8, lb * div_up(tiles, kEmaGroup) * kEmaLanes * 8, lb * osm::kEmaTicketStride * 4};
+  return {lb * osm::kEmaLine * 4, lb * tiles * kEmaLanes * 8, lb * div_up(tiles, kEmaGroup) * kEmaLanes * 8};
 }
 
 // (the stride of a single token is not used: it can be anything)
@@ -107,10 +111,11 @@ EmaParams params_of(const osm_ema_args* a, int tile, void* workspace) {
   p.n_groups = (int)div_up(p.n_tiles, kEmaGroup);
   const Sizes n = sizes_of(a, tile);
   char* const w = static_cast<char*>(workspace);
-  p.words = reinterpret_cast<unsigned long long*>(w);
-  p.marks = reinterpret_cast<unsigned long long*>(w + n.words);
-  p.tickets = reinterpret_cast<unsigned*>(w + n.words + n.marks);
-  const int es = a->dtype == OSM_F32 ? 4 : 2;
+  p.lines = reinterpret_cast<unsigned*>(w);
+  p.words = reinterpret_cast<unsigned long long*>(w + n.lines);
+  p.marks = reinterpret_cast<unsigned long long*>(w + n.lines + n.words);
+  p.poll_limit = (a->dtype & OSM_FLAG_POLL_LIMIT_ZERO) ? 0u : osm::kSpinLimit;
+  const int es = esize_of(a);
   p.vec = a->D % 2 == 0 && pairs(a->x, a->S, es) && pairs(a->gate, a->S, es);
   return p;
 }
@@ -153,14 +158,14 @@ int osm_gated_ema_fwd(const osm_ema_args* a, void* workspace, size_t workspace_b
   if (rc != OSM_OK) return rc;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (a->B == 0 || a->S == 0) return pass_state(a, a->state_init, a->state_out, st);
-  const int es = a->dtype == OSM_F32 ? 4 : 2;
+  const int es = esize_of(a);
   if ((rc = check_out(a->out, es, a->B, a->S, a->D, "out")) != OSM_OK) return rc;
   if ((rc = prepare(a, kEmaTile, workspace, workspace_bytes, st)) != OSM_OK) return rc;
   EmaParams p = params_of(a, kEmaTile, workspace);
   p.out = seq_of(a->out, a->S);
   p.fin = a->state_out;
   p.vec = p.vec && pairs(a->out, a->S, es);
-  const hipError_t e = osm::launch_ema_fwd(p, a->dtype, st);
+  const hipError_t e = osm::launch_ema_fwd(p, type_of(a), st);
   return e == hipSuccess ? ok() : fail(OSM_E_HIP, "gated EMA launch: %s", hipGetErrorString(e));
 }
 
@@ -173,7 +178,7 @@ int osm_gated_ema_bwd(const osm_ema_args* a, const osm_ema_bwd_args* b, void* wo
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (a->B == 0 || a->S == 0) return pass_state(a, b->grad_state, b->grad_init, st);
   if (!a->saved) return fail(OSM_E_ARG, "saved is NULL");
-  const int es = a->dtype == OSM_F32 ? 4 : 2;
+  const int es = esize_of(a);
   if ((rc = check_seq(b->grad_out, es, a->S, "grad_out")) != OSM_OK ||
       (rc = check_out(b->grad_x, es, a->B, a->S, a->D, "grad_x")) != OSM_OK ||
       (rc = check_out(b->grad_gate, es, a->B, a->S, a->D, "grad_gate")) != OSM_OK)
@@ -186,7 +191,7 @@ int osm_gated_ema_bwd(const osm_ema_args* a, const osm_ema_bwd_args* b, void* wo
   p.gstate = b->grad_state;
   p.ginit = b->grad_init;
   p.vec = p.vec && pairs(b->grad_out, a->S, es) && pairs(b->grad_x, a->S, es) && pairs(b->grad_gate, a->S, es);
-  const hipError_t e = osm::launch_ema_bwd(p, a->dtype, st);
+  const hipError_t e = osm::launch_ema_bwd(p, type_of(a), st);
   return e == hipSuccess ? ok() : fail(OSM_E_HIP, "gated EMA backward launch: %s", hipGetErrorString(e));
 }
 

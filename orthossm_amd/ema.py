@@ -27,8 +27,14 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native as nat
+from . import ops
 from .delta import _dest, _lengths, _scratch, _state, apart, differentiable, on_device, written
-from .ops import _current_stream, _dtype_code, _fast
+from .ops import _after_launch, _current_stream, _dtype_code, _fast
+
+
+def _extension():
+    """The native launch path, which carries no test aids."""
+    return None if ops._poll_limit_zero else _fast()
 
 
 def _set_seq(r: nat.Seq, t: torch.Tensor) -> None:
@@ -60,7 +66,8 @@ def _prepare(x, gate, state_init, lengths):
     init = _state(state_init, (B, D), dev, "state_init")
     lens = _lengths(lengths, B, S, dev)
     a = nat.EmaArgs()
-    a.abi_version, a.dtype = nat.ABI_VERSION, _dtype_code(x.dtype)
+    a.abi_version = nat.ABI_VERSION
+    a.dtype = _dtype_code(x.dtype) | (nat.FLAG_POLL_LIMIT_ZERO if ops._poll_limit_zero else 0)
     a.B, a.S, a.D = B, S, D
     _set_seq(a.x, x)
     _set_seq(a.gate, gate)
@@ -95,8 +102,10 @@ def _forward(x, gate, state_init, lengths, out, return_state, state_out, save):
         a.saved = saved.data_ptr()
     ws = _scratch(lib.osm_gated_ema_workspace_bytes(ctypes.byref(a)), dev)
     with on_device(dev):
-        nat.check(lib.osm_gated_ema_fwd(ctypes.byref(a), ctypes.c_void_p(ws.data_ptr()), ws.numel(),
-                                        ctypes.c_void_p(_current_stream(dev))))
+        stream = _current_stream(dev)
+        nat.check(lib.osm_gated_ema_fwd(ctypes.byref(a), ctypes.c_void_p(ws.data_ptr()), ws.numel(), ctypes.c_void_p(stream)))
+        if ws.numel():
+            _after_launch(ws, stream, "gated_ema_forward")
     written(*given)
     return out, state_out, saved, keep
 
@@ -109,7 +118,7 @@ def gated_ema_forward(x: torch.Tensor, gate: torch.Tensor, *, state_init: torch.
     fp32 when ``return_state``.  ``out`` and ``state_out`` (contiguous; state_out
     may be state_init, else they lie in no argument's memory) receive the results
     instead of new tensors."""
-    fast = _fast()
+    fast = _extension()
     if fast is not None and out is None and state_out is None:
         res = fast.ema_forward(x, gate, lengths, state_init, return_state)
         if res is not None:
@@ -141,8 +150,11 @@ def _backward(x, gate, lengths, saved, grad_out, grad_state, need_init: bool):
     b.grad_init = gi.data_ptr() if gi is not None else None
     ws = _scratch(lib.osm_gated_ema_bwd_workspace_bytes(ctypes.byref(a)), dev)
     with on_device(dev):
+        stream = _current_stream(dev)
         nat.check(lib.osm_gated_ema_bwd(ctypes.byref(a), ctypes.byref(b), ctypes.c_void_p(ws.data_ptr()), ws.numel(),
-                                        ctypes.c_void_p(_current_stream(dev))))
+                                        ctypes.c_void_p(stream)))
+        if ws.numel():
+            _after_launch(ws, stream, "gated_ema_backward")
     return gx, gg, gi
 
 
@@ -184,7 +196,7 @@ def gated_ema(x: torch.Tensor, gate: torch.Tensor, *, state_init: torch.Tensor |
     """``gated_ema_forward`` as a differentiable op: gradients flow to x, gate
     and state_init, from the output and the final state.  Returns h, or (h,
     final state) when ``return_state``."""
-    fast = _fast()
+    fast = _extension()
     if fast is not None:
         res = fast.gated_ema(x, gate, lengths, state_init)
         if res is not None:
@@ -202,7 +214,7 @@ def gated_ema_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, *, 
     device, no slot twice): a negative one marks an idle row, whose output is 0;
     one past the pool gives NaN; neither touches a state.  Returns h [B,D] in x's
     type, in ``out`` (contiguous, in no argument's memory) if given."""
-    fast = _fast()
+    fast = _extension()
     if fast is not None and out is None:
         res = fast.ema_step(x, gate, state, slots)
         if res is not None:

@@ -61,7 +61,7 @@ def set_timing_jitter(on: bool) -> bool:
 
 
 # Test aid: with the poll limit at zero, the forward, TTT, backward and
-# table-forward scan launches carry OSM_FLAG_POLL_LIMIT_ZERO: a look-back wait whose word is not
+# table-forward scan launches, and the gated EMA's, carry OSM_FLAG_POLL_LIMIT_ZERO: a look-back wait whose word is not
 # yet published gives up at once (the fault word is set and the outputs that
 # depend on the missing value are NaN), as a wait that passes its poll limit
 # does.
