@@ -497,7 +497,7 @@ typedef struct osm_ema_step_args {
   int32_t abi_version;          /* = OSM_ABI_VERSION */
   int32_t dtype;                /* osm_dtype of x, gate and out */
   int64_t B, D;
-  osm_seq x, gate, out;         /* [B,D] */
+  osm_seq x, gate, out;         /* [B,D]; in no state's memory (x and gate may be the states where slots is NULL) */
   float* state;                 /* [n_slots,D], slots state_stride elements apart; updated in place */
   int64_t state_stride, n_slots;
   const int64_t* slots;         /* as osm_delta_step_args' */

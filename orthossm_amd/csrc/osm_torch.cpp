@@ -1497,12 +1497,22 @@ PyObject* run_gated_ema(PyObject* const* p) {
   return Py_BuildValue("(NN)", THPVariable_Wrap(out), THPVariable_Wrap(fin));
 }
 
+// Whether the bytes from the first element to the last of two matrices meet.
+bool extents_meet(const at::Tensor& a, const at::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  auto end = [](const at::Tensor& t) {
+    const int64_t last = (t.size(0) - 1) * t.stride(0) + (t.size(1) - 1) * t.stride(1);
+    return static_cast<const char*>(t.data_ptr()) + (last + 1) * (int64_t)t.element_size();
+  };
+  return a.data_ptr() < end(b) && b.data_ptr() < end(a);
+}
+
 // ema_step(x, gate, state, slots): None, or out.
 PyObject* run_ema_step(PyObject* const* p) {
   const at::Tensor *x = plain(p[0]), *gate = plain(p[1]), *state = plain(p[2]);
   if (!x || !gate || !state || !ema_tensor(*x, 2) || !ema_tensor(*gate, 2) || !alike(*gate, *x) || state->dim() != 2 || !is_f32(*state) ||
       state->device() != x->device() || state->size(1) != x->size(1) || (state->stride(1) != 1 && state->size(1) > 1) ||
-      state->stride(0) < state->size(1) || state->requires_grad())
+      state->stride(0) < state->size(1) || state->requires_grad() || extents_meet(*x, *state) || extents_meet(*gate, *state))
     Py_RETURN_NONE;
   osm_ema_step_args a{};
   a.abi_version = OSM_ABI_VERSION;

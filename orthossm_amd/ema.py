@@ -28,7 +28,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _native as nat
 from . import ops
-from .delta import _dest, _lengths, _scratch, _state, apart, differentiable, on_device, written
+from .delta import _dest, _extent, _lengths, _scratch, _state, apart, differentiable, on_device, written
 from .ops import _after_launch, _current_stream, _dtype_code, _fast
 
 
@@ -207,12 +207,27 @@ def gated_ema(x: torch.Tensor, gate: torch.Tensor, *, state_init: torch.Tensor |
     return gated_ema_forward(x, gate, state_init=state_init, lengths=lengths, return_state=return_state)
 
 
+def _reads_states(t: torch.Tensor, state: torch.Tensor, slots) -> bool:
+    """Whether a row of ``t`` [B,D] lies where another row's state is written (its
+    own, at the same place in both, it reads before)."""
+    (a, b), (c, d) = _extent(t), _extent(state)
+    if not t.numel() or not state.numel() or a >= d or c >= b:
+        return False
+    step, rows = t.stride(0) * t.element_size() if t.shape[0] > 1 else 0, state.stride(0) * 4
+    if slots is None and a == c and t.dtype == state.dtype and (step == rows or t.shape[0] == 1):
+        return False
+    # beside the states: in the gaps between them, at whole times their distance
+    gap = (a - c) % rows
+    return step % rows != 0 or gap < 4 * state.shape[1] or gap + t.shape[1] * t.element_size() > rows
+
+
 def gated_ema_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, *, slots: torch.Tensor | None = None,
                    out: torch.Tensor | None = None) -> torch.Tensor:
     """One token a row: x, gate [B,D], and the states [slots,D] fp32, which are
     updated in place.  Row b's state is slot b, or ``slots[b]`` (int64, on the
     device, no slot twice): a negative one marks an idle row, whose output is 0;
-    one past the pool gives NaN; neither touches a state.  Returns h [B,D] in x's
+    one past the pool gives NaN; neither touches a state.  x and gate lie in no
+    state's memory (without slots they may be the states).  Returns h [B,D] in x's
     type, in ``out`` (contiguous, in no argument's memory) if given."""
     fast = _extension()
     if fast is not None and out is None:
@@ -232,6 +247,9 @@ def gated_ema_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, *, 
     elif not isinstance(slots, torch.Tensor) or tuple(slots.shape) != (B,) or slots.dtype != torch.int64 or \
             slots.device != dev or not slots.is_contiguous():
         raise ValueError(f"slots must be a contiguous int64 tensor of shape ({B},) on {dev}")
+    for name, t in (("x", x), ("gate", gate)):
+        if _reads_states(t, state, slots):
+            raise ValueError(f"{name} shares memory with state")
     given = out
     if out is None:
         out = torch.empty((B, D), dtype=x.dtype, device=dev)
