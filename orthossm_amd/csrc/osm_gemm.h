@@ -14,7 +14,7 @@
 // sum of the six products of parts that are not below 2^-24: the product of the first
 // parts, and in accumulators of their own the five small ones.  All parts of a step lie in
 // LDS together: they come from memory and are read once for the six products (5003 x 981 x
-// 448: 34 us; with a walk over k for each product 49).
+// 448: 36 us; with a walk over k for each product 49).
 //
 // What bounds it: the matrix instructions, half of the time (50176 x 8192 x 1024 in tiles of
 // 256 x 256: 680 us, 1238 TFLOP/s, by columns both ways 1170; 16384 x 4096 x 1024 of three

@@ -89,9 +89,10 @@ int64_t next_piece(int64_t left, int64_t piece, int64_t D) {
 Plan plan_of(const osm_loss_args* a, bool bwd) {
   Plan n;
   n.parts = a->dtype == OSM_F32 ? 3 : 1;
-  // (P rounded to bf16 adds as much to a gradient's error as the gradient's own rounding, and
-  // no more where many tokens' errors mean out: of few tokens, which cost little, it is held
-  // to twice the bits.)
+  // (P rounded to bf16 puts a gradient off by 0.0002 to 0.0013 of its size, whatever the number
+  // of tokens, where its own rounding puts it off by 0.0017: together 0.0018 for 65 tokens of 256
+  // over 5000 classes, 0.0021 for 300 of 64 over 50.  A second part doubles both products; of few
+  // tokens, whose products are bounded by the weights' bytes, it is held to twice the bits.)
   n.p_parts = n.parts == 1 && a->N <= 64 ? 2 : n.parts;
   n.Npad = up(std::max<int64_t>(a->N, 1), kLossPad);
   n.Dpad = up(a->D, 64);

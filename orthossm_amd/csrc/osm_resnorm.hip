@@ -9,11 +9,15 @@
 //   dw = sum_rows dn rh,  db = sum_rows dn,  dscale = sum_rows dr u      (no mean(g), mean(e) with rms)
 //
 // What bounds both: the bytes of x, y, gate, r, n (x, y, gate, dr, dn, dx, dy, dgate);
-// 262144 rows of 1024, blocks in bf16 around an fp32 stream: forward 650 us, 5.8 TB/s,
-// backward 1210 us, 4.9 TB/s.
+// 262144 rows of 1024, blocks in bf16 around an fp32 stream: forward 640 us, 5.9 TB/s,
+// backward 1230 us, 4.8 TB/s; all in bf16 449 and 897 us, 6.0 and 4.8 TB/s.
 // A row is held in the registers of a quarter of a wave, of one, of four or of
 // sixteen, so every input is read once, and the next row is on its way while one is
-// worked on.  The backward forms r again from x, y and gate and the saved statistics,
+// worked on.  Not all registers fit where a thread holds 16 elements with an fp32 stream
+// (rows of 513 to 1024 and 2049 to 4096) or 1024 threads hold a row: the backward then
+// spills up to 97 of fp32 blocks (175 by 1024 threads) and 23 of bf16 ones (92), the
+// forward by 1024 threads up to 80, and the rate falls (fp32, backward, 2^27 elements: rows of
+// 512 834 us, 5.2 TB/s; of 1024 1318, 3.3; of 4096 1340, 3.2; of 8192 2108, 2.0).  The backward forms r again from x, y and gate and the saved statistics,
 // unrounded as the forward had it; its workgroups walk rows a grid apart and keep
 // their columns' sums in registers, each writes one line of them, and a second launch
 // adds the lines in order, so the result does not depend on timing.
