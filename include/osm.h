@@ -121,8 +121,10 @@ typedef enum osm_status {
                                       on the missing value are NaN (out,
                                       ema_final, the TTT gradient, the
                                       backward's gradients, the table
-                                      forward's out and ema_final); every kernel
-                                      still exits normally */
+                                      forward's out and ema_final, the gated
+                                      EMA's outputs and gradients, which take
+                                      it beside their type); every kernel still
+                                      exits normally */
 
 /* TTT target y */
 typedef enum osm_ttt_target { OSM_TARGET_X = 0, OSM_TARGET_SOFTSIGN = 1 } osm_ttt_target;
